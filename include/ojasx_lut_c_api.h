@@ -310,6 +310,69 @@ OJASX_API int ojasx_attention_stream_finalize_device(const double *state, int ro
                                                      void *out, int out_dtype, double *lse,
                                                      void *stream);
 
+/* ---- 4-bit paged KV cache and packed prompts (no reference counterpart) --- */
+/* A cache of num_sequences sequences, K and V held in 4 bits.  Of a token's
+ * row of one kv head, each group of group_size dimensions is held as lo =
+ * fp16(min), s = fp16(fp32((max - lo) / 15)) and codes clamp(round_half_even((x
+ * - lo) / s), 0, 15), for the values lo + s * code; a group with an infinity or
+ * a NaN reads back as NaN.  Tokens fill pages of page_size slots; position t
+ * lies in its sequence's page j = t / page_size, which entry e = j < sink_pages
+ * ? j : sink_pages + (j - sink_pages) % (max_pages - sink_pages) of its row of
+ * block_table maps: opening a page beyond max_pages evicts the oldest one after
+ * the sink_pages first.  An entry outside [0, num_pages) is a page that is not
+ * there: its tokens are not written, read as 0 and are not attended.
+ * Lengths are the caller's: int32 arrays on the device, read by the kernels,
+ * so every call can be captured and replayed while they advance.
+ * head_dim 64, 128 or 256; group_size 32, 64 or 128, at most head_dim;
+ * page_size a power of two from 16 to 32768.  Codes and steps are 16-byte
+ * aligned, num_pages * num_kv_heads * page_size * head_dim / 2 bytes of codes
+ * and * 4 / group_size * head_dim bytes of steps for K and V each; the layout
+ * within a page is the library's.  The struct is read during the call. */
+typedef struct OjasxKV4Cache {
+    uint8_t *k_codes, *v_codes;
+    void *k_steps, *v_steps;       /* fp16 pairs (s, lo) */
+    const int *block_table;        /* [num_sequences][max_pages] */
+    const double *turns;           /* [rotary_dim / 2]: frequency / (2 pi), turns per position */
+    int num_sequences, max_pages, sink_pages, page_size, num_pages;
+    int num_kv_heads, head_dim, group_size;
+    int rotary_dim;                /* dimensions that rotate: a multiple of 16, 0: none */
+    int interleaved;               /* pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2) */
+} OjasxKV4Cache;
+/* Rotates queries and keys by their positions and appends keys and values.
+ * Rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32, num_sequences + 1) are
+ * sequence b's tokens at positions start[b], start[b] + 1, ...; cu_seqlens NULL:
+ * one token for each sequence.  q [num_tokens][num_q_heads][head_dim] and k, v
+ * [num_tokens][num_kv_heads][head_dim] in dtype F32, BF16 or F16, with element
+ * strides of tokens and heads, rows 16-byte aligned.  Rotation in fp64, rounded
+ * to fp32: q_out (and k_out, unless NULL) receive it in dtype, contiguous; the
+ * cache encodes the fp32 keys.  num_q_heads 0: no queries.  A token whose page
+ * the same call evicts again is not written.  Rows of no sequence: zeros in
+ * q_out and k_out. */
+OJASX_API int ojasx_kv4_append_device(const OjasxKV4Cache *cache, const void *q, long q_token_stride,
+                                      long q_head_stride, int num_q_heads, void *q_out, const void *k,
+                                      long k_token_stride, long k_head_stride, void *k_out, const void *v,
+                                      long v_token_stride, long v_head_stride, int num_tokens, int dtype,
+                                      const int *start, const int *cu_seqlens, void *stream);
+/* The held values of tokens addressed as in ojasx_kv4_append_device, into
+ * contiguous k_out, v_out [num_tokens][num_kv_heads][head_dim] (dtype F32, BF16
+ * or F16).  seen: the tokens of each sequence so far (NULL: up to the last one
+ * read); a token that they have evicted, and a row of no sequence, reads as 0. */
+OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start, const int *cu_seqlens,
+                                    const int *seen, int num_tokens, void *k_out, void *v_out, int dtype,
+                                    void *stream);
+/* Attention of one query token per sequence over its resident tokens:
+ * q, out [num_sequences][num_q_heads][head_dim] in dtype (F32, BF16, F16), head
+ * j reading kv head j / (num_q_heads / num_kv_heads); seen: the tokens of each
+ * sequence so far (0: a row of zeros).  scale_factor <= 0: 1/sqrt(head_dim).
+ * max_seen bounds seen[] (0: the cache's capacity) and sets how far a sequence
+ * is split; larger entries of seen are attended in full all the same.
+ * workspace: ojasx_kv4_decode_workspace(...) bytes for the same arguments,
+ * 16-byte aligned, one for each call that may run at the same time. */
+OJASX_API long ojasx_kv4_decode_workspace(const OjasxKV4Cache *cache, int num_q_heads, int max_seen);
+OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q, int num_q_heads, int dtype,
+                                      const int *seen, int max_seen, float scale_factor, void *out,
+                                      void *workspace, long workspace_bytes, void *stream);
+
 /* ---- MoE (ref.h:125-150) ---------------------------------------------- */
 OJASX_API OjasxMoEHandle ojasx_create_moe(int num_experts, int hidden_dim,
                                           int intermediate_dim, int top_k, int block_dim,

@@ -78,6 +78,11 @@ SIGNATURES = {
                                                   ctypes.c_longlong, ctypes.c_longlong,
                                                   ctypes.c_double, vp]),
     "ojasx_attention_stream_finalize_device": (ci, [vp, ci, ci, vp, ci, vp, vp]),
+    "ojasx_kv4_append_device": (ci, [vp, vp, cl, cl, ci, vp, vp, cl, cl, vp, vp, cl, cl, ci, ci, vp,
+                                     vp, vp]),
+    "ojasx_kv4_read_device": (ci, [vp, vp, vp, vp, ci, vp, vp, ci, vp]),
+    "ojasx_kv4_decode_workspace": (cl, [vp, ci, ci]),
+    "ojasx_kv4_decode_device": (ci, [vp, vp, ci, ci, vp, ci, cf, vp, vp, cl, vp]),
 }
 
 
@@ -90,6 +95,16 @@ class AttnTile(ctypes.Structure):
                 ("scale_batch_stride", ctypes.c_longlong),
                 ("scale_head_stride", ctypes.c_longlong),
                 ("scale_token_stride", ctypes.c_longlong)]
+
+
+class KV4Cache(ctypes.Structure):
+    """OjasxKV4Cache: the buffers and shape of a 4-bit paged KV cache."""
+    _fields_ = [("k_codes", vp), ("v_codes", vp), ("k_steps", vp), ("v_steps", vp),
+                ("block_table", vp), ("turns", vp),
+                ("num_sequences", ci), ("max_pages", ci), ("sink_pages", ci), ("page_size", ci),
+                ("num_pages", ci), ("num_kv_heads", ci), ("head_dim", ci), ("group_size", ci),
+                ("rotary_dim", ci), ("interleaved", ci)]
+
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1

@@ -1,0 +1,76 @@
+// kv4.h -- the 4-bit paged KV cache's format, shared by its write side
+// (kv4_append.hip) and its attention (kv4_decode.hip).
+//
+// Of a token's K or V row of one kv head (D values, fp32), each group of GS
+// consecutive dimensions is held as lo = fp16(min), s = fp16(fp32((max - lo) /
+// 15)) and codes c_d = clamp(round_half_even((x_d - lo) / s), 0, 15), for the
+// values lo + s c_d.  s = 0 holds codes 0.  lo and s saturate at +-65504; a
+// group with an infinity or a NaN holds s = lo = NaN.
+//
+// A block is 16 slots of a page; block b of a page and kv head holds
+//   K codes  [16 slots][D / 2 bytes]: a row is 4-byte words, word h (D / 32) +
+//            j the 8 dimensions 32 j + 8 h .. + 7: the code of dimension 2 i
+//            of them in bits 4 i, of 2 i + 1 in bits 16 + 4 i (the pairs that a
+//            mask with 0x000f000f leaves are neighbours);
+//   V codes  [D / 2 pairs][16 slots], byte = dimension 2 i in the low four
+//            bits, 2 i + 1 in the high ones;
+//   steps    [D / GS][16 slots] fp16 pairs (s, lo), K and V alike;
+// blocks in the order [page][kv head][block of the page].
+//
+// Position t of a sequence lies in its page j = t / P; the first `sink` pages
+// stay, the others take turns: entry e = j < sink ? j : sink + (j - sink) mod
+// (max_pages - sink) of the sequence's row of the block table.
+#pragma once
+
+#include "common.h"
+
+namespace ojx {
+
+struct Kv4View {
+    uint8_t *kc, *vc;
+    __half2 *ks, *vs;
+    const int *bt;              // [B][max_pages]
+    const double *turns;        // [rot / 2] or null
+    int B, max_pages, sink, pshift, num_pages;   // page = 1 << pshift slots
+    int Hkv, rot, interleaved;
+};
+
+int kv4_view(const OjasxKV4Cache *c, Kv4View *v);   // 0 or an error code
+
+// Entry of the block table that holds page j of a sequence.
+__device__ __forceinline__ int kv4_entry(const Kv4View &c, int j) {
+    return j < c.sink ? j : c.sink + (j - c.sink) % (c.max_pages - c.sink);
+}
+
+// First page after the sink ones that a sequence of `seen` tokens still holds.
+__device__ __forceinline__ int kv4_first_page(const Kv4View &c, int seen) {
+    const int opened = (int)(((long)seen + (1 << c.pshift) - 1) >> c.pshift);
+    return opened - (c.max_pages - c.sink);
+}
+
+// The block that position t of sequence b lies in, in whole-pool block order,
+// or -1: a position before the first, of a page that a sequence of `seen`
+// tokens no longer holds, or of a page the block table does not map.
+__device__ __forceinline__ long kv4_block(const Kv4View &c, int b, int t, int seen, int h) {
+    if (t < 0) return -1;
+    const int j = t >> c.pshift;
+    if (j >= c.sink && j < kv4_first_page(c, seen)) return -1;
+    const int page = c.bt[(long)b * c.max_pages + kv4_entry(c, j)];
+    if (page < 0 || page >= c.num_pages) return -1;
+    return ((((long)page * c.Hkv + h) << c.pshift) + (t & ((1 << c.pshift) - 1))) >> 4;
+}
+
+// The sequence that row n of a packed batch belongs to: the last b with
+// cu[b] <= n (cu has B + 1 entries), -1 or B where it is none.  The whole wave
+// calls it with one n.
+__device__ __forceinline__ int packed_sequence(const int *cu, int B, int n) {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int i0 = 0; i0 <= B; i0 += 64) {
+        const int i = i0 + lane;
+        count += __popcll(__ballot(i <= B && cu[min(i, B)] <= n));
+    }
+    return count - 1;
+}
+
+}  // namespace ojx

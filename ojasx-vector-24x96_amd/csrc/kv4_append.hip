@@ -1,0 +1,449 @@
+// kv4_append.hip -- the write side of the 4-bit paged KV cache (format: kv4.h):
+// rotation of queries and keys by their positions, encoding of keys and values
+// into the pages, and reading tokens back.
+//
+// Rotation: dimensions (i, i + rot / 2), or (2 i, 2 i + 1) interleaved, turn by
+// the angle pos inv_freq[i].  The angle is held in turns, pos (inv_freq / 2 pi),
+// as an fp64 product and its rounding error, so that taking the whole turns
+// away leaves 2^-53 of the frequency's own rounding at any position (fp32
+// angles are off by 0.004 at position 65536).  (x, y) -> (x c - y s, y c + x s)
+// runs in fp64 with one rounding to fp32: the codes then follow from the
+// format's definition, and do not depend on how a product was rounded.
+#include "kv4.h"
+
+namespace ojx {
+
+namespace {
+constexpr int kNT = 256;
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+
+struct Kv4AppendParams {
+    Kv4View c;
+    const void *q, *k, *v;
+    long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;    // token and head strides, elements
+    void *q_out, *k_out;                        // contiguous [n][heads][D]
+    const int *start, *cu;
+    int n, Hq;
+};
+
+// Eight consecutive values as fp32 (16-byte aligned).
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+    const v4f a = *reinterpret_cast<const v4f *>(p), b = *reinterpret_cast<const v4f *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+__device__ __forceinline__ void load8(const __hip_bfloat16 *p, float (&x)[8]) {
+    const v4u a = *reinterpret_cast<const v4u *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(a[i] << 16);
+        x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void load8(const __half *p, float (&x)[8]) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    const h8 a = *reinterpret_cast<const h8 *>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+}
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+    *reinterpret_cast<v4f *>(p) = v4f{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<v4f *>(p + 4) = v4f{x[4], x[5], x[6], x[7]};
+}
+__device__ __forceinline__ void store8(__hip_bfloat16 *p, const float (&x)[8]) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    b8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (__bf16)x[i];
+    *reinterpret_cast<b8 *>(p) = a;
+}
+__device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    h8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (_Float16)x[i];
+    *reinterpret_cast<h8 *>(p) = a;
+}
+
+// Minimum, maximum and sum over the LANES (4, 8 or 16) lanes of a group.
+template <int LANES>
+__device__ __forceinline__ void group_stats(float &mn, float &mx, float &sum) {
+#define OJX_GROUP_STEP(CTRL)                                          \
+    mn = fminf(mn, __int_as_float(dpp_i<CTRL>(__float_as_int(mn)))); \
+    mx = fmaxf(mx, __int_as_float(dpp_i<CTRL>(__float_as_int(mx)))); \
+    sum += __int_as_float(dpp_i<CTRL>(__float_as_int(sum)));
+    OJX_GROUP_STEP(0xB1)
+    OJX_GROUP_STEP(0x4E)
+    if (LANES > 4) { OJX_GROUP_STEP(0x141) }
+    if (LANES > 8) { OJX_GROUP_STEP(0x140) }
+#undef OJX_GROUP_STEP
+}
+
+// fp16 of a float, rounded to nearest even.  The value passes through a
+// register the compiler cannot see behind: it would round the fp64 expression
+// it came from to fp16 at once, where the format rounds to fp32 first.
+__device__ __forceinline__ _Float16 to_half(float f) {
+    asm volatile("" : "+v"(f));
+    return (_Float16)f;
+}
+
+// Encodes a lane's eight dimensions of a K (V) row into block `blk`, slot t.
+// unit: which eight of the row's D / 8.
+template <int D, int GS>
+__device__ __forceinline__ void encode_unit(const float (&x)[8], bool value, int unit, long blk, int t,
+                                            uint8_t *codes, __half2 *steps) {
+    float mn = x[0], mx = x[0], poison = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        mn = fminf(mn, x[i]);
+        mx = fmaxf(mx, x[i]);
+        poison = fmaf(x[i], 0.f, poison);       // NaN from an infinity or a NaN, else 0
+    }
+    group_stats<GS / 8>(mn, mx, poison);
+    const _Float16 lo = to_half(fminf(fmaxf(mn, -65504.f), 65504.f) + poison);
+    const float step = (float)(((double)mx - (double)(float)lo) / 15.0);
+    const _Float16 s = to_half(fminf(step, 65504.f) + poison);
+    const float lo32 = (float)lo, s32 = (float)s, inv = s32 > 0.f ? 1.0f / s32 : 0.f;
+    int code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = (x[i] - lo32) * inv;
+        float r = rintf(f);
+        // f is off by less than 2^-18: only beside a half can the fp32 quotient
+        // round another way than the exact one, whose remainder decides there
+        if (fabsf(f - r) > 0.4999f && s32 > 0.f) {
+            const double e = fma(-(double)r, (double)s32, (double)x[i] - (double)lo32);
+            const double half = 0.5 * (double)s32;
+            const bool odd = ((int)r & 1) != 0;
+            if (e > half || (e == half && odd)) r += 1.f;
+            else if (e < -half || (e == -half && odd)) r -= 1.f;
+        }
+        code[i] = (int)fminf(fmaxf(r, 0.f), 15.f);   // NaN: 0
+    }
+    if (blk < 0) return;
+    if (!value) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (uint32_t)code[2 * i] << (4 * i) | (uint32_t)code[2 * i + 1] << (16 + 4 * i);
+        const int word = (unit & 3) * (D / 32) + (unit >> 2);
+        reinterpret_cast<uint32_t *>(codes + blk * (D * 8) + t * (D / 2))[word] = w;
+    } else {
+        uint8_t *dst = codes + blk * (D * 8) + unit * 64 + t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[16 * i] = (uint8_t)(code[2 * i] | code[2 * i + 1] << 4);
+    }
+    if (unit % (GS / 8) == 0) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        reinterpret_cast<h2 *>(steps)[(blk * (D / GS) + unit / (GS / 8)) * 16 + t] = h2{s, lo};
+    }
+}
+}  // namespace
+
+// A workgroup takes one token (blockIdx.x); its threads each eight dimensions
+// of a query, key or value row at a time.
+template <typename T, int D, int GS>
+__global__ __launch_bounds__(kNT) void kv4_append_kernel(Kv4AppendParams p) {
+    __shared__ double2 cs[D / 2];               // cos and sin of the token's angles
+    const int tid = threadIdx.x, n = blockIdx.x;
+    constexpr int UPR = D / 8;                  // units of eight per row
+    int b = n, pos, seen;
+    if (p.cu) {
+        b = packed_sequence(p.cu, p.c.B, n);
+        const bool none = b < 0 || b >= p.c.B;  // a row of no sequence
+        const int bb = none ? 0 : b;
+        const int first = p.cu[bb], s0 = p.start[bb];
+        pos = s0 + (n - first);
+        seen = s0 + (p.cu[bb + 1] - first);
+        if (none) b = -1;
+    } else {
+        pos = p.start[b];
+        seen = pos + 1;
+    }
+    const int half = p.c.rot >> 1;
+    if (b >= 0) {
+        for (int i = tid; i < half; i += kNT) {
+            const double f = p.c.turns[i], t = (double)pos * f;
+            const double frac = (t - rint(t)) + fma((double)pos, f, -t);
+            double s, c;
+            sincospi(2.0 * frac, &s, &c);
+            cs[i] = make_double2(c, s);
+        }
+    }
+    __syncthreads();
+    const int Hkv = p.c.Hkv, units = (p.Hq + 2 * Hkv) * UPR;
+    const int t = pos & 15;
+    for (int u0 = blockIdx.y * kNT; u0 < units; u0 += gridDim.y * kNT) {
+        const int u = u0 + tid;
+        if (u >= units) break;
+        const int row = u / UPR, unit = u % UPR;
+        const bool isq = row < p.Hq, isv = row >= p.Hq + Hkv;
+        const int head = isq ? row : isv ? row - p.Hq - Hkv : row - p.Hq;
+        const T *src = isq ? static_cast<const T *>(p.q) + n * p.q_ts + head * p.q_hs
+                     : isv ? static_cast<const T *>(p.v) + n * p.v_ts + head * p.v_hs
+                           : static_cast<const T *>(p.k) + n * p.k_ts + head * p.k_hs;
+        const int d0 = unit * 8;
+        float x[8];
+        T *out = isq ? static_cast<T *>(p.q_out) : isv ? nullptr : static_cast<T *>(p.k_out);
+        if (out) out += ((size_t)n * (isq ? p.Hq : Hkv) + head) * D + d0;
+        if (b < 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 0.f;
+            if (out) store8(out, x);
+            continue;
+        }
+        load8(src + d0, x);
+        if (!isv && d0 < p.c.rot) {
+            if (p.c.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double2 r = cs[d0 / 2 + i];
+                    const double a = x[2 * i], c = x[2 * i + 1];
+                    x[2 * i] = (float)(a * r.x - c * r.y);
+                    x[2 * i + 1] = (float)(c * r.x + a * r.y);
+                }
+            } else {
+                const bool low = d0 < half;
+                float y[8];
+                load8(src + (low ? d0 + half : d0 - half), y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const double2 r = cs[(low ? d0 : d0 - half) + i];
+                    const double a = x[i], c = y[i];
+                    x[i] = (float)(low ? a * r.x - c * r.y : a * r.x + c * r.y);
+                }
+            }
+        }
+        if (out) store8(out, x);
+        if (!isq) {
+            const long blk = kv4_block(p.c, b, pos, seen, head);
+            encode_unit<D, GS>(x, isv, unit, blk, t, isv ? p.c.vc : p.c.kc, isv ? p.c.vs : p.c.ks);
+        }
+    }
+}
+
+struct Kv4ReadParams {
+    Kv4View c;
+    const int *start, *cu, *seen;
+    void *k_out, *v_out;        // contiguous [n][Hkv][D]
+    int n;
+};
+
+// The appended tokens' values: workgroup = token, thread = eight dimensions of
+// a K or V row at a time.
+template <typename T, int D, int GS>
+__global__ __launch_bounds__(kNT) void kv4_read_kernel(Kv4ReadParams p) {
+    const int tid = threadIdx.x, n = blockIdx.x;
+    constexpr int UPR = D / 8;
+    int b = n, pos, seen;
+    if (p.cu) {
+        b = packed_sequence(p.cu, p.c.B, n);
+        const bool none = b < 0 || b >= p.c.B;
+        const int bb = none ? 0 : b;
+        const int first = p.cu[bb], s0 = p.start[bb];
+        pos = s0 + (n - first);
+        seen = s0 + (p.cu[bb + 1] - first);
+        if (none) b = -1;
+    } else {
+        pos = p.start[b];
+        seen = pos + 1;
+    }
+    if (p.seen && b >= 0) seen = p.seen[b];
+    const int Hkv = p.c.Hkv, units = 2 * Hkv * UPR, t = pos & 15;
+    for (int u0 = blockIdx.y * kNT; u0 < units; u0 += gridDim.y * kNT) {
+        const int u = u0 + tid;
+        if (u >= units) break;
+        const int row = u / UPR, unit = u % UPR;
+        const bool isv = row >= Hkv;
+        const int head = isv ? row - Hkv : row;
+        const long blk = b < 0 || pos >= seen ? -1 : kv4_block(p.c, b, pos, seen, head);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (blk >= 0) {
+            const __half2 st = (isv ? p.c.vs : p.c.ks)[(blk * (D / GS) + unit / (GS / 8)) * 16 + t];
+            const float s = __low2float(st), lo = __high2float(st);
+            if (!isv) {
+                const int word = (unit & 3) * (D / 32) + (unit >> 2);
+                const uint32_t w =
+                    reinterpret_cast<const uint32_t *>(p.c.kc + blk * (D * 8) + t * (D / 2))[word];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[2 * i] = fmaf(s, (float)(w >> (4 * i) & 15u), lo);
+                    x[2 * i + 1] = fmaf(s, (float)(w >> (16 + 4 * i) & 15u), lo);
+                }
+            } else {
+                const uint8_t *src = p.c.vc + blk * (D * 8) + unit * 64 + t;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t w = src[16 * i];
+                    x[2 * i] = fmaf(s, (float)(w & 15u), lo);
+                    x[2 * i + 1] = fmaf(s, (float)(w >> 4), lo);
+                }
+            }
+        }
+        store8(static_cast<T *>(isv ? p.v_out : p.k_out) + ((size_t)n * Hkv + head) * D + unit * 8, x);
+    }
+}
+
+int kv4_view(const OjasxKV4Cache *c, Kv4View *v) {
+    if (!c || !c->k_codes || !c->v_codes || !c->k_steps || !c->v_steps || !c->block_table) {
+        set_error("4-bit KV cache: a NULL buffer");
+        return OJASX_ERR_NULL;
+    }
+    const int D = c->head_dim, GS = c->group_size;
+    if ((D != 64 && D != 128 && D != 256) || (GS != 32 && GS != 64 && GS != 128) || GS > D) {
+        set_error("4-bit KV cache: head_dim %d, group_size %d (64, 128 or 256; 32, 64 or 128 and at most "
+                  "head_dim)", D, GS);
+        return OJASX_ERR_INVALID;
+    }
+    const int P = c->page_size;
+    if (P < 16 || P > 32768 || (P & (P - 1))) {
+        set_error("4-bit KV cache: page_size %d is no power of two from 16 to 32768", P);
+        return OJASX_ERR_INVALID;
+    }
+    if (c->num_sequences <= 0 || c->num_kv_heads <= 0 || c->num_kv_heads > 65535 || c->num_pages <= 0 ||
+        c->sink_pages < 0 || c->max_pages <= c->sink_pages) {
+        set_error("4-bit KV cache: %d sequences, %d kv heads, %d pages, %d of a sequence with %d sink pages",
+                  c->num_sequences, c->num_kv_heads, c->num_pages, c->max_pages, c->sink_pages);
+        return OJASX_ERR_INVALID;
+    }
+    if (c->rotary_dim < 0 || c->rotary_dim > D || c->rotary_dim % 16 || (c->rotary_dim && !c->turns)) {
+        set_error("4-bit KV cache: rotary_dim %d (a multiple of 16 up to %d, with turns)", c->rotary_dim, D);
+        return OJASX_ERR_INVALID;
+    }
+    if ((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes) |
+         reinterpret_cast<uintptr_t>(c->k_steps) | reinterpret_cast<uintptr_t>(c->v_steps)) & 15) {
+        set_error("4-bit KV cache: codes and steps are 16-byte aligned");
+        return OJASX_ERR_INVALID;
+    }
+    v->kc = c->k_codes;
+    v->vc = c->v_codes;
+    v->ks = static_cast<__half2 *>(c->k_steps);
+    v->vs = static_cast<__half2 *>(c->v_steps);
+    v->bt = c->block_table;
+    v->turns = c->turns;
+    v->B = c->num_sequences;
+    v->max_pages = c->max_pages;
+    v->sink = c->sink_pages;
+    v->pshift = __builtin_ctz((unsigned)P);
+    v->num_pages = c->num_pages;
+    v->Hkv = c->num_kv_heads;
+    v->rot = c->rotary_dim;
+    v->interleaved = c->interleaved != 0;
+    return OJASX_OK;
+}
+
+namespace {
+// Workgroups per token: one for each kNT units while the tokens are fewer than
+// the card's CUs, else one that takes the token's units in turn and computes
+// its angles once.
+int row_split(int n, long units) { return n < 256 ? (int)((units + kNT - 1) / kNT) : 1; }
+
+// The (element type, head_dim, group_size) instances of a kernel.
+#define OJX_KV4_DISPATCH(KERNEL, T, D, GS, ...)                                               \
+    do {                                                                                      \
+        if (D == 64 && GS == 32) OJX_LAUNCH((KERNEL<T, 64, 32>), __VA_ARGS__);                \
+        else if (D == 64) OJX_LAUNCH((KERNEL<T, 64, 64>), __VA_ARGS__);                       \
+        else if (D == 128 && GS == 32) OJX_LAUNCH((KERNEL<T, 128, 32>), __VA_ARGS__);         \
+        else if (D == 128 && GS == 64) OJX_LAUNCH((KERNEL<T, 128, 64>), __VA_ARGS__);         \
+        else if (D == 128) OJX_LAUNCH((KERNEL<T, 128, 128>), __VA_ARGS__);                    \
+        else if (GS == 32) OJX_LAUNCH((KERNEL<T, 256, 32>), __VA_ARGS__);                     \
+        else if (GS == 64) OJX_LAUNCH((KERNEL<T, 256, 64>), __VA_ARGS__);                     \
+        else OJX_LAUNCH((KERNEL<T, 256, 128>), __VA_ARGS__);                                  \
+    } while (0)
+
+#define OJX_KV4_DISPATCH_T(KERNEL, dtype, D, GS, ...)                                         \
+    do {                                                                                      \
+        if (dtype == OJASX_DTYPE_F32) OJX_KV4_DISPATCH(KERNEL, float, D, GS, __VA_ARGS__);    \
+        else if (dtype == OJASX_DTYPE_BF16)                                                   \
+            OJX_KV4_DISPATCH(KERNEL, __hip_bfloat16, D, GS, __VA_ARGS__);                     \
+        else OJX_KV4_DISPATCH(KERNEL, __half, D, GS, __VA_ARGS__);                            \
+    } while (0)
+
+bool rows_ok(const void *p, long ts, long hs, size_t es) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ts >= 0 && hs >= 0 &&
+           (ts * es) % 16 == 0 && (hs * es) % 16 == 0;
+}
+}  // namespace
+
+}  // namespace ojx
+
+extern "C" {
+
+OJASX_API int ojasx_kv4_append_device(const OjasxKV4Cache *cache, const void *q, long q_token_stride,
+                                      long q_head_stride, int num_q_heads, void *q_out, const void *k,
+                                      long k_token_stride, long k_head_stride, void *k_out, const void *v,
+                                      long v_token_stride, long v_head_stride, int num_tokens, int dtype,
+                                      const int *start, const int *cu_seqlens, void *stream) {
+    using namespace ojx;
+    Kv4AppendParams p{};
+    int rc = kv4_view(cache, &p.c);
+    if (rc) return rc;
+    if (dtype != OJASX_DTYPE_F32 && dtype != OJASX_DTYPE_BF16 && dtype != OJASX_DTYPE_F16) {
+        set_error("unsupported dtype %d", dtype);
+        return OJASX_ERR_INVALID;
+    }
+    if (num_tokens < 0 || num_q_heads < 0 || num_q_heads > 65535 ||
+        (!cu_seqlens && num_tokens != cache->num_sequences)) {
+        set_error("4-bit KV append: %d tokens, %d query heads (without cu_seqlens one token for each of the "
+                  "%d sequences)", num_tokens, num_q_heads, cache->num_sequences);
+        return OJASX_ERR_INVALID;
+    }
+    if (num_tokens == 0) return OJASX_OK;
+    if (!k || !v || !start || (num_q_heads && (!q || !q_out))) return OJASX_ERR_NULL;
+    const size_t es = dtype == OJASX_DTYPE_F32 ? 4 : 2;
+    if (!rows_ok(k, k_token_stride, k_head_stride, es) || !rows_ok(v, v_token_stride, v_head_stride, es) ||
+        (num_q_heads && (!rows_ok(q, q_token_stride, q_head_stride, es) || !rows_ok(q_out, 0, 0, es))) ||
+        (k_out && !rows_ok(k_out, 0, 0, es))) {
+        set_error("4-bit KV append: rows are 16-byte aligned");
+        return OJASX_ERR_INVALID;
+    }
+    p.q = q, p.k = k, p.v = v;
+    p.q_ts = q_token_stride, p.q_hs = q_head_stride;
+    p.k_ts = k_token_stride, p.k_hs = k_head_stride;
+    p.v_ts = v_token_stride, p.v_hs = v_head_stride;
+    p.q_out = q_out, p.k_out = k_out;
+    p.start = start, p.cu = cu_seqlens;
+    p.n = num_tokens, p.Hq = num_q_heads;
+    const int D = cache->head_dim, GS = cache->group_size;
+    const long units = ((long)num_q_heads + 2L * cache->num_kv_heads) * (D / 8);
+    const dim3 grid(num_tokens, row_split(num_tokens, units));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    OJX_KV4_DISPATCH_T(kv4_append_kernel, dtype, D, GS, grid, dim3(kNT), 0, st, p);
+    OJX_HIP(hipGetLastError());
+    return OJASX_OK;
+}
+
+OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start, const int *cu_seqlens,
+                                    const int *seen, int num_tokens, void *k_out, void *v_out, int dtype, void *stream) {
+    using namespace ojx;
+    Kv4ReadParams p{};
+    int rc = kv4_view(cache, &p.c);
+    if (rc) return rc;
+    if (dtype != OJASX_DTYPE_F32 && dtype != OJASX_DTYPE_BF16 && dtype != OJASX_DTYPE_F16) {
+        set_error("unsupported dtype %d", dtype);
+        return OJASX_ERR_INVALID;
+    }
+    if (num_tokens < 0 || (!cu_seqlens && num_tokens != cache->num_sequences)) {
+        set_error("4-bit KV read: %d tokens (without cu_seqlens one for each of the %d sequences)", num_tokens,
+                  cache->num_sequences);
+        return OJASX_ERR_INVALID;
+    }
+    if (num_tokens == 0) return OJASX_OK;
+    if (!start || !k_out || !v_out) return OJASX_ERR_NULL;
+    if (!rows_ok(k_out, 0, 0, 4) || !rows_ok(v_out, 0, 0, 4)) {
+        set_error("4-bit KV read: outputs are 16-byte aligned");
+        return OJASX_ERR_INVALID;
+    }
+    p.start = start, p.cu = cu_seqlens, p.seen = seen, p.k_out = k_out, p.v_out = v_out, p.n = num_tokens;
+    const int D = cache->head_dim, GS = cache->group_size;
+    const dim3 grid(num_tokens, row_split(num_tokens, 2L * cache->num_kv_heads * (D / 8)));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    OJX_KV4_DISPATCH_T(kv4_read_kernel, dtype, D, GS, grid, dim3(kNT), 0, st, p);
+    OJX_HIP(hipGetLastError());
+    return OJASX_OK;
+}
+
+}  // extern "C"

@@ -25,6 +25,11 @@ csrc/lut_kv.hip.
   pages are then read in place and dequantised in registers, all pages in
   one update.
 
+* ``PagedInt4KVCache`` is the cache of a serving batch: the keys and values of
+  several sequences in 4 bits, with the position rotation applied on the way
+  in (csrc/kv4_append.hip, csrc/kv4_decode.hip).  The sequences' lengths are
+  the caller's, in device memory, so its calls can be captured.
+
 Everything runs on the GPU; CPU queries raise.
 """
 from __future__ import annotations
@@ -643,3 +648,296 @@ class PagedCodeKVCache:
         """Codes and scales of the resident tokens (K and V)."""
         G = self.head_dim // self.block_dim
         return 2 * self.seq_len * self.num_kv_heads * (G + 4)
+
+
+def _inference_tag(what, *tensors):
+    """The C-ABI tag of the tensors' one dtype; they have no gradient here."""
+    torch = _torch()
+    t = tensors[0]
+    for u in tensors:
+        _require_gpu(u, what)
+        if u.dtype != t.dtype or u.device != t.device:
+            raise ValueError(f"{what}: tensors of {t.dtype} on {t.device} and of {u.dtype} on {u.device}")
+        if u.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or with detached "
+                               "tensors")
+    tag = _attn_tag(t.dtype)
+    if tag is None or tag == _lib.DTYPE_F64:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype}: float32, bfloat16 or float16")
+    return tag
+
+
+def _aligned_rows(t):
+    """t [n, heads, D] itself where its rows are contiguous and 16-byte aligned,
+    else a contiguous copy."""
+    es = t.element_size()
+    s = t.stride()
+    if s[2] != 1 or t.data_ptr() % 16 or s[0] * es % 16 or s[1] * es % 16 or s[0] < 0 or s[1] < 0:
+        t = t.contiguous()
+        if t.data_ptr() % 16:               # contiguous() returns a contiguous slice as it is
+            t = t.clone()
+    return t
+
+
+def _lengths_tensor(t, n, device, what):
+    torch = _torch()
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or \
+            t.device != device:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries on {device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+class _on_device:
+    """Makes ``device`` the current one for a call where another is."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device):
+        self.index = device.index
+        self.before = None
+
+    def __enter__(self):
+        torch = _torch()
+        current = torch.cuda.current_device()
+        if current != self.index:
+            self.before = current
+            torch.cuda.set_device(self.index)
+        return _lib.raw_stream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            _torch().cuda.set_device(self.before)
+
+
+class PagedInt4KVCache:
+    """Paged KV cache of one attention layer for ``num_sequences`` sequences, in
+    4 bits, on the GPU.
+
+    Of a token's key or value row of one head, each group of ``group_size``
+    dimensions is held as its smallest value lo and the step s = (largest - lo)
+    / 15 in fp16 and 4-bit codes, for the values lo + s * code: 4 + 32 /
+    group_size bits per value.  A group with an infinity or a NaN reads back as
+    NaN.
+
+    Tokens fill pages of ``page_size`` (a power of two from 16).  A sequence
+    keeps at most ``max_resident_pages`` of them: opening one more evicts the
+    oldest after the ``sink_pages`` first ones.  Its page j sits in entry e = j
+    < sink_pages ? j : sink_pages + (j - sink_pages) % (max_resident_pages -
+    sink_pages) of its row of ``block_table`` (int32 [num_sequences,
+    max_resident_pages], physical pages): by default every sequence has pages
+    of its own.  With ``num_pages`` given, the pool has that many pages and the
+    table starts as -1, no page; the caller fills it in (sequences may share
+    pages that none of them writes).
+
+    Keys, and queries given to ``append``, are rotated by their positions:
+    dimensions (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with ``interleaved``,
+    by the angle position * inv_freq[i], inv_freq[i] = rope_theta ** (-2 i /
+    rotary_dim) unless ``inv_freq`` (rotary_dim / 2 values) is given;
+    ``rope_theta=None`` without ``inv_freq``: no rotation.  Angles are held in
+    64 bits.
+
+    The sequences' lengths are the caller's: int32 tensors on the cache's
+    device, one for all layers, that a captured graph advances itself.  Calls
+    on one cache write its pages: order them on one stream."""
+
+    def __init__(self, num_kv_heads: int, head_dim: int = 128, *, num_sequences: int = 1,
+                 page_size: int = 16, max_resident_pages: int = 2048, sink_pages: int = 2,
+                 group_size: int = 32, rope_theta: Optional[float] = 1e6, inv_freq=None,
+                 rotary_dim: Optional[int] = None, interleaved: bool = False,
+                 num_pages: Optional[int] = None, device="cuda") -> None:
+        torch = _torch()
+        if head_dim not in (64, 128, 256) or group_size not in (32, 64, 128) or group_size > head_dim:
+            raise ValueError(f"head_dim must be 64, 128 or 256 and group_size 32, 64 or 128, at most "
+                             f"head_dim: got {head_dim} and {group_size}")
+        if not 16 <= page_size <= 32768 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 32768, got {page_size}")
+        if num_kv_heads <= 0 or num_sequences <= 0 or sink_pages < 0 or \
+                max_resident_pages <= sink_pages or (num_pages is not None and num_pages <= 0):
+            raise ValueError("Invalid page configuration for PagedInt4KVCache")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("PagedInt4KVCache runs on the GPU only")
+        if inv_freq is None and rope_theta is None:
+            if rotary_dim:
+                raise ValueError("rotary_dim without rope_theta or inv_freq")
+            rotary_dim = 0
+        elif rotary_dim is None:
+            rotary_dim = head_dim
+        if rotary_dim < 0 or rotary_dim > head_dim or rotary_dim % 16:
+            raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim, got {rotary_dim}")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        dev = self.device
+        turns = None
+        if rotary_dim:
+            if inv_freq is None:
+                inv_freq = float(rope_theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+                                                 / rotary_dim)
+            inv_freq = torch.as_tensor(inv_freq).to(device="cpu", dtype=torch.float64)
+            if tuple(inv_freq.shape) != (rotary_dim // 2,):
+                raise ValueError(f"inv_freq must hold {rotary_dim // 2} values, got "
+                                 f"{tuple(inv_freq.shape)}")
+            turns = (inv_freq / (2.0 * math.pi)).to(dev)
+        self.num_kv_heads, self.head_dim, self.group_size = num_kv_heads, head_dim, group_size
+        self.num_sequences, self.page_size = num_sequences, page_size
+        self.max_resident_pages, self.sink_pages = max_resident_pages, sink_pages
+        self.rotary_dim, self.interleaved = rotary_dim, bool(interleaved)
+        self.num_pages = num_sequences * max_resident_pages if num_pages is None else num_pages
+        rows = self.num_pages * num_kv_heads * page_size
+        self.k_codes = torch.zeros(rows * head_dim // 2, dtype=torch.uint8, device=dev)
+        self.v_codes = torch.zeros_like(self.k_codes)
+        self.k_steps = torch.zeros(rows * head_dim // group_size * 2, dtype=torch.float16, device=dev)
+        self.v_steps = torch.zeros_like(self.k_steps)
+        if num_pages is None:
+            table = torch.arange(self.num_pages, dtype=torch.int32, device=dev)
+        else:
+            table = torch.full((num_sequences * max_resident_pages,), -1, dtype=torch.int32, device=dev)
+        self.block_table = table.view(num_sequences, max_resident_pages)
+        self._turns = turns
+        self._c = _lib.KV4Cache(_vp(self.k_codes), _vp(self.v_codes), _vp(self.k_steps),
+                                _vp(self.v_steps), _vp(self.block_table),
+                                _vp(turns) if turns is not None else None, num_sequences,
+                                max_resident_pages, sink_pages, page_size, self.num_pages,
+                                num_kv_heads, head_dim, group_size, rotary_dim, int(self.interleaved))
+        self._ref = ctypes.addressof(self._c)
+        self._workspace_bytes = {}       # (query heads, max_seen) -> bytes
+
+    @property
+    def capacity(self) -> int:
+        """Tokens of one sequence that its pages hold at most."""
+        return self.max_resident_pages * self.page_size
+
+    @property
+    def storage_bytes(self) -> int:
+        """Bytes of the pool: codes, steps and block table."""
+        return sum(t.numel() * t.element_size() for t in
+                   (self.k_codes, self.v_codes, self.k_steps, self.v_steps, self.block_table))
+
+    def _check_rows(self, t, n, heads, name):
+        if t.dim() != 3 or t.shape[0] != n or t.shape[2] != self.head_dim or \
+                (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"{name} must be [{n}, {heads or 'heads'}, {self.head_dim}], got "
+                             f"{tuple(t.shape)}")
+        if t.device != self.device:
+            raise ValueError(f"{name} lives on {t.device}, the cache on {self.device}")
+
+    def _packed(self, n, start, cu_seqlens):
+        B = self.num_sequences
+        at = _lengths_tensor(start, B, self.device, "start")
+        if cu_seqlens is None:
+            if n != B:
+                raise ValueError(f"{n} tokens: without cu_seqlens each of the {B} sequences gets one")
+            return at, None
+        return at, _lengths_tensor(cu_seqlens, B + 1, self.device, "cu_seqlens")
+
+    def append(self, key, value, start, cu_seqlens=None, *, query=None, return_key: bool = False):
+        """Rotate and append ``key`` and ``value`` [N, num_kv_heads, head_dim]
+        (float32, bfloat16 or float16, any strides): rows cu_seqlens[b] ..
+        cu_seqlens[b + 1] - 1 are sequence b's tokens at positions start[b],
+        start[b] + 1, ...; without ``cu_seqlens`` row b is sequence b's one
+        token.  ``start`` (int32 [num_sequences]) is read, not advanced.
+
+        Returns (query rotated by the same positions or None, the rotated key
+        before its encoding or None without ``return_key``), contiguous, in
+        their dtype; rows that belong to no sequence are zeros there."""
+        torch = _torch()
+        what = "PagedInt4KVCache.append"
+        tensors = (key, value) if query is None else (key, value, query)
+        tag = _inference_tag(what, *tensors)
+        n = key.shape[0] if key.dim() else 0
+        self._check_rows(key, n, self.num_kv_heads, "key")
+        self._check_rows(value, n, self.num_kv_heads, "value")
+        if query is not None:
+            self._check_rows(query, n, None, "query")
+        at, cu = self._packed(n, start, cu_seqlens)
+        with _on_device(self.device) as stream:
+            k, v = _aligned_rows(key), _aligned_rows(value)
+            ks, vs = k.stride(), v.stride()
+            qp = qo = ko = None
+            qs, heads = (0, 0), 0
+            if query is not None:
+                q = _aligned_rows(query)
+                qs, heads = q.stride(), q.shape[1]
+                qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                qp = q.data_ptr()
+            if return_key:
+                ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            rc = _lib.lib().ojasx_kv4_append_device(
+                self._ref, qp, qs[0], qs[1], heads, None if qo is None else qo.data_ptr(),
+                k.data_ptr(), ks[0], ks[1], None if ko is None else ko.data_ptr(), v.data_ptr(),
+                vs[0], vs[1], n, tag, at, cu, stream)
+        if rc:
+            _lib.check(rc, "ojasx_kv4_append_device")
+        return qo, ko
+
+    def read(self, start, cu_seqlens=None, num_tokens: Optional[int] = None, *, seen=None, dtype=None):
+        """The held keys (rotated) and values of tokens addressed as in
+        ``append``: (k, v), each [num_tokens, num_kv_heads, head_dim] in
+        ``dtype`` (float32 unless given).  ``seen`` (int32 [num_sequences]): the
+        tokens of each sequence so far, where that is more than the last one
+        read; a token its sequence has evicted reads as 0."""
+        torch = _torch()
+        dtype = torch.float32 if dtype is None else dtype
+        tag = _attn_tag(dtype)
+        if tag is None or tag == _lib.DTYPE_F64:
+            raise TypeError(f"unsupported dtype {dtype}: float32, bfloat16 or float16")
+        if num_tokens is None:
+            if cu_seqlens is not None:
+                raise ValueError("give num_tokens with cu_seqlens: the rows of the result")
+            num_tokens = self.num_sequences
+        if num_tokens < 0:
+            raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
+        at, cu = self._packed(num_tokens, start, cu_seqlens)
+        sp = None if seen is None else _lengths_tensor(seen, self.num_sequences, self.device, "seen")
+        with _on_device(self.device) as stream:
+            k = torch.empty(num_tokens, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
+            rc = _lib.lib().ojasx_kv4_read_device(self._ref, at, cu, sp, num_tokens, k.data_ptr(),
+                                                  v.data_ptr(), tag, stream)
+        if rc:
+            _lib.check(rc, "ojasx_kv4_read_device")
+        return k, v
+
+    def decode(self, query, seen, scale_factor: float = -1.0, *, max_seen: int = 0, out=None):
+        """Attention of one query token per sequence, ``query``
+        [num_sequences, num_q_heads, head_dim] (rotated; float32, bfloat16 or
+        float16), over the resident ones of the ``seen[b]`` tokens (int32
+        [num_sequences], the current one included) of each sequence; q head j
+        reads kv head j // (num_q_heads // num_kv_heads).  ``scale_factor <= 0``
+        means 1/sqrt(head_dim); a sequence without tokens gives 0.
+        ``max_seen``, a bound on ``seen`` where the caller knows one, keeps
+        short sequences from being split as far as the capacity asks for."""
+        torch = _torch()
+        what = "PagedInt4KVCache.decode"
+        tag = _inference_tag(what, query)
+        self._check_rows(query, self.num_sequences, None, "query")
+        heads = query.shape[1]
+        if heads == 0 or heads % self.num_kv_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {self.num_kv_heads} kv heads")
+        if max_seen < 0:
+            raise ValueError(f"max_seen must not be negative, got {max_seen}")
+        sp = _lengths_tensor(seen, self.num_sequences, self.device, "seen")
+        lib = _lib.lib()
+        need = self._workspace_bytes.get((heads, max_seen))
+        if need is None:
+            need = lib.ojasx_kv4_decode_workspace(self._ref, heads, max_seen)
+            if need < 0:
+                _lib.check(need, "ojasx_kv4_decode_workspace")
+            if len(self._workspace_bytes) > 64:
+                self._workspace_bytes.clear()
+            self._workspace_bytes[(heads, max_seen)] = need
+        if out is None:
+            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or \
+                not out.is_contiguous():
+            raise ValueError("out must be contiguous and of the query's shape, dtype and device")
+        with _on_device(self.device) as stream:
+            q = query.contiguous()
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            rc = lib.ojasx_kv4_decode_device(self._ref, q.data_ptr(), heads, tag, sp, max_seen,
+                                             float(scale_factor), out.data_ptr(),
+                                             ws.data_ptr() if need else None, need, stream)
+        if rc:
+            _lib.check(rc, "ojasx_kv4_decode_device")
+        return out
