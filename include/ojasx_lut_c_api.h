@@ -313,7 +313,7 @@ OJASX_API int ojasx_attention_stream_finalize_device(const double *state, int ro
 /* ---- 4-bit paged KV cache and packed prompts (no reference counterpart) --- */
 /* A cache of num_sequences sequences, K and V held in 4 bits.  Of a token's
  * row of one kv head, each group of group_size dimensions is held as lo =
- * fp16(min), s = fp16(fp32((max - lo) / 15)) and codes clamp(round_half_even((x
+ * fp16(min), s = fp16(fp32((max - lo) / 15)), at least 0, and codes clamp(round_half_even((x
  * - lo) / s), 0, 15), for the values lo + s * code; a group with an infinity or
  * a NaN reads back as NaN.  Tokens fill pages of page_size slots; position t
  * lies in its sequence's page j = t / page_size, which entry e = j < sink_pages

@@ -104,7 +104,8 @@ __device__ __forceinline__ void encode_unit(const float (&x)[8], bool value, int
     group_stats<GS / 8>(mn, mx, poison);
     const _Float16 lo = to_half(fminf(fmaxf(mn, -65504.f), 65504.f) + poison);
     const float step = (float)(((double)mx - (double)(float)lo) / 15.0);
-    const _Float16 s = to_half(fminf(step, 65504.f) + poison);
+    // lo may have been rounded above max: no step below 0
+    const _Float16 s = to_half(fminf(fmaxf(step, 0.f), 65504.f) + poison);
     const float lo32 = (float)lo, s32 = (float)s, inv = s32 > 0.f ? 1.0f / s32 : 0.f;
     int code[8];
 #pragma unroll

@@ -1,11 +1,15 @@
 // kv4_decode.hip -- attention of one query token per sequence over the 4-bit
 // paged KV cache (format: kv4.h), on v_mfma_f32_16x16x32_f16 over the codes.
 //
-// With K_d = lo_g + s_g c_d and V_d likewise (g the group of dimension d),
-//   <q, K> = sum_g s_g <q_g, c_g> + lo_g sum(q_g),
-//   out_d  = sum_t (p_t s_tg) c_td + sum_t p_t lo_tg  (over sum_t p_t),
-// so the matrix operands are the integers 0 .. 15, exact in fp16, and the
-// steps stay outside in fp32.  A column of the products is a (query head j,
+// With e = c - 8, K_d = lo_g + s_g c_d = mid_g + s_g e_d, mid = lo + 8 s, and V_d
+// likewise (g the group of dimension d),
+//   <q, K> = sum_g s_g <q_g, e_g> + mid_g sum(q_g),
+//   out_d  = sum_t (p_t s_tg) e_td + sum_t p_t mid_tg  (over sum_t p_t),
+// so the matrix operands are the integers -8 .. 7, exact in fp16, and the steps
+// stay outside in fp32.  (With the codes 0 .. 15 themselves the two terms are
+// each as large as lo, about two standard deviations of V, and their sum, an
+// average over many tokens, much smaller: what fp32 rounds off them would show.)
+// A column of the products is a (query head j,
 // group g) pair: column j G + g of the score product holds q_j with every
 // group but g zeroed, so one accumulator gives all groups' partial sums, each
 // lane applies the steps of its own group only, and a sum over the G
@@ -74,18 +78,18 @@ __device__ __forceinline__ Kv4Extent kv4_extent(const Kv4View &c, int seen) {
 }
 
 __device__ __forceinline__ h2_t as_h2(uint32_t u) { return __builtin_bit_cast(h2_t, u); }
-// Four codes' fp16 pairs of a mask with 0x000f000f << SH: (code in the low
-// half, code in the high half).  0x6400 | c is 1024 + c, 0x6400 | 16 c is
-// 1024 + 16 c.
+// c - 8 of the two codes that a mask with 0x000f000f (0x00f000f0) leaves, as
+// fp16: 0x6400 | c is 1024 + c, 0x6400 | 16 c is 1024 + 16 c.
 __device__ __forceinline__ h2_t codes_low(uint32_t w) {
     const uint32_t u = (w & 0x000f000fu) | 0x64006400u;
-    return as_h2(u) - h2_t{(_Float16)1024.f, (_Float16)1024.f};
+    return as_h2(u) - h2_t{(_Float16)1032.f, (_Float16)1032.f};
 }
 __device__ __forceinline__ h2_t codes_high(uint32_t w) {
     const uint32_t u = (w & 0x00f000f0u) | 0x64006400u;
     return as_h2(u) * h2_t{(_Float16)0.0625f, (_Float16)0.0625f} -
-           h2_t{(_Float16)64.f, (_Float16)64.f};
+           h2_t{(_Float16)72.f, (_Float16)72.f};
 }
+__device__ __forceinline__ float mid(h2_t st) { return fmaf(8.f, (float)st[0], (float)st[1]); }
 __device__ __forceinline__ h8_t join(h2_t a, h2_t b, h2_t c, h2_t d) {
     return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
@@ -248,7 +252,7 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const h2_t st = as_h2(ksr[i][r]);
-                float v = group_sum<G>(fmaf((float)st[1], qsum, (float)st[0] * a[r]));
+                float v = group_sum<G>(fmaf(mid(st), qsum, (float)st[0] * a[r]));
                 if (!whole && 4 * i + r >= held) v = -INFINITY;
                 sc[i][r] = v;
                 tmax = fmaxf(tmax, v);
@@ -260,12 +264,21 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
         const float fn = fminf(to_range(quarters_max((float)smax[0])), 0x1p100f);
         const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - ref) * kq);
         m = mn;
-        if (!__all(alpha == 1.f && fn == f)) {
-            const float fa = alpha * (fn / f);
+        const float fa = alpha * (fn / f);
+        if (WP == 1 && !__all(fa == 1.f)) {
 #pragma unroll
             for (int i = 0; i < NJ; ++i) acc[i][0] *= fa, acc[i][1] *= fa;
-            l *= alpha;
-            z *= alpha;
+        }
+        l *= alpha;
+        z *= alpha;
+        // where the outputs have fp16's or fp32's bits a tile's products get an
+        // accumulator of their own, added to the sum so far in one rounding per
+        // value (512 fp32 tokens per wave: 3.3e-7 off the exact sum, 4.3e-7 when
+        // the matrix instructions add to the running sum themselves)
+        f4_t part[WP == 1 ? 1 : NJ][2];
+        if (WP > 1) {
+#pragma unroll
+            for (int i = 0; i < NJ; ++i) part[i][0] = part[i][1] = f4_t{0.f, 0.f, 0.f, 0.f};
         }
         f = fn;
         // ---- weights and the value product
@@ -281,8 +294,11 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
                     const h2_t st = as_h2(vsr[i][r]);
                     const float pv = __builtin_amdgcn_exp2f((sc[i][r] - ref) * kq);
                     l += pv;
-                    z = fmaf(pv, (float)st[1], z);
+                    z = fmaf(pv, mid(st), z);
                     wv[r] = pv * ((float)st[0] * f);
+                    // rounded to fp32 here: the pieces below are of one value (the
+                    // compiler rounds the product to fp16 at once for one of them)
+                    if (WP > 1) asm volatile("" : "+v"(wv[r]));
                 }
                 // token order of a mask with 0x000f000f: 0, 2, then 1, 3
                 constexpr int order[4] = {0, 2, 1, 3};
@@ -298,12 +314,21 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
                 const uint32_t a = vw[i][2 * u], c = vw[i][2 * u + 1];
                 const h8_t ev = join(codes_low(a), codes_low(a >> 8), codes_low(c), codes_low(c >> 8));
                 const h8_t od = join(codes_high(a), codes_high(a >> 8), codes_high(c), codes_high(c >> 8));
+                f4_t *to = WP == 1 ? acc[i] : part[WP == 1 ? 0 : i];
 #pragma unroll
                 for (int x = WP - 1; x >= 0; --x) {
-                    acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ev, wf[x], acc[i][0], 0, 0, 0);
-                    acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(od, wf[x], acc[i][1], 0, 0, 0);
+                    to[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ev, wf[x], to[0], 0, 0, 0);
+                    to[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(od, wf[x], to[1], 0, 0, 0);
                 }
             }
+        }
+        if (WP > 1) {
+#pragma unroll
+            for (int i = 0; i < NJ; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][e][r] = fmaf(acc[i][e][r], fa, part[WP == 1 ? 0 : i][e][r]);
         }
     }
     l = quarters_sum(l);

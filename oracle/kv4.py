@@ -28,7 +28,7 @@ def held(x, group):
     y = np.where(bad, 0.0, y)
     lo = np.clip(y.min(-1, keepdims=True), -65504, 65504).astype(np.float16).astype(np.float64)
     step = np.float32((y.max(-1, keepdims=True) - lo) / 15)
-    s = np.minimum(step, np.float32(65504)).astype(np.float16).astype(np.float64)
+    s = np.clip(step, np.float32(0), np.float32(65504)).astype(np.float16).astype(np.float64)
     with np.errstate(divide="ignore", invalid="ignore"):
         code = np.where(s > 0, np.clip(np.rint((y - lo) / s), 0, 15), 0)
     return np.where(bad, np.nan, lo + s * code).reshape(x.shape)

@@ -344,6 +344,25 @@ def test_decode_large_and_small_values(lc, dev):
         check_decode(c.decode(q, i32(dev, [n])), q, hk, hv, [n], 2, "float32", 1 / 8, 32)
 
 
+def test_decode_constant_groups(lc, dev):
+    """Groups of one value that fp16 rounds up or down: their step is 0 (or the smallest there is), never
+    negative, and the weights' scaling holds beside them."""
+    import torch
+    n = 500
+    for seed in range(3):
+        g = np.random.default_rng(seed)
+        x = [np.repeat(g.normal(size=(n, 1, 4, 1)), 32, -1).reshape(n, 1, 128).astype(np.float32) for _ in range(2)]
+        x[1][::9, 0, 5] += 1e-3
+        c = lc.PagedInt4KVCache(1, 128, rope_theta=None, device=dev)
+        k, v = (torch.from_numpy(a).to(dev) for a in x)
+        q = rand(dev, "float32", 1, 4, 128, seed=3)
+        c.append(k, v, i32(dev, [0]), i32(dev, [0, n]))
+        assert (c.k_steps.view(-1, 2)[:, 0] >= 0).all() and (c.v_steps.view(-1, 2)[:, 0] >= 0).all()
+        hk, hv = kv4.held(x[0], 32), kv4.held(x[1], 32)
+        for ms in (0, 64):
+            check_decode(c.decode(q, i32(dev, [n]), max_seen=ms), q, hk, hv, [n], 4, "float32", 128 ** -0.5, 32)
+
+
 def test_captured_steps(lc, dev):
     """A captured decode step replays as the sequences grow: rotation, append and attention follow the
     lengths that the graph advances itself; every replay equals the eager step."""
