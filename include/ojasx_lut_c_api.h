@@ -373,6 +373,27 @@ OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q,
                                       const int *seen, int max_seen, float scale_factor, void *out,
                                       void *workspace, long workspace_bytes, void *stream);
 
+/* Attention of packed prompts: sequence b's queries, rows cu_seqlens_q[b] ..
+ * cu_seqlens_q[b + 1] - 1 (int32 on the device, num_sequences + 1 entries,
+ * ascending), over its keys, rows cu_seqlens_kv[b] .. of k and v.  With causal !=
+ * 0 query i of Lq sees keys j <= i + Lk - Lq (the last query all of them); a row
+ * that sees none is 0, with lse -inf.  q [num_q_tokens][num_heads][head_dim], k, v
+ * [num_kv_tokens][num_kv_heads][head_dim] in dtype F32, BF16 or F16, element
+ * strides of tokens and heads, rows 16-byte aligned; head_dim a multiple of 8 up
+ * to 256; query head h reads kv head h / (num_heads / num_kv_heads).  out
+ * [num_q_tokens][num_heads][head_dim] contiguous in dtype; lse [num_q_tokens][num_heads]
+ * fp32, the natural log of sum exp(scale * score), or NULL.  Keys that a row does
+ * not see reach nothing, whatever they hold.  Rows of no sequence are left as
+ * they are, or with zero_rest != 0 written as 0 (lse -inf). */
+OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, long q_head_stride,
+                                            const void *k, long k_token_stride, long k_head_stride,
+                                            const void *v, long v_token_stride, long v_head_stride,
+                                            int dtype, int num_q_tokens, int num_kv_tokens, int num_heads,
+                                            int num_kv_heads, int head_dim, const int *cu_seqlens_q,
+                                            const int *cu_seqlens_kv, int num_sequences, int causal,
+                                            float scale, int zero_rest, void *out, float *lse,
+                                            void *stream);
+
 /* ---- MoE (ref.h:125-150) ---------------------------------------------- */
 OJASX_API OjasxMoEHandle ojasx_create_moe(int num_experts, int hidden_dim,
                                           int intermediate_dim, int top_k, int block_dim,

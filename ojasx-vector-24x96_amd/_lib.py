@@ -83,6 +83,8 @@ SIGNATURES = {
     "ojasx_kv4_read_device": (ci, [vp, vp, vp, vp, ci, vp, vp, ci, vp]),
     "ojasx_kv4_decode_workspace": (cl, [vp, ci, ci]),
     "ojasx_kv4_decode_device": (ci, [vp, vp, ci, ci, vp, ci, cf, vp, vp, cl, vp]),
+    "ojasx_prompt_attention_device": (ci, [vp, cl, cl, vp, cl, cl, vp, cl, cl, ci, ci, ci, ci, ci, ci,
+                                           vp, vp, ci, ci, cf, ci, vp, vp, vp]),
 }
 
 

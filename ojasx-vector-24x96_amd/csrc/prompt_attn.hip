@@ -1,0 +1,649 @@
+// prompt_attn.hip -- attention of packed prompts: every sequence's queries over
+// its own keys, causal or not, grouped heads, one pass with a running maximum
+// and sum.
+//
+// out_i = sum_{j <= i + Lk - Lq} softmax_j(scale <q_i, k_j>) v_j  (all j < Lk
+// without the mask); a row that sees no key is 0.
+//
+// Both products are computed transposed, so that nothing crosses lanes between
+// them.  S^T = K Q^T on 32x32 tiles: lane (q = lane % 32, h = lane / 32) ends
+// with the scores of its query row against keys 8 (r / 4) + 4 h + r % 4, r < 16.
+// O^T = V^T P^T takes P^T as the operand whose lane holds one query row and any
+// keys of its half, as long as V^T's lanes hold the same ones: the softmax's
+// results go in as they are, V is read from LDS in that key order.  Maxima and
+// sums are a query row's, a lane's own: one exchange between the halves per
+// tile.
+//
+// A workgroup's waves take HW query heads of one kv head (the largest power of
+// two up to 8 that divides the heads per kv head) by 8 / HW blocks of 32 rows:
+// K and V are staged once for all of them, and the causal diagonal cuts through
+// 32 (8 / HW) rows instead of 256.
+#include <cmath>
+#include <type_traits>
+
+#include "common.h"
+
+namespace ojx {
+
+namespace {
+constexpr int kKeys = 64;                        // keys per tile
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+struct PromptParams {
+    const void *q, *k, *v;
+    long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;     // token and head strides, elements
+    void *out;                                   // [Nq][Hq][D]
+    float *lse;                                  // [Nq][Hq] or null
+    const int *cu_q, *cu_k;                      // [B + 1]
+    int B, Nq, Nk, Hq, Hkv, D;
+    int hw, causal, zero_rest;                   // log2 of the heads per workgroup
+    float scale2;                                // scale x log2(e)
+};
+
+struct Bf16 {
+    typedef __hip_bfloat16 T;
+    typedef bf16x8_t V8;
+    static __device__ __forceinline__ f32x16_t mma(V8 a, V8 b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ __bf16 from(float f) { return (__bf16)f; }
+};
+struct F16 {
+    typedef __half T;
+    typedef f16x8_t V8;
+    static __device__ __forceinline__ f32x16_t mma(V8 a, V8 b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ _Float16 from(float f) { return (_Float16)f; }
+};
+
+// The rows of a workgroup: slot t of the grid.  Sequence b takes the slots from
+// s(b) = cu[b] / BM + b + 1 (its rows need at most the next sequence's slots
+// less one), rows before the first sequence the slots from 0 and rows behind
+// the last one those from s(B).  cu is clamped to the rows there are, whatever
+// it holds.
+struct Rows {
+    int b, first, len, tile;     // sequence (-1 or B: rows of none), its rows, the tile in it
+};
+__device__ __forceinline__ int cu_at(const int *cu, int b, int n) { return min(max(cu[b], 0), n); }
+__device__ __forceinline__ Rows rows_of_slot(const int *cu, int B, int n, int bm_shift, int t) {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int i0 = 0; i0 <= B; i0 += 64) {
+        const int i = min(i0 + lane, B);
+        count += __popcll(__ballot(i0 + lane <= B && (cu_at(cu, i, n) >> bm_shift) + i + 1 <= t));
+    }
+    Rows r;
+    r.b = count - 1;
+    r.first = r.b < 0 ? 0 : cu_at(cu, r.b, n);
+    r.len = (r.b < B ? cu_at(cu, r.b + 1, n) : n) - r.first;
+    r.tile = t - (r.b < 0 ? 0 : (r.first >> bm_shift) + r.b + 1);
+    return r;
+}
+
+// 16-byte unit `u` of row `row` in a K tile, and 32-byte unit of a V tile: XOR
+// swizzles under which the 16 rows of a K read, and the 8 rows of a transposed V
+// read, spread over all the banks.
+template <int ROWB>
+__device__ __forceinline__ int k_unit(int row, int u) {
+    return ROWB >= 256 ? u ^ (row & 15) : u ^ (row >> 1 & 7);
+}
+template <int ROWB>
+__device__ __forceinline__ int v_unit(int row, int u) {
+    return ROWB >= 256 ? u ^ (row & 7) : u ^ (row >> 1 & 3);
+}
+
+__device__ __forceinline__ float swap_halves(float v) { return __shfl_xor(v, 32); }
+
+// The key that accumulator register r of a lane's half h stands for.
+__device__ __forceinline__ constexpr int key_of(int r) { return 8 * (r / 4) + r % 4; }
+
+// Running softmax of one query row per lane over a tile's scores s (two blocks
+// of 32 keys): rescales acc and l where the row's maximum grew by more than 2^8,
+// turns s into weights.  Weights up to 2^8 above 1 lose nothing: they are
+// rounded relative to their size and all sums are fp32.
+template <int NT>
+__device__ __forceinline__ void softmax_tile(f32x16_t (&s)[2], float scale2, float &m, float &ref, float &l,
+                                             f32x16_t (&acc)[NT]) {
+    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[1][r]);
+    float t = fmaxf(t0, t1);
+    t = fmaxf(t, swap_halves(t)) * scale2;
+    if (__any(t > m + 8.f)) {
+        const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
+        m = mn;
+        ref = rn;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] *= alpha;
+    }
+    float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], scale2, -ref));
+        s[1][r] = __builtin_amdgcn_exp2f(fmaf(s[1][r], scale2, -ref));
+        a0 += s[0][r];
+        a1 += s[1][r];
+    }
+    l += a0 + a1;
+}
+
+// Hides the keys past `lim` from the lane's row; k0 = the tile's first key.
+__device__ __forceinline__ void mask_tile(f32x16_t (&s)[2], int lim, int k0, int h) {
+    const int rel = lim - k0 - 4 * h;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        if (key_of(r) > rel) s[0][r] = -INFINITY;
+        if (32 + key_of(r) > rel) s[1][r] = -INFINITY;
+    }
+}
+}  // namespace
+
+// Workgroups: slots x head groups, the head group fastest: consecutive
+// workgroups go to different XCDs, so with 8 head groups (or a multiple) an XCD
+// keeps the K and V of its own heads; the last rows of the batch, the longest
+// tiles of a single causal sequence, start first.
+struct PromptBlock {
+    Rows rows;
+    int head0, k_first, Lk;
+};
+__device__ __forceinline__ bool prompt_block(const PromptParams &p, int slots, int bm_shift, PromptBlock &o) {
+    const int hg = p.Hq >> p.hw;
+    const int t = slots - 1 - (int)blockIdx.x / hg;
+    o.head0 = (int)blockIdx.x % hg << p.hw;
+    o.rows = rows_of_slot(p.cu_q, p.B, p.Nq, bm_shift, t);
+    const int r0 = o.rows.tile << bm_shift;
+    if (o.rows.tile < 0 || r0 >= o.rows.len) return false;
+    o.k_first = o.Lk = 0;
+    if (o.rows.b >= 0 && o.rows.b < p.B) {
+        o.k_first = cu_at(p.cu_k, o.rows.b, p.Nk);
+        o.Lk = max(cu_at(p.cu_k, o.rows.b + 1, p.Nk) - o.k_first, 0);
+    }
+    return true;
+}
+
+// Rows of no sequence: zeros, where the caller wants them written.
+template <typename T>
+__device__ __forceinline__ void zero_rows(const PromptParams &p, const PromptBlock &o, int bm_shift) {
+    if (!p.zero_rest) return;
+    const int r0 = o.rows.tile << bm_shift, n = min(1 << bm_shift, o.rows.len - r0);
+    const int heads = 1 << p.hw, per = heads * p.D;
+    for (int x = threadIdx.x; x < n * per; x += blockDim.x) {
+        const size_t row = (size_t)(o.rows.first + r0 + x / per) * p.Hq + o.head0 + x % per / p.D;
+        store_act(static_cast<T *>(p.out), row * p.D + x % p.D, 0.f);
+        if (p.lse && x % p.D == 0) p.lse[row] = -INFINITY;
+    }
+}
+
+// bf16 and fp16: v_mfma_f32_32x32x16, head dims up to DP (the dims past D are
+// zeros in Q and K).
+template <typename E, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void prompt_attn_kernel(
+    PromptParams p, int slots) {
+    typedef typename E::T T;
+    typedef typename E::V8 V8;
+    constexpr int NT = 64 * NW, ROWB = 2 * DP, UPR = DP / 8, TILE = kKeys * ROWB;
+    constexpr int CH = kKeys * UPR / NT;             // 16-byte units of a tile per thread
+    extern __shared__ __align__(16) unsigned char sm[];   // [2 buffers][K tile, V tile]
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int bm_shift = 5 + __builtin_ctz(NW) - p.hw;
+    PromptBlock o;
+    if (!prompt_block(p, slots, bm_shift, o)) return;
+    if (o.rows.b < 0 || o.rows.b >= p.B) {
+        zero_rows<T>(p, o, bm_shift);
+        return;
+    }
+    const int head = o.head0 + (w & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
+    const int Lq = o.rows.len, Lk = o.Lk, off = Lk - Lq;
+    const int tile0 = o.rows.tile << bm_shift;                  // the workgroup's first row
+    const int row0 = tile0 + 32 * (w >> p.hw), row = row0 + n;  // the wave's, the lane's
+    const int qrow = min(row, Lq - 1);
+    const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;       // last key the row sees
+    const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;    // the wave's least,
+    const int lim_hi = p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;   // and most
+    const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
+    const int tiles = last < 0 ? 0 : last / kKeys + 1;
+
+    // ---- this lane's query row: dims 16 c + 8 h ..
+    V8 qf[DP / 16];
+    {
+        const T *qp = static_cast<const T *>(p.q) + (long)(o.rows.first + qrow) * p.q_ts + head * p.q_hs;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (16 * c + 8 * h < p.D) x = *reinterpret_cast<const u32x4_t *>(qp + 16 * c + 8 * h);
+            qf[c] = __builtin_bit_cast(V8, x);
+        }
+    }
+    // ---- staging: unit i of a tile is (key, unit) = ((tid + i NT) / UPR, % UPR)
+    const int su = tid % UPR, sr = tid / UPR;        // NT is a multiple of UPR
+    const T *kp = static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + su * 8;
+    const T *vp = static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + su * 8;
+    const bool in = su * 8 < p.D;
+    u32x4_t kr[CH], vr[CH];
+    auto load = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const long key = min(tile * kKeys + sr + i * (NT / UPR), Lk - 1);   // past the end: the last again
+            kr[i] = vr[i] = u32x4_t{0, 0, 0, 0};
+            if (in) {
+                kr[i] = *reinterpret_cast<const u32x4_t *>(kp + key * p.k_ts);
+                vr[i] = *reinterpret_cast<const u32x4_t *>(vp + key * p.v_ts);
+            }
+        }
+    };
+    auto store = [&](int tile) __attribute__((always_inline)) {
+        unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int r = sr + i * (NT / UPR);
+            *reinterpret_cast<u32x4_t *>(ks + r * ROWB + k_unit<ROWB>(r, su) * 16) = kr[i];
+            *reinterpret_cast<u32x4_t *>(vs + r * ROWB + v_unit<ROWB>(r, su >> 1) * 32 + (su & 1) * 16) = vr[i];
+        }
+    };
+    f32x16_t acc[DP / 32] = {};
+    float m = -INFINITY, ref = 0.f, l = 0.f;
+    if (tiles) {
+        load(0);
+        store(0);
+    }
+    // this lane's part of a transposed V read: key 4 h + i / 4, dims 16 g + 4 (i % 4) .. of 32
+    const int vkey = 4 * h + ((lane & 15) >> 2), vg = lane >> 4 & 1, vb = (lane & 3) * 8;
+    for (int tile = 0; tile < tiles; ++tile) {
+        __syncthreads();
+        if (tile + 1 < tiles) load(tile + 1);
+        const int k0 = tile * kKeys;
+        if (k0 <= lim_hi) {
+            const unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
+            f32x16_t s[2] = {};
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int r = 32 * b + n;
+                    const u32x4_t x =
+                        *reinterpret_cast<const u32x4_t *>(ks + r * ROWB + k_unit<ROWB>(r, 2 * c + h) * 16);
+                    s[b] = E::mma(__builtin_bit_cast(V8, x), qf[c], s[b]);
+                }
+            if (k0 + kKeys - 1 > lim_lo) mask_tile(s, lim, k0, h);
+            softmax_tile(s, p.scale2, m, ref, l, acc);
+            V8 pf[2][2];                             // the weights, rounded to the inputs' type
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pf[b][u][e] = E::from(s[b][8 * u + e]);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        s16x4_t x[2];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const int r = 32 * b + 16 * u + 8 * y + vkey;
+                            auto *at = (__attribute__((address_space(3))) s16x4_t *)(vs + r * ROWB +
+                                                                                  v_unit<ROWB>(r, 2 * t + vg) * 32 + vb);
+                            x[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+                        }
+                        typedef short s16x8_t __attribute__((ext_vector_type(8)));
+                        const s16x8_t z = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                        acc[t] = E::mma(__builtin_bit_cast(V8, z), pf[b][u], acc[t]);
+                    }
+        }
+        if (tile + 1 < tiles) store(tile + 1);
+    }
+    l += swap_halves(l);
+    // A weight of 0 times an infinity or a NaN is a NaN in the matrix product: an
+    // output that is NaN may come from a key its row does not see.  Where the
+    // wave has one, its rows run again, key by key, with hidden keys left out.
+    bool again = false;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) again |= acc[t][r] != acc[t][r];
+    if (__any(again)) {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+        const T *k1 = static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs;
+        const T *v1 = static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs;
+        for (int key = 0; key <= lim_hi; ++key) {
+            float x = 0.f;
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c)
+                if (16 * c + 8 * h < p.D)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        x = fmaf((float)qf[c][e], load_act(k1, key * p.k_ts + 16 * c + 8 * h + e), x);
+            x = (x + swap_halves(x)) * p.scale2;
+            if (key > lim) continue;                 // the lane's; the loop is the wave's
+            const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
+            const float pv = __builtin_amdgcn_exp2f(x - rn);
+            m = mn;
+            ref = rn;
+            l = fmaf(l, alpha, pv);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * t + 4 * h + key_of(r);
+                    if (d < p.D) acc[t][r] = fmaf(pv, load_act(v1, key * p.v_ts + d), acc[t][r] * alpha);
+                }
+        }
+    }
+    if (row >= Lq) return;
+    const size_t at = (size_t)(o.rows.first + row) * p.Hq + head;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T *op = static_cast<T *>(p.out) + at * p.D;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = 32 * t + 8 * x + 4 * h;
+            if (d < p.D) {
+                typedef decltype(E::from(0.f)) e4_t __attribute__((ext_vector_type(4)));
+                e4_t y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = E::from(l == 0.f ? 0.f : acc[t][4 * x + e] * inv);
+                *reinterpret_cast<e4_t *>(op + d) = y;
+            }
+        }
+    if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// fp32: v_mfma_f32_32x32x2, exact products.  A lane's operand of a step is one
+// value; the dims of a step are 8 c + i of half 0 and 8 c + 4 + i of half 1, so
+// that K is read from LDS 16 bytes at a time.
+template <int DP, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void prompt_attn_f32_kernel(
+    PromptParams p, int slots) {
+    constexpr int NT = 64 * NW, ROWB = 4 * DP, UPR = DP / 4, KEYS = 32, TILE = KEYS * ROWB;
+    constexpr int CH = KEYS * UPR / NT;
+    extern __shared__ __align__(16) unsigned char sm[];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int bm_shift = 5 + __builtin_ctz(NW) - p.hw;
+    PromptBlock o;
+    if (!prompt_block(p, slots, bm_shift, o)) return;
+    if (o.rows.b < 0 || o.rows.b >= p.B) {
+        zero_rows<float>(p, o, bm_shift);
+        return;
+    }
+    const int head = o.head0 + (w & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
+    const int Lq = o.rows.len, Lk = o.Lk, off = Lk - Lq;
+    const int tile0 = o.rows.tile << bm_shift;
+    const int row0 = tile0 + 32 * (w >> p.hw), row = row0 + n;
+    const int qrow = min(row, Lq - 1);
+    const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;
+    const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;
+    const int lim_hi = p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;
+    const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
+    const int tiles = last < 0 ? 0 : last / KEYS + 1;
+
+    f32x4_t qf[DP / 8];                              // dims 8 c + 4 h ..
+    {
+        const float *qp = static_cast<const float *>(p.q) + (long)(o.rows.first + qrow) * p.q_ts + head * p.q_hs;
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+            qf[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (8 * c < p.D) qf[c] = *reinterpret_cast<const f32x4_t *>(qp + 8 * c + 4 * h);
+        }
+    }
+    const int su = tid % UPR, sr = tid / UPR;
+    const float *kp = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + su * 4;
+    const float *vp = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + su * 4;
+    const bool in = su * 4 < p.D;
+    f32x4_t kr[CH], vr[CH];
+    auto load = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const long key = min(tile * KEYS + sr + i * (NT / UPR), Lk - 1);
+            kr[i] = vr[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (in) {
+                kr[i] = *reinterpret_cast<const f32x4_t *>(kp + key * p.k_ts);
+                vr[i] = *reinterpret_cast<const f32x4_t *>(vp + key * p.v_ts);
+            }
+        }
+    };
+    auto store = [&](int tile) __attribute__((always_inline)) {
+        unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int r = sr + i * (NT / UPR);
+            *reinterpret_cast<f32x4_t *>(ks + r * ROWB + (su ^ (r & 15)) * 16) = kr[i];
+            // rows 4 apart are read together: their 128-byte units swap
+            *reinterpret_cast<f32x4_t *>(vs + r * ROWB + (su ^ (r << 1 & 8)) * 16) = vr[i];
+        }
+    };
+    f32x16_t acc[DP / 32] = {};
+    float m = -INFINITY, ref = 0.f, l = 0.f;
+    if (tiles) {
+        load(0);
+        store(0);
+    }
+    for (int tile = 0; tile < tiles; ++tile) {
+        __syncthreads();
+        if (tile + 1 < tiles) load(tile + 1);
+        const int k0 = tile * KEYS;
+        if (k0 <= lim_hi) {
+            const unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
+            f32x16_t s[2] = {};
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c) {
+                const f32x4_t x =
+                    *reinterpret_cast<const f32x4_t *>(ks + n * ROWB + ((2 * c + h) ^ (n & 15)) * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], qf[c][i], s[i & 1], 0, 0, 0);
+            }
+            s[0] += s[1];
+            if (k0 + KEYS - 1 > lim_lo) {
+                const int rel = lim - k0 - 4 * h;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key_of(r) > rel) s[0][r] = -INFINITY;
+            }
+            float t = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t = fmaxf(t, s[0][r]);
+            t = fmaxf(t, swap_halves(t)) * p.scale2;
+            if (__any(t > m)) {
+                const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
+                m = mn;
+                ref = rn;
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) acc[i] *= alpha;
+            }
+            float a = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -ref));
+                a += s[0][r];
+            }
+            l += a;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int key = key_of(r) + 4 * h;
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) {
+                    const float x = *reinterpret_cast<const float *>(
+                        vs + key * ROWB + ((8 * i + (n >> 2)) ^ (key << 1 & 8)) * 16 + (n & 3) * 4);
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[0][r], acc[i], 0, 0, 0);
+                }
+            }
+        }
+        if (tile + 1 < tiles) store(tile + 1);
+    }
+    l += swap_halves(l);
+    bool again = false;                              // as in prompt_attn_kernel
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) again |= acc[t][r] != acc[t][r];
+    if (__any(again)) {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+        const float *k1 = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs;
+        const float *v1 = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs;
+        for (int key = 0; key <= lim_hi; ++key) {
+            float x = 0.f;
+#pragma unroll
+            for (int c = 0; c < DP / 8; ++c)
+                if (8 * c < p.D)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x = fmaf(qf[c][e], k1[key * p.k_ts + 8 * c + 4 * h + e], x);
+            x = (x + swap_halves(x)) * p.scale2;
+            if (key > lim) continue;
+            const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
+            const float pv = __builtin_amdgcn_exp2f(x - rn);
+            m = mn;
+            ref = rn;
+            l = fmaf(l, alpha, pv);
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * t + 4 * h + key_of(r);
+                    if (d < p.D) acc[t][r] = fmaf(pv, v1[key * p.v_ts + d], acc[t][r] * alpha);
+                }
+        }
+    }
+    if (row >= Lq) return;
+    const size_t at = (size_t)(o.rows.first + row) * p.Hq + head;
+    float *op = static_cast<float *>(p.out) + at * p.D;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int d = 32 * t + 8 * x + 4 * h;
+            if (d < p.D) {
+                f32x4_t y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = l == 0.f ? 0.f : acc[t][4 * x + e] / l;
+                *reinterpret_cast<f32x4_t *>(op + d) = y;
+            }
+        }
+    if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+namespace {
+template <typename K>
+int launch(K kernel, const PromptParams &p, int nw, size_t lds, size_t *granted, hipStream_t st) {
+    const int rc = ensure_dyn_lds(reinterpret_cast<const void *>(kernel), lds, granted);
+    if (rc) return rc;
+    const int bm_shift = 5 + __builtin_ctz((unsigned)nw) - p.hw;
+    const long slots = (long)(p.Nq >> bm_shift) + p.B + 2, groups = slots * (p.Hq >> p.hw);
+    if (groups > 0x7fffffffL) {
+        set_error("prompt attention: %ld workgroups", groups);
+        return OJASX_ERR_INVALID;
+    }
+    OJX_LAUNCH(kernel, dim3((unsigned)groups), dim3(64 * nw), lds, st, p, (int)slots);
+    OJX_HIP(hipGetLastError());
+    return OJASX_OK;
+}
+template <typename E, int DP, int NW>
+int launch16(const PromptParams &p, hipStream_t st) {
+    static size_t granted = 0;
+    return launch(&prompt_attn_kernel<E, DP, NW>, p, NW, (size_t)4 * kKeys * 2 * DP, &granted, st);
+}
+template <int DP, int NW>
+int launch32(const PromptParams &p, hipStream_t st) {
+    static size_t granted = 0;
+    return launch(&prompt_attn_f32_kernel<DP, NW>, p, NW, (size_t)4 * 32 * 4 * DP, &granted, st);
+}
+
+bool rows16(const void *p, long ts, long hs, size_t es) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ts >= 0 && hs >= 0 && ts * es % 16 == 0 &&
+           hs * es % 16 == 0;
+}
+}  // namespace
+
+}  // namespace ojx
+
+extern "C" {
+
+OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, long q_head_stride,
+                                            const void *k, long k_token_stride, long k_head_stride,
+                                            const void *v, long v_token_stride, long v_head_stride,
+                                            int dtype, int num_q_tokens, int num_kv_tokens, int num_heads,
+                                            int num_kv_heads, int head_dim, const int *cu_seqlens_q,
+                                            const int *cu_seqlens_kv, int num_sequences, int causal,
+                                            float scale, int zero_rest, void *out, float *lse,
+                                            void *stream) {
+    using namespace ojx;
+    if (dtype != OJASX_DTYPE_F32 && dtype != OJASX_DTYPE_BF16 && dtype != OJASX_DTYPE_F16) {
+        set_error("unsupported dtype %d", dtype);
+        return OJASX_ERR_INVALID;
+    }
+    if (num_q_tokens < 0 || num_kv_tokens < 0 || num_heads <= 0 || num_heads > 65535 || num_kv_heads <= 0 ||
+        num_heads % num_kv_heads || num_sequences <= 0 || num_sequences > (1 << 24)) {
+        set_error("prompt attention: %d query and %d key tokens of %d sequences, %d query and %d kv heads",
+                  num_q_tokens, num_kv_tokens, num_sequences, num_heads, num_kv_heads);
+        return OJASX_ERR_INVALID;
+    }
+    if (head_dim <= 0 || head_dim > 256 || head_dim % 8) {
+        set_error("prompt attention: head_dim %d is no multiple of 8 up to 256", head_dim);
+        return OJASX_ERR_INVALID;
+    }
+    if (!(scale > 0.f) || !(scale < INFINITY)) {
+        set_error("prompt attention: scale must be positive and finite");
+        return OJASX_ERR_INVALID;
+    }
+    if (num_q_tokens == 0) return OJASX_OK;
+    if (!q || !out || !cu_seqlens_q || !cu_seqlens_kv || (num_kv_tokens && (!k || !v))) return OJASX_ERR_NULL;
+    const size_t es = dtype == OJASX_DTYPE_F32 ? 4 : 2;
+    if (!rows16(q, q_token_stride, q_head_stride, es) || !rows16(out, 0, 0, es) ||
+        (num_kv_tokens && (!rows16(k, k_token_stride, k_head_stride, es) ||
+                           !rows16(v, v_token_stride, v_head_stride, es)))) {
+        set_error("prompt attention: rows are 16-byte aligned");
+        return OJASX_ERR_INVALID;
+    }
+    PromptParams p{};
+    p.q = q, p.k = k, p.v = v;
+    p.q_ts = q_token_stride, p.q_hs = q_head_stride;
+    p.k_ts = k_token_stride, p.k_hs = k_head_stride;
+    p.v_ts = v_token_stride, p.v_hs = v_head_stride;
+    p.out = out, p.lse = lse, p.cu_q = cu_seqlens_q, p.cu_k = cu_seqlens_kv;
+    p.B = num_sequences, p.Nq = num_q_tokens, p.Nk = num_kv_tokens;
+    p.Hq = num_heads, p.Hkv = num_kv_heads, p.D = head_dim;
+    p.causal = causal != 0, p.zero_rest = zero_rest != 0, p.scale2 = scale * kLog2e;
+    const int share = num_heads / num_kv_heads, max_hw = head_dim > 128 ? 2 : 3;   // 4 waves there
+    p.hw = __builtin_ctz((unsigned)share);
+    if (p.hw > max_hw) p.hw = max_hw;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == OJASX_DTYPE_F32)
+        return head_dim <= 64 ? launch32<64, 8>(p, st) : head_dim <= 128 ? launch32<128, 8>(p, st)
+                                                                        : launch32<256, 4>(p, st);
+    if (dtype == OJASX_DTYPE_BF16)
+        return head_dim <= 64    ? launch16<Bf16, 64, 8>(p, st)
+               : head_dim <= 128 ? launch16<Bf16, 128, 8>(p, st)
+                                 : launch16<Bf16, 256, 4>(p, st);
+    return head_dim <= 64    ? launch16<F16, 64, 8>(p, st)
+           : head_dim <= 128 ? launch16<F16, 128, 8>(p, st)
+                             : launch16<F16, 256, 4>(p, st);
+}
+
+}  // extern "C"

@@ -29,6 +29,9 @@ csrc/lut_kv.hip.
   several sequences in 4 bits, with the position rotation applied on the way
   in (csrc/kv4_append.hip, csrc/kv4_decode.hip).  The sequences' lengths are
   the caller's, in device memory, so its calls can be captured.
+* ``PackedPromptAttention`` is the prefill beside it: attention of a batch of
+  prompts of different lengths, packed row by row, causal, grouped heads
+  (csrc/prompt_attn.hip).
 
 Everything runs on the GPU; CPU queries raise.
 """
@@ -941,3 +944,87 @@ class PagedInt4KVCache:
         if rc:
             _lib.check(rc, "ojasx_kv4_decode_device")
         return out
+
+
+class PackedPromptAttention:
+    """Attention of packed prompts: the queries of every sequence over its own
+    keys, in one launch.  float32, bfloat16 or float16; head_dim a multiple of
+    8 up to 256; scores times ``scale`` (1/sqrt(head_dim) unless given), sums
+    and softmax in float32.  Where OnlineSoftmaxBlockAttention is exact (fp64)
+    over one sequence's tiles, this is the batch's prefill at the speed of the
+    inputs' own type."""
+
+    def __init__(self, num_heads: int, num_kv_heads: Optional[int] = None, head_dim: int = 128, *,
+                 causal: bool = True, scale: Optional[float] = None) -> None:
+        self.num_heads = int(num_heads)
+        self.num_kv_heads = int(num_kv_heads or num_heads)
+        self.head_dim = int(head_dim)
+        if self.num_heads <= 0 or self.num_kv_heads <= 0 or self.num_heads % self.num_kv_heads:
+            raise ValueError(f"num_heads ({self.num_heads}) must be divisible by num_kv_heads "
+                             f"({self.num_kv_heads})")
+        if self.head_dim <= 0 or self.head_dim > 256 or self.head_dim % 8:
+            raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {self.head_dim}")
+        self.causal = bool(causal)
+        self.scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+        if not 0.0 < self.scale < math.inf:
+            raise ValueError(f"scale must be positive and finite, got {scale}")
+
+    def _check(self, t, heads, name):
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim:
+            raise ValueError(f"{name} must be [tokens, {heads}, {self.head_dim}], got {tuple(t.shape)}")
+
+    def forward(self, query, key, value, cu_seqlens, cu_seqlens_kv=None, *, out=None,
+                return_lse: bool = False):
+        """``query`` [N, num_heads, head_dim] over ``key`` and ``value`` [M,
+        num_kv_heads, head_dim] (any strides): rows cu_seqlens[b] ..
+        cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device) are sequence b's.
+        With ``cu_seqlens_kv`` its keys are those rows instead, and query i of
+        Lq sees keys j <= i + Lk - Lq: a prompt's last rows over keys that
+        begin earlier.  A row that sees no key is 0.
+
+        Returns the output [N, num_heads, head_dim] in the query's dtype, or
+        (output, lse float32 [N, num_heads]) with ``return_lse``.  Rows of no
+        sequence are 0 (lse -inf); in a given ``out`` they stay as they are."""
+        torch = _torch()
+        what = "PackedPromptAttention"
+        tag = _inference_tag(what, query, key, value)
+        self._check(query, self.num_heads, "query")
+        self._check(key, self.num_kv_heads, "key")
+        self._check(value, self.num_kv_heads, "value")
+        if key.shape[0] != value.shape[0]:
+            raise ValueError(f"{key.shape[0]} keys and {value.shape[0]} values")
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+            raise ValueError(f"cu_seqlens must hold the B + 1 bounds of B sequences, got "
+                             f"{tuple(cu_seqlens.shape)}")
+        dev = query.device
+        B = cu_seqlens.shape[0] - 1
+        cq = _lengths_tensor(cu_seqlens, B + 1, dev, "cu_seqlens")
+        if cu_seqlens_kv is None:
+            if key.shape[0] != query.shape[0]:
+                raise ValueError(f"{query.shape[0]} queries and {key.shape[0]} keys without cu_seqlens_kv")
+            ck = cq
+        else:
+            ck = _lengths_tensor(cu_seqlens_kv, B + 1, dev, "cu_seqlens_kv")
+        fresh = out is None
+        if fresh:
+            out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or \
+                not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("out must be contiguous, 16-byte aligned and of the query's shape, dtype and "
+                             "device")
+        with _on_device(dev) as stream:
+            q, k, v = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+            if lse is not None and not fresh:
+                lse.fill_(-math.inf)
+            qs, ks, vs = q.stride(), k.stride(), v.stride()
+            rc = _lib.lib().ojasx_prompt_attention_device(
+                q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], tag,
+                q.shape[0], k.shape[0], self.num_heads, self.num_kv_heads, self.head_dim, cq, ck, B,
+                int(self.causal), self.scale, int(fresh), out.data_ptr(),
+                None if lse is None else lse.data_ptr(), stream)
+        if rc:
+            _lib.check(rc, "ojasx_prompt_attention_device")
+        return (out, lse) if return_lse else out
+
+    __call__ = forward

@@ -120,3 +120,21 @@ def test_oracle_residents_and_rotation():
         assert np.array_equal(y[0], x[0])
         assert np.allclose((y ** 2).sum(-1), (x ** 2).sum(-1), rtol=1e-13)
     assert not np.allclose(kv4.rotate(x, [1] * 3, f), kv4.rotate(x, [1] * 3, f, True))
+
+
+def test_prompt_attention_refusals(pkg):
+    L = pkg.lib()
+
+    def call(q=FAKE, k=FAKE, v=FAKE, ts=512, hs=128, dtype=0, nq=4, nk=4, H=4, Hkv=2, D=128, cu=FAKE, ck=FAKE,
+             B=1, scale=0.1, out=FAKE):
+        return L.ojasx_prompt_attention_device(q, ts, hs, k, ts, hs, v, ts, hs, dtype, nq, nk, H, Hkv, D, cu, ck,
+                                               B, 1, scale, 0, out, None, None)
+
+    assert call(dtype=3) == -3 and call(nq=-1) == -3 and call(nk=-1) == -3 and call(H=3) == -3
+    assert call(Hkv=0) == -3 and call(D=0) == -3 and call(D=12) == -3 and call(D=264) == -3 and call(B=0) == -3
+    assert call(scale=0.0) == -3 and call(scale=-1.0) == -3 and call(scale=float("inf")) == -3
+    assert call(scale=float("nan")) == -3 and call(ts=514) == -3 and call(hs=-128) == -3
+    assert call(q=FAKE + 8) == -3 and call(k=FAKE + 4) == -3 and call(out=FAKE + 2) == -3
+    assert call(q=None) == -1 and call(k=None) == -1 and call(cu=None) == -1 and call(ck=None) == -1
+    assert call(out=None) == -1 and call(nq=0, q=None) == 0
+    assert L.ojasx_get_last_error()
