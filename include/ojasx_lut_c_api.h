@@ -364,10 +364,11 @@ OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start
  * q, out [num_sequences][num_q_heads][head_dim] in dtype (F32, BF16, F16), head
  * j reading kv head j / (num_q_heads / num_kv_heads); seen: the tokens of each
  * sequence so far (0: a row of zeros).  scale_factor <= 0: 1/sqrt(head_dim).
- * max_seen bounds seen[] (0: the cache's capacity) and sets how far a sequence
- * is split; larger entries of seen are attended in full all the same.
- * workspace: ojasx_kv4_decode_workspace(...) bytes for the same arguments,
- * 16-byte aligned, one for each call that may run at the same time. */
+ * max_seen bounds seen[] (0: the cache's capacity) and with it the size of the
+ * launch; larger entries of seen are attended in full all the same.
+ * q is 16-byte aligned.  workspace: ojasx_kv4_decode_workspace(...) bytes for the
+ * same arguments, 16-byte aligned, one for each call that may run at the same
+ * time. */
 OJASX_API long ojasx_kv4_decode_workspace(const OjasxKV4Cache *cache, int num_q_heads, int max_seen);
 OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q, int num_q_heads, int dtype,
                                       const int *seen, int max_seen, float scale_factor, void *out,

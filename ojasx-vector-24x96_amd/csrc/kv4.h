@@ -37,6 +37,30 @@ struct Kv4View {
 
 int kv4_view(const OjasxKV4Cache *c, Kv4View *v);   // 0 or an error code
 
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef unsigned int u4_t __attribute__((ext_vector_type(4)));
+
+// Eight consecutive values as fp32 (16-byte aligned).
+__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
+    const f4_t a = *reinterpret_cast<const f4_t *>(p), b = *reinterpret_cast<const f4_t *>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+}
+__device__ __forceinline__ void load8(const __hip_bfloat16 *p, float (&x)[8]) {
+    const u4_t a = *reinterpret_cast<const u4_t *>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(a[i] << 16);
+        x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void load8(const __half *p, float (&x)[8]) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    const h8 a = *reinterpret_cast<const h8 *>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+}
+
 // Entry of the block table that holds page j of a sequence.
 __device__ __forceinline__ int kv4_entry(const Kv4View &c, int j) {
     return j < c.sink ? j : c.sink + (j - c.sink) % (c.max_pages - c.sink);

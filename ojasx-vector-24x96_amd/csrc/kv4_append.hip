@@ -17,7 +17,6 @@ namespace {
 constexpr int kNT = 256;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 
 struct Kv4AppendParams {
     Kv4View c;
@@ -28,26 +27,6 @@ struct Kv4AppendParams {
     int n, Hq;
 };
 
-// Eight consecutive values as fp32 (16-byte aligned).
-__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-    const v4f a = *reinterpret_cast<const v4f *>(p), b = *reinterpret_cast<const v4f *>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-}
-__device__ __forceinline__ void load8(const __hip_bfloat16 *p, float (&x)[8]) {
-    const v4u a = *reinterpret_cast<const v4u *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(a[i] << 16);
-        x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void load8(const __half *p, float (&x)[8]) {
-    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    const h8 a = *reinterpret_cast<const h8 *>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-}
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
     *reinterpret_cast<v4f *>(p) = v4f{x[0], x[1], x[2], x[3]};
     *reinterpret_cast<v4f *>(p + 4) = v4f{x[4], x[5], x[6], x[7]};
@@ -308,6 +287,11 @@ int kv4_view(const OjasxKV4Cache *c, Kv4View *v) {
         c->sink_pages < 0 || c->max_pages <= c->sink_pages) {
         set_error("4-bit KV cache: %d sequences, %d kv heads, %d pages, %d of a sequence with %d sink pages",
                   c->num_sequences, c->num_kv_heads, c->num_pages, c->max_pages, c->sink_pages);
+        return OJASX_ERR_INVALID;
+    }
+    if ((long)c->num_pages * c->num_kv_heads * (P / 16) > 0x7fffffffL) {
+        set_error("4-bit KV cache: %d pages of %d slots for %d heads are more than 2^31 blocks of 16", c->num_pages,
+                  P, c->num_kv_heads);
         return OJASX_ERR_INVALID;
     }
     if (c->rotary_dim < 0 || c->rotary_dim > D || c->rotary_dim % 16 || (c->rotary_dim && !c->turns)) {

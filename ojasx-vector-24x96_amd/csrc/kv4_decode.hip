@@ -8,7 +8,8 @@
 // so the matrix operands are the integers -8 .. 7, exact in fp16, and the steps
 // stay outside in fp32.  (With the codes 0 .. 15 themselves the two terms are
 // each as large as lo, about two standard deviations of V, and their sum, an
-// average over many tokens, much smaller: what fp32 rounds off them would show.)
+// average over many tokens, much smaller: what fp32 rounds off them would show.
+// Keys for bf16 outputs keep 0 .. 15 and lo: the scores are exact enough.)
 // A column of the products is a (query head j,
 // group g) pair: column j G + g of the score product holds q_j with every
 // group but g zeroed, so one accumulator gives all groups' partial sums, each
@@ -33,8 +34,11 @@
 // outputs, a second one for what it leaves for fp16 and fp32 outputs.  Scores,
 // maxima, sums and outputs are fp32.
 //
-// The pass is split over the slots (gridDim.x); kv4_merge_kernel joins the
-// splits' (out, max, sum).
+// Work: the tiles of all sequences in one row, cut into equal runs, one for each
+// of the W workgroups of a (kv head, slice of its query heads), whatever the
+// sequences' lengths.  A workgroup goes through the sequences of its run; a
+// sequence that lies in one run is written whole, of the others each run leaves
+// (out, max, sum) in slot run + sequence, and kv4_merge_kernel joins them.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -47,19 +51,18 @@ namespace {
 constexpr int kNT = 256;
 constexpr int kNW = kNT / 64;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kMostRange = 0x1p40f;              // takes the smallest fp16 step to 2^16
 
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
-typedef unsigned int u4_t __attribute__((ext_vector_type(4)));
 
 struct Kv4DecodeParams {
     Kv4View c;
     const void *q;
     void *out;
-    float *part_o, *part_ml;    // [B][Hq][splits][D], [B][Hq][splits][2]
+    float *part_o, *part_ml;    // [W + B][Hq][D], [W + B][Hq][2]
     const int *seen;
-    int Hq, R, splits;
+    int Hq, R, W;
     float scale;                // scale factor x log2(e)
 };
 
@@ -78,53 +81,115 @@ __device__ __forceinline__ Kv4Extent kv4_extent(const Kv4View &c, int seen) {
 }
 
 __device__ __forceinline__ h2_t as_h2(uint32_t u) { return __builtin_bit_cast(h2_t, u); }
-// c - 8 of the two codes that a mask with 0x000f000f (0x00f000f0) leaves, as
-// fp16: 0x6400 | c is 1024 + c, 0x6400 | 16 c is 1024 + 16 c.
-__device__ __forceinline__ h2_t codes_low(uint32_t w) {
-    const uint32_t u = (w & 0x000f000fu) | 0x64006400u;
-    return as_h2(u) - h2_t{(_Float16)1032.f, (_Float16)1032.f};
+__device__ __forceinline__ int kv4_tiles(const Kv4View &c, int seen) {
+    const Kv4Extent x = kv4_extent(c, seen);
+    return ((x.entries << (c.pshift - 4)) + 3) >> 2;
 }
-__device__ __forceinline__ h2_t codes_high(uint32_t w) {
-    const uint32_t u = (w & 0x00f000f0u) | 0x64006400u;
-    return as_h2(u) * h2_t{(_Float16)0.0625f, (_Float16)0.0625f} -
-           h2_t{(_Float16)72.f, (_Float16)72.f};
+// Sum over the lanes before and with this one.
+__device__ __forceinline__ int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
 }
-__device__ __forceinline__ float mid(h2_t st) { return fmaf(8.f, (float)st[0], (float)st[1]); }
+// Run i of a row of T tiles in W runs: q + 1 tiles each for the first T % W, then q.
+struct Runs {
+    int W, q, r;
+    __device__ __forceinline__ Runs(int T, int most) : W(min(most, T)), q(0), r(0) {
+        if (W) q = T / W, r = T - q * W;
+    }
+    __device__ __forceinline__ int start(int i) const { return i * q + min(i, r); }
+    __device__ __forceinline__ int of(int tile) const {
+        const int big = (q + 1) * r;
+        return tile < big ? tile / (q + 1) : r + (tile - big) / q;
+    }
+};
+// The tiles of all sequences, and those before sequence b.  Whole waves call it.
+__device__ __forceinline__ int kv4_all_tiles(const Kv4View &c, const int *seen, int b, int *before) {
+    const int lane = threadIdx.x & 63;
+    int all = 0, bef = 0;
+    for (int i = lane; i < c.B; i += 64) {
+        const int n = kv4_tiles(c, seen[i]);
+        all += n;
+        if (i < b) bef += n;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o), bef += __shfl_xor(bef, o);
+    *before = bef;
+    return all;
+}
+
+// The two codes that a mask with 0x000f000f (0x00f000f0) leaves, as fp16, less 8
+// with MID: 0x6400 | c is 1024 + c, 0x6400 | 16 c is 1024 + 16 c.  `magic` is
+// 0x64006400 in a register, where the mask and the or are one instruction.
+template <bool MID>
+__device__ __forceinline__ h2_t codes_low(uint32_t w, uint32_t magic) {
+    constexpr _Float16 k = (_Float16)(MID ? 1032.f : 1024.f);
+    return as_h2((w & 0x000f000fu) | magic) - h2_t{k, k};
+}
+template <bool MID>
+__device__ __forceinline__ h2_t codes_high(uint32_t w, uint32_t magic) {
+    constexpr _Float16 k = (_Float16)(MID ? 72.f : 64.f);
+    return as_h2((w & 0x00f000f0u) | magic) * h2_t{(_Float16)0.0625f, (_Float16)0.0625f} - h2_t{k, k};
+}
+// lo, or the value of code 8.
+template <bool MID>
+__device__ __forceinline__ float base(h2_t st) {
+    return MID ? fmaf(8.f, (float)st[0], (float)st[1]) : (float)st[1];
+}
 __device__ __forceinline__ h8_t join(h2_t a, h2_t b, h2_t c, h2_t d) {
     return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // Sum over the G neighbouring lanes of a column group (G = 1, 2, 4, 8).
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {   // folds into the instruction that uses it
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
-    if (G > 1) v += __int_as_float(dpp_i<0xB1>(__float_as_int(v)));
-    if (G > 2) v += __int_as_float(dpp_i<0x4E>(__float_as_int(v)));
-    if (G > 4) v += __int_as_float(dpp_i<0x141>(__float_as_int(v)));
+    if (G > 1) v += dpp_f<0xB1>(v);
+    if (G > 2) v += dpp_f<0x4E>(v);
+    if (G > 4) v += dpp_f<0x141>(v);
     return v;
 }
 template <int G>
 __device__ __forceinline__ float group_max(float v) {
-    if (G > 1) v = fmaxf(v, __int_as_float(dpp_i<0xB1>(__float_as_int(v))));
-    if (G > 2) v = fmaxf(v, __int_as_float(dpp_i<0x4E>(__float_as_int(v))));
-    if (G > 4) v = fmaxf(v, __int_as_float(dpp_i<0x141>(__float_as_int(v))));
+    if (G > 1) v = fmaxf(v, dpp_f<0xB1>(v));
+    if (G > 2) v = fmaxf(v, dpp_f<0x4E>(v));
+    if (G > 4) v = fmaxf(v, dpp_f<0x141>(v));
     return v;
 }
-// Over the four quarters of the wave (lanes of one column).
+// Over the four quarters of the wave (lanes of one column): v_permlane16_swap of a
+// register with itself leaves row 2 i and row 2 i + 1 of each pair side by side,
+// v_permlane32_swap the halves.
 __device__ __forceinline__ float quarters_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float quarters_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// 2^e that takes |v| > 0 to [2^14, 2^15); 1 for 0, infinities and NaN.
+// 2^e that takes |v| > 0 to [2^14, 2^15), held to normal numbers; 2^126 for 0, 1
+// for infinities and NaN.
 __device__ __forceinline__ float to_range(float v) {
     const int e = (int)((__float_as_uint(v) >> 23) & 0xff);
-    // 2^(14 - (e - 127)), held to normal numbers
-    return e == 0 || e == 255 ? (e == 0 && v != 0.f ? 0x1p126f : 1.f)
-                              : __uint_as_float((uint32_t)min(max(268 - e, 1), 254) << 23);
+    return e == 255 ? 1.f : __uint_as_float((uint32_t)min(max(268 - e, 1), 253) << 23);
+}
+
+// A wave-uniform read of what no kernel of this file writes: a scalar load.
+__device__ __forceinline__ int uniform_int(const int *p) {
+    typedef __attribute__((address_space(4))) const int const_t;
+    return *reinterpret_cast<const_t *>(reinterpret_cast<uintptr_t>(p));
 }
 
 template <int NW>
@@ -143,37 +208,79 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[NW]) 
 }
 }  // namespace
 
-template <typename T, int D, int GS>
-__global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
+template <typename T_, int D, int GS>
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, 8))) void kv4_decode_kernel(Kv4DecodeParams p) {
     constexpr int G = D / GS, HS = 16 / G, NJ = D / 32;
-    constexpr int QP = sizeof(T) == 4 ? 2 : 1;                      // fp16 pieces of a query value
-    constexpr int WP = std::is_same<T, __hip_bfloat16>::value ? 1 : 2;   // and of a weight
-    __shared__ float so[kNW][HS][D];
-    __shared__ float sm[kNW][HS][2];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    constexpr int QP = sizeof(T_) == 4 ? 2 : 1;                     // fp16 pieces of a query value
+    constexpr int WP = std::is_same<T_, __hip_bfloat16>::value ? 1 : 2;   // and of a weight
+    constexpr bool KMID = WP > 1;             // keys: codes 0 .. 15 do for bf16 outputs
+    __shared__ float so[kNW][HS][D];                                 // the waves' outputs
+    __shared__ float sm[kNW][HS][2];                                 // and (max, sum)
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, h = lane >> 4, j = n / G, g = n % G;
-    const int b = blockIdx.z, slices = (p.R + HS - 1) / HS;
+    const int slices = (p.R + HS - 1) / HS;
     const int kvh = blockIdx.y / slices, j0 = blockIdx.y % slices * HS;
     const int nj = min(HS, p.R - j0), head0 = kvh * p.R + j0;
-    const Kv4Extent ext = kv4_extent(p.c, p.seen[b]);
     const int bps = p.c.pshift - 4;                                  // log2 of blocks per page
-    const int blocks = ext.entries << bps, tiles = (blocks + 3) >> 2;
-    const int per = (tiles + p.splits - 1) / p.splits;
-    const int t0 = blockIdx.x * per, t1 = min(tiles, t0 + per);
-    if (t0 >= t1 && blockIdx.x > 0) return;                          // the merge knows the same
+    // ---- this workgroup's run of tiles, and the sequence that it begins in
+    int pos, end, b, first;                                          // first: number of b's first tile
+    if (p.c.B <= 64) {
+        const int own = lane < p.c.B ? kv4_tiles(p.c, p.seen[lane]) : 0;
+        const int up = p.c.B == 1 ? __builtin_amdgcn_readfirstlane(own) : wave_scan(own);
+        const Runs runs(__builtin_amdgcn_readlane(up, 63), p.W);
+        if ((int)blockIdx.x >= runs.W) return;
+        pos = runs.start(blockIdx.x);
+        end = runs.start(blockIdx.x + 1);
+        b = p.c.B == 1 ? 0 : __builtin_ctzll(__ballot(up > pos));
+        first = __builtin_amdgcn_readlane(up - own, b);
+    } else {
+        int none;
+        const Runs runs(kv4_all_tiles(p.c, p.seen, 0, &none), p.W);
+        if ((int)blockIdx.x >= runs.W) return;
+        pos = runs.start(blockIdx.x);
+        end = runs.start(blockIdx.x + 1);
+        first = 0;
+        for (int i0 = 0;; i0 += 64) {
+            const int i = i0 + lane, own = i < p.c.B ? kv4_tiles(p.c, p.seen[i]) : 0, up = wave_scan(own);
+            const unsigned long long over = __ballot(first + up > pos);
+            if (over) {
+                const int at = __builtin_ctzll(over);
+                first += __shfl(up - own, at);
+                b = i0 + at;
+                break;
+            }
+            first += __shfl(up, 63);
+        }
+    }
+    pos = __builtin_amdgcn_readfirstlane(pos);
+    end = __builtin_amdgcn_readfirstlane(end);
+    b = __builtin_amdgcn_readfirstlane(b);
+    first = __builtin_amdgcn_readfirstlane(first);
+    uint32_t magic = 0x64006400u;
+    asm volatile("" : "+v"(magic));
+    for (; pos < end; ++b) {
+    const Kv4Extent ext = kv4_extent(p.c, uniform_int(p.seen + b));
+    const int tiles = ((ext.entries << bps) + 3) >> 2;
+    if (tiles == 0) continue;
+    const int t0 = pos - first, t1 = min(tiles, end - first);
+    const bool whole_sequence = t0 == 0 && t1 == tiles;
+    pos = first + t1;
+    first += tiles;
 
     // ---- the column's query: its group's dimensions, as fp16 pieces
     h8_t qf[QP][NJ];
     float qsum = 0.f, kq;
     {
         float x[NJ][8], mx = 0.f;
-        const T *qr = static_cast<const T *>(p.q) + ((size_t)b * p.Hq + head0 + min(j, nj - 1)) * D;
+        const T_ *qr = static_cast<const T_ *>(p.q) + ((size_t)b * p.Hq + head0 + min(j, nj - 1)) * D;
+#pragma unroll
+        for (int jj = 0; jj < NJ; ++jj) load8(qr + 32 * jj + 8 * h, x[jj]);
 #pragma unroll
         for (int jj = 0; jj < NJ; ++jj) {
             const bool mine = jj * 32 / GS == g && j < nj;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[jj][e] = mine ? load_act(qr, 32 * jj + 8 * h + e) : 0.f;
+                if (!mine) x[jj][e] = 0.f;
                 mx = fmaxf(mx, fabsf(x[jj][e]));
             }
         }
@@ -195,46 +302,65 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
     f4_t acc[NJ][2];
 #pragma unroll
     for (int i = 0; i < NJ; ++i) acc[i][0] = acc[i][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f, z = 0.f, f = 1.f;
+    // m: an integer no less than the largest score (log2), so that rescaling is
+    // exact; f: the weights' power of two, which only falls
+    float m = -INFINITY, l = 0.f, z = 0.f, f = kMostRange;
     const int *bt = p.c.bt + (size_t)b * p.c.max_pages;
-    for (int tile = t0 + w; tile < t1; tile += kNW) {
-        // the block of this lane's K rows (n / 4 of the tile) and of its
-        // weights (h): index in the pool, and the tokens it holds
-        long kblk, vblk;
-        int held;
-        {
-            auto at = [&](int x, int *tokens) __attribute__((always_inline)) {
-                const int blk = 4 * tile + x, e = blk >> bps, o = blk & ((1 << bps) - 1);
-                const int page = e < ext.entries ? bt[e] : -1;
-                const bool ok = page >= 0 && page < p.c.num_pages;
-                const int in_page = e == ext.last ? ext.tail : 1 << p.c.pshift;
-                if (tokens) *tokens = ok ? min(max(in_page - 16 * o, 0), 16) : 0;
-                return ((((long)(ok ? page : 0)) * p.c.Hkv + kvh) << bps) + o;
-            };
-            kblk = at(n >> 2, nullptr);
-            vblk = at(h, &held);
+    int page[4], blk[4], held[4];
+    auto read_pages = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) page[x] = uniform_int(bt + min((4 * tile + x) >> bps, ext.entries - 1));
+    };
+    // The tile's four blocks in the pool and the tokens they hold.
+    auto locate = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int i = 4 * tile + x, e = i >> bps, o = i & ((1 << bps) - 1);
+            const bool ok = e < ext.entries && page[x] >= 0 && page[x] < p.c.num_pages;
+            held[x] = ok ? min(max((e == ext.last ? ext.tail : 1 << p.c.pshift) - 16 * o, 0), 16) : 0;
+            blk[x] = (((ok ? page[x] : 0) * p.c.Hkv + kvh) << bps) + o;
         }
-        uint32_t kw[4][NJ], vw[NJ][4];
-        u4_t ksr[4], vsr[4];
-        const uint8_t *kp = p.c.kc + kblk * (D * 8) + (n & 3) * (D / 2) + h * NJ * 4;
+    };
+    auto pick = [&](const int (&v)[4], int x) __attribute__((always_inline)) {
+        return x == 0 ? v[0] : x == 1 ? v[1] : x == 2 ? v[2] : v[3];
+    };
+    // K rows (of block n / 4) and steps (of block h) of the tile that locate() found.
+    uint32_t kw[4][NJ];
+    u4_t ksr[4];
+    auto load_k = [&]() __attribute__((always_inline)) {
+        const uint8_t *kp = p.c.kc + (long)pick(blk, n >> 2) * (D * 8) + (n & 3) * (D / 2) + h * NJ * 4;
+        const u4_t *ksp = reinterpret_cast<const u4_t *>(p.c.ks) + ((long)pick(blk, h) * G + g) * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_words<NJ>(kp + 4 * i * (D / 2), kw[i]);
-        const u4_t *ksp = reinterpret_cast<const u4_t *>(p.c.ks + (vblk * G + g) * 16);
-        const u4_t *vsp = reinterpret_cast<const u4_t *>(p.c.vs + (vblk * G + g) * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) ksr[i] = ksp[i];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vsr[i] = vsp[i];
+    };
+    // A tile's V is loaded while its scores are computed, the next tile's K while
+    // the weights are: both in flight without registers of their own.
+    if (t0 + w < t1) {
+        read_pages(t0 + w);
+        locate(t0 + w);
+        load_k();
+        read_pages(t0 + w + kNW);
+    }
+    for (int tile = t0 + w; tile < t1; tile += kNW) {
+        uint32_t vw[NJ][4];
+        u4_t vsr[4];
+        const long vblk = pick(blk, h);
+        const u4_t *vsp = reinterpret_cast<const u4_t *>(p.c.vs) + (vblk * G + g) * 4;
         const uint8_t *vp = p.c.vc + vblk * (D * 8) + n * 16;
 #pragma unroll
+        for (int i = 0; i < 4; ++i) vsr[i] = vsp[i];
+#pragma unroll
         for (int i = 0; i < NJ; ++i) load_words<4>(vp + i * 256, vw[i]);
-        const bool whole = __all(held == 16);
+        const bool whole = held[0] + held[1] + held[2] + held[3] == 64;
+        const int mine = pick(held, h);
         if (!whole) {           // what a slot without a token holds reaches nothing
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (4 * i + r >= held) ksr[i][r] = 0, vsr[i][r] = 0;
+                    if (4 * i + r >= mine) ksr[i][r] = 0, vsr[i][r] = 0;
         }
         // ---- scores of the 16 tokens of block h, for this lane's column
         float sc[4][4], tmax = -INFINITY;
@@ -245,32 +371,44 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
 #pragma unroll
             for (int jj = 0; jj < NJ; ++jj) {
                 const uint32_t v = kw[i][jj];
-                const h8_t kf = join(codes_low(v), codes_high(v), codes_low(v >> 8), codes_high(v >> 8));
+                const h8_t kf = join(codes_low<KMID>(v, magic), codes_high<KMID>(v, magic),
+                                     codes_low<KMID>(v >> 8, magic), codes_high<KMID>(v >> 8, magic));
                 if (QP > 1) a = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[QP - 1][jj], a, 0, 0, 0);
                 a = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[0][jj], a, 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const h2_t st = as_h2(ksr[i][r]);
-                float v = group_sum<G>(fmaf(mid(st), qsum, (float)st[0] * a[r]));
-                if (!whole && 4 * i + r >= held) v = -INFINITY;
+                float v = group_sum<G>(fmaf(base<KMID>(st), qsum, (float)st[0] * a[r]));
+                if (!whole && 4 * i + r >= mine) v = -INFINITY;
                 sc[i][r] = v;
                 tmax = fmaxf(tmax, v);
                 smax = __builtin_elementwise_max(smax, as_h2(vsr[i][r]));
             }
         }
-        // ---- running maximum and the weights' power of two
-        const float mn = fmaxf(m, quarters_max(tmax)), ref = mn == -INFINITY ? 0.f : mn;
-        const float fn = fminf(to_range(quarters_max((float)smax[0])), 0x1p100f);
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - ref) * kq);
-        m = mn;
-        const float fa = alpha * (fn / f);
-        if (WP == 1 && !__all(fa == 1.f)) {
-#pragma unroll
-            for (int i = 0; i < NJ; ++i) acc[i][0] *= fa, acc[i][1] *= fa;
+        if (tile + kNW < t1) {
+            locate(tile + kNW);
+            load_k();
+            read_pages(tile + 2 * kNW);
         }
-        l *= alpha;
-        z *= alpha;
+        // ---- running maximum and the weights' power of two
+        const float mn = fmaxf(m, ceilf(quarters_max(tmax) * kq));
+        const float fn = fminf(f, to_range(quarters_max((float)smax[0])));
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - ref);
+        const float fa = alpha * (fn / f);
+        m = mn;
+        f = fn;
+        // bf16 outputs: the weights' factor 2^k goes into the exponent, and l and z
+        // carry it as the products do; the others multiply the steps, exactly
+        const float shift = (WP == 1 ? (float)((int)(__float_as_uint(f) >> 23) - 127) : 0.f) - ref;
+        if (!__all(fa == 1.f)) {
+            if (WP == 1)
+#pragma unroll
+                for (int i = 0; i < NJ; ++i) acc[i][0] *= fa, acc[i][1] *= fa;
+            l *= WP == 1 ? fa : alpha;
+            z *= WP == 1 ? fa : alpha;
+        }
         // where the outputs have fp16's or fp32's bits a tile's products get an
         // accumulator of their own, added to the sum so far in one rounding per
         // value (512 fp32 tokens per wave: 3.3e-7 off the exact sum, 4.3e-7 when
@@ -280,7 +418,6 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
 #pragma unroll
             for (int i = 0; i < NJ; ++i) part[i][0] = part[i][1] = f4_t{0.f, 0.f, 0.f, 0.f};
         }
-        f = fn;
         // ---- weights and the value product
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -292,10 +429,10 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
                 for (int r = 0; r < 4; ++r) {
                     const int i = 2 * u + y;
                     const h2_t st = as_h2(vsr[i][r]);
-                    const float pv = __builtin_amdgcn_exp2f((sc[i][r] - ref) * kq);
+                    const float pv = __builtin_amdgcn_exp2f(fmaf(sc[i][r], kq, shift));
                     l += pv;
-                    z = fmaf(pv, mid(st), z);
-                    wv[r] = pv * ((float)st[0] * f);
+                    z = fmaf(pv, base<true>(st), z);
+                    wv[r] = pv * (WP == 1 ? (float)st[0] : (float)st[0] * f);
                     // rounded to fp32 here: the pieces below are of one value (the
                     // compiler rounds the product to fp16 at once for one of them)
                     if (WP > 1) asm volatile("" : "+v"(wv[r]));
@@ -312,8 +449,10 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
 #pragma unroll
             for (int i = 0; i < NJ; ++i) {
                 const uint32_t a = vw[i][2 * u], c = vw[i][2 * u + 1];
-                const h8_t ev = join(codes_low(a), codes_low(a >> 8), codes_low(c), codes_low(c >> 8));
-                const h8_t od = join(codes_high(a), codes_high(a >> 8), codes_high(c), codes_high(c >> 8));
+                const h8_t ev = join(codes_low<true>(a, magic), codes_low<true>(a >> 8, magic),
+                                     codes_low<true>(c, magic), codes_low<true>(c >> 8, magic));
+                const h8_t od = join(codes_high<true>(a, magic), codes_high<true>(a >> 8, magic),
+                                     codes_high<true>(c, magic), codes_high<true>(c >> 8, magic));
                 f4_t *to = WP == 1 ? acc[i] : part[WP == 1 ? 0 : i];
 #pragma unroll
                 for (int x = WP - 1; x >= 0; --x) {
@@ -333,7 +472,6 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
     }
     l = quarters_sum(l);
     z = quarters_sum(z);
-    m *= kq;                                   // in log2 units, the same for a head's groups
 
     // ---- the waves' passes joined
     if (j < nj) {
@@ -345,8 +483,8 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        so[w][j][32 * i + 2 * (4 * h + r) + e] = fmaf(acc[i][e][r], inv, z);
-        if (g == 0 && h == 0) sm[w][j][0] = m, sm[w][j][1] = l;
+                        so[w][j][32 * i + 2 * (4 * h + r) + e] = WP == 1 ? (acc[i][e][r] + z) * inv : fmaf(acc[i][e][r], inv, z);
+        if (g == 0 && h == 0) sm[w][j][0] = m, sm[w][j][1] = WP == 1 ? l * inv : l;
     }
     __syncthreads();
     for (int x = tid; x < nj * D; x += kNT) {
@@ -362,64 +500,124 @@ __global__ __launch_bounds__(kNT) void kv4_decode_kernel(Kv4DecodeParams p) {
             o = fmaf(a, so[k][jj][d], o);
             ll = fmaf(a, sm[k][jj][1], ll);
         }
-        const size_t row = (size_t)b * p.Hq + head0 + jj;
-        if (p.splits == 1) {
-            store_act(static_cast<T *>(p.out), row * D + d, ll == 0.f ? 0.f : o / ll);
+        if (whole_sequence) {
+            store_act(static_cast<T_ *>(p.out), ((size_t)b * p.Hq + head0 + jj) * D + d, ll == 0.f ? 0.f : o / ll);
         } else {
-            p.part_o[(row * p.splits + blockIdx.x) * D + d] = o;
+            const size_t row = (size_t)(blockIdx.x + b) * p.Hq + head0 + jj;
+            p.part_o[row * D + d] = o;
             if (d == 0) {
-                float *ml = p.part_ml + (row * p.splits + blockIdx.x) * 2;
-                ml[0] = mm;
-                ml[1] = ll;
+                p.part_ml[2 * row] = mm;
+                p.part_ml[2 * row + 1] = ll;
             }
         }
     }
+    __syncthreads();                           // so and sm are free for the next sequence
+    }
 }
 
-// One workgroup per (query head, sequence): the splits that took tokens.
-template <typename T>
-__global__ __launch_bounds__(kNT) void kv4_merge_kernel(Kv4DecodeParams p, int D) {
-    const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-    const Kv4Extent ext = kv4_extent(p.c, p.seen[b]);
-    const int tiles = ((ext.entries << (p.c.pshift - 4)) + 3) >> 2;
-    const int per = (tiles + p.splits - 1) / p.splits;
-    const int used = per ? (tiles + per - 1) / per : 0;
-    const size_t row = (size_t)b * p.Hq + head;
-    const float *ml = p.part_ml + row * p.splits * 2, *po = p.part_o + row * p.splits * D;
-    float mm = -INFINITY;
-    for (int s = 0; s < used; ++s) mm = fmaxf(mm, ml[2 * s]);
-    const float ref = mm == -INFINITY ? 0.f : mm;
-    if (d >= D) return;
-    float o = 0.f, l = 0.f;
-    for (int s = 0; s < used; ++s) {
-        const float a = __builtin_amdgcn_exp2f(ml[2 * s] - ref);
-        o = fmaf(a, po[(size_t)s * D + d], o);
-        l = fmaf(a, ml[2 * s + 1], l);
+// One workgroup per (query head, sequence).  A sequence cut by runs: thread
+// (four dims, group of slots) adds every SG-th slot's output times its weight,
+// kPre of them loaded before the weights are known.
+template <typename T, int D>
+__global__ __launch_bounds__(kNT) void kv4_merge_kernel(Kv4DecodeParams p) {
+    constexpr int DQ = D / 4, SG = kNT / DQ, kPre = 4;
+    __shared__ float ws[kNT], wm[kNW], wl[kNW];
+    __shared__ float4 os[SG][DQ];
+    const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int d = tid % DQ, sg = tid / DQ;
+    const int tiles = kv4_tiles(p.c, p.seen[b]);
+    T *out = static_cast<T *>(p.out) + ((size_t)b * p.Hq + head) * D;
+    if (tiles == 0) {
+        if (tid < DQ)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_act(out, 4 * d + e, 0.f);
+        return;
     }
-    store_act(static_cast<T *>(p.out), row * D + d, l == 0.f ? 0.f : o / l);
+    int first;
+    const Runs runs(kv4_all_tiles(p.c, p.seen, b, &first), p.W);
+    const int i0 = runs.of(first), used = runs.of(first + tiles - 1) - i0 + 1;
+    if (used == 1) return;                               // written whole
+    const size_t row0 = (size_t)(i0 + b) * p.Hq + head;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row0;
+    const float4 *po = reinterpret_cast<const float4 *>(p.part_o) + row0 * DQ + d;
+    const size_t step = (size_t)p.Hq * DQ;
+    float4 pre[kPre];
+#pragma unroll
+    for (int u = 0; u < kPre; ++u) pre[u] = po[step * min(sg + u * SG, used - 1)];
+    float m = -INFINITY;
+    for (int s = tid; s < used; s += kNT) m = fmaxf(m, ml[(size_t)s * p.Hq].x);
+    m = wave_max_f(m);
+    if ((tid & 63) == 0) wm[tid >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kNW; ++k) m = fmaxf(m, wm[k]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, const float4 &x) __attribute__((always_inline)) {
+        o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    };
+    for (int s0 = 0; s0 < used; s0 += kNT) {             // kNT slots' weights at a time
+        const int s = s0 + tid, n = min(kNT, used - s0);
+        float w = 0.f;
+        if (s < used) {
+            const float2 x = ml[(size_t)s * p.Hq];
+            w = __builtin_amdgcn_exp2f(x.x - ref);
+            l = fmaf(w, x.y, l);
+        }
+        __syncthreads();
+        ws[tid] = w;
+        __syncthreads();
+        int k = sg;
+        if (s0 == 0) {
+#pragma unroll
+            for (int u = 0; u < kPre; ++u)
+                if (sg + u * SG < n) add(ws[sg + u * SG], pre[u]);
+            k += kPre * SG;
+        }
+        for (; k < n; k += kPre * SG) {
+            float4 x[kPre];
+#pragma unroll
+            for (int u = 0; u < kPre; ++u) x[u] = po[step * min(s0 + k + u * SG, used - 1)];
+#pragma unroll
+            for (int u = 0; u < kPre; ++u)
+                if (k + u * SG < n) add(ws[k + u * SG], x[u]);
+        }
+    }
+    l = wave_sum_f(l);
+    if ((tid & 63) == 0) wl[tid >> 6] = l;
+    os[sg][d] = o;
+    __syncthreads();
+    if (tid >= D) return;
+    l = 0.f;
+#pragma unroll
+    for (int k = 0; k < kNW; ++k) l += wl[k];
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < SG; ++k) v += reinterpret_cast<const float *>(os[k])[tid];
+    store_act(out, tid, l == 0.f ? 0.f : v / l);
 }
 
 namespace {
 int decode_heads_per_slice(int D, int GS) { return 16 / (D / GS); }
 
-// Splits of the slots of a sequence: about four workgroups per CU over the
-// whole call, each at least four tiles (one per wave) long.
-int decode_splits(const OjasxKV4Cache *c, int Hq, int max_seen) {
+// Runs W: two workgroups per CU over the whole call (what the registers of the
+// main kernel leave room for), no more than there can be tiles.
+int decode_runs(const OjasxKV4Cache *c, int Hq, int max_seen) {
     const int HS = decode_heads_per_slice(c->head_dim, c->group_size);
     const int R = Hq / c->num_kv_heads;
-    const long groups = (long)c->num_sequences * c->num_kv_heads * ((R + HS - 1) / HS);
-    const long slots = max_seen > 0 ? std::min((long)max_seen, (long)c->max_pages * c->page_size)
-                                    : (long)c->max_pages * c->page_size;
-    const long tiles = (slots + 63) / 64;
-    long s = (1024 + groups - 1) / groups;
-    if (s > (tiles + kNW - 1) / kNW) s = (tiles + kNW - 1) / kNW;
-    return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+    const long groups = (long)c->num_kv_heads * ((R + HS - 1) / HS);
+    const long cap = (long)c->max_pages * c->page_size;
+    const long slots = max_seen > 0 ? std::min((long)max_seen, cap) : cap;
+    const long tiles = (slots + 63) / 64 * c->num_sequences;
+    return (int)std::max(1L, std::min((512 + groups - 1) / groups, tiles));
 }
 
 int decode_check(const OjasxKV4Cache *c, int Hq) {
-    if (Hq <= 0 || Hq > 65535 || Hq % c->num_kv_heads || c->num_sequences > 65535) {
-        set_error("4-bit KV decode: %d query heads for %d kv heads, %d sequences (at most 65535)", Hq,
-                  c->num_kv_heads, c->num_sequences);
+    const long tiles = ((long)c->max_pages * c->page_size + 63) / 64 * c->num_sequences;
+    if (Hq <= 0 || Hq > 65535 || Hq % c->num_kv_heads || c->num_sequences > 65535 || tiles > 0x3fffffffL) {
+        set_error("4-bit KV decode: %d query heads for %d kv heads, %d sequences (at most 65535) of up to %d pages "
+                  "(2^36 tokens in all)", Hq, c->num_kv_heads, c->num_sequences, c->max_pages);
         return OJASX_ERR_INVALID;
     }
     return OJASX_OK;
@@ -428,7 +626,7 @@ int decode_check(const OjasxKV4Cache *c, int Hq) {
 template <typename T>
 int launch_decode(const Kv4DecodeParams &p, int D, int GS, hipStream_t st) {
     const int HS = decode_heads_per_slice(D, GS);
-    const dim3 grid(p.splits, p.c.Hkv * ((p.R + HS - 1) / HS), p.c.B);
+    const dim3 grid(p.W, p.c.Hkv * ((p.R + HS - 1) / HS));
     if (D == 64 && GS == 32) OJX_LAUNCH((kv4_decode_kernel<T, 64, 32>), grid, dim3(kNT), 0, st, p);
     else if (D == 64) OJX_LAUNCH((kv4_decode_kernel<T, 64, 64>), grid, dim3(kNT), 0, st, p);
     else if (D == 128 && GS == 32) OJX_LAUNCH((kv4_decode_kernel<T, 128, 32>), grid, dim3(kNT), 0, st, p);
@@ -437,8 +635,10 @@ int launch_decode(const Kv4DecodeParams &p, int D, int GS, hipStream_t st) {
     else if (GS == 32) OJX_LAUNCH((kv4_decode_kernel<T, 256, 32>), grid, dim3(kNT), 0, st, p);
     else if (GS == 64) OJX_LAUNCH((kv4_decode_kernel<T, 256, 64>), grid, dim3(kNT), 0, st, p);
     else OJX_LAUNCH((kv4_decode_kernel<T, 256, 128>), grid, dim3(kNT), 0, st, p);
-    if (p.splits > 1)
-        OJX_LAUNCH(kv4_merge_kernel<T>, dim3(p.Hq, p.c.B), dim3(kNT), 0, st, p, D);
+    const dim3 rows(p.Hq, p.c.B);
+    if (D == 64) OJX_LAUNCH((kv4_merge_kernel<T, 64>), rows, dim3(kNT), 0, st, p);
+    else if (D == 128) OJX_LAUNCH((kv4_merge_kernel<T, 128>), rows, dim3(kNT), 0, st, p);
+    else OJX_LAUNCH((kv4_merge_kernel<T, 256>), rows, dim3(kNT), 0, st, p);
     OJX_HIP(hipGetLastError());
     return OJASX_OK;
 }
@@ -454,8 +654,8 @@ OJASX_API long ojasx_kv4_decode_workspace(const OjasxKV4Cache *cache, int num_q_
     int rc = kv4_view(cache, &v);
     if (!rc) rc = decode_check(cache, num_q_heads);
     if (rc) return rc;
-    const long s = decode_splits(cache, num_q_heads, max_seen);
-    return s == 1 ? 0 : s * cache->num_sequences * num_q_heads * (cache->head_dim + 2) * (long)sizeof(float);
+    return ((long)decode_runs(cache, num_q_heads, max_seen) + cache->num_sequences) * num_q_heads *
+           (cache->head_dim + 2) * (long)sizeof(float);
 }
 
 OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q, int num_q_heads, int dtype,
@@ -467,23 +667,25 @@ OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q,
     if (!rc) rc = decode_check(cache, num_q_heads);
     if (rc) return rc;
     if (!q || !seen || !out) return OJASX_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(q) & 15) {
+        set_error("4-bit KV decode: q is 16-byte aligned");
+        return OJASX_ERR_INVALID;
+    }
     if (dtype != OJASX_DTYPE_F32 && dtype != OJASX_DTYPE_BF16 && dtype != OJASX_DTYPE_F16) {
         set_error("unsupported dtype %d", dtype);
         return OJASX_ERR_INVALID;
     }
     const int D = cache->head_dim;
-    p.splits = decode_splits(cache, num_q_heads, max_seen);
-    const size_t rows = (size_t)cache->num_sequences * num_q_heads;
-    if (p.splits > 1) {
-        if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-            workspace_bytes < (long)(rows * p.splits * (D + 2) * sizeof(float))) {
-            set_error("4-bit KV decode: workspace of %ld bytes at %p (ojasx_kv4_decode_workspace; 16-byte "
-                      "aligned)", workspace_bytes, workspace);
-            return OJASX_ERR_INVALID;
-        }
-        p.part_o = static_cast<float *>(workspace);
-        p.part_ml = p.part_o + rows * p.splits * D;
+    p.W = decode_runs(cache, num_q_heads, max_seen);
+    const size_t rows = ((size_t)p.W + cache->num_sequences) * num_q_heads;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < (long)(rows * (D + 2) * sizeof(float))) {
+        set_error("4-bit KV decode: workspace of %ld bytes at %p (ojasx_kv4_decode_workspace; 16-byte aligned)",
+                  workspace_bytes, workspace);
+        return OJASX_ERR_INVALID;
     }
+    p.part_o = static_cast<float *>(workspace);
+    p.part_ml = p.part_o + rows * D;
     p.q = q, p.out = out, p.seen = seen, p.Hq = num_q_heads, p.R = num_q_heads / cache->num_kv_heads;
     p.scale = (scale_factor > 0.f ? scale_factor : 1.0f / sqrtf((float)D)) * kLog2e;
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -909,8 +909,8 @@ class PagedInt4KVCache:
         [num_sequences], the current one included) of each sequence; q head j
         reads kv head j // (num_q_heads // num_kv_heads).  ``scale_factor <= 0``
         means 1/sqrt(head_dim); a sequence without tokens gives 0.
-        ``max_seen``, a bound on ``seen`` where the caller knows one, keeps
-        short sequences from being split as far as the capacity asks for."""
+        ``max_seen``, a bound on ``seen`` where the caller knows one, keeps the
+        launch of short sequences as small as they are."""
         torch = _torch()
         what = "PagedInt4KVCache.decode"
         tag = _inference_tag(what, query)
@@ -936,11 +936,13 @@ class PagedInt4KVCache:
                 not out.is_contiguous():
             raise ValueError("out must be contiguous and of the query's shape, dtype and device")
         with _on_device(self.device) as stream:
-            q = query.contiguous()
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            q = _aligned_rows(query)
+            if not q.is_contiguous():
+                q = q.contiguous()
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             rc = lib.ojasx_kv4_decode_device(self._ref, q.data_ptr(), heads, tag, sp, max_seen,
                                              float(scale_factor), out.data_ptr(),
-                                             ws.data_ptr() if need else None, need, stream)
+                                             ws.data_ptr(), need, stream)
         if rc:
             _lib.check(rc, "ojasx_kv4_decode_device")
         return out

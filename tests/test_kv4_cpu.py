@@ -68,18 +68,17 @@ def test_bad_calls_are_refused(pkg):
     decode = lambda heads=4, dtype=0, q=FAKE, ws=FAKE, n=need: L.ojasx_kv4_decode_device(  # noqa: E731
         ref, q, heads, dtype, FAKE, 0, -1.0, FAKE, ws, n, None)
     assert decode(heads=3) == -3 and decode(heads=0) == -3 and decode(dtype=3) == -3 and decode(q=None) == -1
-    if need:
-        assert decode(n=need - 1) == -3 and decode(ws=None) == -3 and decode(ws=FAKE + 4) == -3
+    assert decode(n=need - 1) == -3 and decode(ws=None) == -3 and decode(ws=FAKE + 4) == -3
 
 
-def test_workspace_covers_the_splits(pkg):
+def test_workspace_covers_the_runs(pkg):
+    """(runs + sequences) x query heads x (head_dim + 2) floats; no more runs than tiles."""
     L = pkg.lib()
     big = cache(pkg, num_sequences=1, max_pages=2048, num_pages=2048)
-    few = cache(pkg, num_sequences=64, max_pages=2048, num_pages=131072, num_kv_heads=16)
-    one = L.ojasx_kv4_decode_workspace(ctypes.addressof(big), 4, 0)
-    assert one > 0 and one % (4 * 130 * 4) == 0
-    assert L.ojasx_kv4_decode_workspace(ctypes.addressof(big), 4, 64) == 0       # one pass of one workgroup
-    assert L.ojasx_kv4_decode_workspace(ctypes.addressof(few), 64, 0) == 0       # enough heads without splits
+    row = 4 * 130 * 4
+    need = [L.ojasx_kv4_decode_workspace(ctypes.addressof(big), 4, m) for m in (0, 64, 65, 1 << 30)]
+    assert all(n > 0 and n % row == 0 for n in need)
+    assert need[1] == 2 * row and need[2] == 3 * row and need[0] == need[3]
 
 
 def test_python_refusals(pkg):
