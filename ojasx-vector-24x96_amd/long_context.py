@@ -653,21 +653,35 @@ class PagedCodeKVCache:
         return 2 * self.seq_len * self.num_kv_heads * (G + 4)
 
 
+_INFERENCE_TAGS = {}
+
+
 def _inference_tag(what, *tensors):
     """The C-ABI tag of the tensors' one dtype; they have no gradient here."""
-    torch = _torch()
     t = tensors[0]
+    dtype, device = t.dtype, t.device
+    _require_gpu(t, what)
     for u in tensors:
-        _require_gpu(u, what)
-        if u.dtype != t.dtype or u.device != t.device:
-            raise ValueError(f"{what}: tensors of {t.dtype} on {t.device} and of {u.dtype} on {u.device}")
-        if u.requires_grad and torch.is_grad_enabled():
+        if u.dtype != dtype or u.device != device:
+            raise ValueError(f"{what}: tensors of {dtype} on {device} and of {u.dtype} on {u.device}")
+        if u.requires_grad and _torch().is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or with detached "
                                "tensors")
-    tag = _attn_tag(t.dtype)
-    if tag is None or tag == _lib.DTYPE_F64:
-        raise TypeError(f"{what}: unsupported dtype {t.dtype}: float32, bfloat16 or float16")
+    tag = _INFERENCE_TAGS.get(dtype)
+    if tag is None:
+        tag = _attn_tag(dtype)
+        if tag is None or tag == _lib.DTYPE_F64:
+            raise TypeError(f"{what}: unsupported dtype {dtype}: float32, bfloat16 or float16")
+        _INFERENCE_TAGS[dtype] = tag
     return tag
+
+
+def _new_like(t):
+    """An uninitialised contiguous tensor of t's shape, dtype and device."""
+    torch = _torch()
+    if t.is_contiguous():
+        return torch.empty_like(t)      # takes half the time of torch.empty with a device
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _aligned_rows(t):
@@ -691,26 +705,15 @@ def _lengths_tensor(t, n, device, what):
     return t.data_ptr()
 
 
-class _on_device:
-    """Makes ``device`` the current one for a call where another is."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, device):
-        self.index = device.index
-        self.before = None
-
-    def __enter__(self):
-        torch = _torch()
-        current = torch.cuda.current_device()
-        if current != self.index:
-            self.before = current
-            torch.cuda.set_device(self.index)
-        return _lib.raw_stream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            _torch().cuda.set_device(self.before)
+def _launch(device, call):
+    """``call(stream)`` on the device's current stream, the device made current
+    where another is."""
+    torch = _torch()
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return call(_lib.raw_stream(index))
+    with torch.cuda.device(index):
+        return call(_lib.raw_stream(index))
 
 
 class PagedInt4KVCache:
@@ -854,22 +857,21 @@ class PagedInt4KVCache:
         if query is not None:
             self._check_rows(query, n, None, "query")
         at, cu = self._packed(n, start, cu_seqlens)
-        with _on_device(self.device) as stream:
-            k, v = _aligned_rows(key), _aligned_rows(value)
-            ks, vs = k.stride(), v.stride()
-            qp = qo = ko = None
-            qs, heads = (0, 0), 0
-            if query is not None:
-                q = _aligned_rows(query)
-                qs, heads = q.stride(), q.shape[1]
-                qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-                qp = q.data_ptr()
-            if return_key:
-                ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            rc = _lib.lib().ojasx_kv4_append_device(
-                self._ref, qp, qs[0], qs[1], heads, None if qo is None else qo.data_ptr(),
-                k.data_ptr(), ks[0], ks[1], None if ko is None else ko.data_ptr(), v.data_ptr(),
-                vs[0], vs[1], n, tag, at, cu, stream)
+        k, v = _aligned_rows(key), _aligned_rows(value)
+        ks, vs = k.stride(), v.stride()
+        qp = qo = ko = None
+        qs, heads = (0, 0), 0
+        if query is not None:
+            q = _aligned_rows(query)
+            qs, heads = q.stride(), q.shape[1]
+            qo = _new_like(q)
+            qp = q.data_ptr()
+        if return_key:
+            ko = _new_like(k)
+        rc = _launch(self.device, lambda stream: _lib.lib().ojasx_kv4_append_device(
+            self._ref, qp, qs[0], qs[1], heads, None if qo is None else qo.data_ptr(),
+            k.data_ptr(), ks[0], ks[1], None if ko is None else ko.data_ptr(), v.data_ptr(),
+            vs[0], vs[1], n, tag, at, cu, stream))
         if rc:
             _lib.check(rc, "ojasx_kv4_append_device")
         return qo, ko
@@ -893,11 +895,10 @@ class PagedInt4KVCache:
             raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
         at, cu = self._packed(num_tokens, start, cu_seqlens)
         sp = None if seen is None else _lengths_tensor(seen, self.num_sequences, self.device, "seen")
-        with _on_device(self.device) as stream:
-            k = torch.empty(num_tokens, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
-            v = torch.empty_like(k)
-            rc = _lib.lib().ojasx_kv4_read_device(self._ref, at, cu, sp, num_tokens, k.data_ptr(),
-                                                  v.data_ptr(), tag, stream)
+        k = torch.empty(num_tokens, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        rc = _launch(self.device, lambda stream: _lib.lib().ojasx_kv4_read_device(
+            self._ref, at, cu, sp, num_tokens, k.data_ptr(), v.data_ptr(), tag, stream))
         if rc:
             _lib.check(rc, "ojasx_kv4_read_device")
         return k, v
@@ -931,18 +932,17 @@ class PagedInt4KVCache:
                 self._workspace_bytes.clear()
             self._workspace_bytes[(heads, max_seen)] = need
         if out is None:
-            out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+            out = _new_like(query)
         elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or \
                 not out.is_contiguous():
             raise ValueError("out must be contiguous and of the query's shape, dtype and device")
-        with _on_device(self.device) as stream:
-            q = _aligned_rows(query)
-            if not q.is_contiguous():
-                q = q.contiguous()
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            rc = lib.ojasx_kv4_decode_device(self._ref, q.data_ptr(), heads, tag, sp, max_seen,
-                                             float(scale_factor), out.data_ptr(),
-                                             ws.data_ptr(), need, stream)
+        q = _aligned_rows(query)
+        if not q.is_contiguous():
+            q = q.contiguous()
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        rc = _launch(self.device, lambda stream: lib.ojasx_kv4_decode_device(
+            self._ref, q.data_ptr(), heads, tag, sp, max_seen, scale_factor, out.data_ptr(),
+            ws.data_ptr(), need, stream))
         if rc:
             _lib.check(rc, "ojasx_kv4_decode_device")
         return out
@@ -1009,22 +1009,21 @@ class PackedPromptAttention:
             ck = _lengths_tensor(cu_seqlens_kv, B + 1, dev, "cu_seqlens_kv")
         fresh = out is None
         if fresh:
-            out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+            out = _new_like(query)
         elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or \
                 not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous, 16-byte aligned and of the query's shape, dtype and "
                              "device")
-        with _on_device(dev) as stream:
-            q, k, v = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-            if lse is not None and not fresh:
-                lse.fill_(-math.inf)
-            qs, ks, vs = q.stride(), k.stride(), v.stride()
-            rc = _lib.lib().ojasx_prompt_attention_device(
-                q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], tag,
-                q.shape[0], k.shape[0], self.num_heads, self.num_kv_heads, self.head_dim, cq, ck, B,
-                int(self.causal), self.scale, int(fresh), out.data_ptr(),
-                None if lse is None else lse.data_ptr(), stream)
+        q, k, v = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+        if lse is not None and not fresh:
+            lse.fill_(-math.inf)
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        rc = _launch(dev, lambda stream: _lib.lib().ojasx_prompt_attention_device(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], tag,
+            q.shape[0], k.shape[0], self.num_heads, self.num_kv_heads, self.head_dim, cq, ck, B,
+            self.causal, self.scale, fresh, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), stream))
         if rc:
             _lib.check(rc, "ojasx_prompt_attention_device")
         return (out, lse) if return_lse else out
