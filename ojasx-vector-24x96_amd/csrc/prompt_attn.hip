@@ -99,23 +99,37 @@ __device__ __forceinline__ int v_unit(int row, int u) {
     return ROWB >= 256 ? u ^ (row & 7) : u ^ (row >> 1 & 3);
 }
 
-__device__ __forceinline__ float swap_halves(float v) { return __shfl_xor(v, 32); }
+// max and sum of a lane's value and the other half's: v_permlane32_swap of a register
+// with itself leaves the low half's in the first result, the high half's in the second.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// Waits for the loads so far.  Without it before a loop the compiler waits inside
+// it, for the loop's own loads too, before the first use of what was loaded
+// before it.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0) alone
 
 // The key that accumulator register r of a lane's half h stands for.
 __device__ __forceinline__ constexpr int key_of(int r) { return 8 * (r / 4) + r % 4; }
 
-// Running softmax of one query row per lane over a tile's scores s (two blocks
-// of 32 keys): rescales acc and l where the row's maximum grew by more than 2^8,
-// turns s into weights.  Weights up to 2^8 above 1 lose nothing: they are
-// rounded relative to their size and all sums are fp32.
+// Running maximum of one query row per lane with a tile's scores s (two blocks of
+// 32 keys): rescales acc and l where the row's maximum grew by more than 2^8.
+// Weights up to 2^8 above 1 lose nothing: they are rounded relative to their
+// size and all sums are fp32.
 template <int NT>
-__device__ __forceinline__ void softmax_tile(f32x16_t (&s)[2], float scale2, float &m, float &ref, float &l,
-                                             f32x16_t (&acc)[NT]) {
+__device__ __forceinline__ void raise_max(const f32x16_t (&s)[2], float scale2, float &m, float &ref, float &l,
+                                          f32x16_t (&acc)[NT]) {
     float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[1][r]);
     float t = fmaxf(t0, t1);
-    t = fmaxf(t, swap_halves(t)) * scale2;
+    t = halves_max(t) * scale2;
     if (__any(t > m + 8.f)) {
         const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
         const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
@@ -125,20 +139,12 @@ __device__ __forceinline__ void softmax_tile(f32x16_t (&s)[2], float scale2, flo
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= alpha;
     }
-    float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], scale2, -ref));
-        s[1][r] = __builtin_amdgcn_exp2f(fmaf(s[1][r], scale2, -ref));
-        a0 += s[0][r];
-        a1 += s[1][r];
-    }
-    l += a0 + a1;
 }
 
 // Hides the keys past `lim` from the lane's row; k0 = the tile's first key.
 __device__ __forceinline__ void mask_tile(f32x16_t (&s)[2], int lim, int k0, int h) {
-    const int rel = lim - k0 - 4 * h;
+    int rel = lim - k0 - 4 * h;
+    asm volatile("" : "+v"(rel));                // keeps the selects behind the wave's branch
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         if (key_of(r) > rel) s[0][r] = -INFINITY;
@@ -186,7 +192,7 @@ __device__ __forceinline__ void zero_rows(const PromptParams &p, const PromptBlo
 // bf16 and fp16: v_mfma_f32_32x32x16, head dims up to DP (the dims past D are
 // zeros in Q and K).
 template <typename E, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void prompt_attn_kernel(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2, DP > 128 ? 1 : 2))) void prompt_attn_kernel(
     PromptParams p, int slots) {
     typedef typename E::T T;
     typedef typename E::V8 V8;
@@ -226,22 +232,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
     }
     // ---- staging: unit i of a tile is (key, unit) = ((tid + i NT) / UPR, % UPR)
     const int su = tid % UPR, sr = tid / UPR;        // NT is a multiple of UPR
-    const T *kp = static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + su * 8;
-    const T *vp = static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + su * 8;
-    const bool in = su * 8 < p.D;
+    const bool in = su * 8 < p.D;               // past the head's dims: unit 0's, and zeros stored
+    const T *kp = static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + (in ? su * 8 : 0);
+    const T *vp = static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + (in ? su * 8 : 0);
+    const T *kn = kp + sr * p.k_ts, *vn = vp + sr * p.v_ts;    // this thread's first row of the next tile
     u32x4_t kr[CH], vr[CH];
     auto load = [&](int tile) __attribute__((always_inline)) {
+        if ((tile + 1) * kKeys <= Lk) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const long key = min(tile * kKeys + sr + i * (NT / UPR), Lk - 1);   // past the end: the last again
-            kr[i] = vr[i] = u32x4_t{0, 0, 0, 0};
-            if (in) {
+            for (int i = 0; i < CH; ++i) {
+                kr[i] = *reinterpret_cast<const u32x4_t *>(kn + i * (NT / UPR) * p.k_ts);
+                vr[i] = *reinterpret_cast<const u32x4_t *>(vn + i * (NT / UPR) * p.v_ts);
+            }
+            kn += kKeys * p.k_ts;
+            vn += kKeys * p.v_ts;
+        } else {                                       // past the end: the last key again
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const long key = min(tile * kKeys + sr + i * (NT / UPR), Lk - 1);
                 kr[i] = *reinterpret_cast<const u32x4_t *>(kp + key * p.k_ts);
                 vr[i] = *reinterpret_cast<const u32x4_t *>(vp + key * p.v_ts);
             }
         }
     };
     auto store = [&](int tile) __attribute__((always_inline)) {
+        if (p.D < DP && !in)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) kr[i] = vr[i] = u32x4_t{0, 0, 0, 0};
         unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -256,6 +273,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
         load(0);
         store(0);
     }
+    loads_done();
     // this lane's part of a transposed V read: key 4 h + i / 4, dims 16 g + 4 (i % 4) .. of 32
     const int vkey = 4 * h + ((lane & 15) >> 2), vg = lane >> 4 & 1, vb = (lane & 3) * 8;
     for (int tile = 0; tile < tiles; ++tile) {
@@ -265,46 +283,74 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
         if (k0 <= lim_hi) {
             const unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
             f32x16_t s[2] = {};
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c)
+            // operands are read two steps before the products that take them; the
+            // barriers keep the compiler from moving the reads back to their use
+            constexpr int NC = DP / 16;
+            u32x4_t kf[3][2];
+            auto read_k = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     const int r = 32 * b + n;
-                    const u32x4_t x =
-                        *reinterpret_cast<const u32x4_t *>(ks + r * ROWB + k_unit<ROWB>(r, 2 * c + h) * 16);
-                    s[b] = E::mma(__builtin_bit_cast(V8, x), qf[c], s[b]);
+                    kf[c % 3][b] = *reinterpret_cast<const u32x4_t *>(ks + r * ROWB + k_unit<ROWB>(r, 2 * c + h) * 16);
                 }
+            };
+            read_k(0);
+            read_k(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                if (c + 2 < NC) read_k(c + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) s[b] = E::mma(__builtin_bit_cast(V8, kf[c % 3][b]), qf[c], s[b]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (k0 + kKeys - 1 > lim_lo) mask_tile(s, lim, k0, h);
-            softmax_tile(s, p.scale2, m, ref, l, acc);
-            V8 pf[2][2];                             // the weights, rounded to the inputs' type
+            raise_max(s, p.scale2, m, ref, l, acc);
+            // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block),
+            // rounded to the inputs' type; between the products of one 16 go the
+            // exponentials and the V reads of the next.
+            constexpr int NT2 = DP / 32, VB = NT2 < 4 ? NT2 : 4, PART = 8 / NT2;
+            V8 pf[4];
+            auto weight = [&](int f, int e) __attribute__((always_inline)) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[f >> 1][8 * (f & 1) + e], p.scale2, -ref));
+                l += x;
+                pf[f][e] = E::from(x);
+            };
+            // V operands (f, t) in order, VB of them read ahead
+            s16x4_t vf[2 * VB][2];
+            auto read_v = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+                for (int y = 0; y < 2; ++y) {
+                    const int r = 16 * (i / NT2) + 8 * y + vkey, t = i % NT2;
+                    auto *at = (__attribute__((address_space(3))) s16x4_t *)(vs + r * ROWB +
+                                                                          v_unit<ROWB>(r, 2 * t + vg) * 32 + vb);
+                    vf[i % (2 * VB)][y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+                }
+            };
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+            for (int i = 0; i < VB; ++i) read_v(i);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) pf[b][u][e] = E::from(s[b][8 * u + e]);
+            for (int e = 0; e < 8; ++e) weight(0, e);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
+            for (int i = 0; i < 4 * NT2; ++i) {
+                const int f = i / NT2, t = i % NT2;
+                if (i + VB < 4 * NT2) read_v(i + VB);
+                __builtin_amdgcn_sched_barrier(0);
+                typedef short s16x8_t __attribute__((ext_vector_type(8)));
+                const s16x8_t z = __builtin_shufflevector(vf[i % (2 * VB)][0], vf[i % (2 * VB)][1], 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[t] = E::mma(__builtin_bit_cast(V8, z), pf[f], acc[t]);
+                if (f < 3)
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        s16x4_t x[2];
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const int r = 32 * b + 16 * u + 8 * y + vkey;
-                            auto *at = (__attribute__((address_space(3))) s16x4_t *)(vs + r * ROWB +
-                                                                                  v_unit<ROWB>(r, 2 * t + vg) * 32 + vb);
-                            x[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
-                        }
-                        typedef short s16x8_t __attribute__((ext_vector_type(8)));
-                        const s16x8_t z = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                        acc[t] = E::mma(__builtin_bit_cast(V8, z), pf[b][u], acc[t]);
-                    }
+                    for (int e = 0; e < PART; ++e) weight(f + 1, t * PART + e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if (tile + 1 < tiles) store(tile + 1);
     }
-    l += swap_halves(l);
+    l = halves_sum(l);
     // A weight of 0 times an infinity or a NaN is a NaN in the matrix product: an
     // output that is NaN may come from a key its row does not see.  Where the
     // wave has one, its rows run again, key by key, with hidden keys left out.
@@ -330,7 +376,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         x = fmaf((float)qf[c][e], load_act(k1, key * p.k_ts + 16 * c + 8 * h + e), x);
-            x = (x + swap_halves(x)) * p.scale2;
+            x = halves_sum(x) * p.scale2;
             if (key > lim) continue;                 // the lane's; the loop is the wave's
             const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
@@ -371,7 +417,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
 // value; the dims of a step are 8 c + i of half 0 and 8 c + 4 + i of half 1, so
 // that K is read from LDS 16 bytes at a time.
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void prompt_attn_f32_kernel(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2, DP > 128 ? 1 : 2))) void prompt_attn_f32_kernel(
     PromptParams p, int slots) {
     constexpr int NT = 64 * NW, ROWB = 4 * DP, UPR = DP / 4, KEYS = 32, TILE = KEYS * ROWB;
     constexpr int CH = KEYS * UPR / NT;
@@ -406,22 +452,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
         }
     }
     const int su = tid % UPR, sr = tid / UPR;
-    const float *kp = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + su * 4;
-    const float *vp = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + su * 4;
-    const bool in = su * 4 < p.D;
+    const bool in = su * 4 < p.D;               // past the head's dims: unit 0's, and zeros stored
+    const float *kp = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + (in ? su * 4 : 0);
+    const float *vp = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + (in ? su * 4 : 0);
+    const float *kn = kp + sr * p.k_ts, *vn = vp + sr * p.v_ts;    // this thread's first row of the next tile
     f32x4_t kr[CH], vr[CH];
     auto load = [&](int tile) __attribute__((always_inline)) {
+        if ((tile + 1) * KEYS <= Lk) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const long key = min(tile * KEYS + sr + i * (NT / UPR), Lk - 1);
-            kr[i] = vr[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (in) {
+            for (int i = 0; i < CH; ++i) {
+                kr[i] = *reinterpret_cast<const f32x4_t *>(kn + i * (NT / UPR) * p.k_ts);
+                vr[i] = *reinterpret_cast<const f32x4_t *>(vn + i * (NT / UPR) * p.v_ts);
+            }
+            kn += KEYS * p.k_ts;
+            vn += KEYS * p.v_ts;
+        } else {                                       // past the end: the last key again
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const long key = min(tile * KEYS + sr + i * (NT / UPR), Lk - 1);
                 kr[i] = *reinterpret_cast<const f32x4_t *>(kp + key * p.k_ts);
                 vr[i] = *reinterpret_cast<const f32x4_t *>(vp + key * p.v_ts);
             }
         }
     };
     auto store = [&](int tile) __attribute__((always_inline)) {
+        if (p.D < DP && !in)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) kr[i] = vr[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
@@ -437,6 +494,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
         load(0);
         store(0);
     }
+    loads_done();
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
         if (tile + 1 < tiles) load(tile + 1);
@@ -454,7 +512,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
             }
             s[0] += s[1];
             if (k0 + KEYS - 1 > lim_lo) {
-                const int rel = lim - k0 - 4 * h;
+                int rel = lim - k0 - 4 * h;
+                asm volatile("" : "+v"(rel));
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (key_of(r) > rel) s[0][r] = -INFINITY;
@@ -462,7 +521,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
             float t = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s[0][r]);
-            t = fmaxf(t, swap_halves(t)) * p.scale2;
+            t = halves_max(t) * p.scale2;
             if (__any(t > m)) {
                 const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
                 const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
@@ -492,7 +551,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
         }
         if (tile + 1 < tiles) store(tile + 1);
     }
-    l += swap_halves(l);
+    l = halves_sum(l);
     bool again = false;                              // as in prompt_attn_kernel
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -514,7 +573,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW / 4,
                 if (8 * c < p.D)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x = fmaf(qf[c][e], k1[key * p.k_ts + 8 * c + 4 * h + e], x);
-            x = (x + swap_halves(x)) * p.scale2;
+            x = halves_sum(x) * p.scale2;
             if (key > lim) continue;
             const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
@@ -630,19 +689,19 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
     p.B = num_sequences, p.Nq = num_q_tokens, p.Nk = num_kv_tokens;
     p.Hq = num_heads, p.Hkv = num_kv_heads, p.D = head_dim;
     p.causal = causal != 0, p.zero_rest = zero_rest != 0, p.scale2 = scale * kLog2e;
-    const int share = num_heads / num_kv_heads, max_hw = head_dim > 128 ? 2 : 3;   // 4 waves there
+    const int share = num_heads / num_kv_heads, max_hw = 2;   // 4 waves there
     p.hw = __builtin_ctz((unsigned)share);
     if (p.hw > max_hw) p.hw = max_hw;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == OJASX_DTYPE_F32)
-        return head_dim <= 64 ? launch32<64, 8>(p, st) : head_dim <= 128 ? launch32<128, 8>(p, st)
+        return head_dim <= 64 ? launch32<64, 4>(p, st) : head_dim <= 128 ? launch32<128, 4>(p, st)
                                                                         : launch32<256, 4>(p, st);
     if (dtype == OJASX_DTYPE_BF16)
-        return head_dim <= 64    ? launch16<Bf16, 64, 8>(p, st)
-               : head_dim <= 128 ? launch16<Bf16, 128, 8>(p, st)
+        return head_dim <= 64    ? launch16<Bf16, 64, 4>(p, st)
+               : head_dim <= 128 ? launch16<Bf16, 128, 4>(p, st)
                                  : launch16<Bf16, 256, 4>(p, st);
-    return head_dim <= 64    ? launch16<F16, 64, 8>(p, st)
-           : head_dim <= 128 ? launch16<F16, 128, 8>(p, st)
+    return head_dim <= 64    ? launch16<F16, 64, 4>(p, st)
+           : head_dim <= 128 ? launch16<F16, 128, 4>(p, st)
                              : launch16<F16, 256, 4>(p, st);
 }
 
