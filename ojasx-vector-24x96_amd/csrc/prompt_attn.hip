@@ -63,29 +63,8 @@ struct F16 {
     static __device__ __forceinline__ _Float16 from(float f) { return (_Float16)f; }
 };
 
-// The rows of a workgroup: slot t of the grid.  Sequence b takes the slots from
-// s(b) = cu[b] / BM + b + 1 (its rows need at most the next sequence's slots
-// less one), rows before the first sequence the slots from 0 and rows behind
-// the last one those from s(B).  cu is clamped to the rows there are, whatever
-// it holds.
-struct Rows {
-    int b, first, len, tile;     // sequence (-1 or B: rows of none), its rows, the tile in it
-};
+// Entry b of cumulative lengths, clamped to the n rows there are, whatever it holds.
 __device__ __forceinline__ int cu_at(const int *cu, int b, int n) { return min(max(cu[b], 0), n); }
-__device__ __forceinline__ Rows rows_of_slot(const int *cu, int B, int n, int bm_shift, int t) {
-    const int lane = threadIdx.x & 63;
-    int count = 0;
-    for (int i0 = 0; i0 <= B; i0 += 64) {
-        const int i = min(i0 + lane, B);
-        count += __popcll(__ballot(i0 + lane <= B && (cu_at(cu, i, n) >> bm_shift) + i + 1 <= t));
-    }
-    Rows r;
-    r.b = count - 1;
-    r.first = r.b < 0 ? 0 : cu_at(cu, r.b, n);
-    r.len = (r.b < B ? cu_at(cu, r.b + 1, n) : n) - r.first;
-    r.tile = t - (r.b < 0 ? 0 : (r.first >> bm_shift) + r.b + 1);
-    return r;
-}
 
 // 16-byte unit `u` of row `row` in a K tile, and 32-byte unit of a V tile: XOR
 // swizzles under which the 16 rows of a K read, and the 8 rows of a transposed V
@@ -118,18 +97,12 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70
 // The key that accumulator register r of a lane's half h stands for.
 __device__ __forceinline__ constexpr int key_of(int r) { return 8 * (r / 4) + r % 4; }
 
-// Running maximum of one query row per lane with a tile's scores s (two blocks of
-// 32 keys): rescales acc and l where the row's maximum grew by more than 2^8.
+// Running maximum (log2) of one query row per lane with a tile's largest score t:
+// rescales acc and l where the row's maximum grew by more than 2^8.
 // Weights up to 2^8 above 1 lose nothing: they are rounded relative to their
 // size and all sums are fp32.
 template <int NT>
-__device__ __forceinline__ void raise_max(const f32x16_t (&s)[2], float scale2, float &m, float &ref, float &l,
-                                          f32x16_t (&acc)[NT]) {
-    float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[1][r]);
-    float t = fmaxf(t0, t1);
-    t = halves_max(t) * scale2;
+__device__ __forceinline__ void raise_max(float t, float &m, float &ref, float &l, f32x16_t (&acc)[NT]) {
     if (__any(t > m + 8.f)) {
         const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
         const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
@@ -138,6 +111,42 @@ __device__ __forceinline__ void raise_max(const f32x16_t (&s)[2], float scale2, 
         l *= alpha;
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] *= alpha;
+    }
+}
+
+// The lane's row again, key by key, with hidden keys left out: acc, m / ref and l as
+// the tiles' passes leave them (dims 32 t + 4 h + key_of(r), and 16 c + 8 h .. of
+// the scores' halves).
+template <typename T, int DP>
+__device__ __forceinline__ void rows_again(const PromptParams &p, const T *q, const T *k, const T *v, int lim,
+                                           int lim_hi, int h, float &m, float &ref, float &l,
+                                           f32x16_t (&acc)[DP / 32]) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
+    for (int key = 0; key <= lim_hi; ++key) {
+        float x = 0.f;
+        for (int c = 8 * h; c < p.D; c += 16)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x = fmaf(load_act(q, c + e), load_act(k, key * p.k_ts + c + e), x);
+        x = halves_sum(x) * p.scale2;
+        if (key > lim) continue;                 // the lane's; the loop is the wave's
+        const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
+        const float pv = __builtin_amdgcn_exp2f(x - rn);
+        m = mn;
+        ref = rn;
+        l = fmaf(l, alpha, pv);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * t + 4 * h + key_of(r);
+                if (d < p.D) acc[t][r] = fmaf(pv, load_act(v, key * p.v_ts + d), acc[t][r] * alpha);
+            }
     }
 }
 
@@ -153,37 +162,66 @@ __device__ __forceinline__ void mask_tile(f32x16_t (&s)[2], int lim, int k0, int
 }
 }  // namespace
 
+// The rows and keys of a workgroup.
+struct PromptBlock {
+    int b, first, len, tile;     // sequence (-1 or B: rows of none), its rows, the tile in it
+    int head0, k_first, Lk;
+};
+
 // Workgroups: slots x head groups, the head group fastest: consecutive
 // workgroups go to different XCDs, so with 8 head groups (or a multiple) an XCD
 // keeps the K and V of its own heads; the last rows of the batch, the longest
 // tiles of a single causal sequence, start first.
-struct PromptBlock {
-    Rows rows;
-    int head0, k_first, Lk;
-};
+// Sequence b takes the slots from s(b) = cu[b] / BM + b + 1 (its rows need at most
+// the next sequence's slots less one), rows before the first sequence the slots
+// from 0 and rows behind the last one those from s(B).
 __device__ __forceinline__ bool prompt_block(const PromptParams &p, int slots, int bm_shift, PromptBlock &o) {
-    const int hg = p.Hq >> p.hw;
+    const int hg = p.Hq >> p.hw, lane = threadIdx.x & 63;
     const int t = slots - 1 - (int)blockIdx.x / hg;
     o.head0 = (int)blockIdx.x % hg << p.hw;
-    o.rows = rows_of_slot(p.cu_q, p.B, p.Nq, bm_shift, t);
-    const int r0 = o.rows.tile << bm_shift;
-    if (o.rows.tile < 0 || r0 >= o.rows.len) return false;
-    o.k_first = o.Lk = 0;
-    if (o.rows.b >= 0 && o.rows.b < p.B) {
-        o.k_first = cu_at(p.cu_k, o.rows.b, p.Nk);
-        o.Lk = max(cu_at(p.cu_k, o.rows.b + 1, p.Nk) - o.k_first, 0);
+    o.k_first = 0;
+    int next, k_next = 0;
+    if (p.B < 64) {              // both lists in one load each, the entries by lane
+        const int i = min(lane, p.B), cq = cu_at(p.cu_q, i, p.Nq), ck = cu_at(p.cu_k, i, p.Nk);
+        o.b = __popcll(__ballot(lane <= p.B && (cq >> bm_shift) + lane + 1 <= t)) - 1;
+        o.first = o.b < 0 ? 0 : __builtin_amdgcn_readlane(cq, max(o.b, 0));
+        next = o.b < p.B ? __builtin_amdgcn_readlane(cq, o.b + 1) : p.Nq;
+        if (o.b >= 0 && o.b < p.B) {
+            o.k_first = __builtin_amdgcn_readlane(ck, max(o.b, 0));
+            k_next = __builtin_amdgcn_readlane(ck, o.b + 1);
+        }
+    } else {
+        int count = 0;
+        for (int i0 = 0; i0 <= p.B; i0 += 64) {
+            const int i = min(i0 + lane, p.B);
+            count += __popcll(__ballot(i0 + lane <= p.B && (cu_at(p.cu_q, i, p.Nq) >> bm_shift) + i + 1 <= t));
+        }
+        o.b = count - 1;
+        o.first = o.b < 0 ? 0 : cu_at(p.cu_q, o.b, p.Nq);
+        next = o.b < p.B ? cu_at(p.cu_q, o.b + 1, p.Nq) : p.Nq;
+        if (o.b >= 0 && o.b < p.B) {
+            o.k_first = cu_at(p.cu_k, o.b, p.Nk);
+            k_next = cu_at(p.cu_k, o.b + 1, p.Nk);
+        }
+        next = __builtin_amdgcn_readfirstlane(next);
+        k_next = __builtin_amdgcn_readfirstlane(k_next);
+        o.first = __builtin_amdgcn_readfirstlane(o.first);
+        o.k_first = __builtin_amdgcn_readfirstlane(o.k_first);
     }
-    return true;
+    o.len = next - o.first;
+    o.tile = t - (o.b < 0 ? 0 : (o.first >> bm_shift) + o.b + 1);
+    o.Lk = max(k_next - o.k_first, 0);
+    return o.tile >= 0 && o.tile << bm_shift < o.len;
 }
 
 // Rows of no sequence: zeros, where the caller wants them written.
 template <typename T>
 __device__ __forceinline__ void zero_rows(const PromptParams &p, const PromptBlock &o, int bm_shift) {
     if (!p.zero_rest) return;
-    const int r0 = o.rows.tile << bm_shift, n = min(1 << bm_shift, o.rows.len - r0);
+    const int r0 = o.tile << bm_shift, n = min(1 << bm_shift, o.len - r0);
     const int heads = 1 << p.hw, per = heads * p.D;
     for (int x = threadIdx.x; x < n * per; x += blockDim.x) {
-        const size_t row = (size_t)(o.rows.first + r0 + x / per) * p.Hq + o.head0 + x % per / p.D;
+        const size_t row = (size_t)(o.first + r0 + x / per) * p.Hq + o.head0 + x % per / p.D;
         store_act(static_cast<T *>(p.out), row * p.D + x % p.D, 0.f);
         if (p.lse && x % p.D == 0) p.lse[row] = -INFINITY;
     }
@@ -204,13 +242,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
     const int bm_shift = 5 + __builtin_ctz(NW) - p.hw;
     PromptBlock o;
     if (!prompt_block(p, slots, bm_shift, o)) return;
-    if (o.rows.b < 0 || o.rows.b >= p.B) {
+    if (o.b < 0 || o.b >= p.B) {
         zero_rows<T>(p, o, bm_shift);
         return;
     }
     const int head = o.head0 + (w & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
-    const int Lq = o.rows.len, Lk = o.Lk, off = Lk - Lq;
-    const int tile0 = o.rows.tile << bm_shift;                  // the workgroup's first row
+    const int Lq = o.len, Lk = o.Lk, off = Lk - Lq;
+    const int tile0 = o.tile << bm_shift;                  // the workgroup's first row
     const int row0 = tile0 + 32 * (w >> p.hw), row = row0 + n;  // the wave's, the lane's
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;       // last key the row sees
@@ -222,7 +260,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
     // ---- this lane's query row: dims 16 c + 8 h ..
     V8 qf[DP / 16];
     {
-        const T *qp = static_cast<const T *>(p.q) + (long)(o.rows.first + qrow) * p.q_ts + head * p.q_hs;
+        const T *qp = static_cast<const T *>(p.q) + (long)(o.first + qrow) * p.q_ts + head * p.q_hs;
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) {
             u32x4_t x = {0, 0, 0, 0};
@@ -306,7 +344,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (k0 + kKeys - 1 > lim_lo) mask_tile(s, lim, k0, h);
-            raise_max(s, p.scale2, m, ref, l, acc);
+            float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[1][r]);
+            raise_max(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
             // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block),
             // rounded to the inputs' type; between the products of one 16 go the
             // exponentials and the V reads of the next.
@@ -359,42 +400,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
     for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) again |= acc[t][r] != acc[t][r];
-    if (__any(again)) {
-        m = -INFINITY;
-        l = 0.f;
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-        const T *k1 = static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs;
-        const T *v1 = static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs;
-        for (int key = 0; key <= lim_hi; ++key) {
-            float x = 0.f;
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c)
-                if (16 * c + 8 * h < p.D)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        x = fmaf((float)qf[c][e], load_act(k1, key * p.k_ts + 16 * c + 8 * h + e), x);
-            x = halves_sum(x) * p.scale2;
-            if (key > lim) continue;                 // the lane's; the loop is the wave's
-            const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
-            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
-            const float pv = __builtin_amdgcn_exp2f(x - rn);
-            m = mn;
-            ref = rn;
-            l = fmaf(l, alpha, pv);
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = 32 * t + 4 * h + key_of(r);
-                    if (d < p.D) acc[t][r] = fmaf(pv, load_act(v1, key * p.v_ts + d), acc[t][r] * alpha);
-                }
-        }
-    }
+    if (__any(again))
+        rows_again<T, DP>(p, static_cast<const T *>(p.q) + (long)(o.first + qrow) * p.q_ts + head * p.q_hs,
+                          static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs,
+                          static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs, lim, lim_hi, h, m,
+                          ref, l, acc);
     if (row >= Lq) return;
-    const size_t at = (size_t)(o.rows.first + row) * p.Hq + head;
+    const size_t at = (size_t)(o.first + row) * p.Hq + head;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T *op = static_cast<T *>(p.out) + at * p.D;
 #pragma unroll
@@ -413,27 +425,33 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
     if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// fp32: v_mfma_f32_32x32x2, exact products.  A lane's operand of a step is one
-// value; the dims of a step are 8 c + i of half 0 and 8 c + 4 + i of half 1, so
-// that K is read from LDS 16 bytes at a time.
-template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2, DP > 128 ? 1 : 2))) void prompt_attn_f32_kernel(
-    PromptParams p, int slots) {
-    constexpr int NT = 64 * NW, ROWB = 4 * DP, UPR = DP / 4, KEYS = 32, TILE = KEYS * ROWB;
-    constexpr int CH = KEYS * UPR / NT;
-    extern __shared__ __align__(16) unsigned char sm[];
+// fp32 on v_mfma_f32_32x32x16_bf16: every operand as three bf16 pieces whose sum it
+// is (v1 = bf16(v), v2 = bf16(v - v1), v3 the rest; an fp32 value's 24 bits), the
+// products of pieces i and j with i + j <= 4, six of nine; the others are below
+// 2^-25 of the term.  The first pieces' products have accumulators of their own,
+// the five smaller kinds others: no small product is added to a large sum before
+// the end (head dims past 128 have registers for one set).  Six bf16 products take 3 / 8 of the time of v_mfma_f32_32x32x2 on the
+// same operands.  K and V are split as they are staged, in [piece][key] planes; one
+// wave per SIMD, for the registers of two sets of accumulators.
+template <int DP, int BUFFERS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void prompt_attn_f32_kernel(PromptParams p,
+                                                                                                        int slots) {
+    constexpr int NW = 4, NT = 64 * NW, ROWB = 2 * DP, UPR = DP / 8, KEYS = 32, PLANE = KEYS * ROWB;
+    constexpr int CH = KEYS * UPR / NT, NT2 = DP / 32, NC = DP / 16;
+    constexpr int SETS = DP > 128 ? 1 : 2;           // of output accumulators
+    extern __shared__ __align__(16) unsigned char sm[];   // [buffer][K pieces, V pieces][32 keys]
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int bm_shift = 5 + __builtin_ctz(NW) - p.hw;
     PromptBlock o;
     if (!prompt_block(p, slots, bm_shift, o)) return;
-    if (o.rows.b < 0 || o.rows.b >= p.B) {
+    if (o.b < 0 || o.b >= p.B) {
         zero_rows<float>(p, o, bm_shift);
         return;
     }
     const int head = o.head0 + (w & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
-    const int Lq = o.rows.len, Lk = o.Lk, off = Lk - Lq;
-    const int tile0 = o.rows.tile << bm_shift;
+    const int Lq = o.len, Lk = o.Lk, off = Lk - Lq;
+    const int tile0 = o.tile << bm_shift;
     const int row0 = tile0 + 32 * (w >> p.hw), row = row0 + n;
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;
@@ -442,166 +460,179 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
     const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
     const int tiles = last < 0 ? 0 : last / KEYS + 1;
 
-    f32x4_t qf[DP / 8];                              // dims 8 c + 4 h ..
-    {
-        const float *qp = static_cast<const float *>(p.q) + (long)(o.rows.first + qrow) * p.q_ts + head * p.q_hs;
+    const float *qp = static_cast<const float *>(p.q) + (long)(o.first + qrow) * p.q_ts + head * p.q_hs;
+    bf16x8_t qf[NC][3];                              // dims 16 c + 8 h ..
 #pragma unroll
-        for (int c = 0; c < DP / 8; ++c) {
-            qf[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (8 * c < p.D) qf[c] = *reinterpret_cast<const f32x4_t *>(qp + 8 * c + 4 * h);
+    for (int c = 0; c < NC; ++c) {
+        float x[8] = {};
+        if (16 * c + 8 * h < p.D) {
+            const f32x4_t a = *reinterpret_cast<const f32x4_t *>(qp + 16 * c + 8 * h);
+            const f32x4_t b = *reinterpret_cast<const f32x4_t *>(qp + 16 * c + 8 * h + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
         }
+        split3_bf16(x, qf[c]);
     }
     const int su = tid % UPR, sr = tid / UPR;
-    const bool in = su * 4 < p.D;               // past the head's dims: unit 0's, and zeros stored
-    const float *kp = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + (in ? su * 4 : 0);
-    const float *vp = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + (in ? su * 4 : 0);
-    const float *kn = kp + sr * p.k_ts, *vn = vp + sr * p.v_ts;    // this thread's first row of the next tile
-    f32x4_t kr[CH], vr[CH];
+    const bool in = su * 8 < p.D;
+    const float *kp = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs + (in ? su * 8 : 0);
+    const float *vp = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs + (in ? su * 8 : 0);
+    f32x4_t kr[CH][2], vr[CH][2];
     auto load = [&](int tile) __attribute__((always_inline)) {
-        if ((tile + 1) * KEYS <= Lk) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                kr[i] = *reinterpret_cast<const f32x4_t *>(kn + i * (NT / UPR) * p.k_ts);
-                vr[i] = *reinterpret_cast<const f32x4_t *>(vn + i * (NT / UPR) * p.v_ts);
-            }
-            kn += KEYS * p.k_ts;
-            vn += KEYS * p.v_ts;
-        } else {                                       // past the end: the last key again
+        for (int i = 0; i < CH; ++i) {
+            const long key = min(tile * KEYS + sr + i * (NT / UPR), Lk - 1);   // past the end: the last again
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const long key = min(tile * KEYS + sr + i * (NT / UPR), Lk - 1);
-                kr[i] = *reinterpret_cast<const f32x4_t *>(kp + key * p.k_ts);
-                vr[i] = *reinterpret_cast<const f32x4_t *>(vp + key * p.v_ts);
+            for (int y = 0; y < 2; ++y) {
+                kr[i][y] = *reinterpret_cast<const f32x4_t *>(kp + key * p.k_ts + 4 * y);
+                vr[i][y] = *reinterpret_cast<const f32x4_t *>(vp + key * p.v_ts + 4 * y);
             }
         }
     };
     auto store = [&](int tile) __attribute__((always_inline)) {
-        if (p.D < DP && !in)
-#pragma unroll
-            for (int i = 0; i < CH; ++i) kr[i] = vr[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
+        unsigned char *ks = sm + (BUFFERS == 2 ? tile & 1 : 0) * 6 * PLANE, *vs = ks + 3 * PLANE;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int r = sr + i * (NT / UPR);
-            *reinterpret_cast<f32x4_t *>(ks + r * ROWB + (su ^ (r & 15)) * 16) = kr[i];
-            // rows 4 apart are read together: their 128-byte units swap
-            *reinterpret_cast<f32x4_t *>(vs + r * ROWB + (su ^ (r << 1 & 8)) * 16) = vr[i];
+            float kx[8], vx[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                kx[e] = p.D < DP && !in ? 0.f : kr[i][e / 4][e % 4];
+                vx[e] = p.D < DP && !in ? 0.f : vr[i][e / 4][e % 4];
+            }
+            bf16x8_t kb[3], vb[3];
+            split3_bf16(kx, kb);
+            split3_bf16(vx, vb);
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                *reinterpret_cast<bf16x8_t *>(ks + x * PLANE + r * ROWB + k_unit<ROWB>(r, su) * 16) = kb[x];
+                *reinterpret_cast<bf16x8_t *>(vs + x * PLANE + r * ROWB + v_unit<ROWB>(r, su >> 1) * 32 +
+                                              (su & 1) * 16) = vb[x];
+            }
         }
     };
-    f32x16_t acc[DP / 32] = {};
+    // c += the six products of a and b, the largest into c0
+    auto mma6 = [&](const bf16x8_t (&a)[3], const bf16x8_t (&b)[3], f32x16_t &c0, f32x16_t &c1)
+                    __attribute__((always_inline)) {
+        c1 = Bf16::mma(a[0], b[2], c1);
+        c1 = Bf16::mma(a[1], b[1], c1);
+        c1 = Bf16::mma(a[2], b[0], c1);
+        c1 = Bf16::mma(a[0], b[1], c1);
+        c1 = Bf16::mma(a[1], b[0], c1);
+        c0 = Bf16::mma(a[0], b[0], c0);
+    };
+    f32x16_t acc[SETS * NT2] = {};                   // [t]: first pieces; the other set: the smaller products
     float m = -INFINITY, ref = 0.f, l = 0.f;
     if (tiles) {
         load(0);
         store(0);
     }
     loads_done();
+    const int vkey = 4 * h + ((lane & 15) >> 2), vg = lane >> 4 & 1, vb8 = (lane & 3) * 8;
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
         if (tile + 1 < tiles) load(tile + 1);
         const int k0 = tile * KEYS;
         if (k0 <= lim_hi) {
-            const unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
-            f32x16_t s[2] = {};
+            const unsigned char *ks = sm + (BUFFERS == 2 ? tile & 1 : 0) * 6 * PLANE, *vs = ks + 3 * PLANE;
+            f32x16_t s0 = {}, s1 = {};
+            bf16x8_t kf[2][3];
+            auto read_k = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-            for (int c = 0; c < DP / 8; ++c) {
-                const f32x4_t x =
-                    *reinterpret_cast<const f32x4_t *>(ks + n * ROWB + ((2 * c + h) ^ (n & 15)) * 16);
+                for (int x = 0; x < 3; ++x)
+                    kf[c % 2][x] = *reinterpret_cast<const bf16x8_t *>(ks + x * PLANE + n * ROWB +
+                                                                      k_unit<ROWB>(n, 2 * c + h) * 16);
+            };
+            read_k(0);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], qf[c][i], s[i & 1], 0, 0, 0);
+            for (int c = 0; c < NC; ++c) {
+                if (c + 1 < NC) read_k(c + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                mma6(kf[c % 2], qf[c], s0, s1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            s[0] += s[1];
+            s0 += s1;
             if (k0 + KEYS - 1 > lim_lo) {
                 int rel = lim - k0 - 4 * h;
                 asm volatile("" : "+v"(rel));
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (key_of(r) > rel) s[0][r] = -INFINITY;
+                    if (key_of(r) > rel) s0[r] = -INFINITY;
             }
             float t = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) t = fmaxf(t, s[0][r]);
-            t = halves_max(t) * p.scale2;
-            if (__any(t > m)) {
-                const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
-                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
-                m = mn;
-                ref = rn;
-                l *= alpha;
+            for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
+            raise_max(halves_max(t) * p.scale2, m, ref, l, acc);
+            bf16x8_t pf[2][3];
+            auto weights = [&](int f) __attribute__((always_inline)) {
+                float x[8];
 #pragma unroll
-                for (int i = 0; i < DP / 32; ++i) acc[i] *= alpha;
-            }
-            float a = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[0][r] = __builtin_amdgcn_exp2f(fmaf(s[0][r], p.scale2, -ref));
-                a += s[0][r];
-            }
-            l += a;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int key = key_of(r) + 4 * h;
-#pragma unroll
-                for (int i = 0; i < DP / 32; ++i) {
-                    const float x = *reinterpret_cast<const float *>(
-                        vs + key * ROWB + ((8 * i + (n >> 2)) ^ (key << 1 & 8)) * 16 + (n & 3) * 4);
-                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[0][r], acc[i], 0, 0, 0);
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(s0[8 * f + e], p.scale2, -ref));
+                    l += x[e];
                 }
+                split3_bf16(x, pf[f]);
+            };
+            s16x4_t vf[2][3][2];
+            auto read_v = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int r = 16 * (i / NT2) + 8 * y + vkey, t2 = i % NT2;
+                        auto *at = (__attribute__((address_space(3))) s16x4_t *)(
+                            vs + x * PLANE + r * ROWB + v_unit<ROWB>(r, 2 * t2 + vg) * 32 + vb8);
+                        vf[i % 2][x][y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+                    }
+            };
+            read_v(0);
+            __builtin_amdgcn_sched_barrier(0);
+            weights(0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 2 * NT2; ++i) {
+                if (i + 1 < 2 * NT2) read_v(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                bf16x8_t z[3];
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+                    z[x] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vf[i % 2][x][0], vf[i % 2][x][1], 0, 1, 2,
+                                                                               3, 4, 5, 6, 7));
+                mma6(z, pf[i / NT2], acc[i % NT2], acc[(SETS - 1) * NT2 + i % NT2]);
+                if (i == 0) weights(1);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        if (BUFFERS == 1) __syncthreads();
         if (tile + 1 < tiles) store(tile + 1);
     }
     l = halves_sum(l);
+    f32x16_t sum[NT2];
     bool again = false;                              // as in prompt_attn_kernel
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+    for (int t = 0; t < NT2; ++t) {
+        sum[t] = acc[t];
+        if (SETS == 2) sum[t] += acc[(SETS - 1) * NT2 + t];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) again |= acc[t][r] != acc[t][r];
-    if (__any(again)) {
-        m = -INFINITY;
-        l = 0.f;
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-        const float *k1 = static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs;
-        const float *v1 = static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs;
-        for (int key = 0; key <= lim_hi; ++key) {
-            float x = 0.f;
-#pragma unroll
-            for (int c = 0; c < DP / 8; ++c)
-                if (8 * c < p.D)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x = fmaf(qf[c][e], k1[key * p.k_ts + 8 * c + 4 * h + e], x);
-            x = halves_sum(x) * p.scale2;
-            if (key > lim) continue;
-            const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
-            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
-            const float pv = __builtin_amdgcn_exp2f(x - rn);
-            m = mn;
-            ref = rn;
-            l = fmaf(l, alpha, pv);
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = 32 * t + 4 * h + key_of(r);
-                    if (d < p.D) acc[t][r] = fmaf(pv, v1[key * p.v_ts + d], acc[t][r] * alpha);
-                }
-        }
+        for (int r = 0; r < 16; ++r) again |= sum[t][r] != sum[t][r];
     }
+    if (__any(again))
+        rows_again<float, DP>(p, qp, static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs,
+                              static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs, lim, lim_hi, h,
+                              m, ref, l, sum);
     if (row >= Lq) return;
-    const size_t at = (size_t)(o.rows.first + row) * p.Hq + head;
+    const size_t at = (size_t)(o.first + row) * p.Hq + head;
     float *op = static_cast<float *>(p.out) + at * p.D;
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+    for (int t = 0; t < NT2; ++t)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const int d = 32 * t + 8 * x + 4 * h;
             if (d < p.D) {
                 f32x4_t y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = l == 0.f ? 0.f : acc[t][4 * x + e] / l;
+                for (int e = 0; e < 4; ++e) y[e] = l == 0.f ? 0.f : sum[t][4 * x + e] / l;
                 *reinterpret_cast<f32x4_t *>(op + d) = y;
             }
         }
@@ -628,10 +659,10 @@ int launch16(const PromptParams &p, hipStream_t st) {
     static size_t granted = 0;
     return launch(&prompt_attn_kernel<E, DP, NW>, p, NW, (size_t)4 * kKeys * 2 * DP, &granted, st);
 }
-template <int DP, int NW>
+template <int DP, int BUFFERS>
 int launch32(const PromptParams &p, hipStream_t st) {
     static size_t granted = 0;
-    return launch(&prompt_attn_f32_kernel<DP, NW>, p, NW, (size_t)4 * 32 * 4 * DP, &granted, st);
+    return launch(&prompt_attn_f32_kernel<DP, BUFFERS>, p, 4, (size_t)BUFFERS * 6 * 32 * 2 * DP, &granted, st);
 }
 
 bool rows16(const void *p, long ts, long hs, size_t es) {
@@ -694,8 +725,8 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
     if (p.hw > max_hw) p.hw = max_hw;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == OJASX_DTYPE_F32)
-        return head_dim <= 64 ? launch32<64, 4>(p, st) : head_dim <= 128 ? launch32<128, 4>(p, st)
-                                                                        : launch32<256, 4>(p, st);
+        return head_dim <= 64 ? launch32<64, 2>(p, st) : head_dim <= 128 ? launch32<128, 2>(p, st)
+                                                                        : launch32<256, 1>(p, st);
     if (dtype == OJASX_DTYPE_BF16)
         return head_dim <= 64    ? launch16<Bf16, 64, 4>(p, st)
                : head_dim <= 128 ? launch16<Bf16, 128, 4>(p, st)
