@@ -84,17 +84,35 @@ __device__ __forceinline__ long kv4_block(const Kv4View &c, int b, int t, int se
     return ((((long)page * c.Hkv + h) << c.pshift) + (t & ((1 << c.pshift) - 1))) >> 4;
 }
 
-// The sequence that row n of a packed batch belongs to: the last b with
-// cu[b] <= n (cu has B + 1 entries), -1 or B where it is none.  The whole wave
-// calls it with one n.
-__device__ __forceinline__ int packed_sequence(const int *cu, int B, int n) {
+// Where row n of a packed batch lies: its sequence b (-1: of none), the token's
+// position and the tokens of the sequence after the batch.  Sequence b owns rows
+// cu[b] .. cu[b + 1] - 1 at positions start[b] ..; without cu row n is sequence
+// n's one token.  Whole waves call it with one n.
+struct Kv4Row {
+    int b, pos, seen;
+};
+__device__ __forceinline__ Kv4Row kv4_row(const int *cu, const int *start, int B, int n) {
+    if (!cu) {
+        const int s = start[n];
+        return {n, s, s + 1};
+    }
     const int lane = threadIdx.x & 63;
+    if (B < 64) {                // both lists in one load each, the entries by lane
+        const int c = cu[min(lane, B)], s = start[min(lane, B - 1)];
+        const int b = __popcll(__ballot(lane <= B && c <= n)) - 1;
+        if (b < 0 || b >= B) return {-1, 0, 0};
+        const int first = __builtin_amdgcn_readlane(c, b), s0 = __builtin_amdgcn_readlane(s, b);
+        return {b, s0 + (n - first), s0 + (__builtin_amdgcn_readlane(c, b + 1) - first)};
+    }
     int count = 0;
     for (int i0 = 0; i0 <= B; i0 += 64) {
         const int i = i0 + lane;
         count += __popcll(__ballot(i <= B && cu[min(i, B)] <= n));
     }
-    return count - 1;
+    const int b = count - 1;
+    if (b < 0 || b >= B) return {-1, 0, 0};
+    const int first = cu[b], s0 = start[b];
+    return {b, s0 + (n - first), s0 + (cu[b + 1] - first)};
 }
 
 }  // namespace ojx

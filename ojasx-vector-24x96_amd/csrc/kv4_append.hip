@@ -24,7 +24,7 @@ struct Kv4AppendParams {
     long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;    // token and head strides, elements
     void *q_out, *k_out;                        // contiguous [n][heads][D]
     const int *start, *cu;
-    int n, Hq;
+    int n, Hq, parts;
 };
 
 __device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
@@ -68,6 +68,15 @@ __device__ __forceinline__ _Float16 to_half(float f) {
     return (_Float16)f;
 }
 
+// fp32 of x / 15: the product with the double nearest 1 / 15, corrected by its
+// remainder, is the quotient to a double's last place (a full fp64 division
+// takes three times the instructions).
+__device__ __forceinline__ float div15(double x) {
+    constexpr double r = 1.0 / 15.0;
+    const double q = x * r;
+    return (float)fma(fma(-15.0, q, x), r, q);
+}
+
 // Encodes a lane's eight dimensions of a K (V) row into block `blk`, slot t.
 // unit: which eight of the row's D / 8.
 template <int D, int GS>
@@ -82,31 +91,38 @@ __device__ __forceinline__ void encode_unit(const float (&x)[8], bool value, int
     }
     group_stats<GS / 8>(mn, mx, poison);
     const _Float16 lo = to_half(fminf(fmaxf(mn, -65504.f), 65504.f) + poison);
-    const float step = (float)(((double)mx - (double)(float)lo) / 15.0);
+    const float step = div15((double)mx - (double)(float)lo);
     // lo may have been rounded above max: no step below 0
     const _Float16 s = to_half(fminf(fmaxf(step, 0.f), 65504.f) + poison);
     const float lo32 = (float)lo, s32 = (float)s, inv = s32 > 0.f ? 1.0f / s32 : 0.f;
-    int code[8];
+    // An fp32 quotient is off by less than 2^-18: only beside a half can it round
+    // another way than the exact one, whose remainder decides there.
+    float near[8];
+    bool beside = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float f = (x[i] - lo32) * inv;
-        float r = rintf(f);
-        // f is off by less than 2^-18: only beside a half can the fp32 quotient
-        // round another way than the exact one, whose remainder decides there
-        if (fabsf(f - r) > 0.4999f && s32 > 0.f) {
-            const double e = fma(-(double)r, (double)s32, (double)x[i] - (double)lo32);
-            const double half = 0.5 * (double)s32;
-            const bool odd = ((int)r & 1) != 0;
-            if (e > half || (e == half && odd)) r += 1.f;
-            else if (e < -half || (e == -half && odd)) r -= 1.f;
-        }
-        code[i] = (int)fminf(fmaxf(r, 0.f), 15.f);   // NaN: 0
+        near[i] = rintf(f);
+        beside |= fabsf(f - near[i]) > 0.4999f;
     }
+    if (beside && s32 > 0.f) {
+        const double half = 0.5 * (double)s32;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double e = fma(-(double)near[i], (double)s32, (double)x[i] - (double)lo32);
+            const bool odd = fabsf(near[i]) < 16.f && ((int)near[i] & 1) != 0;
+            if (e > half || (e == half && odd)) near[i] += 1.f;
+            else if (e < -half || (e == -half && odd)) near[i] -= 1.f;
+        }
+    }
+    uint32_t code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = (uint32_t)fminf(fmaxf(near[i], 0.f), 15.f);   // NaN: 0
     if (blk < 0) return;
     if (!value) {
         uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= (uint32_t)code[2 * i] << (4 * i) | (uint32_t)code[2 * i + 1] << (16 + 4 * i);
+        for (int i = 0; i < 4; ++i) w |= code[2 * i] << (4 * i) | code[2 * i + 1] << (16 + 4 * i);
         const int word = (unit & 3) * (D / 32) + (unit >> 2);
         reinterpret_cast<uint32_t *>(codes + blk * (D * 8) + t * (D / 2))[word] = w;
     } else {
@@ -121,84 +137,85 @@ __device__ __forceinline__ void encode_unit(const float (&x)[8], bool value, int
 }
 }  // namespace
 
-// A workgroup takes one token (blockIdx.x); its threads each eight dimensions
-// of a query, key or value row at a time.
+// Waves: wave i of the launch takes token i / parts and every parts-th 64 units of
+// eight dimensions of its query, key and value rows.  It computes the token's
+// angles itself (a lane per pair), so waves need no barrier.  64 units are whole
+// rows: a lane's dimensions are the same in all of them, and its eight angles stay
+// in registers (read from LDS for every unit they cost more than the rest).
+// kAtOnce units' loads are in flight together.
+constexpr int kAtOnce = 3;
+
 template <typename T, int D, int GS>
 __global__ __launch_bounds__(kNT) void kv4_append_kernel(Kv4AppendParams p) {
-    __shared__ double2 cs[D / 2];               // cos and sin of the token's angles
-    const int tid = threadIdx.x, n = blockIdx.x;
-    constexpr int UPR = D / 8;                  // units of eight per row
-    int b = n, pos, seen;
-    if (p.cu) {
-        b = packed_sequence(p.cu, p.c.B, n);
-        const bool none = b < 0 || b >= p.c.B;  // a row of no sequence
-        const int bb = none ? 0 : b;
-        const int first = p.cu[bb], s0 = p.start[bb];
-        pos = s0 + (n - first);
-        seen = s0 + (p.cu[bb + 1] - first);
-        if (none) b = -1;
-    } else {
-        pos = p.start[b];
-        seen = pos + 1;
+    __shared__ double2 angles[kNT / 64][D / 2];  // cos and sin of the token's angles
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int UPR = D / 8, RPW = 64 / UPR;   // units of eight per row, rows per 64 units
+    const int wave = blockIdx.x * (kNT / 64) + w, n = wave / p.parts, part = wave - n * p.parts;
+    if (n >= p.n) return;
+    const int Hkv = p.c.Hkv, rows = p.Hq + 2 * Hkv, step = p.parts * RPW;
+    const int half = p.c.rot >> 1, d0 = lane % UPR * 8, unit = lane % UPR;
+    const bool turns = d0 < p.c.rot, low = d0 < half;
+    const int other = !turns || p.c.interleaved ? 0 : low ? half : -half;   // where the values lie they turn with
+    const Kv4Row r = kv4_row(p.cu, p.start, p.c.B, n);
+    // the token's block of kv head 0; head h's is h pages of blocks further
+    const long blk0 = r.b < 0 ? -1 : kv4_block(p.c, r.b, r.pos, r.seen, 0);
+    double2 *cs = angles[w];
+    for (int i = lane; i < half; i += 64) {
+        const double f = p.c.turns[i], t = (double)r.pos * f;
+        const double frac = (t - rint(t)) + fma((double)r.pos, f, -t);
+        double sn, co;
+        sincospi(2.0 * frac, &sn, &co);
+        cs[i] = make_double2(co, sn);
     }
-    const int half = p.c.rot >> 1;
-    if (b >= 0) {
-        for (int i = tid; i < half; i += kNT) {
-            const double f = p.c.turns[i], t = (double)pos * f;
-            const double frac = (t - rint(t)) + fma((double)pos, f, -t);
-            double s, c;
-            sincospi(2.0 * frac, &s, &c);
-            cs[i] = make_double2(c, s);
-        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    double co[8], sn[8];                         // x_e <- x_e co + (its other) sn
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int i = p.c.interleaved ? (d0 + e) / 2 : low ? d0 + e : d0 - half + e;
+        const double2 a = turns ? cs[i] : make_double2(1.0, 0.0);
+        co[e] = a.x;
+        sn[e] = (p.c.interleaved ? e % 2 == 0 : low) ? -a.y : a.y;
     }
-    __syncthreads();
-    const int Hkv = p.c.Hkv, units = (p.Hq + 2 * Hkv) * UPR;
-    const int t = pos & 15;
-    for (int u0 = blockIdx.y * kNT; u0 < units; u0 += gridDim.y * kNT) {
-        const int u = u0 + tid;
-        if (u >= units) break;
-        const int row = u / UPR, unit = u % UPR;
-        const bool isq = row < p.Hq, isv = row >= p.Hq + Hkv;
-        const int head = isq ? row : isv ? row - p.Hq - Hkv : row - p.Hq;
-        const T *src = isq ? static_cast<const T *>(p.q) + n * p.q_ts + head * p.q_hs
-                     : isv ? static_cast<const T *>(p.v) + n * p.v_ts + head * p.v_hs
-                           : static_cast<const T *>(p.k) + n * p.k_ts + head * p.k_hs;
-        const int d0 = unit * 8;
-        float x[8];
-        T *out = isq ? static_cast<T *>(p.q_out) : isv ? nullptr : static_cast<T *>(p.k_out);
-        if (out) out += ((size_t)n * (isq ? p.Hq : Hkv) + head) * D + d0;
-        if (b < 0) {
+    for (int row0 = part * RPW + lane / UPR; row0 - lane / UPR < rows; row0 += kAtOnce * step) {
+        float x[kAtOnce][8], y[kAtOnce][8];
+        // past the last row: row 0's values, not used
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = 0.f;
-            if (out) store8(out, x);
-            continue;
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int row = row0 + i * step < rows ? row0 + i * step : 0;
+            const bool isq = row < p.Hq, isv = row >= p.Hq + Hkv;
+            const T *src = d0 + (isq ? static_cast<const T *>(p.q) + n * p.q_ts + row * p.q_hs
+                                 : isv ? static_cast<const T *>(p.v) + n * p.v_ts + (row - p.Hq - Hkv) * p.v_hs
+                                       : static_cast<const T *>(p.k) + n * p.k_ts + (row - p.Hq) * p.k_hs);
+            load8(src, x[i]);
+            load8(src + other, y[i]);
         }
-        load8(src + d0, x);
-        if (!isv && d0 < p.c.rot) {
-            if (p.c.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const double2 r = cs[d0 / 2 + i];
-                    const double a = x[2 * i], c = x[2 * i + 1];
-                    x[2 * i] = (float)(a * r.x - c * r.y);
-                    x[2 * i + 1] = (float)(c * r.x + a * r.y);
-                }
-            } else {
-                const bool low = d0 < half;
-                float y[8];
-                load8(src + (low ? d0 + half : d0 - half), y);
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int row = row0 + i * step;
+            if (row >= rows) continue;
+            const bool isq = row < p.Hq, isv = row >= p.Hq + Hkv;
+            const int head = isq ? row : isv ? row - p.Hq - Hkv : row - p.Hq;
+            T *out = isq ? static_cast<T *>(p.q_out) : isv ? nullptr : static_cast<T *>(p.k_out);
+            if (out) out += ((size_t)n * (isq ? p.Hq : Hkv) + head) * D + d0;
+            if (r.b < 0) {                           // a row of no sequence
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const double2 r = cs[(low ? d0 : d0 - half) + i];
-                    const double a = x[i], c = y[i];
-                    x[i] = (float)(low ? a * r.x - c * r.y : a * r.x + c * r.y);
-                }
+                for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+                if (out) store8(out, x[i]);
+                continue;
             }
-        }
-        if (out) store8(out, x);
-        if (!isq) {
-            const long blk = kv4_block(p.c, b, pos, seen, head);
-            encode_unit<D, GS>(x, isv, unit, blk, t, isv ? p.c.vc : p.c.kc, isv ? p.c.vs : p.c.ks);
+            if (turns && !isv) {
+                if (p.c.interleaved)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[i][e] = x[i][e ^ 1];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = (float)fma((double)x[i][e], co[e], (double)y[i][e] * sn[e]);
+            }
+            if (out) store8(out, x[i]);
+            if (!isq) {
+                const long blk = blk0 < 0 ? -1 : blk0 + ((long)head << (p.c.pshift - 4));
+                encode_unit<D, GS>(x[i], isv, unit, blk, r.pos & 15, isv ? p.c.vc : p.c.kc, isv ? p.c.vs : p.c.ks);
+            }
         }
     }
 }
@@ -207,59 +224,48 @@ struct Kv4ReadParams {
     Kv4View c;
     const int *start, *cu, *seen;
     void *k_out, *v_out;        // contiguous [n][Hkv][D]
-    int n;
+    int n, parts;
 };
 
-// The appended tokens' values: workgroup = token, thread = eight dimensions of
-// a K or V row at a time.
+// The appended tokens' values: waves as in kv4_append_kernel.
 template <typename T, int D, int GS>
 __global__ __launch_bounds__(kNT) void kv4_read_kernel(Kv4ReadParams p) {
-    const int tid = threadIdx.x, n = blockIdx.x;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     constexpr int UPR = D / 8;
-    int b = n, pos, seen;
-    if (p.cu) {
-        b = packed_sequence(p.cu, p.c.B, n);
-        const bool none = b < 0 || b >= p.c.B;
-        const int bb = none ? 0 : b;
-        const int first = p.cu[bb], s0 = p.start[bb];
-        pos = s0 + (n - first);
-        seen = s0 + (p.cu[bb + 1] - first);
-        if (none) b = -1;
-    } else {
-        pos = p.start[b];
-        seen = pos + 1;
-    }
-    if (p.seen && b >= 0) seen = p.seen[b];
-    const int Hkv = p.c.Hkv, units = 2 * Hkv * UPR, t = pos & 15;
-    for (int u0 = blockIdx.y * kNT; u0 < units; u0 += gridDim.y * kNT) {
-        const int u = u0 + tid;
-        if (u >= units) break;
+    const int wave = blockIdx.x * (kNT / 64) + w, n = wave / p.parts, part = wave - n * p.parts;
+    if (n >= p.n) return;
+    Kv4Row r = kv4_row(p.cu, p.start, p.c.B, n);
+    if (p.seen && r.b >= 0) r.seen = p.seen[r.b];
+    const int Hkv = p.c.Hkv, units = 2 * Hkv * UPR, t = r.pos & 15;
+    // the token's block of kv head 0; head h's is h pages of blocks further
+    const long blk0 = r.b < 0 || r.pos >= r.seen ? -1 : kv4_block(p.c, r.b, r.pos, r.seen, 0);
+    for (int u = part * 64 + lane; u < units; u += p.parts * 64) {
         const int row = u / UPR, unit = u % UPR;
         const bool isv = row >= Hkv;
         const int head = isv ? row - Hkv : row;
-        const long blk = b < 0 || pos >= seen ? -1 : kv4_block(p.c, b, pos, seen, head);
+        const long blk = blk0 + ((long)head << (p.c.pshift - 4));
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        if (blk >= 0) {
+        if (blk0 >= 0) {
             const __half2 st = (isv ? p.c.vs : p.c.ks)[(blk * (D / GS) + unit / (GS / 8)) * 16 + t];
             const float s = __low2float(st), lo = __high2float(st);
             if (!isv) {
                 const int word = (unit & 3) * (D / 32) + (unit >> 2);
-                const uint32_t w =
+                const uint32_t c =
                     reinterpret_cast<const uint32_t *>(p.c.kc + blk * (D * 8) + t * (D / 2))[word];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[2 * i] = fmaf(s, (float)(w >> (4 * i) & 15u), lo);
-                    x[2 * i + 1] = fmaf(s, (float)(w >> (16 + 4 * i) & 15u), lo);
+                    x[2 * i] = fmaf(s, (float)(c >> (4 * i) & 15u), lo);
+                    x[2 * i + 1] = fmaf(s, (float)(c >> (16 + 4 * i) & 15u), lo);
                 }
             } else {
                 const uint8_t *src = p.c.vc + blk * (D * 8) + unit * 64 + t;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t w = src[16 * i];
-                    x[2 * i] = fmaf(s, (float)(w & 15u), lo);
-                    x[2 * i + 1] = fmaf(s, (float)(w >> 4), lo);
+                    const uint32_t c = src[16 * i];
+                    x[2 * i] = fmaf(s, (float)(c & 15u), lo);
+                    x[2 * i + 1] = fmaf(s, (float)(c >> 4), lo);
                 }
             }
         }
@@ -321,10 +327,13 @@ int kv4_view(const OjasxKV4Cache *c, Kv4View *v) {
 }
 
 namespace {
-// Workgroups per token: one for each kNT units while the tokens are fewer than
-// the card's CUs, else one that takes the token's units in turn and computes
-// its angles once.
-int row_split(int n, long units) { return n < 256 ? (int)((units + kNT - 1) / kNT) : 1; }
+// Waves per token: one for each 64 units while the launch is small, one in all from
+// 4096 tokens (16 waves a CU).
+int wave_parts(int n, long units) {
+    const long most = (units + 63) / 64, want = 4096 / n;
+    return (int)(want < 1 ? 1 : want < most ? want : most);
+}
+unsigned wave_groups(int n, int parts) { return (unsigned)(((long)n * parts + kNT / 64 - 1) / (kNT / 64)); }
 
 // The (element type, head_dim, group_size) instances of a kernel.
 #define OJX_KV4_DISPATCH(KERNEL, T, D, GS, ...)                                               \
@@ -394,7 +403,8 @@ OJASX_API int ojasx_kv4_append_device(const OjasxKV4Cache *cache, const void *q,
     p.n = num_tokens, p.Hq = num_q_heads;
     const int D = cache->head_dim, GS = cache->group_size;
     const long units = ((long)num_q_heads + 2L * cache->num_kv_heads) * (D / 8);
-    const dim3 grid(num_tokens, row_split(num_tokens, units));
+    p.parts = wave_parts(num_tokens, units);
+    const dim3 grid(wave_groups(num_tokens, p.parts));
     hipStream_t st = static_cast<hipStream_t>(stream);
     OJX_KV4_DISPATCH_T(kv4_append_kernel, dtype, D, GS, grid, dim3(kNT), 0, st, p);
     OJX_HIP(hipGetLastError());
@@ -424,7 +434,8 @@ OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start
     }
     p.start = start, p.cu = cu_seqlens, p.seen = seen, p.k_out = k_out, p.v_out = v_out, p.n = num_tokens;
     const int D = cache->head_dim, GS = cache->group_size;
-    const dim3 grid(num_tokens, row_split(num_tokens, 2L * cache->num_kv_heads * (D / 8)));
+    p.parts = wave_parts(num_tokens, 2L * cache->num_kv_heads * (D / 8));
+    const dim3 grid(wave_groups(num_tokens, p.parts));
     hipStream_t st = static_cast<hipStream_t>(stream);
     OJX_KV4_DISPATCH_T(kv4_read_kernel, dtype, D, GS, grid, dim3(kNT), 0, st, p);
     OJX_HIP(hipGetLastError());

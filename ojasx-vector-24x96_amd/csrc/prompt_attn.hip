@@ -27,6 +27,13 @@ namespace ojx {
 
 namespace {
 constexpr int kKeys = 64;                        // keys per tile
+// Workgroups up to which half as many rows go to each and the keys of a tile to two
+// waves: as many as are resident at once (three, two or one to a CU by head dim).
+// Below it the longest rows' way through their keys sets the time (1500 tokens of
+// 8 / 2 heads of 128: 98 workgroups, 35.0 -> 26.8 us; 3000 of 16 of 64: 416, 43.9 ->
+// 36.0), above it the splits' own cost (2048 tokens of 32 / 8 heads of 128: 536, 54.4
+// -> 57.7; 4096 of 16 / 2 of 256: 524, 190 -> 284).
+constexpr long split_below(int DP) { return 256 * (DP <= 64 ? 3 : DP <= 128 ? 2 : 1); }
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -151,13 +158,14 @@ __device__ __forceinline__ void rows_again(const PromptParams &p, const T *q, co
 }
 
 // Hides the keys past `lim` from the lane's row; k0 = the tile's first key.
-__device__ __forceinline__ void mask_tile(f32x16_t (&s)[2], int lim, int k0, int h) {
+template <int NB>
+__device__ __forceinline__ void mask_tile(f32x16_t (&s)[NB], int lim, int k0, int h) {
     int rel = lim - k0 - 4 * h;
     asm volatile("" : "+v"(rel));                // keeps the selects behind the wave's branch
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         if (key_of(r) > rel) s[0][r] = -INFINITY;
-        if (32 + key_of(r) > rel) s[1][r] = -INFINITY;
+        if (NB > 1 && 32 + key_of(r) > rel) s[NB - 1][r] = -INFINITY;
     }
 }
 }  // namespace
@@ -228,28 +236,33 @@ __device__ __forceinline__ void zero_rows(const PromptParams &p, const PromptBlo
 }
 
 // bf16 and fp16: v_mfma_f32_32x32x16, head dims up to DP (the dims past D are
-// zeros in Q and K).
-template <typename E, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : 2, DP > 128 ? 1 : 2))) void prompt_attn_kernel(
+// zeros in Q and K).  KS = 2: half the waves take the first 32 keys of every tile,
+// the other half the last 32, and the pairs join their sums in LDS: twice the
+// workgroups with half the work in a row, for grids too small to hide how long
+// their longest rows take.
+template <typename E, int DP, int KS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : DP > 64 ? 2 : 3))) void prompt_attn_kernel(
     PromptParams p, int slots) {
     typedef typename E::T T;
     typedef typename E::V8 V8;
+    constexpr int NW = 4, WR = NW / KS, NB = 2 / KS;  // waves of different rows, 32-key blocks of a wave
     constexpr int NT = 64 * NW, ROWB = 2 * DP, UPR = DP / 8, TILE = kKeys * ROWB;
     constexpr int CH = kKeys * UPR / NT;             // 16-byte units of a tile per thread
     extern __shared__ __align__(16) unsigned char sm[];   // [2 buffers][K tile, V tile]
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
-    const int bm_shift = 5 + __builtin_ctz(NW) - p.hw;
+    const int wr = w % WR, kb = KS == 1 ? 0 : 32 * (w / WR);    // the wave's keys begin at kb
+    const int bm_shift = 5 + __builtin_ctz(WR) - p.hw;
     PromptBlock o;
     if (!prompt_block(p, slots, bm_shift, o)) return;
     if (o.b < 0 || o.b >= p.B) {
         zero_rows<T>(p, o, bm_shift);
         return;
     }
-    const int head = o.head0 + (w & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
+    const int head = o.head0 + (wr & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
     const int Lq = o.len, Lk = o.Lk, off = Lk - Lq;
     const int tile0 = o.tile << bm_shift;                  // the workgroup's first row
-    const int row0 = tile0 + 32 * (w >> p.hw), row = row0 + n;  // the wave's, the lane's
+    const int row0 = tile0 + 32 * (wr >> p.hw), row = row0 + n;  // the wave's, the lane's
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;       // last key the row sees
     const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;    // the wave's least,
@@ -316,19 +329,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
     const int vkey = 4 * h + ((lane & 15) >> 2), vg = lane >> 4 & 1, vb = (lane & 3) * 8;
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
-        if (tile + 1 < tiles) load(tile + 1);
-        const int k0 = tile * kKeys;
+        load(tile + 1);                              // past the end: the last key's rows again
+        const int k0 = tile * kKeys + kb;
         if (k0 <= lim_hi) {
             const unsigned char *ks = sm + (tile & 1) * 2 * TILE, *vs = ks + TILE;
-            f32x16_t s[2] = {};
+            f32x16_t s[NB] = {};
             // operands are read two steps before the products that take them; the
             // barriers keep the compiler from moving the reads back to their use
             constexpr int NC = DP / 16;
-            u32x4_t kf[3][2];
+            u32x4_t kf[3][NB];
             auto read_k = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int r = 32 * b + n;
+                for (int b = 0; b < NB; ++b) {
+                    const int r = kb + 32 * b + n;
                     kf[c % 3][b] = *reinterpret_cast<const u32x4_t *>(ks + r * ROWB + k_unit<ROWB>(r, 2 * c + h) * 16);
                 }
             };
@@ -340,19 +353,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
                 if (c + 2 < NC) read_k(c + 2);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) s[b] = E::mma(__builtin_bit_cast(V8, kf[c % 3][b]), qf[c], s[b]);
+                for (int b = 0; b < NB; ++b) s[b] = E::mma(__builtin_bit_cast(V8, kf[c % 3][b]), qf[c], s[b]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (k0 + kKeys - 1 > lim_lo) mask_tile(s, lim, k0, h);
+            if (k0 + 32 * NB - 1 > lim_lo) mask_tile(s, lim, k0, h);
             float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[1][r]);
+            for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[NB - 1][r]);
             raise_max(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
             // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block),
             // rounded to the inputs' type; between the products of one 16 go the
             // exponentials and the V reads of the next.
             constexpr int NT2 = DP / 32, VB = NT2 < 4 ? NT2 : 4, PART = 8 / NT2;
-            V8 pf[4];
+            V8 pf[2 * NB];
             auto weight = [&](int f, int e) __attribute__((always_inline)) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[f >> 1][8 * (f & 1) + e], p.scale2, -ref));
                 l += x;
@@ -363,7 +376,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
             auto read_v = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    const int r = 16 * (i / NT2) + 8 * y + vkey, t = i % NT2;
+                    const int r = kb + 16 * (i / NT2) + 8 * y + vkey, t = i % NT2;
                     auto *at = (__attribute__((address_space(3))) s16x4_t *)(vs + r * ROWB +
                                                                           v_unit<ROWB>(r, 2 * t + vg) * 32 + vb);
                     vf[i % (2 * VB)][y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
@@ -376,14 +389,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
             for (int e = 0; e < 8; ++e) weight(0, e);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 4 * NT2; ++i) {
+            for (int i = 0; i < 2 * NB * NT2; ++i) {
                 const int f = i / NT2, t = i % NT2;
-                if (i + VB < 4 * NT2) read_v(i + VB);
+                if (i + VB < 2 * NB * NT2) read_v(i + VB);
                 __builtin_amdgcn_sched_barrier(0);
                 typedef short s16x8_t __attribute__((ext_vector_type(8)));
                 const s16x8_t z = __builtin_shufflevector(vf[i % (2 * VB)][0], vf[i % (2 * VB)][1], 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[t] = E::mma(__builtin_bit_cast(V8, z), pf[f], acc[t]);
-                if (f < 3)
+                if (f < 2 * NB - 1)
 #pragma unroll
                     for (int e = 0; e < PART; ++e) weight(f + 1, t * PART + e);
                 __builtin_amdgcn_sched_barrier(0);
@@ -392,6 +405,32 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP > 12
         if (tile + 1 < tiles) store(tile + 1);
     }
     l = halves_sum(l);
+    if (KS == 2) {
+        // [row wave][acc registers, m, l][lane]
+        constexpr int REGS = DP / 2 + 2;
+        float *pair = reinterpret_cast<float *>(sm) + wr * REGS * 64 + lane;
+        __syncthreads();
+        if (kb) {
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) pair[(16 * t + r) * 64] = acc[t][r];
+            pair[(REGS - 2) * 64] = m;
+            pair[(REGS - 1) * 64] = l;
+        }
+        __syncthreads();
+        if (kb) return;
+        const float m1 = pair[(REGS - 2) * 64], mn = fmaxf(m, m1);
+        ref = mn == -INFINITY ? 0.f : mn;
+        const float a0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - ref);
+        const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - ref);
+        m = mn;
+        l = fmaf(a0, l, a1 * pair[(REGS - 1) * 64]);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][r] = fmaf(a0, acc[t][r], a1 * pair[(16 * t + r) * 64]);
+    }
     // A weight of 0 times an infinity or a NaN is a NaN in the matrix product: an
     // output that is NaN may come from a key its row does not see.  Where the
     // wave has one, its rows run again, key by key, with hidden keys left out.
@@ -640,24 +679,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 }
 
 namespace {
+// Workgroups of a call whose wr waves (of different rows) take 1 << hw heads.
+long slots_of(const PromptParams &p, int wr, int hw) {
+    return (long)(p.Nq >> (5 + __builtin_ctz((unsigned)wr) - hw)) + p.B + 2;
+}
+int heads_shift(const PromptParams &p, int wr) {
+    const int share = __builtin_ctz((unsigned)(p.Hq / p.Hkv)), most = __builtin_ctz((unsigned)wr);
+    return share < most ? share : most;
+}
 template <typename K>
-int launch(K kernel, const PromptParams &p, int nw, size_t lds, size_t *granted, hipStream_t st) {
+int launch(K kernel, PromptParams p, int wr, size_t lds, size_t *granted, hipStream_t st) {
     const int rc = ensure_dyn_lds(reinterpret_cast<const void *>(kernel), lds, granted);
     if (rc) return rc;
-    const int bm_shift = 5 + __builtin_ctz((unsigned)nw) - p.hw;
-    const long slots = (long)(p.Nq >> bm_shift) + p.B + 2, groups = slots * (p.Hq >> p.hw);
+    p.hw = heads_shift(p, wr);
+    const long slots = slots_of(p, wr, p.hw), groups = slots * (p.Hq >> p.hw);
     if (groups > 0x7fffffffL) {
         set_error("prompt attention: %ld workgroups", groups);
         return OJASX_ERR_INVALID;
     }
-    OJX_LAUNCH(kernel, dim3((unsigned)groups), dim3(64 * nw), lds, st, p, (int)slots);
+    OJX_LAUNCH(kernel, dim3((unsigned)groups), dim3(256), lds, st, p, (int)slots);
     OJX_HIP(hipGetLastError());
     return OJASX_OK;
 }
-template <typename E, int DP, int NW>
+template <typename E, int DP>
 int launch16(const PromptParams &p, hipStream_t st) {
-    static size_t granted = 0;
-    return launch(&prompt_attn_kernel<E, DP, NW>, p, NW, (size_t)4 * kKeys * 2 * DP, &granted, st);
+    static size_t granted[2] = {0, 0};
+    const int hw = heads_shift(p, 4);
+    const size_t lds = (size_t)4 * kKeys * 2 * DP;
+    if (slots_of(p, 4, hw) * (p.Hq >> hw) > split_below(DP))
+        return launch(&prompt_attn_kernel<E, DP, 1>, p, 4, lds, &granted[0], st);
+    return launch(&prompt_attn_kernel<E, DP, 2>, p, 2, lds, &granted[1], st);
 }
 template <int DP, int BUFFERS>
 int launch32(const PromptParams &p, hipStream_t st) {
@@ -720,20 +771,17 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
     p.B = num_sequences, p.Nq = num_q_tokens, p.Nk = num_kv_tokens;
     p.Hq = num_heads, p.Hkv = num_kv_heads, p.D = head_dim;
     p.causal = causal != 0, p.zero_rest = zero_rest != 0, p.scale2 = scale * kLog2e;
-    const int share = num_heads / num_kv_heads, max_hw = 2;   // 4 waves there
-    p.hw = __builtin_ctz((unsigned)share);
-    if (p.hw > max_hw) p.hw = max_hw;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == OJASX_DTYPE_F32)
         return head_dim <= 64 ? launch32<64, 2>(p, st) : head_dim <= 128 ? launch32<128, 2>(p, st)
                                                                         : launch32<256, 1>(p, st);
     if (dtype == OJASX_DTYPE_BF16)
-        return head_dim <= 64    ? launch16<Bf16, 64, 4>(p, st)
-               : head_dim <= 128 ? launch16<Bf16, 128, 4>(p, st)
-                                 : launch16<Bf16, 256, 4>(p, st);
-    return head_dim <= 64    ? launch16<F16, 64, 4>(p, st)
-           : head_dim <= 128 ? launch16<F16, 128, 4>(p, st)
-                             : launch16<F16, 256, 4>(p, st);
+        return head_dim <= 64    ? launch16<Bf16, 64>(p, st)
+               : head_dim <= 128 ? launch16<Bf16, 128>(p, st)
+                                 : launch16<Bf16, 256>(p, st);
+    return head_dim <= 64    ? launch16<F16, 64>(p, st)
+           : head_dim <= 128 ? launch16<F16, 128>(p, st)
+                             : launch16<F16, 256>(p, st);
 }
 
 }  // extern "C"
