@@ -3,9 +3,9 @@
 //
 // Of a token's K or V row of one kv head (D values, fp32), each group of GS
 // consecutive dimensions is held as lo = fp16(min), s = fp16(fp32((max - lo) /
-// 15)), at least 0, and codes c_d = clamp(round_half_even((x_d - lo) / s), 0, 15), for the
-// values lo + s c_d.  s = 0 holds codes 0.  lo and s saturate at +-65504; a
-// group with an infinity or a NaN holds s = lo = NaN.
+// 15)), at least 0, and codes c_d = clamp(round_half_even((x_d - lo) / s), 0,
+// 15), for the values lo + s c_d.  s = 0 holds codes 0.  lo and s saturate at
+// +-65504; a group with an infinity or a NaN holds s = lo = NaN.
 //
 // A block is 16 slots of a page; block b of a page and kv head holds
 //   K codes  [16 slots][D / 2 bytes]: a row is 4-byte words, word h (D / 32) +

@@ -14,10 +14,20 @@
 // sums are a query row's, a lane's own: one exchange between the halves per
 // tile.
 //
-// A workgroup's waves take HW query heads of one kv head (the largest power of
-// two up to 8 that divides the heads per kv head) by 8 / HW blocks of 32 rows:
-// K and V are staged once for all of them, and the causal diagonal cuts through
-// 32 (8 / HW) rows instead of 256.
+// A workgroup's four waves (two pairs where a tile's keys are split) take HW query
+// heads of one kv head, the largest power of two up to four (two) that divides the
+// heads per kv head, by 4 / HW (2 / HW) blocks of 32 rows: K and V are staged once
+// for all of them, and with four heads the causal diagonal cuts through 32 rows
+// instead of 128.
+//
+// Bound by the matrix instructions where rows are long, and by exponentials with
+// narrow heads: a score costs 4 D operations there and one exp2 at a quarter of the
+// vector rate, about as long as its products at D = 64.  Measured, one pass, causal,
+// 32 / 8 heads of 128 but where said: 16384 bf16 tokens of one sequence 2.16 ms, 1015
+// TFLOP/s (a large bf16 matrix product of the library runs at 1200 here); 8192 of
+// eight 0.12 ms; 4999 fp16 tokens of five sequences, 16 heads of 64, 30 us; 2048 fp32
+// of two 157 us, 116 TFLOP/s where the library's fp32 product has 153; 150 of three
+// 7.4 us, of which a launch with nothing to do is half.
 #include <cmath>
 #include <type_traits>
 
@@ -219,7 +229,7 @@ __device__ __forceinline__ bool prompt_block(const PromptParams &p, int slots, i
     o.len = next - o.first;
     o.tile = t - (o.b < 0 ? 0 : (o.first >> bm_shift) + o.b + 1);
     o.Lk = max(k_next - o.k_first, 0);
-    return o.tile >= 0 && o.tile << bm_shift < o.len;
+    return o.tile >= 0 && (long)o.tile << bm_shift < o.len;   // whatever cu holds
 }
 
 // Rows of no sequence: zeros, where the caller wants them written.
@@ -361,9 +371,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
 #pragma unroll
             for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[NB - 1][r]);
             raise_max(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
-            // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block),
-            // rounded to the inputs' type; between the products of one 16 go the
-            // exponentials and the V reads of the next.
+            // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block);
+            // between the products of one 16 go the exponentials and the V reads of
+            // the next.  They are rounded to the inputs' type, relative to their size
+            // and each by itself, as the output is once more: over many keys the errors
+            // average out.  Their sum is of the unrounded ones, in fp32.
             constexpr int NT2 = DP / 32, VB = NT2 < 4 ? NT2 : 4, PART = 8 / NT2;
             V8 pf[2 * NB];
             auto weight = [&](int f, int e) __attribute__((always_inline)) {
@@ -469,9 +481,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
 // products of pieces i and j with i + j <= 4, six of nine; the others are below
 // 2^-25 of the term.  The first pieces' products have accumulators of their own,
 // the five smaller kinds others: no small product is added to a large sum before
-// the end (head dims past 128 have registers for one set).  Six bf16 products take 3 / 8 of the time of v_mfma_f32_32x32x2 on the
-// same operands.  K and V are split as they are staged, in [piece][key] planes; one
-// wave per SIMD, for the registers of two sets of accumulators.
+// the end (head dims past 128 have registers for one set).  Six bf16 products take
+// 3 / 8 of the time of v_mfma_f32_32x32x2 on the same operands: 2048 tokens of two
+// sequences, 32 / 8 heads of 128, 328 -> 157 us.  K and V are split as they are
+// staged, in [piece][key] planes; one wave per SIMD, for the registers of two sets
+// of accumulators.
 template <int DP, int BUFFERS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void prompt_attn_f32_kernel(PromptParams p,
                                                                                                         int slots) {
@@ -693,8 +707,9 @@ int launch(K kernel, PromptParams p, int wr, size_t lds, size_t *granted, hipStr
     if (rc) return rc;
     p.hw = heads_shift(p, wr);
     const long slots = slots_of(p, wr, p.hw), groups = slots * (p.Hq >> p.hw);
-    if (groups > 0x7fffffffL) {
-        set_error("prompt attention: %ld workgroups", groups);
+    if (groups > 0xffffffL) {                        // a grid has fewer than 2^32 threads
+        set_error("prompt attention: %d tokens of %d sequences and %d heads need %ld workgroups (at most 2^24 - 1)",
+                  p.Nq, p.B, p.Hq, groups);
         return OJASX_ERR_INVALID;
     }
     OJX_LAUNCH(kernel, dim3((unsigned)groups), dim3(256), lds, st, p, (int)slots);
@@ -739,8 +754,10 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
         set_error("unsupported dtype %d", dtype);
         return OJASX_ERR_INVALID;
     }
-    if (num_q_tokens < 0 || num_kv_tokens < 0 || num_heads <= 0 || num_heads > 65535 || num_kv_heads <= 0 ||
-        num_heads % num_kv_heads || num_sequences <= 0 || num_sequences > (1 << 24)) {
+    constexpr int most = 0x7fffffff - 1024;          // row numbers of tiles that end past them are ints
+    if (num_q_tokens < 0 || num_kv_tokens < 0 || num_q_tokens > most || num_kv_tokens > most || num_heads <= 0 ||
+        num_heads > 65535 || num_kv_heads <= 0 || num_heads % num_kv_heads || num_sequences <= 0 ||
+        num_sequences > (1 << 24)) {
         set_error("prompt attention: %d query and %d key tokens of %d sequences, %d query and %d kv heads",
                   num_q_tokens, num_kv_tokens, num_sequences, num_heads, num_kv_heads);
         return OJASX_ERR_INVALID;

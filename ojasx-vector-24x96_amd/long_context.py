@@ -799,15 +799,20 @@ class PagedInt4KVCache:
             table = torch.arange(self.num_pages, dtype=torch.int32, device=dev)
         else:
             table = torch.full((num_sequences * max_resident_pages,), -1, dtype=torch.int32, device=dev)
-        self.block_table = table.view(num_sequences, max_resident_pages)
+        self._block_table = table.view(num_sequences, max_resident_pages)
         self._turns = turns
         self._c = _lib.KV4Cache(_vp(self.k_codes), _vp(self.v_codes), _vp(self.k_steps),
-                                _vp(self.v_steps), _vp(self.block_table),
+                                _vp(self.v_steps), _vp(table),
                                 _vp(turns) if turns is not None else None, num_sequences,
                                 max_resident_pages, sink_pages, page_size, self.num_pages,
                                 num_kv_heads, head_dim, group_size, rotary_dim, int(self.interleaved))
         self._ref = ctypes.addressof(self._c)
         self._workspace_bytes = {}       # (query heads, max_seen) -> bytes
+
+    @property
+    def block_table(self):
+        """The table itself: the kernels read this tensor, so it is filled in, never replaced."""
+        return self._block_table
 
     @property
     def capacity(self) -> int:
@@ -909,7 +914,8 @@ class PagedInt4KVCache:
         float16), over the resident ones of the ``seen[b]`` tokens (int32
         [num_sequences], the current one included) of each sequence; q head j
         reads kv head j // (num_q_heads // num_kv_heads).  ``scale_factor <= 0``
-        means 1/sqrt(head_dim); a sequence without tokens gives 0.
+        means 1/sqrt(head_dim); a sequence without tokens gives 0.  ``out`` may be
+        the query itself.
         ``max_seen``, a bound on ``seen`` where the caller knows one, keeps the
         launch of short sequences as small as they are."""
         torch = _torch()
@@ -986,7 +992,9 @@ class PackedPromptAttention:
 
         Returns the output [N, num_heads, head_dim] in the query's dtype, or
         (output, lse float32 [N, num_heads]) with ``return_lse``.  Rows of no
-        sequence are 0 (lse -inf); in a given ``out`` they stay as they are."""
+        sequence are 0 (lse -inf); in a given ``out`` they stay as they are.
+        ``out`` may be the query itself, and shares no memory with the keys and
+        values."""
         torch = _torch()
         what = "PackedPromptAttention"
         tag = _inference_tag(what, query, key, value)

@@ -473,3 +473,25 @@ def test_offsets_past_32_bits(lc, dev):
     assert np.array_equal(f64(rk), hk.astype(np.float32)) and np.array_equal(f64(rv), hv.astype(np.float32))
     q = rand(dev, "bfloat16", 1, 4, 256, seed=3)
     check_decode(c.decode(q, i32(dev, [100])), q, hk, hv, [100], 2, "bfloat16", 1 / 16, 128)
+
+
+def test_block_table_is_filled_in_not_replaced(lc, dev):
+    import torch
+    c = lc.PagedInt4KVCache(1, 64, max_resident_pages=4, group_size=64, num_pages=4, device=dev)
+    with pytest.raises(AttributeError):
+        c.block_table = torch.zeros(1, 4, dtype=torch.int32, device=dev)
+
+
+def test_decode_into_the_query(lc, dev):
+    """out may be the query: a long sequence, cut into runs, and short ones, written whole."""
+    import torch
+    g = torch.Generator(device=dev).manual_seed(3)
+    c = lc.PagedInt4KVCache(2, 128, num_sequences=3, max_resident_pages=64, device=dev)
+    n = [1000, 3, 0]
+    cu = i32(dev, [0, 1000, 1003, 1003])
+    k, v = (torch.randn(1003, 2, 128, generator=g, device=dev) for _ in range(2))
+    c.append(k, v, i32(dev, [0, 0, 0]), cu)
+    for dtype in (torch.float32, torch.bfloat16):
+        q = torch.randn(3, 16, 128, generator=g, device=dev).to(dtype)
+        want = c.decode(q, i32(dev, n))
+        assert c.decode(q, i32(dev, n), out=q) is q and torch.equal(q, want)

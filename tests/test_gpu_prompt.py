@@ -313,3 +313,15 @@ def test_serving_path(lc, dev, dtype):
                     V = np.abs(hist[b][1][keep, h // 4]).max()
                     tol = V * (2 ** -12 + 1e-5 if dtype == "bfloat16" else 1e-5) + eps_half(dtype) * np.abs(want[0])
                     assert (np.abs(got[b, h] - want[0]) <= tol).all(), (b, h)
+
+
+@pytest.mark.parametrize("name", ["float32", "bfloat16"])
+def test_out_is_the_query(lc, dev, name):
+    import torch
+    dtype = getattr(torch, name)
+    g = torch.Generator(device=dev).manual_seed(4)
+    cu = torch.tensor([0, 70, 70, 301], dtype=torch.int32, device=dev)
+    q, k, v = (torch.randn(301, h, 64, generator=g, device=dev).to(dtype) for h in (4, 2, 2))
+    a = lc.PackedPromptAttention(4, 2, 64)
+    want = a(q, k, v, cu)
+    assert a(q, k, v, cu, out=q) is q and torch.equal(q, want)

@@ -137,3 +137,18 @@ def test_prompt_attention_refusals(pkg):
     assert call(q=None) == -1 and call(k=None) == -1 and call(cu=None) == -1 and call(ck=None) == -1
     assert call(out=None) == -1 and call(nq=0, q=None) == 0
     assert L.ojasx_get_last_error()
+
+
+def test_launches_past_the_grid_are_refused(pkg):
+    """More tokens than a grid of fewer than 2^32 threads, or than row numbers of 32 bits, take."""
+    L, c = pkg.lib(), cache(pkg)
+    ref = ctypes.addressof(c)
+    for n in ((1 << 25) + 1, 0x7fffffff):
+        assert L.ojasx_kv4_append_device(ref, None, 0, 0, 0, None, FAKE, 256, 128, None, FAKE, 256, 128, n, 0,
+                                         FAKE, FAKE, None) == -3
+        assert L.ojasx_kv4_read_device(ref, FAKE, FAKE, None, n, FAKE, FAKE, 0, None) == -3
+    prompt = lambda nq, nk, H, B: L.ojasx_prompt_attention_device(  # noqa: E731
+        FAKE, 64, 8, FAKE, 64, 8, FAKE, 64, 8, 0, nq, nk, H, H, 8, FAKE, FAKE, B, 1, 0.5, 0, FAKE, None, None)
+    assert prompt(0x7fffffff, 1, 1, 1) == -3 and prompt(1, 0x7fffffff, 1, 1) == -3
+    assert prompt(1 << 26, 1, 64, 1) == -3          # 2^19 blocks of rows by 64 heads: 2^25 workgroups
+    assert prompt(1, 1, 8, 1 << 22) == -3           # every sequence has a workgroup for each head
