@@ -10,14 +10,18 @@
 // each as large as lo, about two standard deviations of V, and their sum, an
 // average over many tokens, much smaller: what fp32 rounds off them would show.
 // Keys for bf16 outputs keep 0 .. 15 and lo: the scores are exact enough.)
-// A column of the products is a (query head j,
-// group g) pair: column j G + g of the score product holds q_j with every
-// group but g zeroed, so one accumulator gives all groups' partial sums, each
-// lane applies the steps of its own group only, and a sum over the G
-// neighbouring lanes completes the score.  The weights p_t s_tg of that column
-// are the B operand of the value product, whose rows are all the dimensions;
-// the rows of the column's own group are kept.  16 / G query heads of a kv head
-// share a workgroup's pass over the cache.
+//
+// A column of the products is a (query head j, group g) pair: column j G + g of
+// the score product holds q_j with every group but g zeroed, so one accumulator
+// gives all groups' partial sums, each lane applies the steps of its own group
+// only, and a sum over the G neighbouring lanes completes the score.  The weights
+// p_t s_tg of that column are the B operand of the value product, whose rows are
+// all the dimensions; the rows of the column's own group are kept.  16 / G query
+// heads of a kv head share a workgroup's pass over the cache.  Where a kv head has
+// no more than a quarter of them, its columns come C = 4 times, and copy c has the
+// weights of slots 4 c .. 4 c + 3 of each block, the others' being 0: a quarter of
+// the exponentials and steps for every lane.  The copies are joined as the waves
+// are, each with its own maximum and sum.
 //
 // Tokens go in tiles of 64 = 4 blocks of 16 slots.  Row rho of the score
 // product's A operand in step i is slot 4 i + rho % 4 of block rho / 4, so a
@@ -39,6 +43,12 @@
 // sequences' lengths.  A workgroup goes through the sequences of its run; a
 // sequence that lies in one run is written whole, of the others each run leaves
 // (out, max, sum) in slot run + sequence, and kv4_merge_kernel joins them.
+//
+// Bound by the reading of the pages: 131072 bf16 tokens, 32 / 8 heads of 128, groups
+// of 64, 32 us for 151 MB, 4.6 TB/s (a copy runs at 4.9 here); 64 sequences of 192000
+// tokens in all, groups of 32, 56 us for 246 MB, 4.4 TB/s; with narrow heads by a
+// wave's way through its tiles: 16 sequences of 32000 held fp16 tokens, 16 heads of 64,
+// 15 us for 38 MB.  The merge is a second launch, 4 to 5 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -54,7 +64,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kMostRange = 0x1p40f;              // takes the smallest fp16 step to 2^16
 
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
 
 struct Kv4DecodeParams {
     Kv4View c;
@@ -208,9 +220,11 @@ __device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[NW]) 
 }
 }  // namespace
 
-template <typename T_, int D, int GS>
-__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, 8))) void kv4_decode_kernel(Kv4DecodeParams p) {
+template <typename T_, int D, int GS, int C>
+__global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 1 : 2, 8))) void kv4_decode_kernel(
+    Kv4DecodeParams p) {
     constexpr int G = D / GS, HS = 16 / G, NJ = D / 32;
+    constexpr int HE = HS / C, NI = 4 / C;                           // heads of a slice, slot groups of a copy
     constexpr int QP = sizeof(T_) == 4 ? 2 : 1;                     // fp16 pieces of a query value
     constexpr int WP = std::is_same<T_, __hip_bfloat16>::value ? 1 : 2;   // and of a weight
     constexpr bool KMID = WP > 1;             // keys: codes 0 .. 15 do for bf16 outputs
@@ -218,9 +232,10 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     __shared__ float sm[kNW][HS][2];                                 // and (max, sum)
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, h = lane >> 4, j = n / G, g = n % G;
-    const int slices = (p.R + HS - 1) / HS;
-    const int kvh = blockIdx.y / slices, j0 = blockIdx.y % slices * HS;
-    const int nj = min(HS, p.R - j0), head0 = kvh * p.R + j0;
+    const int slices = (p.R + HE - 1) / HE;
+    const int kvh = blockIdx.y / slices, j0 = blockIdx.y % slices * HE;
+    const int jh = j % HE, cp = j / HE;
+    const int nj = min(HE, p.R - j0), head0 = kvh * p.R + j0;
     const int bps = p.c.pshift - 4;                                  // log2 of blocks per page
     // ---- this workgroup's run of tiles, and the sequence that it begins in
     int pos, end, b, first;                                          // first: number of b's first tile
@@ -272,12 +287,12 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     float qsum = 0.f, kq;
     {
         float x[NJ][8], mx = 0.f;
-        const T_ *qr = static_cast<const T_ *>(p.q) + ((size_t)b * p.Hq + head0 + min(j, nj - 1)) * D;
+        const T_ *qr = static_cast<const T_ *>(p.q) + ((size_t)b * p.Hq + head0 + min(jh, nj - 1)) * D;
 #pragma unroll
         for (int jj = 0; jj < NJ; ++jj) load8(qr + 32 * jj + 8 * h, x[jj]);
 #pragma unroll
         for (int jj = 0; jj < NJ; ++jj) {
-            const bool mine = jj * 32 / GS == g && j < nj;
+            const bool mine = jj * 32 / GS == g && jh < nj;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (!mine) x[jj][e] = 0.f;
@@ -326,14 +341,14 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     };
     // K rows (of block n / 4) and steps (of block h) of the tile that locate() found.
     uint32_t kw[4][NJ];
-    u4_t ksr[4];
+    u4_t ksr[NI];
     auto load_k = [&]() __attribute__((always_inline)) {
         const uint8_t *kp = p.c.kc + (long)pick(blk, n >> 2) * (D * 8) + (n & 3) * (D / 2) + h * NJ * 4;
-        const u4_t *ksp = reinterpret_cast<const u4_t *>(p.c.ks) + ((long)pick(blk, h) * G + g) * 4;
+        const u4_t *ksp = reinterpret_cast<const u4_t *>(p.c.ks) + ((long)pick(blk, h) * G + g) * 4 + cp * NI;
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_words<NJ>(kp + 4 * i * (D / 2), kw[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ksr[i] = ksp[i];
+        for (int i = 0; i < NI; ++i) ksr[i] = ksp[i];
     };
     // A tile's V is loaded while its scores are computed, the next tile's K while
     // the weights are: both in flight without registers of their own.
@@ -345,25 +360,25 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     }
     for (int tile = t0 + w; tile < t1; tile += kNW) {
         uint32_t vw[NJ][4];
-        u4_t vsr[4];
+        u4_t vsr[NI];
         const long vblk = pick(blk, h);
-        const u4_t *vsp = reinterpret_cast<const u4_t *>(p.c.vs) + (vblk * G + g) * 4;
+        const u4_t *vsp = reinterpret_cast<const u4_t *>(p.c.vs) + (vblk * G + g) * 4 + cp * NI;
         const uint8_t *vp = p.c.vc + vblk * (D * 8) + n * 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vsr[i] = vsp[i];
+        for (int i = 0; i < NI; ++i) vsr[i] = vsp[i];
 #pragma unroll
         for (int i = 0; i < NJ; ++i) load_words<4>(vp + i * 256, vw[i]);
         const bool whole = held[0] + held[1] + held[2] + held[3] == 64;
-        const int mine = pick(held, h);
+        const int mine = pick(held, h) - 4 * NI * cp;     // of this copy's slots
         if (!whole) {           // what a slot without a token holds reaches nothing
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (4 * i + r >= mine) ksr[i][r] = 0, vsr[i][r] = 0;
         }
-        // ---- scores of the 16 tokens of block h, for this lane's column
-        float sc[4][4], tmax = -INFINITY;
+        // ---- scores of the copy's tokens of block h, for this lane's column
+        float sc[NI][4], tmax = -INFINITY;
         h2_t smax = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -377,9 +392,14 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
                 a = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[0][jj], a, 0, 0, 0);
             }
 #pragma unroll
+            for (int r = 0; r < 4; ++r) sc[i % NI][r] = i < NI || i / NI == cp ? a[r] : sc[i % NI][r];
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+#pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const h2_t st = as_h2(ksr[i][r]);
-                float v = group_sum<G>(fmaf(base<KMID>(st), qsum, (float)st[0] * a[r]));
+                float v = group_sum<G>(fmaf(base<KMID>(st), qsum, (float)st[0] * sc[i][r]));
                 if (!whole && 4 * i + r >= mine) v = -INFINITY;
                 sc[i][r] = v;
                 tmax = fmaxf(tmax, v);
@@ -419,32 +439,43 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
             for (int i = 0; i < NJ; ++i) part[i][0] = part[i][1] = f4_t{0.f, 0.f, 0.f, 0.f};
         }
         // ---- weights and the value product
+        h4_t wt[WP][NI];
+        auto weigh = [&](int i) __attribute__((always_inline)) {
+            float wv[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const h2_t st = as_h2(vsr[i][r]);
+                const float pv = __builtin_amdgcn_exp2f(fmaf(sc[i][r], kq, shift));
+                l += pv;
+                z = fmaf(pv, base<true>(st), z);
+                wv[r] = pv * (WP == 1 ? (float)st[0] : (float)st[0] * f);
+                // rounded to fp32 here: the pieces below are of one value (the
+                // compiler rounds the product to fp16 at once for one of them)
+                if (WP > 1) asm volatile("" : "+v"(wv[r]));
+            }
+            // token order of a mask with 0x000f000f: 0, 2, then 1, 3
+            constexpr int order[4] = {0, 2, 1, 3};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const _Float16 a = (_Float16)wv[order[e]];
+                wt[0][i][e] = a;
+                if (WP > 1) wt[WP - 1][i][e] = (_Float16)(wv[order[e]] - (float)a);
+            }
+        };
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             h8_t wf[WP];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                float wv[4];
+            for (int y = 0; y < 2; ++y)
+                if (2 * u + y < NI) weigh(2 * u + y);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 2 * u + y;
-                    const h2_t st = as_h2(vsr[i][r]);
-                    const float pv = __builtin_amdgcn_exp2f(fmaf(sc[i][r], kq, shift));
-                    l += pv;
-                    z = fmaf(pv, base<true>(st), z);
-                    wv[r] = pv * (WP == 1 ? (float)st[0] : (float)st[0] * f);
-                    // rounded to fp32 here: the pieces below are of one value (the
-                    // compiler rounds the product to fp16 at once for one of them)
-                    if (WP > 1) asm volatile("" : "+v"(wv[r]));
-                }
-                // token order of a mask with 0x000f000f: 0, 2, then 1, 3
-                constexpr int order[4] = {0, 2, 1, 3};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const _Float16 a = (_Float16)wv[order[e]];
-                    wf[0][4 * y + e] = a;
-                    if (WP > 1) wf[WP - 1][4 * y + e] = (_Float16)(wv[order[e]] - (float)a);
-                }
+            for (int x = 0; x < WP; ++x) {
+                const int i = 2 * u;                 // slots of other copies: no weight
+                const u32x2_t none = {0, 0};
+                const u32x2_t a = __builtin_bit_cast(u32x2_t, wt[x][i % NI]);
+                const u32x2_t c = __builtin_bit_cast(u32x2_t, wt[x][(i + 1) % NI]);
+                const u32x2_t ma = C == 1 || i / NI == cp ? a : none, mc = C == 1 || (i + 1) / NI == cp ? c : none;
+                wf[x] = __builtin_bit_cast(h8_t, u4_t{ma[0], ma[1], mc[0], mc[1]});
             }
 #pragma unroll
             for (int i = 0; i < NJ; ++i) {
@@ -474,7 +505,7 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     z = quarters_sum(z);
 
     // ---- the waves' passes joined
-    if (j < nj) {
+    if (jh < nj) {
         const float inv = 1.f / f;
 #pragma unroll
         for (int i = 0; i < NJ; ++i)
@@ -483,7 +514,8 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        so[w][j][32 * i + 2 * (4 * h + r) + e] = WP == 1 ? (acc[i][e][r] + z) * inv : fmaf(acc[i][e][r], inv, z);
+                        so[w][j][32 * i + 2 * (4 * h + r) + e] =
+                            WP == 1 ? (acc[i][e][r] + z) * inv : fmaf(acc[i][e][r], inv, z);
         if (g == 0 && h == 0) sm[w][j][0] = m, sm[w][j][1] = WP == 1 ? l * inv : l;
     }
     __syncthreads();
@@ -491,14 +523,15 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         const int jj = x / D, d = x % D;
         float mm = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kNW; ++k) mm = fmaxf(mm, sm[k][jj][0]);
+        for (int k = 0; k < kNW * C; ++k) mm = fmaxf(mm, sm[k / C][k % C * HE + jj][0]);
         const float ref = mm == -INFINITY ? 0.f : mm;
         float o = 0.f, ll = 0.f;
 #pragma unroll
-        for (int k = 0; k < kNW; ++k) {
-            const float a = __builtin_amdgcn_exp2f(sm[k][jj][0] - ref);
-            o = fmaf(a, so[k][jj][d], o);
-            ll = fmaf(a, sm[k][jj][1], ll);
+        for (int k = 0; k < kNW * C; ++k) {
+            const int col = k % C * HE + jj;
+            const float a = __builtin_amdgcn_exp2f(sm[k / C][col][0] - ref);
+            o = fmaf(a, so[k / C][col][d], o);
+            ll = fmaf(a, sm[k / C][col][1], ll);
         }
         if (whole_sequence) {
             store_act(static_cast<T_ *>(p.out), ((size_t)b * p.Hq + head0 + jj) * D + d, ll == 0.f ? 0.f : o / ll);
@@ -599,13 +632,18 @@ __global__ __launch_bounds__(kNT) void kv4_merge_kernel(Kv4DecodeParams p) {
 }
 
 namespace {
-int decode_heads_per_slice(int D, int GS) { return 16 / (D / GS); }
+// Copies of the columns, kernel us with one and with four: 64 sequences of 3000 bf16
+// tokens, 16 / 16 heads of 64 (G = 1) 68.6, 52.7; 32 / 8 of 64 (G = 1) 35.5, 28.5; 16 /
+// 8 of 128 (G = 2) 45.1, 40.5; one sequence of 500 5.5 to 7.1 either way.  With more
+// heads than a quarter of the columns four copies would pass over the cache twice.
+int decode_copies(int R, int D, int GS) { return 4 * R <= 16 / (D / GS) ? 4 : 1; }
+int decode_heads_per_slice(int R, int D, int GS) { return 16 / (D / GS) / decode_copies(R, D, GS); }
 
-// Runs W: two workgroups per CU over the whole call (what the registers of the
-// main kernel leave room for), no more than there can be tiles.
+// Runs W: two workgroups per CU over the whole call, no more than there can be tiles.
+// A call of 64 sequences of 192000 bf16 tokens in all, 32 / 8 heads of 128, with one,
+// two, three and four: 77, 65, 71 and 73 us; 131072 of one sequence 42, 38, 42, 44.
 int decode_runs(const OjasxKV4Cache *c, int Hq, int max_seen) {
-    const int HS = decode_heads_per_slice(c->head_dim, c->group_size);
-    const int R = Hq / c->num_kv_heads;
+    const int R = Hq / c->num_kv_heads, HS = decode_heads_per_slice(R, c->head_dim, c->group_size);
     const long groups = (long)c->num_kv_heads * ((R + HS - 1) / HS);
     const long cap = (long)c->max_pages * c->page_size;
     const long slots = max_seen > 0 ? std::min((long)max_seen, cap) : cap;
@@ -625,16 +663,24 @@ int decode_check(const OjasxKV4Cache *c, int Hq) {
 
 template <typename T>
 int launch_decode(const Kv4DecodeParams &p, int D, int GS, hipStream_t st) {
-    const int HS = decode_heads_per_slice(D, GS);
+    const int HS = decode_heads_per_slice(p.R, D, GS);
     const dim3 grid(p.W, p.c.Hkv * ((p.R + HS - 1) / HS));
-    if (D == 64 && GS == 32) OJX_LAUNCH((kv4_decode_kernel<T, 64, 32>), grid, dim3(kNT), 0, st, p);
-    else if (D == 64) OJX_LAUNCH((kv4_decode_kernel<T, 64, 64>), grid, dim3(kNT), 0, st, p);
-    else if (D == 128 && GS == 32) OJX_LAUNCH((kv4_decode_kernel<T, 128, 32>), grid, dim3(kNT), 0, st, p);
-    else if (D == 128 && GS == 64) OJX_LAUNCH((kv4_decode_kernel<T, 128, 64>), grid, dim3(kNT), 0, st, p);
-    else if (D == 128) OJX_LAUNCH((kv4_decode_kernel<T, 128, 128>), grid, dim3(kNT), 0, st, p);
-    else if (GS == 32) OJX_LAUNCH((kv4_decode_kernel<T, 256, 32>), grid, dim3(kNT), 0, st, p);
-    else if (GS == 64) OJX_LAUNCH((kv4_decode_kernel<T, 256, 64>), grid, dim3(kNT), 0, st, p);
-    else OJX_LAUNCH((kv4_decode_kernel<T, 256, 128>), grid, dim3(kNT), 0, st, p);
+    const bool copies = decode_copies(p.R, D, GS) > 1;
+#define OJX_KV4_DECODE(D_, GS_)                                                                            \
+    if (D == D_ && GS == GS_) {                                                                            \
+        if constexpr (D_ / GS_ <= 4)                                                                       \
+            if (copies) OJX_LAUNCH((kv4_decode_kernel<T, D_, GS_, 4>), grid, dim3(kNT), 0, st, p);         \
+        if (!copies) OJX_LAUNCH((kv4_decode_kernel<T, D_, GS_, 1>), grid, dim3(kNT), 0, st, p);            \
+    }
+    OJX_KV4_DECODE(64, 32)
+    OJX_KV4_DECODE(64, 64)
+    OJX_KV4_DECODE(128, 32)
+    OJX_KV4_DECODE(128, 64)
+    OJX_KV4_DECODE(128, 128)
+    OJX_KV4_DECODE(256, 32)
+    OJX_KV4_DECODE(256, 64)
+    OJX_KV4_DECODE(256, 128)
+#undef OJX_KV4_DECODE
     const dim3 rows(p.Hq, p.c.B);
     if (D == 64) OJX_LAUNCH((kv4_merge_kernel<T, 64>), rows, dim3(kNT), 0, st, p);
     else if (D == 128) OJX_LAUNCH((kv4_merge_kernel<T, 128>), rows, dim3(kNT), 0, st, p);

@@ -495,3 +495,24 @@ def test_decode_into_the_query(lc, dev):
         q = torch.randn(3, 16, 128, generator=g, device=dev).to(dtype)
         want = c.decode(q, i32(dev, n))
         assert c.decode(q, i32(dev, n), out=q) is q and torch.equal(q, want)
+
+
+FEW = [  # as DECODE: no more heads per kv head than a quarter of the columns
+    (128, 32, "float32", 16, 3, 1, [0, 1, 3, 4, 5, 11, 12, 13, 16, 17, 63, 64, 65, 700], 64),
+    (128, 64, "bfloat16", 32, 2, 2, [1, 4, 6, 900, 0, 31], 64),
+    (128, 128, "float16", 16, 1, 3, [1030, 7], 128),
+    (64, 32, "bfloat16", 16, 2, 1, [2, 500, 66], 64),
+    (64, 64, "float32", 64, 2, 4, [1, 8, 129, 0], 16),
+    (64, 64, "bfloat16", 16, 16, 1, [1300, 5, 9, 14], 128),
+    (256, 64, "bfloat16", 16, 2, 1, [10, 333], 64),
+    (256, 128, "float32", 16, 1, 2, [3, 260], 64),
+]
+
+
+@pytest.mark.parametrize("case", FEW, ids=lambda c: f"d{c[0]}g{c[1]}{c[2]}x{c[5]}")
+def test_decode_few_heads(lc, dev, case):
+    D, group, dtype, page, Hkv, share, lengths, pages = case
+    c, q, hk, hv = decode_case(lc, dev, *case)
+    seen = i32(dev, lengths)
+    for kw in (dict(), dict(max_seen=max(lengths))):
+        check_decode(c.decode(q, seen, **kw), q, hk, hv, lengths, share, dtype, D ** -0.5, group)
