@@ -653,17 +653,18 @@ class PagedCodeKVCache:
         return 2 * self.seq_len * self.num_kv_heads * (G + 4)
 
 
+# The calls below serve single tokens, where the host's time is the call's: their checks
+# read each property once, and hold devices by index.
 _INFERENCE_TAGS = {}
 
 
 def _inference_tag(what, *tensors):
-    """The C-ABI tag of the tensors' one dtype; they have no gradient here."""
-    t = tensors[0]
-    dtype, device = t.dtype, t.device
-    _require_gpu(t, what)
+    """(C-ABI tag, device index) of tensors of one dtype on one GPU, without a gradient."""
+    dtype, index = tensors[0].dtype, tensors[0].get_device()
     for u in tensors:
-        if u.dtype != dtype or u.device != device:
-            raise ValueError(f"{what}: tensors of {dtype} on {device} and of {u.dtype} on {u.device}")
+        if u.dtype != dtype or u.get_device() != index or index < 0:
+            _require_gpu(u, what)
+            raise ValueError(f"{what}: tensors of {dtype} on {tensors[0].device} and of {u.dtype} on {u.device}")
         if u.requires_grad and _torch().is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or with detached "
                                "tensors")
@@ -673,7 +674,7 @@ def _inference_tag(what, *tensors):
         if tag is None or tag == _lib.DTYPE_F64:
             raise TypeError(f"{what}: unsupported dtype {dtype}: float32, bfloat16 or float16")
         _INFERENCE_TAGS[dtype] = tag
-    return tag
+    return tag, index
 
 
 def _new_like(t):
@@ -684,36 +685,40 @@ def _new_like(t):
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _aligned_rows(t):
-    """t [n, heads, D] itself where its rows are contiguous and 16-byte aligned,
-    else a contiguous copy."""
-    es = t.element_size()
-    s = t.stride()
-    if s[2] != 1 or t.data_ptr() % 16 or s[0] * es % 16 or s[1] * es % 16 or s[0] < 0 or s[1] < 0:
+def _aligned_rows(t, es):
+    """(t [n, heads, D] itself where its rows are contiguous and 16-byte aligned, else a
+    contiguous copy; its address, its token and its head stride).  es: bytes per element."""
+    ts, hs, ds = t.stride()
+    at = t.data_ptr()
+    if ds != 1 or (at | ts * es | hs * es) & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:               # contiguous() returns a contiguous slice as it is
+        if t.data_ptr() & 15:               # contiguous() returns a contiguous slice as it is
             t = t.clone()
-    return t
+        ts, hs, _ = t.stride()
+        at = t.data_ptr()
+    return t, at, ts, hs
 
 
-def _lengths_tensor(t, n, device, what):
-    torch = _torch()
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or \
-            t.device != device:
-        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries on {device}, got "
+def _lengths_tensor(t, n, index, what):
+    if t.dtype != _torch().int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or \
+            t.get_device() != index:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries on cuda:{index}, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _launch(device, call):
-    """``call(stream)`` on the device's current stream, the device made current
+def _launch(index, what, *args):
+    """The entry point ``what`` on the device's current stream, the device made current
     where another is."""
     torch = _torch()
-    index = device.index
+    call = getattr(_lib.lib(), what)
     if torch.cuda.current_device() == index:
-        return call(_lib.raw_stream(index))
-    with torch.cuda.device(index):
-        return call(_lib.raw_stream(index))
+        rc = call(*args, _lib.raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, _lib.raw_stream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
 class PagedInt4KVCache:
@@ -775,6 +780,7 @@ class PagedInt4KVCache:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         dev = self.device
+        self._index = dev.index
         turns = None
         if rotary_dim:
             if inv_freq is None:
@@ -826,21 +832,26 @@ class PagedInt4KVCache:
                    (self.k_codes, self.v_codes, self.k_steps, self.v_steps, self.block_table))
 
     def _check_rows(self, t, n, heads, name):
-        if t.dim() != 3 or t.shape[0] != n or t.shape[2] != self.head_dim or \
-                (heads is not None and t.shape[1] != heads):
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != n or shape[2] != self.head_dim or \
+                (heads is not None and shape[1] != heads):
             raise ValueError(f"{name} must be [{n}, {heads or 'heads'}, {self.head_dim}], got "
-                             f"{tuple(t.shape)}")
-        if t.device != self.device:
-            raise ValueError(f"{name} lives on {t.device}, the cache on {self.device}")
+                             f"{tuple(shape)}")
+
+    def _tag(self, what, *tensors):
+        tag, index = _inference_tag(what, *tensors)
+        if index != self._index:
+            raise ValueError(f"{what}: tensors on {tensors[0].device}, the cache on {self.device}")
+        return tag
 
     def _packed(self, n, start, cu_seqlens):
         B = self.num_sequences
-        at = _lengths_tensor(start, B, self.device, "start")
+        at = _lengths_tensor(start, B, self._index, "start")
         if cu_seqlens is None:
             if n != B:
                 raise ValueError(f"{n} tokens: without cu_seqlens each of the {B} sequences gets one")
             return at, None
-        return at, _lengths_tensor(cu_seqlens, B + 1, self.device, "cu_seqlens")
+        return at, _lengths_tensor(cu_seqlens, B + 1, self._index, "cu_seqlens")
 
     def append(self, key, value, start, cu_seqlens=None, *, query=None, return_key: bool = False):
         """Rotate and append ``key`` and ``value`` [N, num_kv_heads, head_dim]
@@ -852,33 +863,28 @@ class PagedInt4KVCache:
         Returns (query rotated by the same positions or None, the rotated key
         before its encoding or None without ``return_key``), contiguous, in
         their dtype; rows that belong to no sequence are zeros there."""
-        torch = _torch()
         what = "PagedInt4KVCache.append"
-        tensors = (key, value) if query is None else (key, value, query)
-        tag = _inference_tag(what, *tensors)
+        tag = self._tag(what, key, value) if query is None else self._tag(what, key, value, query)
         n = key.shape[0] if key.dim() else 0
         self._check_rows(key, n, self.num_kv_heads, "key")
         self._check_rows(value, n, self.num_kv_heads, "value")
+        at, cu = self._packed(n, start, cu_seqlens)
+        es = 4 if tag == _lib.DTYPE_F32 else 2
+        k, ka, kt, kh = _aligned_rows(key, es)
+        v, va, vt, vh = _aligned_rows(value, es)
+        qo = ko = qa = qp = kp = None
+        heads = qt = qh = 0
         if query is not None:
             self._check_rows(query, n, None, "query")
-        at, cu = self._packed(n, start, cu_seqlens)
-        k, v = _aligned_rows(key), _aligned_rows(value)
-        ks, vs = k.stride(), v.stride()
-        qp = qo = ko = None
-        qs, heads = (0, 0), 0
-        if query is not None:
-            q = _aligned_rows(query)
-            qs, heads = q.stride(), q.shape[1]
+            heads = query.shape[1]
+            q, qa, qt, qh = _aligned_rows(query, es)
             qo = _new_like(q)
-            qp = q.data_ptr()
+            qp = qo.data_ptr()
         if return_key:
             ko = _new_like(k)
-        rc = _launch(self.device, lambda stream: _lib.lib().ojasx_kv4_append_device(
-            self._ref, qp, qs[0], qs[1], heads, None if qo is None else qo.data_ptr(),
-            k.data_ptr(), ks[0], ks[1], None if ko is None else ko.data_ptr(), v.data_ptr(),
-            vs[0], vs[1], n, tag, at, cu, stream))
-        if rc:
-            _lib.check(rc, "ojasx_kv4_append_device")
+            kp = ko.data_ptr()
+        _launch(self._index, "ojasx_kv4_append_device", self._ref, qa, qt, qh, heads, qp, ka, kt, kh, kp, va,
+                vt, vh, n, tag, at, cu)
         return qo, ko
 
     def read(self, start, cu_seqlens=None, num_tokens: Optional[int] = None, *, seen=None, dtype=None):
@@ -899,13 +905,11 @@ class PagedInt4KVCache:
         if num_tokens < 0:
             raise ValueError(f"num_tokens must not be negative, got {num_tokens}")
         at, cu = self._packed(num_tokens, start, cu_seqlens)
-        sp = None if seen is None else _lengths_tensor(seen, self.num_sequences, self.device, "seen")
+        sp = None if seen is None else _lengths_tensor(seen, self.num_sequences, self._index, "seen")
         k = torch.empty(num_tokens, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        rc = _launch(self.device, lambda stream: _lib.lib().ojasx_kv4_read_device(
-            self._ref, at, cu, sp, num_tokens, k.data_ptr(), v.data_ptr(), tag, stream))
-        if rc:
-            _lib.check(rc, "ojasx_kv4_read_device")
+        _launch(self._index, "ojasx_kv4_read_device", self._ref, at, cu, sp, num_tokens, k.data_ptr(),
+                v.data_ptr(), tag)
         return k, v
 
     def decode(self, query, seen, scale_factor: float = -1.0, *, max_seen: int = 0, out=None):
@@ -919,19 +923,17 @@ class PagedInt4KVCache:
         ``max_seen``, a bound on ``seen`` where the caller knows one, keeps the
         launch of short sequences as small as they are."""
         torch = _torch()
-        what = "PagedInt4KVCache.decode"
-        tag = _inference_tag(what, query)
+        tag = self._tag("PagedInt4KVCache.decode", query)
         self._check_rows(query, self.num_sequences, None, "query")
         heads = query.shape[1]
         if heads == 0 or heads % self.num_kv_heads:
             raise ValueError(f"{heads} query heads are no multiple of {self.num_kv_heads} kv heads")
         if max_seen < 0:
             raise ValueError(f"max_seen must not be negative, got {max_seen}")
-        sp = _lengths_tensor(seen, self.num_sequences, self.device, "seen")
-        lib = _lib.lib()
+        sp = _lengths_tensor(seen, self.num_sequences, self._index, "seen")
         need = self._workspace_bytes.get((heads, max_seen))
         if need is None:
-            need = lib.ojasx_kv4_decode_workspace(self._ref, heads, max_seen)
+            need = _lib.lib().ojasx_kv4_decode_workspace(self._ref, heads, max_seen)
             if need < 0:
                 _lib.check(need, "ojasx_kv4_decode_workspace")
             if len(self._workspace_bytes) > 64:
@@ -942,15 +944,12 @@ class PagedInt4KVCache:
         elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or \
                 not out.is_contiguous():
             raise ValueError("out must be contiguous and of the query's shape, dtype and device")
-        q = _aligned_rows(query)
-        if not q.is_contiguous():
-            q = q.contiguous()
+        q = query if query.is_contiguous() else query.contiguous()
+        if q.data_ptr() & 15:
+            q = q.clone()
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        rc = _launch(self.device, lambda stream: lib.ojasx_kv4_decode_device(
-            self._ref, q.data_ptr(), heads, tag, sp, max_seen, scale_factor, out.data_ptr(),
-            ws.data_ptr(), need, stream))
-        if rc:
-            _lib.check(rc, "ojasx_kv4_decode_device")
+        _launch(self._index, "ojasx_kv4_decode_device", self._ref, q.data_ptr(), heads, tag, sp, max_seen,
+                scale_factor, out.data_ptr(), ws.data_ptr(), need)
         return out
 
 
@@ -978,8 +977,10 @@ class PackedPromptAttention:
             raise ValueError(f"scale must be positive and finite, got {scale}")
 
     def _check(self, t, heads, name):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name} must be [tokens, {heads}, {self.head_dim}], got {tuple(t.shape)}")
+        shape = t.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim:
+            raise ValueError(f"{name} must be [tokens, {heads}, {self.head_dim}], got {tuple(shape)}")
+        return shape[0]
 
     def forward(self, query, key, value, cu_seqlens, cu_seqlens_kv=None, *, out=None,
                 return_lse: bool = False):
@@ -995,45 +996,41 @@ class PackedPromptAttention:
         sequence are 0 (lse -inf); in a given ``out`` they stay as they are.
         ``out`` may be the query itself, and shares no memory with the keys and
         values."""
-        torch = _torch()
-        what = "PackedPromptAttention"
-        tag = _inference_tag(what, query, key, value)
-        self._check(query, self.num_heads, "query")
-        self._check(key, self.num_kv_heads, "key")
-        self._check(value, self.num_kv_heads, "value")
-        if key.shape[0] != value.shape[0]:
-            raise ValueError(f"{key.shape[0]} keys and {value.shape[0]} values")
-        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        tag, dev = _inference_tag("PackedPromptAttention", query, key, value)
+        n = self._check(query, self.num_heads, "query")
+        m = self._check(key, self.num_kv_heads, "key")
+        if self._check(value, self.num_kv_heads, "value") != m:
+            raise ValueError(f"{m} keys and {value.shape[0]} values")
+        B = cu_seqlens.numel() - 1
+        if B < 1:
             raise ValueError(f"cu_seqlens must hold the B + 1 bounds of B sequences, got "
                              f"{tuple(cu_seqlens.shape)}")
-        dev = query.device
-        B = cu_seqlens.shape[0] - 1
-        cq = _lengths_tensor(cu_seqlens, B + 1, dev, "cu_seqlens")
-        if cu_seqlens_kv is None:
-            if key.shape[0] != query.shape[0]:
-                raise ValueError(f"{query.shape[0]} queries and {key.shape[0]} keys without cu_seqlens_kv")
-            ck = cq
-        else:
+        cq = ck = _lengths_tensor(cu_seqlens, B + 1, dev, "cu_seqlens")
+        if cu_seqlens_kv is not None:
             ck = _lengths_tensor(cu_seqlens_kv, B + 1, dev, "cu_seqlens_kv")
+        elif m != n:
+            raise ValueError(f"{n} queries and {m} keys without cu_seqlens_kv")
         fresh = out is None
         if fresh:
             out = _new_like(query)
-        elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or \
-                not out.is_contiguous() or out.data_ptr() % 16:
+        elif out.shape != query.shape or out.dtype != query.dtype or out.get_device() != dev or \
+                not out.is_contiguous() or out.data_ptr() & 15:
             raise ValueError("out must be contiguous, 16-byte aligned and of the query's shape, dtype and "
                              "device")
-        q, k, v = _aligned_rows(query), _aligned_rows(key), _aligned_rows(value)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-        if lse is not None and not fresh:
-            lse.fill_(-math.inf)
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        rc = _launch(dev, lambda stream: _lib.lib().ojasx_prompt_attention_device(
-            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], tag,
-            q.shape[0], k.shape[0], self.num_heads, self.num_kv_heads, self.head_dim, cq, ck, B,
-            self.causal, self.scale, fresh, out.data_ptr(),
-            None if lse is None else lse.data_ptr(), stream))
-        if rc:
-            _lib.check(rc, "ojasx_prompt_attention_device")
+        es = 4 if tag == _lib.DTYPE_F32 else 2
+        q, qa, qt, qh = _aligned_rows(query, es)
+        k, ka, kt, kh = _aligned_rows(key, es)
+        v, va, vt, vh = _aligned_rows(value, es)
+        lse = la = None
+        if return_lse:
+            torch = _torch()
+            lse = torch.empty(n, self.num_heads, dtype=torch.float32, device=query.device)
+            la = lse.data_ptr()
+            if not fresh:
+                lse.fill_(-math.inf)
+        _launch(dev, "ojasx_prompt_attention_device", qa, qt, qh, ka, kt, kh, va, vt, vh, tag, n, m,
+                self.num_heads, self.num_kv_heads, self.head_dim, cq, ck, B, self.causal, self.scale, fresh,
+                out.data_ptr(), la)
         return (out, lse) if return_lse else out
 
     __call__ = forward
