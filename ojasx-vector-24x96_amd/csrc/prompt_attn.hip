@@ -26,8 +26,8 @@
 // 32 / 8 heads of 128 but where said: 16384 bf16 tokens of one sequence 2.16 ms, 1015
 // TFLOP/s (a large bf16 matrix product of the library runs at 1200 here); 8192 of
 // eight 0.12 ms; 4999 fp16 tokens of five sequences, 16 heads of 64, 30 us; 2048 fp32
-// of two 157 us, 116 TFLOP/s where the library's fp32 product has 153; 150 of three
-// 7.4 us, of which a launch with nothing to do is half.
+// of two 147 us; 150 bf16 of three 7.4 us, of which a launch with nothing to do is
+// half.
 #include <cmath>
 #include <type_traits>
 
@@ -114,11 +114,46 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70
 // The key that accumulator register r of a lane's half h stands for.
 __device__ __forceinline__ constexpr int key_of(int r) { return 8 * (r / 4) + r % 4; }
 
+// a *= f in accumulation registers.  Written as a product the compiler copies all of
+// the kernel's accumulators to vector registers and back on every tile, also where
+// none is rescaled.  The waits that it would put between matrix instructions and these
+// reads and writes stand in the block: 24 states before (the longest needs 19), 4 after.
+__device__ __forceinline__ void scale_acc(f32x16_t &a, float f) {
+    float e[16], t;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = a[i];
+    asm volatile(
+        "s_nop 15\n\ts_nop 7\n\t"
+        "v_accvgpr_read_b32 %16, %0\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %0, %16\n\t"
+        "v_accvgpr_read_b32 %16, %1\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %1, %16\n\t"
+        "v_accvgpr_read_b32 %16, %2\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %2, %16\n\t"
+        "v_accvgpr_read_b32 %16, %3\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %3, %16\n\t"
+        "v_accvgpr_read_b32 %16, %4\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %4, %16\n\t"
+        "v_accvgpr_read_b32 %16, %5\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %5, %16\n\t"
+        "v_accvgpr_read_b32 %16, %6\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %6, %16\n\t"
+        "v_accvgpr_read_b32 %16, %7\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %7, %16\n\t"
+        "v_accvgpr_read_b32 %16, %8\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %8, %16\n\t"
+        "v_accvgpr_read_b32 %16, %9\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %9, %16\n\t"
+        "v_accvgpr_read_b32 %16, %10\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %10, %16\n\t"
+        "v_accvgpr_read_b32 %16, %11\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %11, %16\n\t"
+        "v_accvgpr_read_b32 %16, %12\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %12, %16\n\t"
+        "v_accvgpr_read_b32 %16, %13\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %13, %16\n\t"
+        "v_accvgpr_read_b32 %16, %14\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %14, %16\n\t"
+        "v_accvgpr_read_b32 %16, %15\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %15, %16\n\t"
+        "s_nop 3"
+        : "+a"(e[0]), "+a"(e[1]), "+a"(e[2]), "+a"(e[3]), "+a"(e[4]), "+a"(e[5]), "+a"(e[6]), "+a"(e[7]), "+a"(e[8]), "+a"(e[9]), "+a"(e[10]), "+a"(e[11]), "+a"(e[12]), "+a"(e[13]), "+a"(e[14]), "+a"(e[15]), "=&v"(t)
+        : "v"(f));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a[i] = e[i];
+}
+
 // Running maximum (log2) of one query row per lane with a tile's largest score t:
 // rescales acc and l where the row's maximum grew by more than 2^8.
 // Weights up to 2^8 above 1 lose nothing: they are rounded relative to their
 // size and all sums are fp32.
-template <int NT>
+//
+// ACC: acc stays in accumulation registers.
+template <bool ACC, int NT>
 __device__ __forceinline__ void raise_max(float t, float &m, float &ref, float &l, f32x16_t (&acc)[NT]) {
     if (__any(t > m + 8.f)) {
         const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
@@ -127,7 +162,9 @@ __device__ __forceinline__ void raise_max(float t, float &m, float &ref, float &
         ref = rn;
         l *= alpha;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i] *= alpha;
+        for (int i = 0; i < NT; ++i)
+            if (ACC) scale_acc(acc[i], alpha);
+            else acc[i] *= alpha;
     }
 }
 
@@ -370,7 +407,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
             float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[NB - 1][r]);
-            raise_max(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
+            raise_max<false>(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
             // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block);
             // between the products of one 16 go the exponentials and the V reads of
             // the next.  They are rounded to the inputs' type, relative to their size
@@ -484,8 +521,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
 // the end (head dims past 128 have registers for one set).  Six bf16 products take
 // 3 / 8 of the time of v_mfma_f32_32x32x2 on the same operands: 2048 tokens of two
 // sequences, 32 / 8 heads of 128, 328 -> 157 us.  K and V are split as they are
-// staged, in [piece][key] planes; one wave per SIMD, for the registers of two sets
-// of accumulators.
+// staged, in [piece][key] planes: a tile's loads are issued a tile ahead, and its
+// split goes between the products of the tile before (head dims past 128 have LDS for
+// one buffer and split between barriers).  One wave per SIMD, for the registers of two
+// sets of accumulators; with Q and the sets held in accumulation registers 147 us.
 template <int DP, int BUFFERS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void prompt_attn_f32_kernel(PromptParams p,
                                                                                                         int slots) {
@@ -542,27 +581,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             }
         }
     };
-    auto store = [&](int tile) __attribute__((always_inline)) {
+    // Part j of the loaded tile into its planes: unit j / 2 of K, or of V.
+    auto store_part = [&](int tile, int j) __attribute__((always_inline)) {
         unsigned char *ks = sm + (BUFFERS == 2 ? tile & 1 : 0) * 6 * PLANE, *vs = ks + 3 * PLANE;
+        const int i = j >> 1, r = sr + i * (NT / UPR);
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int r = sr + i * (NT / UPR);
-            float kx[8], vx[8];
+        for (int e = 0; e < 8; ++e) x[e] = p.D < DP && !in ? 0.f : (j & 1 ? vr : kr)[i][e / 4][e % 4];
+        bf16x8_t y[3];
+        split3_bf16(x, y);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                kx[e] = p.D < DP && !in ? 0.f : kr[i][e / 4][e % 4];
-                vx[e] = p.D < DP && !in ? 0.f : vr[i][e / 4][e % 4];
-            }
-            bf16x8_t kb[3], vb[3];
-            split3_bf16(kx, kb);
-            split3_bf16(vx, vb);
+        for (int z = 0; z < 3; ++z)
+            if (j & 1)
+                *reinterpret_cast<bf16x8_t *>(vs + z * PLANE + r * ROWB + v_unit<ROWB>(r, su >> 1) * 32 +
+                                              (su & 1) * 16) = y[z];
+            else
+                *reinterpret_cast<bf16x8_t *>(ks + z * PLANE + r * ROWB + k_unit<ROWB>(r, su) * 16) = y[z];
+    };
+    auto store = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-            for (int x = 0; x < 3; ++x) {
-                *reinterpret_cast<bf16x8_t *>(ks + x * PLANE + r * ROWB + k_unit<ROWB>(r, su) * 16) = kb[x];
-                *reinterpret_cast<bf16x8_t *>(vs + x * PLANE + r * ROWB + v_unit<ROWB>(r, su >> 1) * 32 +
-                                              (su & 1) * 16) = vb[x];
-            }
-        }
+        for (int j = 0; j < 2 * CH; ++j) store_part(tile, j);
     };
     // c += the six products of a and b, the largest into c0
     auto mma6 = [&](const bf16x8_t (&a)[3], const bf16x8_t (&b)[3], f32x16_t &c0, f32x16_t &c1)
@@ -581,14 +619,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         store(0);
     }
     loads_done();
+    if (BUFFERS == 2 && tiles) load(1);              // past the end: the last key's rows again
     const int vkey = 4 * h + ((lane & 15) >> 2), vg = lane >> 4 & 1, vb8 = (lane & 3) * 8;
     for (int tile = 0; tile < tiles; ++tile) {
         __syncthreads();
-        if (tile + 1 < tiles) load(tile + 1);
+        if (BUFFERS == 1 && tile + 1 < tiles) load(tile + 1);
         const int k0 = tile * KEYS;
-        if (k0 <= lim_hi) {
+        if (BUFFERS == 2 || k0 <= lim_hi) {           // all waves split their parts
             const unsigned char *ks = sm + (BUFFERS == 2 ? tile & 1 : 0) * 6 * PLANE, *vs = ks + 3 * PLANE;
             f32x16_t s0 = {}, s1 = {};
+            // Q stays in accumulation registers, which the products read as they are
+            if (DP <= 128)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) asm volatile("" : "+a"(qf[c][x]));
             bf16x8_t kf[2][3];
             auto read_k = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
@@ -603,8 +648,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                 if (c + 1 < NC) read_k(c + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 mma6(kf[c % 2], qf[c], s0, s1);
+                // the next tile's split goes between the products
+                if (BUFFERS == 2)
+#pragma unroll
+                    for (int j = c * 2 * CH / NC; j < (c + 1) * 2 * CH / NC; ++j) store_part(tile + 1, j);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (BUFFERS == 2) load(tile + 2);
             s0 += s1;
             if (k0 + KEYS - 1 > lim_lo) {
                 int rel = lim - k0 - 4 * h;
@@ -616,7 +666,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             float t = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
-            raise_max(halves_max(t) * p.scale2, m, ref, l, acc);
+            raise_max<(DP <= 128)>(halves_max(t) * p.scale2, m, ref, l, acc);
             bf16x8_t pf[2][3];
             auto weights = [&](int f) __attribute__((always_inline)) {
                 float x[8];
@@ -657,8 +707,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (BUFFERS == 1) __syncthreads();
-        if (tile + 1 < tiles) store(tile + 1);
+        if (BUFFERS == 1) {
+            __syncthreads();
+            if (tile + 1 < tiles) store(tile + 1);
+        }
     }
     l = halves_sum(l);
     f32x16_t sum[NT2];
