@@ -14,7 +14,9 @@ Faces, each mirroring a reference interface:
   ``subspace_lut_rvq_gemm`` (reference codec container and math engine)
 * ``long_context``: ``PagedCompressedKVCache`` (reference int8 paged KV cache)
   and ``PagedCodeKVCache`` (paged codebook-code KV cache with device append
-  and decode)
+  and decode); for a serving batch ``PagedInt4KVCache`` (4-bit paged cache:
+  append with rotation, decode attention) and ``PackedPromptAttention``
+  (causal attention of packed prompts)
 * ``decoder``: ``LUTDecoder`` / ``synthetic_decoder``, the 4B-shaped greedy
   decoder over LUT linears and the code KV cache (HIP graph per token)
 * ``oqpack``: the reference's oqpack.v1 container (verify, mmap, write) and
