@@ -23,9 +23,9 @@
 // Bound by the matrix instructions where rows are long, and by exponentials with
 // narrow heads: a score costs 4 D operations there and one exp2 at a quarter of the
 // vector rate, about as long as its products at D = 64.  Measured, one pass, causal,
-// 32 / 8 heads of 128 but where said: 16384 bf16 tokens of one sequence 2.16 ms, 1015
-// TFLOP/s (a large bf16 matrix product of the library runs at 1200 here); 8192 of
-// eight 0.12 ms; 4999 fp16 tokens of five sequences, 16 heads of 64, 30 us; 2048 fp32
+// 32 / 8 heads of 128 but where said: 16384 bf16 tokens of one sequence 2.06 to 2.19
+// ms, 1040 TFLOP/s (a large bf16 matrix product of the library runs at 1200 here; the
+// clocks vary); 8192 of eight 0.12 ms; 4999 fp16 tokens of five sequences, 16 heads of 64, 30 us; 2048 fp32
 // of two 147 us; 150 bf16 of three 7.4 us, of which a launch with nothing to do is
 // half.
 #include <cmath>
@@ -403,6 +403,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                 for (int b = 0; b < NB; ++b) s[b] = E::mma(__builtin_bit_cast(V8, kf[c % 3][b]), qf[c], s[b]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            // From here the wave goes before the SIMD's others: its vector work then runs
+            // beside their score products and not after them (16384 tokens, 32 / 8 heads
+            // of 128: 2265 -> 2192 us; the score products first: no gain).
+            __builtin_amdgcn_s_setprio(1);
             if (k0 + 32 * NB - 1 > lim_lo) mask_tile(s, lim, k0, h);
             float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
@@ -451,6 +455,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (tile + 1 < tiles) store(tile + 1);
     }
     l = halves_sum(l);
