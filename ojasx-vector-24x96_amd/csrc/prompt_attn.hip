@@ -673,14 +673,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
             raise_max<(DP <= 128)>(halves_max(t) * p.scale2, m, ref, l, acc);
             bf16x8_t pf[2][3];
-            auto weights = [&](int f) __attribute__((always_inline)) {
-                float x[8];
+            constexpr int PART = NT2 < 4 ? 8 / NT2 : 2;
+            auto weights = [&](int f, int e0, int e1) __attribute__((always_inline)) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(s0[8 * f + e], p.scale2, -ref));
-                    l += x[e];
+                for (int e = e0; e < e1; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s0[8 * f + e], p.scale2, -ref));
+                    l += x;
+                    const __bf16 h1 = (__bf16)x;
+                    const float r1 = x - (float)h1;
+                    const __bf16 h2 = (__bf16)r1;
+                    pf[f][0][e] = h1;
+                    pf[f][1][e] = h2;
+                    pf[f][2][e] = (__bf16)(r1 - (float)h2);
                 }
-                split3_bf16(x, pf[f]);
             };
             s16x4_t vf[2][3][2];
             auto read_v = [&](int i) __attribute__((always_inline)) {
@@ -696,7 +701,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             };
             read_v(0);
             __builtin_amdgcn_sched_barrier(0);
-            weights(0);
+            weights(0, 0, 8);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 2 * NT2; ++i) {
@@ -708,7 +713,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                     z[x] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vf[i % 2][x][0], vf[i % 2][x][1], 0, 1, 2,
                                                                                3, 4, 5, 6, 7));
                 mma6(z, pf[i / NT2], acc[i % NT2], acc[(SETS - 1) * NT2 + i % NT2]);
-                if (i == 0) weights(1);
+                if (i * PART < 8) weights(1, i * PART, i * PART + PART);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
