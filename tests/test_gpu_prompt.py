@@ -325,3 +325,31 @@ def test_out_is_the_query(lc, dev, name):
     a = lc.PackedPromptAttention(4, 2, 64)
     want = a(q, k, v, cu)
     assert a(q, k, v, cu, out=q) is q and torch.equal(q, want)
+
+
+MANY = LENGTHS + [300, 1, 95, 260, 0, 32, 128, 17, 250, 3, 63, 190, 64, 1, 97, 33, 5]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,dtype", [
+    (32, 32, 64, "float16"), (32, 8, 128, "bfloat16"), (16, 16, 128, "float16"), (32, 16, 96, "bfloat16"),
+    (16, 8, 256, "bfloat16")])
+def test_more_workgroups_than_are_resident(lc, dev, Hq, Hkv, D, dtype):
+    """Grids past the rule that splits a tile's keys over two waves: more workgroups (of up to four
+    heads and 128 rows by head) than the 768, 512 or 256 that it has by head dim.  Infinities and
+    NaN in the second half of the longest prompt's keys reach no row before them."""
+    N, cu = sum(MANY), cum(MANY)
+    share = Hq // Hkv
+    heads = min(share & -share, 4)
+    assert (N * heads // 128 + len(MANY) + 2) * (Hq // heads) > (768 if D <= 64 else 512 if D <= 128 else 256)
+    q, k, v = (rand(dev, dtype, N, h, D, seed=s) for h, s in ((Hq, 1), (Hkv, 2), (Hkv, 3)))
+    a = lc.PackedPromptAttention(Hq, Hkv, D)
+    out, lse = a(q, k, v, i32(dev, cu), return_lse=True)
+    check(out, q, k, v, cu, cu, True, D ** -0.5, dtype, lse)
+    b = MANY.index(300)
+    lo, mid = cu[b], cu[b] + 150
+    k[mid:lo + 300:2] = float("inf")
+    k[mid + 1:lo + 300:2] = float("nan")
+    v[mid:lo + 300] = float("-inf")
+    out = a(q, k, v, i32(dev, cu))
+    check(out[lo:mid], q[lo:mid], k[lo:mid], v[lo:mid], [0, 150], [0, 150], True, D ** -0.5, dtype)
+    assert out[mid:lo + 300].isnan().all()
