@@ -516,3 +516,37 @@ def test_decode_few_heads(lc, dev, case):
     seen = i32(dev, lengths)
     for kw in (dict(), dict(max_seen=max(lengths))):
         check_decode(c.decode(q, seen, **kw), q, hk, hv, lengths, share, dtype, D ** -0.5, group)
+
+
+@pytest.mark.parametrize("B,N,dtype", [(3, 1500, "bfloat16"), (70, 2500, "float16"), (130, 5000, "float32")])
+def test_append_many_tokens(lc, dev, B, N, dtype):
+    """Tokens that share their waves' work over fewer of them, and one wave for a whole token; more
+    sequences than lanes."""
+    r = np.random.default_rng(B)
+    cuts = np.sort(r.integers(0, N + 1, B - 1)).tolist()
+    cu = [0] + cuts + [N]
+    lengths = np.diff(cu).tolist()
+    starts = r.integers(0, 100, B).tolist()
+    pages = (max(lengths) + 100) // 16 + 1
+    c = lc.PagedInt4KVCache(2, 128, num_sequences=B, max_resident_pages=pages, sink_pages=1, rope_theta=THETA,
+                            device=dev)
+    k, v, q = (rand(dev, dtype, N, h, 128, seed=s) for h, s in ((2, 1), (2, 2), (12, 3)))
+    qr, _ = c.append(k, v, i32(dev, starts), i32(dev, cu), query=q)
+    pos = positions(starts, lengths)
+    _, hk, hv = want_kv(k, v, pos, 128, 32)
+    rk, rv = c.read(i32(dev, starts), i32(dev, cu), N)
+    assert np.array_equal(f64(rk), hk.astype(np.float32).astype(np.float64))
+    assert np.array_equal(f64(rv), hv.astype(np.float32).astype(np.float64))
+    qf = kv4.rotate(f64(q), pos, kv4.inv_freq(128, THETA))
+    assert (np.abs(f64(qr) - qf) <= 2 * eps_half(dtype) * np.abs(qf) + 1e-7 * (dtype == "float16")).all()
+
+
+@pytest.mark.parametrize("share", [1, 5])
+def test_decode_many_sequences(lc, dev, share):
+    """More sequences than lanes, some without tokens, runs that begin in any of them."""
+    lengths = np.random.default_rng(share).integers(-20, 200, 150).clip(0).tolist()
+    lengths[149] = 1000
+    c, q, hk, hv = decode_case(lc, dev, 64, 32, "float32", 16, 2, share, lengths, 64)
+    seen = i32(dev, lengths)
+    for kw in (dict(), dict(max_seen=40)):
+        check_decode(c.decode(q, seen, **kw), q, hk, hv, lengths, share, "float32", 0.125, 32)
