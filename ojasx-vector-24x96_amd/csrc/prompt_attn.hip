@@ -763,34 +763,52 @@ int heads_shift(const PromptParams &p, int wr) {
     const int share = __builtin_ctz((unsigned)(p.Hq / p.Hkv)), most = __builtin_ctz((unsigned)wr);
     return share < most ? share : most;
 }
-template <typename K>
-int launch(K kernel, PromptParams p, int wr, size_t lds, size_t *granted, hipStream_t st) {
-    const int rc = ensure_dyn_lds(reinterpret_cast<const void *>(kernel), lds, granted);
+// Sets p.hw, the LDS limit of kernel `fn` and the launch's size, or returns an error.
+int prepare(const void *fn, PromptParams &p, int wr, size_t lds, size_t *granted, int *slots, unsigned *groups) {
+    const int rc = ensure_dyn_lds(fn, lds, granted);
     if (rc) return rc;
     p.hw = heads_shift(p, wr);
-    const long slots = slots_of(p, wr, p.hw), groups = slots * (p.Hq >> p.hw);
-    if (groups > 0xffffffL) {                        // a grid has fewer than 2^32 threads
+    const long rows = slots_of(p, wr, p.hw), all = rows * (p.Hq >> p.hw);
+    if (all > 0xffffffL) {                           // a grid has fewer than 2^32 threads
         set_error("prompt attention: %d tokens of %d sequences and %d heads need %ld workgroups (at most 2^24 - 1)",
-                  p.Nq, p.B, p.Hq, groups);
+                  p.Nq, p.B, p.Hq, all);
         return OJASX_ERR_INVALID;
     }
-    OJX_LAUNCH(kernel, dim3((unsigned)groups), dim3(256), lds, st, p, (int)slots);
+    *slots = (int)rows;
+    *groups = (unsigned)all;
+    return OJASX_OK;
+}
+template <typename E, int DP, int KS>
+int launch16_split(PromptParams p, hipStream_t st) {
+    static size_t granted = 0;
+    const size_t lds = (size_t)4 * kKeys * 2 * DP;
+    int slots;
+    unsigned groups;
+    const int rc = prepare(reinterpret_cast<const void *>(&prompt_attn_kernel<E, DP, KS>), p, 4 / KS, lds, &granted,
+                           &slots, &groups);
+    if (rc) return rc;
+    OJX_LAUNCH((prompt_attn_kernel<E, DP, KS>), dim3(groups), dim3(256), lds, st, p, slots);
     OJX_HIP(hipGetLastError());
     return OJASX_OK;
 }
 template <typename E, int DP>
 int launch16(const PromptParams &p, hipStream_t st) {
-    static size_t granted[2] = {0, 0};
     const int hw = heads_shift(p, 4);
-    const size_t lds = (size_t)4 * kKeys * 2 * DP;
-    if (slots_of(p, 4, hw) * (p.Hq >> hw) > split_below(DP))
-        return launch(&prompt_attn_kernel<E, DP, 1>, p, 4, lds, &granted[0], st);
-    return launch(&prompt_attn_kernel<E, DP, 2>, p, 2, lds, &granted[1], st);
+    if (slots_of(p, 4, hw) * (p.Hq >> hw) > split_below(DP)) return launch16_split<E, DP, 1>(p, st);
+    return launch16_split<E, DP, 2>(p, st);
 }
 template <int DP, int BUFFERS>
-int launch32(const PromptParams &p, hipStream_t st) {
+int launch32(PromptParams p, hipStream_t st) {
     static size_t granted = 0;
-    return launch(&prompt_attn_f32_kernel<DP, BUFFERS>, p, 4, (size_t)BUFFERS * 6 * 32 * 2 * DP, &granted, st);
+    const size_t lds = (size_t)BUFFERS * 6 * 32 * 2 * DP;
+    int slots;
+    unsigned groups;
+    const int rc = prepare(reinterpret_cast<const void *>(&prompt_attn_f32_kernel<DP, BUFFERS>), p, 4, lds, &granted,
+                           &slots, &groups);
+    if (rc) return rc;
+    OJX_LAUNCH((prompt_attn_f32_kernel<DP, BUFFERS>), dim3(groups), dim3(256), lds, st, p, slots);
+    OJX_HIP(hipGetLastError());
+    return OJASX_OK;
 }
 
 bool rows16(const void *p, long ts, long hs, size_t es) {
