@@ -313,9 +313,9 @@ OJASX_API int ojasx_attention_stream_finalize_device(const double *state, int ro
 /* ---- 4-bit paged KV cache and packed prompts (no reference counterpart) --- */
 /* A cache of num_sequences sequences, K and V held in 4 bits.  Of a token's
  * row of one kv head, each group of group_size dimensions is held as lo =
- * fp16(min), s = fp16(fp32((max - lo) / 15)), at least 0, and codes clamp(round_half_even((x
- * - lo) / s), 0, 15), for the values lo + s * code; a group with an infinity or
- * a NaN reads back as NaN.  Tokens fill pages of page_size slots; position t
+ * fp16(min), s = fp16(fp32((max - lo) / 15)), at least 0, and codes
+ * clamp(round_half_even((x - lo) / s), 0, 15), for the values lo + s * code; a
+ * group with an infinity or a NaN reads back as NaN.  Tokens fill pages of page_size slots; position t
  * lies in its sequence's page j = t / page_size, which entry e = j < sink_pages
  * ? j : sink_pages + (j - sink_pages) % (max_pages - sink_pages) of its row of
  * block_table maps: opening a page beyond max_pages evicts the oldest one after
@@ -341,7 +341,7 @@ typedef struct OjasxKV4Cache {
 /* Rotates queries and keys by their positions and appends keys and values.
  * Rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32, num_sequences + 1) are
  * sequence b's tokens at positions start[b], start[b] + 1, ...; cu_seqlens NULL:
- * one token for each sequence.  q [num_tokens][num_q_heads][head_dim] and k, v
+ * one token for each sequence.  At most 2^25 tokens a call.  q [num_tokens][num_q_heads][head_dim] and k, v
  * [num_tokens][num_kv_heads][head_dim] in dtype F32, BF16 or F16, with element
  * strides of tokens and heads, rows 16-byte aligned.  Rotation in fp64, rounded
  * to fp32: q_out (and k_out, unless NULL) receive it in dtype, contiguous; the
@@ -385,7 +385,9 @@ OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q,
  * [num_q_tokens][num_heads][head_dim] contiguous in dtype; lse [num_q_tokens][num_heads]
  * fp32, the natural log of sum exp(scale * score), or NULL.  Keys that a row does
  * not see reach nothing, whatever they hold.  Rows of no sequence are left as
- * they are, or with zero_rest != 0 written as 0 (lse -inf). */
+ * they are, or with zero_rest != 0 written as 0 (lse -inf).  A call that would
+ * need 2^24 workgroups (blocks of 32 rows or more by up to four heads) is
+ * refused. */
 OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, long q_head_stride,
                                             const void *k, long k_token_stride, long k_head_stride,
                                             const void *v, long v_token_stride, long v_head_stride,
