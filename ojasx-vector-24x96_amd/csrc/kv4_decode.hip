@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
                 if (QP > 1) qf[QP - 1][jj][e] = (_Float16)(v - (float)a);
             }
         qsum = quarters_sum(qsum);
-        kq = p.scale / f;
+        kq = fmaxf(p.scale / f, 0x1p-126f);    // a query of zeros: never 0, which times a hidden score is NaN
     }
 
     f4_t acc[NJ][2];
