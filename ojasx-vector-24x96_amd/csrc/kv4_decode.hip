@@ -50,6 +50,7 @@
 // wave's way through its tiles: 16 sequences of 32000 held fp16 tokens, 16 heads of 64,
 // 15 us for 38 MB.  The merge is a second launch, 4 to 5 us.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -119,6 +120,12 @@ struct Runs {
         return tile < big ? tile / (q + 1) : r + (tile - big) / q;
     }
 };
+
+// A row's output of its weighted sum o, the weights' sum l and the largest score m.
+__device__ __forceinline__ float kv4_out(float o, float l, float m) {
+    return m == -INFINITY ? 0.f : o / l;         // l = 0: only scores of -inf, no softmax, NaN
+}
+
 // The tiles of all sequences, and those before sequence b.  Whole waves call it.
 __device__ __forceinline__ int kv4_all_tiles(const Kv4View &c, const int *seen, int b, int *before) {
     const int lane = threadIdx.x & 63;
@@ -368,7 +375,8 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         for (int i = 0; i < NI; ++i) vsr[i] = vsp[i];
 #pragma unroll
         for (int i = 0; i < NJ; ++i) load_words<4>(vp + i * 256, vw[i]);
-        const bool whole = held[0] + held[1] + held[2] + held[3] == 64;
+        const int held_all = held[0] + held[1] + held[2] + held[3];
+        const bool whole = held_all == 64;
         const int mine = pick(held, h) - 4 * NI * cp;     // of this copy's slots
         if (!whole) {           // what a slot without a token holds reaches nothing
 #pragma unroll
@@ -411,8 +419,11 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
             load_k();
             read_pages(tile + 2 * kNW);
         }
-        // ---- running maximum and the weights' power of two
-        const float mn = fmaxf(m, ceilf(quarters_max(tmax) * kq));
+        // ---- running maximum and the weights' power of two.  With a token held the
+        // maximum is finite, also where all scores are -inf: a sum of 0 then tells
+        // such a row, which is NaN, from one without tokens, which is 0.
+        const bool any = held_all > 0;
+        const float mn = fmaxf(fmaxf(m, any ? -FLT_MAX : -INFINITY), ceilf(quarters_max(tmax) * kq));
         const float fn = fminf(f, to_range(quarters_max((float)smax[0])));
         const float ref = mn == -INFINITY ? 0.f : mn;
         const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - ref);
@@ -534,7 +545,7 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
             ll = fmaf(a, sm[k / C][col][1], ll);
         }
         if (whole_sequence) {
-            store_act(static_cast<T_ *>(p.out), ((size_t)b * p.Hq + head0 + jj) * D + d, ll == 0.f ? 0.f : o / ll);
+            store_act(static_cast<T_ *>(p.out), ((size_t)b * p.Hq + head0 + jj) * D + d, kv4_out(o, ll, mm));
         } else {
             const size_t row = (size_t)(blockIdx.x + b) * p.Hq + head0 + jj;
             p.part_o[row * D + d] = o;
@@ -628,7 +639,7 @@ __global__ __launch_bounds__(kNT) void kv4_merge_kernel(Kv4DecodeParams p) {
     float v = 0.f;
 #pragma unroll
     for (int k = 0; k < SG; ++k) v += reinterpret_cast<const float *>(os[k])[tid];
-    store_act(out, tid, l == 0.f ? 0.f : v / l);
+    store_act(out, tid, kv4_out(v, l, m));
 }
 
 namespace {

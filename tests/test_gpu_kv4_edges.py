@@ -28,3 +28,51 @@ def test_decode_query_of_zeros(lc, dev, dtype, share):
     for scale in (-1.0, 4e-8, 1e-30, 1e-45):
         out = c.decode(q, i32(dev, lengths), scale)
         check_decode(out, q, hk, hv, lengths, share, dtype, 128 ** -0.5 if scale < 0 else scale, 32)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("share", [1, 4])
+def test_decode_scores_of_minus_infinity(lc, dev, dtype, share):
+    """A head whose held tokens all score -inf has no softmax: NaN, as the definition gives.  A
+    sequence without tokens, or with unmapped pages alone, stays 0."""
+    import torch
+    lengths = [1, 70, 300, 0, 20]
+    N, D = sum(lengths), 64
+    c = lc.PagedInt4KVCache(2, D, num_sequences=5, max_resident_pages=32, rope_theta=None, device=dev, num_pages=160)
+    c.block_table.copy_(torch.arange(160, dtype=torch.int32, device=dev).view(5, 32))
+    k = torch.ones(N, 2, D, device=dev)
+    k[..., 0] = 2                                          # lo 1, step 1 / 15, code 15: both terms of one sign
+    k = k.to(getattr(torch, dtype))
+    v = rand(dev, dtype, N, 2, D, seed=1)
+    c.append(k, v, i32(dev, [0] * 5), i32(dev, cum(lengths)))
+    c.block_table[4] = -1
+    q = rand(dev, dtype, 5, 2 * share, D, seed=2)
+    q[:, 0, 0] = -float("inf")
+    out = c.decode(q, i32(dev, lengths))
+    assert torch.isnan(out[:3, 0]).all()
+    assert torch.isfinite(out[:, 1:]).all() and not out[3:].any()
+    hk, hv = kv4.held(f64(k).astype(np.float32), 32), kv4.held(f64(v).astype(np.float32), 32)
+    q[:, 0], out[:3, 0] = 0, 0
+    hv0 = hv.copy()
+    if share == 1:
+        hv0[:, 0] = 0                                      # head 0 is the one left out
+        check_decode(out[:3], q[:3], hk, hv0, lengths[:3], share, dtype, 0.125, 32)
+
+
+@pytest.mark.parametrize("share", [1, 4])
+def test_decode_some_scores_past_fp32(lc, dev, share):
+    """Tokens whose score is below every fp32 value have no weight beside tokens that have one,
+    whichever wave or run they lie in."""
+    import torch
+    for first in (1, 64, 130, 1000):
+        n, D = first + 137, 64
+        c = lc.PagedInt4KVCache(1, D, max_resident_pages=128, rope_theta=None, device=dev)
+        k = torch.zeros(n, 1, D, device=dev)
+        k[:first] = 6e4
+        v = rand(dev, "float32", n, 1, D, seed=first)
+        c.append(k, v, i32(dev, [0]), i32(dev, [0, n]))
+        q = torch.full((1, share, D), -3e38, device=dev)
+        hv = kv4.held(f64(v).astype(np.float32), 32)[first:, 0]
+        # weights are equal: sums of 137 values in fp32, a pairwise order's error held to 16 half steps
+        got = f64(c.decode(q, i32(dev, [n])))[0]
+        assert (np.abs(got - hv.mean(0)) <= 16 * 2 ** -24 * np.abs(hv).max()).all(), first
