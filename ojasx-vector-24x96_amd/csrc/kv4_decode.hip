@@ -327,6 +327,7 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     // m: an integer no less than the largest score (log2), so that rescaling is
     // exact; f: the weights' power of two, which only falls
     float m = -INFINITY, l = 0.f, z = 0.f, f = kMostRange;
+    bool far = false;            // of any column of the wave
     const int *bt = p.c.bt + (size_t)b * p.c.max_pages;
     int page[4], blk[4], held[4];
     auto read_pages = [&](int tile) __attribute__((always_inline)) {
@@ -432,13 +433,30 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         f = fn;
         // bf16 outputs: the weights' factor 2^k goes into the exponent, and l and z
         // carry it as the products do; the others multiply the steps, exactly
-        const float shift = (WP == 1 ? (float)((int)(__float_as_uint(f) >> 23) - 127) : 0.f) - ref;
+        const float e = WP == 1 ? (float)((int)(__float_as_uint(f) >> 23) - 127) : 0.f;
+        float kw = kq, shift = e - ref;
         if (!__all(fa == 1.f)) {
+            far = __any(fabsf(ref) > 0x1p20f);
             if (WP == 1)
 #pragma unroll
                 for (int i = 0; i < NJ; ++i) acc[i][0] *= fa, acc[i][1] *= fa;
             l *= WP == 1 ? fa : alpha;
             z *= WP == 1 ? fa : alpha;
+        }
+        // A weight is exp2(score kq - ref), the product not rounded.  From 2^24 on the
+        // maximum is rounded by more than 1, and a weight could pass its type's range
+        // (or all of them be 0): there the product is rounded as the maximum was.
+        if (far) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float x = sc[i][r] * kq;
+                    asm volatile("" : "+v"(x));
+                    sc[i][r] = x - ref;
+                }
+            kw = 1.f;
+            shift = e;
         }
         // where the outputs have fp16's or fp32's bits a tile's products get an
         // accumulator of their own, added to the sum so far in one rounding per
@@ -456,7 +474,7 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const h2_t st = as_h2(vsr[i][r]);
-                const float pv = __builtin_amdgcn_exp2f(fmaf(sc[i][r], kq, shift));
+                const float pv = __builtin_amdgcn_exp2f(fmaf(sc[i][r], kw, shift));
                 l += pv;
                 z = fmaf(pv, base<true>(st), z);
                 wv[r] = pv * (WP == 1 ? (float)st[0] : (float)st[0] * f);

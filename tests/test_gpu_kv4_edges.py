@@ -76,3 +76,35 @@ def test_decode_some_scores_past_fp32(lc, dev, share):
         # weights are equal: sums of 137 values in fp32, a pairwise order's error held to 16 half steps
         got = f64(c.decode(q, i32(dev, [n])))[0]
         assert (np.abs(got - hv.mean(0)) <= 16 * 2 ** -24 * np.abs(hv).max()).all(), first
+
+
+@pytest.mark.parametrize("dtype,size", [("bfloat16", 1e2), ("bfloat16", 3e4), ("bfloat16", 1e8), ("bfloat16", 1e15),
+                                        ("float16", 1e3), ("float16", 6e3), ("float32", 3e4), ("float32", 1e8),
+                                        ("float32", 1e15)])
+@pytest.mark.parametrize("share", [1, 4])
+def test_decode_scores_far_apart(lc, dev, dtype, size, share):
+    """Scores of 2^17 to 2^60 and as far apart: all weight on the largest, which fp32 still tells
+    from the next (a head where it does not, by the scores' error in fp32, is only finite)."""
+    import torch
+    n, D, scale = 333, 128, 128 ** -0.5
+    c = lc.PagedInt4KVCache(1, D, max_resident_pages=64, rope_theta=None, device=dev)
+    k, v = rand(dev, dtype, n, 1, D, seed=1) * 5e3, rand(dev, dtype, n, 1, D, seed=2)
+    q = (rand(dev, dtype, 1, share, D, seed=3) * size).to(getattr(torch, dtype))
+    c.append(k, v, i32(dev, [0]), i32(dev, [0, n]))
+    hk, hv = kv4.held(f64(k).astype(np.float32), 32)[:, 0], kv4.held(f64(v).astype(np.float32), 32)[:, 0]
+    got = f64(c.decode(q, i32(dev, [n])))[0]
+    taken = 0
+    for h in range(share):
+        x = f64(q)[0, h]
+        s = hk @ x * scale
+        top = np.argsort(s)[::-1]
+        err = 16 * 2 ** -24 * 3 * (np.abs(x) * np.abs(hk).max(0)).sum() * scale      # as check_decode
+        assert np.abs(s).max() * 1.4427 > 2 ** 17 and np.isfinite(got[h]).all()
+        if s[top[0]] - s[top[1]] <= 2 * err + 40:
+            continue
+        taken += 1
+        want = hv[top[0]]
+        # one weight: fp16 of 2^-12 (bf16 outputs), two pieces else; the output rounds once
+        tol = np.abs(hv).max() * (2 ** -12 if dtype == "bfloat16" else 2 ** -21) + eps_half(dtype) * np.abs(want)
+        assert (np.abs(got[h] - want) <= tol + 1e-7 * (dtype == "float16")).all(), (h, got[h][:4], want[:4])
+    assert 4 * taken >= 3 * share
