@@ -500,7 +500,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                           ref, l, acc);
     if (row >= Lq) return;
     const size_t at = (size_t)(o.first + row) * p.Hq + head;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool none = lim < 0;                       // no key: 0; with keys l = 0 is no softmax, NaN
+    const float inv = 1.f / l;
     T *op = static_cast<T *>(p.out) + at * p.D;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -511,7 +512,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                 typedef decltype(E::from(0.f)) e4_t __attribute__((ext_vector_type(4)));
                 e4_t y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = E::from(l == 0.f ? 0.f : acc[t][4 * x + e] * inv);
+                for (int e = 0; e < 4; ++e) y[e] = E::from(none ? 0.f : acc[t][4 * x + e] * inv);
                 *reinterpret_cast<e4_t *>(op + d) = y;
             }
         }
@@ -747,7 +748,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             if (d < p.D) {
                 f32x4_t y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = l == 0.f ? 0.f : sum[t][4 * x + e] / l;
+                for (int e = 0; e < 4; ++e) y[e] = lim < 0 ? 0.f : sum[t][4 * x + e] / l;   // as in prompt_attn_kernel
                 *reinterpret_cast<f32x4_t *>(op + d) = y;
             }
         }
