@@ -416,12 +416,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
             // between the products of one 16 go the exponentials and the V reads of
             // the next.  They are rounded to the inputs' type, relative to their size
             // and each by itself, as the output is once more: over many keys the errors
-            // average out.  Their sum is of the unrounded ones, in fp32.
+            // average out.  Their sum is of the unrounded ones, in fp32, a tile's by itself
+            // first: many small weights beside a large one are not rounded away one by one.
             constexpr int NT2 = DP / 32, VB = NT2 < 4 ? NT2 : 4, PART = 8 / NT2;
             V8 pf[2 * NB];
+            float lt = 0.f;
             auto weight = [&](int f, int e) __attribute__((always_inline)) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[f >> 1][8 * (f & 1) + e], p.scale2, -ref));
-                l += x;
+                lt += x;
                 pf[f][e] = E::from(x);
             };
             // V operands (f, t) in order, VB of them read ahead
@@ -454,6 +456,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                     for (int e = 0; e < PART; ++e) weight(f + 1, t * PART + e);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            l += lt;
         }
         __builtin_amdgcn_s_setprio(0);
         if (tile + 1 < tiles) store(tile + 1);
@@ -674,12 +677,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
             raise_max<(DP <= 128)>(halves_max(t) * p.scale2, m, ref, l, acc);
             bf16x8_t pf[2][3];
+            float lt = 0.f;                              // a tile's sum by itself, as in prompt_attn_kernel
             constexpr int PART = NT2 < 4 ? 8 / NT2 : 2;
             auto weights = [&](int f, int e0, int e1) __attribute__((always_inline)) {
 #pragma unroll
                 for (int e = e0; e < e1; ++e) {
                     const float x = __builtin_amdgcn_exp2f(fmaf(s0[8 * f + e], p.scale2, -ref));
-                    l += x;
+                    lt += x;
                     const __bf16 h1 = (__bf16)x;
                     const float r1 = x - (float)h1;
                     const __bf16 h2 = (__bf16)r1;
@@ -717,6 +721,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                 if (i * PART < 8) weights(1, i * PART, i * PART + PART);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            l += lt;
         }
         if (BUFFERS == 1) {
             __syncthreads();

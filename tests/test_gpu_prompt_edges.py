@@ -43,3 +43,27 @@ def test_scores_of_minus_infinity(lc, dev, dtype, causal):
     few = a(q2, k[:7], v[:7], i32(dev, [0, N]), i32(dev, [0, 7]))
     if causal:
         assert not few[:N - 7].any()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_small_weights(lc, dev, dtype, D):
+    """One key that takes nearly all the weight and 60000 that have about 2^-25 of it each: their sum
+    is a share of 2^-9, held as exactly as any other."""
+    import torch
+    n, scale = 60000, 1.0
+    k = torch.zeros(n, 1, D, device=dev)
+    k[7, 0, 0] = 25.4 / 1.4427                             # log2 distance 25.4 to the others
+    k = k.to(getattr(torch, dtype))
+    v = torch.ones(n, 1, D, device=dev).to(k.dtype)
+    v[7] = 0
+    q = torch.zeros(3, 2, D, device=dev).to(k.dtype)
+    q[..., 0] = 1
+    a = lc.PackedPromptAttention(2, 1, D, causal=False, scale=scale)
+    got = f64(a(q, k, v, i32(dev, [0, 3]), i32(dev, [0, n])))
+    far = math.exp(-float(k[7, 0, 0]))
+    want = (n - 1) * far / (1 + (n - 1) * far)
+    # equal weights, so their roundings to the inputs' type are all alike: half a step of that type,
+    # of weights and sum; the fp32 sums of 60000 equal terms in blocks of 32, held to 2^-12
+    tol = want * (2 * eps_half(dtype) + 2 ** -12)
+    assert (np.abs(got - want) <= tol + 1e-7 * (dtype == "float16")).all(), (got.ravel()[:4], want)
