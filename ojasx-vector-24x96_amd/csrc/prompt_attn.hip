@@ -37,6 +37,7 @@ namespace ojx {
 
 namespace {
 constexpr int kKeys = 64;                        // keys per tile
+constexpr int kFlags = 16;                       // bytes of LDS behind the tiles: an int per wave
 // Workgroups up to which half as many rows go to each and the keys of a tile to two
 // waves: as many as are resident at once (three, two or one to a CU by head dim).
 // Below it the longest rows' way through their keys sets the time (1500 tokens of
@@ -66,6 +67,7 @@ struct PromptParams {
 struct Bf16 {
     typedef __hip_bfloat16 T;
     typedef bf16x8_t V8;
+    static constexpr int kInf = 0x7f80;          // an infinity's bits
     static __device__ __forceinline__ f32x16_t mma(V8 a, V8 b, f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
@@ -74,6 +76,7 @@ struct Bf16 {
 struct F16 {
     typedef __half T;
     typedef f16x8_t V8;
+    static constexpr int kInf = 0x7c00;
     static __device__ __forceinline__ f32x16_t mma(V8 a, V8 b, f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
@@ -168,40 +171,74 @@ __device__ __forceinline__ void raise_max(float t, float &m, float &ref, float &
     }
 }
 
-// The lane's row again, key by key, with hidden keys left out: acc, m / ref and l as
-// the tiles' passes leave them (dims 32 t + 4 h + key_of(r), and 16 c + 8 h .. of
-// the scores' halves).
-template <typename T, int DP>
-__device__ __forceinline__ void rows_again(const PromptParams &p, const T *q, const T *k, const T *v, int lim,
-                                           int lim_hi, int h, float &m, float &ref, float &l,
-                                           f32x16_t (&acc)[DP / 32]) {
-    m = -INFINITY;
-    l = 0.f;
+// The thread's number, for AGAIN hidden from the compiler: what it computes from it
+// anew would else stay in registers all through the first time.
+template <bool AGAIN>
+__device__ __forceinline__ int own_thread() {
+    int t = threadIdx.x;
+    if (AGAIN) asm volatile("" : "+v"(t));
+    return t;
+}
+
+enum { kDone, kOthersAgain, kAgain };
+
+// Whether a wave of the workgroup has `mine` set.  flags: an int of LDS per wave.
+__device__ __forceinline__ bool any_wave(int *flags, bool mine) {
+    const bool wave = __any(mine);
+    if ((threadIdx.x & 63) == 0) flags[threadIdx.x >> 6] = wave;
+    __syncthreads();
+    return flags[0] | flags[1] | flags[2] | flags[3];
+}
+
+// Exact pieces as split3_bf16 makes them, of any value: one that rounds past bf16's
+// range is cut to eight bits first, an infinity or NaN is the third piece alone.  That
+// piece takes part in one product, with the other operand's first piece, which has its
+// sign and is 0 only with it: the product is what the two values' own would be.
+__device__ __forceinline__ void split3_any(const float (&v)[8], bf16x8_t (&p)[3]) {
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
-    for (int key = 0; key <= lim_hi; ++key) {
-        float x = 0.f;
-        for (int c = 8 * h; c < p.D; c += 16)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x = fmaf(load_act(q, c + e), load_act(k, key * p.k_ts + c + e), x);
-        x = halves_sum(x) * p.scale2;
-        if (key > lim) continue;                 // the lane's; the loop is the wave's
-        const float mn = fmaxf(m, x), rn = mn == -INFINITY ? 0.f : mn;
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
-        const float pv = __builtin_amdgcn_exp2f(x - rn);
-        m = mn;
-        ref = rn;
-        l = fmaf(l, alpha, pv);
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int d = 32 * t + 4 * h + key_of(r);
-                if (d < p.D) acc[t][r] = fmaf(pv, load_act(v, key * p.v_ts + d), acc[t][r] * alpha);
-            }
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t u = __float_as_uint(v[i]), a = u & 0x7fffffffu;
+        const float f = a < 0x7f800000u ? v[i] : 0.f;
+        const __bf16 h1 = (__bf16)(a < 0x7f7f8000u ? f : __uint_as_float(u & 0xffff0000u));
+        const float r1 = f - (float)h1;
+        const __bf16 h2 = (__bf16)r1;
+        p[0][i] = a < 0x7f800000u ? h1 : (__bf16)0.f;
+        p[1][i] = a < 0x7f800000u ? h2 : (__bf16)0.f;
+        p[2][i] = a < 0x7f800000u ? (__bf16)(r1 - (float)h2) : (__bf16)v[i];
     }
+}
+
+// The infinities and NaN of a V operand, taken out of it: 1 for +inf, 2^7 for -inf,
+// 2^14 for NaN in their places, which a product with ones for the keys that a row sees
+// counts exactly (at most 64 keys), and what the counts add to an output.
+template <typename E>
+__device__ __forceinline__ typename E::V8 take_marks(typename E::V8 &v) {
+    typedef short s16x8_t __attribute__((ext_vector_type(8)));
+    s16x8_t z = __builtin_bit_cast(s16x8_t, v);
+    typename E::V8 m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int a = z[i] & 0x7fff;
+        m[i] = E::from(a < E::kInf ? 0.f : a > E::kInf ? 0x1p14f : z[i] < 0 ? 0x1p7f : 1.f);
+        if (a >= E::kInf) z[i] = 0;
+    }
+    v = __builtin_bit_cast(typename E::V8, z);
+    return m;
+}
+// Bit 15 or 31 of the result is set where one of v's values is an infinity or NaN.
+template <typename E>
+__device__ __forceinline__ uint32_t has_marks(const typename E::V8 &v) {
+    constexpr uint32_t inf = E::kInf * 0x10001u, one = (0x8000u - E::kInf) * 0x10001u;
+    const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+    uint32_t x = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x |= (w[i] & inf) + one;
+    return x;
+}
+__device__ __forceinline__ float from_marks(float counts) {
+    const int c = (int)counts;
+    const float up = (c & 127) ? INFINITY : 0.f, down = (c >> 7 & 127) ? -INFINITY : 0.f;
+    return c >> 14 ? NAN : up + down;
 }
 
 // Hides the keys past `lim` from the lane's row; k0 = the tile's first key.
@@ -214,6 +251,16 @@ __device__ __forceinline__ void mask_tile(f32x16_t (&s)[NB], int lim, int k0, in
         if (key_of(r) > rel) s[0][r] = -INFINITY;
         if (NB > 1 && 32 + key_of(r) > rel) s[NB - 1][r] = -INFINITY;
     }
+}
+
+// Ones for the keys of operand f (as the weights lie in it) that come before `rel` or at
+// it, counted from the lane's first.
+template <typename E>
+__device__ __forceinline__ typename E::V8 seen_keys(int f, int rel) {
+    typename E::V8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = E::from(32 * (f >> 1) + key_of(8 * (f & 1) + e) <= rel ? 1.f : 0.f);
+    return x;
 }
 }  // namespace
 
@@ -287,24 +334,27 @@ __device__ __forceinline__ void zero_rows(const PromptParams &p, const PromptBlo
 // the other half the last 32, and the pairs join their sums in LDS: twice the
 // workgroups with half the work in a row, for grids too small to hide how long
 // their longest rows take.
-template <typename E, int DP, int KS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : DP > 64 ? 2 : 3))) void prompt_attn_kernel(
-    PromptParams p, int slots) {
+//
+// AGAIN: with V's infinities and NaN taken out of the product.  Returns what is left to do again: kAgain where the wave's rows are
+// not written yet, kOthersAgain where other waves' are not.  mine: the wave's rows are
+// to be written (the others of AGAIN help with the tiles).
+template <typename E, int DP, int KS, bool AGAIN>
+__device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slots, bool mine) {
     typedef typename E::T T;
     typedef typename E::V8 V8;
     constexpr int NW = 4, WR = NW / KS, NB = 2 / KS;  // waves of different rows, 32-key blocks of a wave
     constexpr int NT = 64 * NW, ROWB = 2 * DP, UPR = DP / 8, TILE = kKeys * ROWB;
     constexpr int CH = kKeys * UPR / NT;             // 16-byte units of a tile per thread
-    extern __shared__ __align__(16) unsigned char sm[];   // [2 buffers][K tile, V tile]
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    extern __shared__ __align__(16) unsigned char sm[];   // [2 buffers][K tile, V tile], flags
+    const int tid = own_thread<AGAIN>(), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int wr = w % WR, kb = KS == 1 ? 0 : 32 * (w / WR);    // the wave's keys begin at kb
     const int bm_shift = 5 + __builtin_ctz(WR) - p.hw;
     PromptBlock o;
-    if (!prompt_block(p, slots, bm_shift, o)) return;
+    if (!prompt_block(p, slots, bm_shift, o)) return kDone;
     if (o.b < 0 || o.b >= p.B) {
         zero_rows<T>(p, o, bm_shift);
-        return;
+        return kDone;
     }
     const int head = o.head0 + (wr & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
     const int Lq = o.len, Lk = o.Lk, off = Lk - Lq;
@@ -313,7 +363,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;       // last key the row sees
     const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;    // the wave's least,
-    const int lim_hi = p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;   // and most
+    const int lim_hi = !mine ? -1 : p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;   // and most
     const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
     const int tiles = last < 0 ? 0 : last / kKeys + 1;
 
@@ -437,6 +487,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                     vf[i % (2 * VB)][y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
                 }
             };
+            auto v_of = [&](int i) __attribute__((always_inline)) {
+                return __builtin_bit_cast(V8, __builtin_shufflevector(vf[i % (2 * VB)][0], vf[i % (2 * VB)][1], 0, 1, 2, 3,
+                                                                      4, 5, 6, 7));
+            };
+            if constexpr (AGAIN) {
+#pragma unroll
+                for (int i = 0; i < 16 * NB; ++i) weight(i / 8, i % 8);
+#pragma unroll
+                for (int t = 0; t < NT2; ++t) {
+                    V8 z[2 * NB];
+                    uint32_t has = 0;
+#pragma unroll
+                    for (int f = 0; f < 2 * NB; ++f) {
+                        read_v(f * NT2 + t);
+                        z[f] = v_of(f * NT2 + t);
+                        has |= has_marks<E>(z[f]);
+                    }
+                    if (__any((has & 0x80008000u) != 0)) {
+                        f32x16_t marks = {};
+#pragma unroll
+                        for (int f = 0; f < 2 * NB; ++f)
+                            marks = E::mma(take_marks<E>(z[f]), seen_keys<E>(f, lim - k0 - 4 * h), marks);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[t][r] += from_marks(marks[r]);
+                    }
+#pragma unroll
+                    for (int f = 0; f < 2 * NB; ++f) acc[t] = E::mma(z[f], pf[f], acc[t]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
 #pragma unroll
             for (int i = 0; i < VB; ++i) read_v(i);
             __builtin_amdgcn_sched_barrier(0);
@@ -448,13 +528,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
                 const int f = i / NT2, t = i % NT2;
                 if (i + VB < 2 * NB * NT2) read_v(i + VB);
                 __builtin_amdgcn_sched_barrier(0);
-                typedef short s16x8_t __attribute__((ext_vector_type(8)));
-                const s16x8_t z = __builtin_shufflevector(vf[i % (2 * VB)][0], vf[i % (2 * VB)][1], 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[t] = E::mma(__builtin_bit_cast(V8, z), pf[f], acc[t]);
+                acc[t] = E::mma(v_of(i), pf[f], acc[t]);
                 if (f < 2 * NB - 1)
 #pragma unroll
                     for (int e = 0; e < PART; ++e) weight(f + 1, t * PART + e);
                 __builtin_amdgcn_sched_barrier(0);
+            }
             }
             l += lt;
         }
@@ -462,11 +541,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
         if (tile + 1 < tiles) store(tile + 1);
     }
     l = halves_sum(l);
+    // A weight of 0 times an infinity or a NaN is a NaN in the matrix product: an
+    // output that is NaN may come from a key its row does not see.  Where a wave has
+    // one, the workgroup goes through its keys once more, with
+    // V's infinities and NaN taken out of the product and counted in one of their own
+    // over the keys that each row sees.  16384 bf16 tokens, 32 / 8 heads of 128: 2.3 ms, with
+    // one NaN among the values 5.0, with nothing but NaN 11.3 (4096 tokens: 0.15, 0.35,
+    // 0.83); fp32, 4096 tokens: 0.74, 1.7, 2.6.
+    int *flags = reinterpret_cast<int *>(sm + 4 * TILE);
+    bool redo = false;
+    if (!AGAIN) {
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) redo |= acc[t][r] != acc[t][r];
+        redo = __any(redo);
+    }
     if (KS == 2) {
         // [row wave][acc registers, m, l][lane]
         constexpr int REGS = DP / 2 + 2;
         float *pair = reinterpret_cast<float *>(sm) + wr * REGS * 64 + lane;
-        __syncthreads();
+        if (any_wave(flags, redo)) return kAgain;    // a barrier: the tiles are done with
         if (kb) {
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
@@ -476,7 +571,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
             pair[(REGS - 1) * 64] = l;
         }
         __syncthreads();
-        if (kb) return;
+        if (kb) return kDone;
         const float m1 = pair[(REGS - 2) * 64], mn = fmaxf(m, m1);
         ref = mn == -INFINITY ? 0.f : mn;
         const float a0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - ref);
@@ -488,38 +583,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[t][r] = fmaf(a0, acc[t][r], a1 * pair[(16 * t + r) * 64]);
     }
-    // A weight of 0 times an infinity or a NaN is a NaN in the matrix product: an
-    // output that is NaN may come from a key its row does not see.  Where the
-    // wave has one, its rows run again, key by key, with hidden keys left out.
-    bool again = false;
+    if (row < Lq && !redo && mine) {
+        const size_t at = (size_t)(o.first + row) * p.Hq + head;
+        const bool none = lim < 0;                   // no key: 0; with keys l = 0 is no softmax, NaN
+        const float inv = 1.f / l;
+        T *op = static_cast<T *>(p.out) + at * p.D;
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+        for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) again |= acc[t][r] != acc[t][r];
-    if (__any(again))
-        rows_again<T, DP>(p, static_cast<const T *>(p.q) + (long)(o.first + qrow) * p.q_ts + head * p.q_hs,
-                          static_cast<const T *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs,
-                          static_cast<const T *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs, lim, lim_hi, h, m,
-                          ref, l, acc);
-    if (row >= Lq) return;
-    const size_t at = (size_t)(o.first + row) * p.Hq + head;
-    const bool none = lim < 0;                       // no key: 0; with keys l = 0 is no softmax, NaN
-    const float inv = 1.f / l;
-    T *op = static_cast<T *>(p.out) + at * p.D;
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * t + 8 * x + 4 * h;
+                if (d < p.D) {
+                    typedef decltype(E::from(0.f)) e4_t __attribute__((ext_vector_type(4)));
+                    e4_t y;
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int d = 32 * t + 8 * x + 4 * h;
-            if (d < p.D) {
-                typedef decltype(E::from(0.f)) e4_t __attribute__((ext_vector_type(4)));
-                e4_t y;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = E::from(none ? 0.f : acc[t][4 * x + e] * inv);
-                *reinterpret_cast<e4_t *>(op + d) = y;
+                    for (int e = 0; e < 4; ++e) y[e] = E::from(none ? 0.f : acc[t][4 * x + e] * inv);
+                    *reinterpret_cast<e4_t *>(op + d) = y;
+                }
             }
-        }
-    if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+        if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+    if (AGAIN || KS == 2 || !any_wave(flags, redo)) return kDone;
+    return redo ? kAgain : kOthersAgain;
+}
+
+template <typename E, int DP, int KS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : DP > 64 ? 2 : 3))) void prompt_attn_kernel(
+    PromptParams p, int slots) {
+    const int left = prompt_block_attn<E, DP, KS, false>(p, slots, true);
+    if (left != kDone) prompt_block_attn<E, DP, KS, true>(p, slots, left == kAgain);
 }
 
 // fp32 on v_mfma_f32_32x32x16_bf16: every operand as three bf16 pieces whose sum it
@@ -534,21 +626,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 
 // split goes between the products of the tile before (head dims past 128 have LDS for
 // one buffer and split between barriers).  One wave per SIMD, for the registers of two
 // sets of accumulators; with Q and the sets held in accumulation registers 147 us.
-template <int DP, int BUFFERS>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void prompt_attn_f32_kernel(PromptParams p,
-                                                                                                        int slots) {
+//
+// AGAIN: as in prompt_block_attn, and with pieces that hold any value.
+template <int DP, int BUFFERS, bool AGAIN>
+__device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots, bool mine) {
     constexpr int NW = 4, NT = 64 * NW, ROWB = 2 * DP, UPR = DP / 8, KEYS = 32, PLANE = KEYS * ROWB;
     constexpr int CH = KEYS * UPR / NT, NT2 = DP / 32, NC = DP / 16;
     constexpr int SETS = DP > 128 ? 1 : 2;           // of output accumulators
-    extern __shared__ __align__(16) unsigned char sm[];   // [buffer][K pieces, V pieces][32 keys]
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    extern __shared__ __align__(16) unsigned char sm[];   // [buffer][K pieces, V pieces][32 keys], flags
+    const int tid = own_thread<AGAIN>(), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int bm_shift = 5 + __builtin_ctz(NW) - p.hw;
     PromptBlock o;
-    if (!prompt_block(p, slots, bm_shift, o)) return;
+    if (!prompt_block(p, slots, bm_shift, o)) return kDone;
     if (o.b < 0 || o.b >= p.B) {
         zero_rows<float>(p, o, bm_shift);
-        return;
+        return kDone;
     }
     const int head = o.head0 + (w & ((1 << p.hw) - 1)), kvh = o.head0 / (p.Hq / p.Hkv);
     const int Lq = o.len, Lk = o.Lk, off = Lk - Lq;
@@ -557,7 +650,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;
     const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;
-    const int lim_hi = p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;
+    const int lim_hi = !mine ? -1 : p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;
     const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
     const int tiles = last < 0 ? 0 : last / KEYS + 1;
 
@@ -572,7 +665,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = a[e], x[4 + e] = b[e];
         }
-        split3_bf16(x, qf[c]);
+        if (AGAIN) split3_any(x, qf[c]);
+        else split3_bf16(x, qf[c]);
     }
     const int su = tid % UPR, sr = tid / UPR;
     const bool in = su * 8 < p.D;
@@ -598,7 +692,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = p.D < DP && !in ? 0.f : (j & 1 ? vr : kr)[i][e / 4][e % 4];
         bf16x8_t y[3];
-        split3_bf16(x, y);
+        if (AGAIN) split3_any(x, y);
+        else split3_bf16(x, y);
 #pragma unroll
         for (int z = 0; z < 3; ++z)
             if (j & 1)
@@ -677,7 +772,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
             raise_max<(DP <= 128)>(halves_max(t) * p.scale2, m, ref, l, acc);
             bf16x8_t pf[2][3];
-            float lt = 0.f;                              // a tile's sum by itself, as in prompt_attn_kernel
+            float lt = 0.f;                              // a tile's sum by itself, as in prompt_block_attn
             constexpr int PART = NT2 < 4 ? 8 / NT2 : 2;
             auto weights = [&](int f, int e0, int e1) __attribute__((always_inline)) {
 #pragma unroll
@@ -704,6 +799,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                         vf[i % 2][x][y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
                     }
             };
+            auto v_of = [&](int i, bf16x8_t (&z)[3]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+                    z[x] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vf[i % 2][x][0], vf[i % 2][x][1], 0, 1, 2,
+                                                                               3, 4, 5, 6, 7));
+            };
+            if constexpr (AGAIN) {                   // infinities and NaN are in the third pieces alone
+                weights(0, 0, 8);
+                weights(1, 0, 8);
+#pragma unroll
+                for (int t2 = 0; t2 < NT2; ++t2) {
+                    bf16x8_t z[2][3];
+                    uint32_t has = 0;
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) {
+                        read_v(f * NT2 + t2);
+                        v_of(f * NT2 + t2, z[f]);
+                        has |= has_marks<Bf16>(z[f][2]);
+                    }
+                    if (__any((has & 0x80008000u) != 0)) {
+                        f32x16_t marks = {};
+#pragma unroll
+                        for (int f = 0; f < 2; ++f)
+                            marks = Bf16::mma(take_marks<Bf16>(z[f][2]), seen_keys<Bf16>(f, lim - k0 - 4 * h), marks);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[t2][r] += from_marks(marks[r]);
+                    }
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) mma6(z[f], pf[f], acc[t2], acc[(SETS - 1) * NT2 + t2]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
             read_v(0);
             __builtin_amdgcn_sched_barrier(0);
             weights(0, 0, 8);
@@ -713,13 +840,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                 if (i + 1 < 2 * NT2) read_v(i + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 bf16x8_t z[3];
-#pragma unroll
-                for (int x = 0; x < 3; ++x)
-                    z[x] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vf[i % 2][x][0], vf[i % 2][x][1], 0, 1, 2,
-                                                                               3, 4, 5, 6, 7));
+                v_of(i, z);
                 mma6(z, pf[i / NT2], acc[i % NT2], acc[(SETS - 1) * NT2 + i % NT2]);
                 if (i * PART < 8) weights(1, i * PART, i * PART + PART);
                 __builtin_amdgcn_sched_barrier(0);
+            }
             }
             l += lt;
         }
@@ -730,34 +855,41 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     l = halves_sum(l);
     f32x16_t sum[NT2];
-    bool again = false;                              // as in prompt_attn_kernel
+    bool redo = false;                               // as in prompt_block_attn
 #pragma unroll
     for (int t = 0; t < NT2; ++t) {
         sum[t] = acc[t];
         if (SETS == 2) sum[t] += acc[(SETS - 1) * NT2 + t];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) again |= sum[t][r] != sum[t][r];
+        for (int r = 0; r < 16; ++r) redo |= sum[t][r] != sum[t][r];
     }
-    if (__any(again))
-        rows_again<float, DP>(p, qp, static_cast<const float *>(p.k) + (long)o.k_first * p.k_ts + kvh * p.k_hs,
-                              static_cast<const float *>(p.v) + (long)o.k_first * p.v_ts + kvh * p.v_hs, lim, lim_hi, h,
-                              m, ref, l, sum);
-    if (row >= Lq) return;
-    const size_t at = (size_t)(o.first + row) * p.Hq + head;
-    float *op = static_cast<float *>(p.out) + at * p.D;
+    redo = !AGAIN && __any(redo);
+    if (row < Lq && !redo && mine) {
+        const size_t at = (size_t)(o.first + row) * p.Hq + head;
+        float *op = static_cast<float *>(p.out) + at * p.D;
 #pragma unroll
-    for (int t = 0; t < NT2; ++t)
+        for (int t = 0; t < NT2; ++t)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int d = 32 * t + 8 * x + 4 * h;
-            if (d < p.D) {
-                f32x4_t y;
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * t + 8 * x + 4 * h;
+                if (d < p.D) {
+                    f32x4_t y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = lim < 0 ? 0.f : sum[t][4 * x + e] / l;   // as in prompt_attn_kernel
-                *reinterpret_cast<f32x4_t *>(op + d) = y;
+                    for (int e = 0; e < 4; ++e) y[e] = lim < 0 ? 0.f : sum[t][4 * x + e] / l;   // as in prompt_block_attn
+                    *reinterpret_cast<f32x4_t *>(op + d) = y;
+                }
             }
-        }
-    if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+        if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+    if (AGAIN || !any_wave(reinterpret_cast<int *>(sm + BUFFERS * 6 * PLANE), redo)) return kDone;
+    return redo ? kAgain : kOthersAgain;
+}
+
+template <int DP, int BUFFERS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void prompt_attn_f32_kernel(PromptParams p,
+                                                                                                        int slots) {
+    const int left = prompt_block_f32<DP, BUFFERS, false>(p, slots, true);
+    if (left != kDone) prompt_block_f32<DP, BUFFERS, true>(p, slots, left == kAgain);
 }
 
 namespace {
@@ -787,7 +919,7 @@ int prepare(const void *fn, PromptParams &p, int wr, size_t lds, size_t *granted
 template <typename E, int DP, int KS>
 int launch16_split(PromptParams p, hipStream_t st) {
     static size_t granted = 0;
-    const size_t lds = (size_t)4 * kKeys * 2 * DP;
+    const size_t lds = (size_t)4 * kKeys * 2 * DP + kFlags;
     int slots;
     unsigned groups;
     const int rc = prepare(reinterpret_cast<const void *>(&prompt_attn_kernel<E, DP, KS>), p, 4 / KS, lds, &granted,
@@ -806,7 +938,7 @@ int launch16(const PromptParams &p, hipStream_t st) {
 template <int DP, int BUFFERS>
 int launch32(PromptParams p, hipStream_t st) {
     static size_t granted = 0;
-    const size_t lds = (size_t)BUFFERS * 6 * 32 * 2 * DP;
+    const size_t lds = (size_t)BUFFERS * 6 * 32 * 2 * DP + kFlags;
     int slots;
     unsigned groups;
     const int rc = prepare(reinterpret_cast<const void *>(&prompt_attn_f32_kernel<DP, BUFFERS>), p, 4, lds, &granted,

@@ -67,3 +67,119 @@ def test_many_small_weights(lc, dev, dtype, D):
     # of weights and sum; the fp32 sums of 60000 equal terms in blocks of 32, held to 2^-12
     tol = want * (2 * eps_half(dtype) + 2 ** -12)
     assert (np.abs(got - want) <= tol + 1e-7 * (dtype == "float16")).all(), (got.ravel()[:4], want)
+
+
+@pytest.mark.parametrize("dtype,D", [(t, D) for t in TYPES for D in (64, 128, 256)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 2), (16, 16)])
+def test_infinities_that_many_rows_see(lc, dev, dtype, D, bad, Hq, Hkv):
+    """One value, one key entry that later rows see and earlier rows do not, in prompts of several
+    tiles and blocks: the value reaches its own dimension of the rows that see it, as itself; the
+    key's rows are what their dot products give; all else is as ever."""
+    import torch
+    lengths = [450, 70, 333]
+    N, cu = sum(lengths), cum(lengths)
+    q, k, v = (rand(dev, dtype, N, h, D, seed=s) for h, s in ((Hq, 1), (Hkv, 2), (Hkv, 3)))
+    share = Hq // Hkv
+    a = lc.PackedPromptAttention(Hq, Hkv, D)
+    v2, k2 = v.clone(), k.clone()
+    v2[140, 0, 3] = v2[cu[1] + 69, 1, 5] = bad             # a value of sequence 0, the last of sequence 1
+    k2[cu[2] + 100, 1, 2] = bad                            # a key of sequence 2
+    out, lse = a(q, k2, v2, i32(dev, cu), return_lse=True)
+    got = f64(out)
+    seen = np.zeros(got.shape, bool)
+    seen[140:450, :share, 3] = seen[cu[1] + 69, share:2 * share, 5] = True
+    if math.isnan(bad):
+        assert np.isnan(got[seen]).all()
+    else:
+        assert (got[seen] == bad).all()
+    # of the key's rows those whose score is +inf or NaN are NaN; a score of -inf weighs nothing
+    rows = slice(cu[2] + 100, N)
+    score = f64(q)[rows, share:2 * share, 2] * bad
+    lost = ~(score == -math.inf)
+    assert np.isnan(got[rows, share:2 * share][lost]).all()
+    seen[rows, share:2 * share] |= lost[..., None]
+    for b in range(3):
+        s = slice(cu[b], cu[b + 1])
+        n = lengths[b]
+        for h in range(Hq):
+            kh, vh = f64(k2)[s, h // share], f64(v2)[s, h // share]
+            # the oracle's sums have no infinite or NaN terms: a key that scores -inf is left out by
+            # rows of its own, values at `seen` are not compared
+            vh = np.where(np.isfinite(vh), vh, 0)
+            clean, _ = kv4.attention(f64(q)[s, h], f64(k)[s, h // share], vh, D ** -0.5, np.arange(n) + 1)
+            if b == 2 and h // share == 1:
+                x = f64(q)[s, h]
+                for i in range(100, n):
+                    if not lost[i - 100, h - share]:
+                        keep = np.r_[0:100, 101:i + 1]
+                        clean[i] = kv4.attention(x[i:i + 1], kh[keep], vh[keep], D ** -0.5)[0][0]
+            absw = np.abs(vh).max()
+            score_err = 2 ** -24 * (16 * D ** -0.5 * np.abs(f64(q)[s, h]).max(0) @ np.abs(f64(k)[s, h // share]).max(0) + 30)
+            tol = absw * (2 * score_err + (eps_half(dtype) if dtype != "float32" else 0) + 2 ** -22)
+            tol = tol + eps_half(dtype) * np.abs(clean) + 1e-7 * (dtype == "float16")
+            ok = (np.abs(got[s, h] - clean) <= tol) | seen[s, h]
+            assert ok.all(), (b, h, np.argwhere(~ok)[:3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_huge_finite_values(lc, dev, dtype):
+    """Values at the type's largest (past bfloat16's range for float32): finite weights of them are
+    finite, hidden ones reach nothing."""
+    import torch
+    n, D = 200, 128
+    most = torch.finfo(getattr(torch, dtype)).max
+    q, k, v = (rand(dev, dtype, n, h, D, seed=s) for h, s in ((2, 1), (1, 2), (1, 3)))
+    k.zero_()                                              # weights of 1: the sums stay in range
+    v[150, 0] = most
+    v[90, 0, :7] = -most
+    out = f64(lc.PackedPromptAttention(2, 1, D)(q, k, v, i32(dev, [0, n])))
+    for h in range(2):
+        want, _ = kv4.attention(f64(q)[:, h], f64(k)[:, 0], f64(v)[:, 0], D ** -0.5, np.arange(n) + 1)
+        absw, _ = kv4.attention(f64(q)[:, h], f64(k)[:, 0], np.abs(f64(v)[:, 0]), D ** -0.5, np.arange(n) + 1)
+        score = 2 ** -24 * (16 * D ** -0.5 * np.abs(f64(q)[:, h]).max(0) @ np.abs(f64(k)[:, 0]).max(0) + 30)
+        # the sums of equal weights run key by key over up to 95 keys where a tile has hidden values:
+        # as many half steps of fp32, at worst, and 33 for the rest
+        tol = absw * (2 * score + (eps_half(dtype) if dtype != "float32" else 0) + 2 ** -17) + eps_half(dtype) * np.abs(want)
+        assert (np.abs(out[:, h] - want) <= tol + 1e-7 * (dtype == "float16")).all()
+
+
+def test_a_nan_does_not_stall_a_batch(lc, dev):
+    """One NaN among the values that almost all rows see costs a second pass, not a walk over every
+    key: a call of 4096 tokens takes less than six times as long with it."""
+    import torch
+    n, D = 4096, 128
+    q, k, v = (rand(dev, "bfloat16", n, h, D, seed=s) for h, s in ((32, 1), (8, 2), (8, 3)))
+    a = lc.PackedPromptAttention(32, 8, D)
+    cu = i32(dev, [0, n])
+
+    def took(v):
+        a(q, k, v, cu)
+        best = math.inf
+        for _ in range(5):
+            t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            t[0].record()
+            a(q, k, v, cu)
+            t[1].record()
+            torch.cuda.synchronize()
+            best = min(best, t[0].elapsed_time(t[1]))
+        return best
+
+    v2 = v.clone()
+    v2[100, :, 3] = float("nan")
+    assert took(v2) < 6 * took(v)
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,n", [("bfloat16", 4, 2, 400), ("bfloat16", 32, 32, 900), ("float32", 4, 1, 300)])
+def test_out_is_the_query_with_a_nan(lc, dev, dtype, Hq, Hkv, n):
+    """A second pass reads the queries again: rows already written into them take no part."""
+    import torch
+    q, k, v = (rand(dev, dtype, n, h, 64, seed=s) for h, s in ((Hq, 1), (Hkv, 2), (Hkv, 3)))
+    v[n // 2, 0, 3] = float("nan")
+    k[n // 3, Hkv - 1, 3] = float("inf")
+    cu = i32(dev, [0, 3, 3, n - 50, n])
+    a = lc.PackedPromptAttention(Hq, Hkv, 64)
+    want, lse = a(q, k, v, cu, return_lse=True)
+    got, l2 = a(q, k, v, cu, out=q, return_lse=True)
+    assert got is q and torch.equal(q.isnan(), want.isnan()) and torch.equal(q.nan_to_num(7), want.nan_to_num(7))
+    assert torch.equal(l2.nan_to_num(7), lse.nan_to_num(7)) and want.isnan().any()
