@@ -45,6 +45,10 @@ constexpr int kFlags = 16;                       // bytes of LDS behind the tile
 // 36.0), above it the splits' own cost (2048 tokens of 32 / 8 heads of 128: 536, 54.4
 // -> 57.7; 4096 of 16 / 2 of 256: 524, 190 -> 284).
 constexpr long split_below(int DP) { return 256 * (DP <= 64 ? 3 : DP <= 128 ? 2 : 1); }
+// A weight is 2^(score scale - max), the product not rounded.  From 2^24 on the maximum
+// is rounded by more than 1, and a weight could pass its type's range, or all of them
+// be 0: scores past this are rounded as their maximum is (rounded_score).
+constexpr float kFar = 0x1p20f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -169,6 +173,13 @@ __device__ __forceinline__ void raise_max(float t, float &m, float &ref, float &
             if (ACC) scale_acc(acc[i], alpha);
             else acc[i] *= alpha;
     }
+}
+
+// A score as the maximum holds it: the product rounded before anything is subtracted.
+__device__ __forceinline__ float rounded_score(float s, float scale2) {
+    float x = s * scale2;
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 // The thread's number, for AGAIN hidden from the compiler: what it computes from it
@@ -335,7 +346,8 @@ __device__ __forceinline__ void zero_rows(const PromptParams &p, const PromptBlo
 // workgroups with half the work in a row, for grids too small to hide how long
 // their longest rows take.
 //
-// AGAIN: with V's infinities and NaN taken out of the product.  Returns what is left to do again: kAgain where the wave's rows are
+// AGAIN: with scores rounded as their maximum is, and V's infinities and NaN taken out
+// of the product.  Returns what is left to do again: kAgain where the wave's rows are
 // not written yet, kOthersAgain where other waves' are not.  mine: the wave's rows are
 // to be written (the others of AGAIN help with the tiles).
 template <typename E, int DP, int KS, bool AGAIN>
@@ -462,6 +474,11 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
 #pragma unroll
             for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[NB - 1][r]);
             raise_max<false>(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
+            if (AGAIN)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[b][r] = rounded_score(s[b][r], p.scale2) - ref;
             // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block);
             // between the products of one 16 go the exponentials and the V reads of
             // the next.  They are rounded to the inputs' type, relative to their size
@@ -472,7 +489,8 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
             V8 pf[2 * NB];
             float lt = 0.f;
             auto weight = [&](int f, int e) __attribute__((always_inline)) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[f >> 1][8 * (f & 1) + e], p.scale2, -ref));
+                const float y = s[f >> 1][8 * (f & 1) + e];
+                const float x = __builtin_amdgcn_exp2f(AGAIN ? y : fmaf(y, p.scale2, -ref));
                 lt += x;
                 pf[f][e] = E::from(x);
             };
@@ -543,7 +561,7 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
     l = halves_sum(l);
     // A weight of 0 times an infinity or a NaN is a NaN in the matrix product: an
     // output that is NaN may come from a key its row does not see.  Where a wave has
-    // one, the workgroup goes through its keys once more, with
+    // one, or a maximum past kFar, the workgroup goes through its keys once more, with
     // V's infinities and NaN taken out of the product and counted in one of their own
     // over the keys that each row sees.  16384 bf16 tokens, 32 / 8 heads of 128: 2.3 ms, with
     // one NaN among the values 5.0, with nothing but NaN 11.3 (4096 tokens: 0.15, 0.35,
@@ -551,6 +569,7 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
     int *flags = reinterpret_cast<int *>(sm + 4 * TILE);
     bool redo = false;
     if (!AGAIN) {
+        redo = fabsf(m) > kFar && m != -INFINITY;
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
@@ -771,13 +790,16 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
 #pragma unroll
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
             raise_max<(DP <= 128)>(halves_max(t) * p.scale2, m, ref, l, acc);
+            if (AGAIN)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s0[r] = rounded_score(s0[r], p.scale2) - ref;
             bf16x8_t pf[2][3];
             float lt = 0.f;                              // a tile's sum by itself, as in prompt_block_attn
             constexpr int PART = NT2 < 4 ? 8 / NT2 : 2;
             auto weights = [&](int f, int e0, int e1) __attribute__((always_inline)) {
 #pragma unroll
                 for (int e = e0; e < e1; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(s0[8 * f + e], p.scale2, -ref));
+                    const float x = __builtin_amdgcn_exp2f(AGAIN ? s0[8 * f + e] : fmaf(s0[8 * f + e], p.scale2, -ref));
                     lt += x;
                     const __bf16 h1 = (__bf16)x;
                     const float r1 = x - (float)h1;
@@ -855,7 +877,7 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
     }
     l = halves_sum(l);
     f32x16_t sum[NT2];
-    bool redo = false;                               // as in prompt_block_attn
+    bool redo = fabsf(m) > kFar && m != -INFINITY;   // as in prompt_block_attn
 #pragma unroll
     for (int t = 0; t < NT2; ++t) {
         sum[t] = acc[t];

@@ -183,3 +183,32 @@ def test_out_is_the_query_with_a_nan(lc, dev, dtype, Hq, Hkv, n):
     got, l2 = a(q, k, v, cu, out=q, return_lse=True)
     assert got is q and torch.equal(q.isnan(), want.isnan()) and torch.equal(q.nan_to_num(7), want.nan_to_num(7))
     assert torch.equal(l2.nan_to_num(7), lse.nan_to_num(7)) and want.isnan().any()
+
+
+@pytest.mark.parametrize("dtype,size", [("bfloat16", 3e3), ("bfloat16", 3e4), ("bfloat16", 1e8), ("bfloat16", 1e15),
+                                        ("float16", 3e3), ("float16", 6e3), ("float32", 3e4), ("float32", 1e8),
+                                        ("float32", 1e15)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scores_far_apart(lc, dev, dtype, size, D):
+    """Scores of 2^23 to 2^100 and as far apart: all weight on the largest, which fp32 still tells from
+    the next (rows where it does not are left out: a few)."""
+    import torch
+    n, scale = 200, D ** -0.5
+    q, k, v = (rand(dev, dtype, n, h, D, seed=s) for h, s in ((2, 1), (1, 2), (1, 3)))
+    q, k = ((x * size).to(x.dtype) for x in (q, k))
+    out, lse = lc.PackedPromptAttention(2, 1, D)(q, k, v, i32(dev, [0, n]), return_lse=True)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    qf, kf, vf, o = f64(q), f64(k)[:, 0], f64(v)[:, 0], f64(out)
+    taken = 0
+    for h in range(2):
+        for i in range(n):
+            s = kf[:i + 1] @ qf[i, h] * scale
+            top = np.argsort(s)[::-1]
+            err = 16 * 2 ** -24 * scale * (np.abs(kf[:i + 1]).max(0) * np.abs(qf[i, h])).sum()
+            assert abs(f64(lse)[i, h] - s.max()) <= 2 * err + 1
+            if i and s[top[0]] - s[top[1]] < 2 * err + 40:
+                continue
+            taken += 1
+            want = vf[top[0]]
+            assert (np.abs(o[i, h] - want) <= (eps_half(dtype) + 2 ** -21) * np.abs(want) + 1e-7 * (dtype == "float16")).all()
+    assert taken > n
