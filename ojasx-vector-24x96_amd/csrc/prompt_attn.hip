@@ -72,6 +72,7 @@ struct Bf16 {
     typedef __hip_bfloat16 T;
     typedef bf16x8_t V8;
     static constexpr int kInf = 0x7f80;          // an infinity's bits
+    static constexpr float kBias = 0.f;
     static __device__ __forceinline__ f32x16_t mma(V8 a, V8 b, f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
@@ -81,6 +82,9 @@ struct F16 {
     typedef __half T;
     typedef f16x8_t V8;
     static constexpr int kInf = 0x7c00;
+    // Weights times 2^7: the largest, 2^8 above 1 (raise_max), still fit, and those
+    // that fp16's subnormals round to 0 are below 2^-32, not 2^-25, of a row's largest
+    static constexpr float kBias = 7.f;
     static __device__ __forceinline__ f32x16_t mma(V8 a, V8 b, f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
@@ -157,14 +161,14 @@ __device__ __forceinline__ void scale_acc(f32x16_t &a, float f) {
 // Running maximum (log2) of one query row per lane with a tile's largest score t:
 // rescales acc and l where the row's maximum grew by more than 2^8.
 // Weights up to 2^8 above 1 lose nothing: they are rounded relative to their
-// size and all sums are fp32.
+// size and all sums are fp32.  A weight is 2^(score - ref), ref = m - bias.
 //
 // ACC: acc stays in accumulation registers.
 template <bool ACC, int NT>
-__device__ __forceinline__ void raise_max(float t, float &m, float &ref, float &l, f32x16_t (&acc)[NT]) {
+__device__ __forceinline__ void raise_max(float t, float bias, float &m, float &ref, float &l, f32x16_t (&acc)[NT]) {
     if (__any(t > m + 8.f)) {
-        const float mn = fmaxf(m, t), rn = mn == -INFINITY ? 0.f : mn;
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - rn);
+        const float mn = fmaxf(m, t), rn = (mn == -INFINITY ? 0.f : mn) - bias;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - rn);
         m = mn;
         ref = rn;
         l *= alpha;
@@ -429,6 +433,7 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
     };
     f32x16_t acc[DP / 32] = {};
     float m = -INFINITY, ref = 0.f, l = 0.f;
+    constexpr float bias = AGAIN ? 0.f : E::kBias;   // in ref; AGAIN, where ref - bias may be rounded, beside it
     if (tiles) {
         load(0);
         store(0);
@@ -473,12 +478,12 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
             float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) t0 = fmaxf(t0, s[0][r]), t1 = fmaxf(t1, s[NB - 1][r]);
-            raise_max<false>(halves_max(fmaxf(t0, t1)) * p.scale2, m, ref, l, acc);
+            raise_max<false>(halves_max(fmaxf(t0, t1)) * p.scale2, bias, m, ref, l, acc);
             if (AGAIN)
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[b][r] = rounded_score(s[b][r], p.scale2) - ref;
+                    for (int r = 0; r < 16; ++r) s[b][r] = rounded_score(s[b][r], p.scale2) - ref + E::kBias;
             // The weights of 16 keys at a time (registers 8 f .. 8 f + 7 of a block);
             // between the products of one 16 go the exponentials and the V reads of
             // the next.  They are rounded to the inputs' type, relative to their size
@@ -591,10 +596,10 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
         }
         __syncthreads();
         if (kb) return kDone;
-        const float m1 = pair[(REGS - 2) * 64], mn = fmaxf(m, m1);
-        ref = mn == -INFINITY ? 0.f : mn;
-        const float a0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - ref);
-        const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - ref);
+        const float m1 = pair[(REGS - 2) * 64], mn = fmaxf(m, m1), rn = (mn == -INFINITY ? 0.f : mn) - bias;
+        const float a0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - rn);
+        const float a1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - bias - rn);
+        ref = rn;
         m = mn;
         l = fmaf(a0, l, a1 * pair[(REGS - 1) * 64]);
 #pragma unroll
@@ -620,7 +625,7 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
                     *reinterpret_cast<e4_t *>(op + d) = y;
                 }
             }
-        if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + __builtin_amdgcn_logf(l)) * kLn2;
+        if (p.lse && h == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + (bias - E::kBias) + __builtin_amdgcn_logf(l)) * kLn2;
     }
     if (AGAIN || KS == 2 || !any_wave(flags, redo)) return kDone;
     return redo ? kAgain : kOthersAgain;
@@ -789,7 +794,7 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
             float t = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) t = fmaxf(t, s0[r]);
-            raise_max<(DP <= 128)>(halves_max(t) * p.scale2, m, ref, l, acc);
+            raise_max<(DP <= 128)>(halves_max(t) * p.scale2, 0.f, m, ref, l, acc);
             if (AGAIN)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s0[r] = rounded_score(s0[r], p.scale2) - ref;
