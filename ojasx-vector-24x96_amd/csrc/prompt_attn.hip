@@ -197,6 +197,21 @@ __device__ __forceinline__ int own_thread() {
 
 enum { kDone, kOthersAgain, kAgain };
 
+// The kernel's first argument, read once more, for the same reason (16-bit kernels of
+// 65 to 128 dims: 29 scalar registers spilled without, 6 with; 8192 tokens of eight
+// sequences, head_dim 80: 104.5 -> 100.8 us).
+__device__ __forceinline__ PromptParams own_params() {
+    typedef __attribute__((address_space(4))) const uint32_t word_t;
+    word_t *a = (word_t *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    uint32_t w[sizeof(PromptParams) / 4];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(PromptParams) / 4; ++i) w[i] = a[i];
+    PromptParams p;
+    __builtin_memcpy(&p, w, sizeof(p));
+    return p;
+}
+
 // Whether a wave of the workgroup has `mine` set.  flags: an int of LDS per wave.
 __device__ __forceinline__ bool any_wave(int *flags, bool mine) {
     const bool wave = __any(mine);
@@ -635,7 +650,7 @@ template <typename E, int DP, int KS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DP > 128 ? 1 : DP > 64 ? 2 : 3))) void prompt_attn_kernel(
     PromptParams p, int slots) {
     const int left = prompt_block_attn<E, DP, KS, false>(p, slots, true);
-    if (left != kDone) prompt_block_attn<E, DP, KS, true>(p, slots, left == kAgain);
+    if (left != kDone) prompt_block_attn<E, DP, KS, true>(own_params(), slots, left == kAgain);
 }
 
 // fp32 on v_mfma_f32_32x32x16_bf16: every operand as three bf16 pieces whose sum it
@@ -916,7 +931,7 @@ template <int DP, int BUFFERS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void prompt_attn_f32_kernel(PromptParams p,
                                                                                                         int slots) {
     const int left = prompt_block_f32<DP, BUFFERS, false>(p, slots, true);
-    if (left != kDone) prompt_block_f32<DP, BUFFERS, true>(p, slots, left == kAgain);
+    if (left != kDone) prompt_block_f32<DP, BUFFERS, true>(own_params(), slots, left == kAgain);
 }
 
 namespace {
