@@ -394,7 +394,9 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;       // last key the row sees
     const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;    // the wave's least,
-    const int lim_hi = !mine ? -1 : p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;   // and most
+    const int lim_hi = !mine || row0 >= Lq ? -1      // and most; none where the wave has no row
+                       : p.causal          ? min(Lk - 1, min(row0 + 31, Lq - 1) + off)
+                                           : Lk - 1;
     const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
     const int tiles = last < 0 ? 0 : last / kKeys + 1;
 
@@ -689,7 +691,9 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
     const int qrow = min(row, Lq - 1);
     const int lim = p.causal ? min(Lk - 1, qrow + off) : Lk - 1;
     const int lim_lo = p.causal ? min(Lk - 1, row0 + off) : Lk - 1;
-    const int lim_hi = !mine ? -1 : p.causal ? min(Lk - 1, min(row0 + 31, Lq - 1) + off) : Lk - 1;
+    const int lim_hi = !mine || row0 >= Lq ? -1
+                       : p.causal          ? min(Lk - 1, min(row0 + 31, Lq - 1) + off)
+                                           : Lk - 1;
     const int last = p.causal ? min(Lk - 1, min(tile0 + (1 << bm_shift), Lq) - 1 + off) : Lk - 1;
     const int tiles = last < 0 ? 0 : last / KEYS + 1;
 
@@ -768,7 +772,9 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
         __syncthreads();
         if (BUFFERS == 1 && tile + 1 < tiles) load(tile + 1);
         const int k0 = tile * KEYS;
-        if (BUFFERS == 2 || k0 <= lim_hi) {           // all waves split their parts
+        // all waves split their parts; with a branch for those without rows 2048 tokens of
+        // two sequences take 146 us instead of 135
+        if (BUFFERS == 2 || k0 <= lim_hi) {
             const unsigned char *ks = sm + (BUFFERS == 2 ? tile & 1 : 0) * 6 * PLANE, *vs = ks + 3 * PLANE;
             f32x16_t s0 = {}, s1 = {};
             // Q stays in accumulation registers, which the products read as they are

@@ -216,3 +216,22 @@ def test_scores_far_apart(lc, dev, dtype, size, D):
             want = vf[top[0]]
             assert (np.abs(o[i, h] - want) <= (eps_half(dtype) + 2 ** -21) * np.abs(want) + 1e-7 * (dtype == "float16")).all()
     assert taken > n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Hq,Hkv,D", [(5, 5, 128), (3, 1, 64), (20, 4, 64), (7, 7, 256)])
+def test_single_rows_over_long_keys(lc, dev, dtype, Hq, Hkv, D):
+    """One to 33 rows of each sequence over some hundred keys, head counts that leave waves of a
+    workgroup without rows: these add nothing, and a NaN in the last row's query stays in it."""
+    nq, nk = [1, 1, 0, 33, 2], [700, 1, 30, 400, 65]
+    q, k, v = rand(dev, dtype, sum(nq), Hq, D, seed=1), rand(dev, dtype, sum(nk), Hkv, D, seed=2), \
+        rand(dev, dtype, sum(nk), Hkv, D, seed=3)
+    a = lc.PackedPromptAttention(Hq, Hkv, D)
+    out, lse = a(q, k, v, i32(dev, cum(nq)), i32(dev, cum(nk)), return_lse=True)
+    check(out, q, k, v, cum(nq), cum(nk), True, D ** -0.5, dtype, lse)
+    q[-1, 0, 0] = float("nan")
+    got = a(q, k, v, i32(dev, cum(nq)), i32(dev, cum(nk)))
+    assert got[-1, 0].isnan().all() and got.isnan().sum() == D
+    got[-1, 0] = out[-1, 0]
+    q[-1, 0, 0] = 0
+    check(got[:-1], q[:-1], k[:-65], v[:-65], cum(nq[:-1]), cum(nk[:-1]), True, D ** -0.5, dtype)
