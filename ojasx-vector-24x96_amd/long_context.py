@@ -691,11 +691,16 @@ def _aligned_rows(t, es):
     ts, hs, ds = t.stride()
     at = t.data_ptr()
     if ds != 1 or (at | ts * es | hs * es) & 15:
-        t = t.contiguous()
-        if t.data_ptr() & 15:               # contiguous() returns a contiguous slice as it is
-            t = t.clone()
-        ts, hs, _ = t.stride()
-        at = t.data_ptr()
+        n, heads, D = t.shape
+        # torch calls a tensor contiguous whatever stride a dimension of one entry has: the
+        # packed one there
+        if n <= 1:
+            ts = heads * D
+        if heads <= 1:
+            hs = D
+        if ds != 1 or (at | ts * es | hs * es) & 15:
+            t = t.clone(memory_format=_torch().contiguous_format)
+            ts, hs, at = heads * D, D, t.data_ptr()
     return t, at, ts, hs
 
 

@@ -108,3 +108,22 @@ def test_decode_scores_far_apart(lc, dev, dtype, size, share):
         tol = np.abs(hv).max() * (2 ** -12 if dtype == "bfloat16" else 2 ** -21) + eps_half(dtype) * np.abs(want)
         assert (np.abs(got[h] - want) <= tol + 1e-7 * (dtype == "float16")).all(), (h, got[h][:4], want[:4])
     assert 4 * taken >= 3 * share
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_append_of_one_row_of_a_wider_projection(lc, dev, dtype):
+    """One token, or one kv head, of a tensor whose other strides are not 16-byte: as contiguous copies."""
+    import torch
+    wide = rand(dev, dtype, 7, 259, seed=1)
+    token = wide[:, :256].view(7, 4, 64)[3:4]
+    head = rand(dev, dtype, 5, 64, 1, seed=2).transpose(1, 2)
+    for t, heads in ((token, 4), (head, 1)):
+        n = len(t)
+        got, want = (lc.PagedInt4KVCache(heads, 64, device=dev) for _ in range(2))
+        s, cu = i32(dev, [3]), i32(dev, [0, n])
+        a = got.append(t, t, s, cu, query=t, return_key=True)
+        p = torch.empty(t.shape, dtype=t.dtype, device=dev).copy_(t)
+        b = want.append(p, p, s, cu, query=p, return_key=True)
+        assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(got.k_codes, want.k_codes)
+        at = lc.PackedPromptAttention(heads, heads, 64)
+        assert torch.equal(at(t, t, t, cu), at(p, p, p, cu))

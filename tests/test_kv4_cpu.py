@@ -152,3 +152,29 @@ def test_launches_past_the_grid_are_refused(pkg):
     assert prompt(0x7fffffff, 1, 1, 1) == -3 and prompt(1, 0x7fffffff, 1, 1) == -3
     assert prompt(1 << 26, 1, 64, 1) == -3          # 2^19 blocks of rows by 64 heads: 2^25 workgroups
     assert prompt(1, 1, 8, 1 << 22) == -3           # every sequence has a workgroup for each head
+
+
+ROWS = [  # shape, strides: torch calls all of them contiguous, or takes them for rows of 16 bytes
+    ((1, 4, 64), (259, 64, 1)), ((7, 1, 64), (64, 1, 1)), ((1, 1, 64), (3, 5, 1)), ((1, 4, 64), (0, 64, 1)),
+    ((5, 1, 64), (72, 3, 1)), ((1, 3, 64), (1, 72, 1)), ((4, 2, 64), (128, 64, 1)), ((4, 2, 64), (200, 64, 1)),
+    ((4, 2, 64), (259, 64, 1)), ((4, 2, 64), (128, 1, 2)), ((4, 2, 64), (0, 0, 1)), ((0, 2, 64), (259, 64, 1)),
+    ((2, 0, 64), (259, 1, 1)),
+]
+
+
+@pytest.mark.parametrize("shape,strides", ROWS, ids=str)
+@pytest.mark.parametrize("offset", [0, 1, 8])
+@pytest.mark.parametrize("es", [2, 4])
+def test_aligned_rows_of_any_strides(pkg, shape, strides, offset, es):
+    """Rows for a kernel: 16-byte aligned, strides of dimensions of one entry too, the same values."""
+    import torch
+    from importlib import import_module
+    lc = import_module(pkg.__name__ + ".long_context")
+    dtype = torch.float32 if es == 4 else torch.bfloat16
+    base = torch.arange(2048 + offset).to(dtype)
+    t = base.as_strided(shape, strides, offset)
+    rows, at, ts, hs = lc._aligned_rows(t, es)
+    assert torch.equal(rows, t) and at == rows.data_ptr()
+    assert at % 16 == 0 and ts * es % 16 == 0 and hs * es % 16 == 0
+    if t.numel():
+        assert torch.equal(rows.as_strided(shape, (ts, hs, 1), rows.storage_offset()), t)
