@@ -655,11 +655,12 @@ class PagedCodeKVCache:
 
 # The calls below serve single tokens, where the host's time is the call's: their checks
 # read each property once, and hold devices by index.
-_INFERENCE_TAGS = {}
+_INFERENCE_TAGS = {}        # dtype -> (C-ABI tag, torch's forward-mode module)
 
 
 def _inference_tag(what, *tensors):
-    """(C-ABI tag, device index) of tensors of one dtype on one GPU, without a gradient."""
+    """(C-ABI tag, device index) of tensors of one dtype on one GPU, without a gradient, reverse
+    or forward."""
     dtype, index = tensors[0].dtype, tensors[0].get_device()
     for u in tensors:
         if u.dtype != dtype or u.get_device() != index or index < 0:
@@ -668,12 +669,17 @@ def _inference_tag(what, *tensors):
         if u.requires_grad and _torch().is_grad_enabled():
             raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or with detached "
                                "tensors")
-    tag = _INFERENCE_TAGS.get(dtype)
-    if tag is None:
+    known = _INFERENCE_TAGS.get(dtype)
+    if known is None:
         tag = _attn_tag(dtype)
         if tag is None or tag == _lib.DTYPE_F64:
             raise TypeError(f"{what}: unsupported dtype {dtype}: float32, bfloat16 or float16")
-        _INFERENCE_TAGS[dtype] = tag
+        known = _INFERENCE_TAGS[dtype] = tag, _torch().autograd.forward_ad
+    tag, forward_ad = known
+    if forward_ad._current_level >= 0 and _torch()._C._is_fwd_grad_enabled() and \
+            any(forward_ad.unpack_dual(u).tangent is not None for u in tensors):
+        raise RuntimeError(f"{what} has no forward-mode gradient: call it with the primal tensors or under "
+                           "torch.inference_mode()")
     return tag, index
 
 

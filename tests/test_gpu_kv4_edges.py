@@ -127,3 +127,25 @@ def test_append_of_one_row_of_a_wider_projection(lc, dev, dtype):
         assert all(torch.equal(x, y) for x, y in zip(a, b)) and torch.equal(got.k_codes, want.k_codes)
         at = lc.PackedPromptAttention(heads, heads, 64)
         assert torch.equal(at(t, t, t, cu), at(p, p, p, cu))
+
+
+def test_forward_tangents_are_refused(lc, dev):
+    """A dual tensor's tangent would be lost without a word: refused, also under no_grad, which keeps
+    forward mode on."""
+    import torch
+    import torch.autograd.forward_ad as fw
+    c = lc.PagedInt4KVCache(2, 64, num_sequences=3, max_resident_pages=4, device=dev)
+    a = lc.PackedPromptAttention(2, 2, 64)
+    k, s, cu = torch.randn(3, 2, 64, device=dev), i32(dev, [0, 0, 0]), i32(dev, [0, 3])
+    with fw.dual_level():
+        d = fw.make_dual(k, torch.ones_like(k))
+        calls = [lambda x: c.append(x, k, s), lambda x: c.append(k, x, s), lambda x: c.append(k, k, s, query=x),
+                 lambda x: c.decode(x, s + 1), lambda x: a(x, k, k, cu), lambda x: a(k, x, k, cu), lambda x: a(k, k, x, cu)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(d)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(d)
+            call(k), call(fw.unpack_dual(d).primal)
+            with torch.inference_mode():
+                call(k)
