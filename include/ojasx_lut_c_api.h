@@ -363,7 +363,8 @@ OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start
 /* Attention of one query token per sequence over its resident tokens:
  * q, out [num_sequences][num_q_heads][head_dim] in dtype (F32, BF16, F16), head
  * j reading kv head j / (num_q_heads / num_kv_heads); seen: the tokens of each
- * sequence so far (0: a row of zeros).  scale_factor <= 0: 1/sqrt(head_dim).
+ * sequence so far (0: a row of zeros).  scale_factor <= 0: 1/sqrt(head_dim);
+ * one that is NaN or not finite times log2(e) is refused.
  * max_seen bounds seen[] (0: the cache's capacity) and with it the size of the
  * launch; larger entries of seen are attended in full all the same.
  * q is 16-byte aligned.  workspace: ojasx_kv4_decode_workspace(...) bytes for the

@@ -751,6 +751,11 @@ OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q,
         return OJASX_ERR_INVALID;
     }
     const int D = cache->head_dim;
+    p.scale = (scale_factor > 0.f ? scale_factor : 1.0f / sqrtf((float)D)) * kLog2e;
+    if (std::isnan(scale_factor) || !std::isfinite(p.scale)) {
+        set_error("4-bit KV decode: scale_factor %g is not finite (times log2(e), in fp32)", (double)scale_factor);
+        return OJASX_ERR_INVALID;
+    }
     p.W = decode_runs(cache, num_q_heads, max_seen);
     const size_t rows = ((size_t)p.W + cache->num_sequences) * num_q_heads;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
@@ -762,7 +767,6 @@ OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q,
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = p.part_o + rows * D;
     p.q = q, p.out = out, p.seen = seen, p.Hq = num_q_heads, p.R = num_q_heads / cache->num_kv_heads;
-    p.scale = (scale_factor > 0.f ? scale_factor : 1.0f / sqrtf((float)D)) * kLog2e;
     hipStream_t st = static_cast<hipStream_t>(stream);
     return dtype == OJASX_DTYPE_F32    ? launch_decode<float>(p, D, cache->group_size, st)
            : dtype == OJASX_DTYPE_BF16 ? launch_decode<__hip_bfloat16>(p, D, cache->group_size, st)

@@ -1032,8 +1032,8 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
         set_error("prompt attention: head_dim %d is no multiple of 8 up to 256", head_dim);
         return OJASX_ERR_INVALID;
     }
-    if (!(scale > 0.f) || !(scale < INFINITY)) {
-        set_error("prompt attention: scale must be positive and finite");
+    if (!(scale > 0.f) || !(scale * kLog2e < INFINITY)) {
+        set_error("prompt attention: scale must be positive and finite (times log2(e), in fp32)");
         return OJASX_ERR_INVALID;
     }
     if (num_q_tokens == 0) return OJASX_OK;

@@ -178,3 +178,17 @@ def test_aligned_rows_of_any_strides(pkg, shape, strides, offset, es):
     assert at % 16 == 0 and ts * es % 16 == 0 and hs * es % 16 == 0
     if t.numel():
         assert torch.equal(rows.as_strided(shape, (ts, hs, 1), rows.storage_offset()), t)
+
+
+def test_scales_that_are_not_finite_are_refused(pkg):
+    """NaN is no request for the default, and a scale whose product with log2(e) overflows fp32 makes
+    every score an infinity or a NaN."""
+    L, c = pkg.lib(), cache(pkg)
+    ref = ctypes.addressof(c)
+    need = L.ojasx_kv4_decode_workspace(ref, 4, 0)
+    for s in (float("nan"), float("inf"), 3e38):
+        assert L.ojasx_kv4_decode_device(ref, FAKE, 4, 0, FAKE, 0, s, FAKE, FAKE, need, None) == -3
+        assert b"scale" in L.ojasx_get_last_error()
+        assert L.ojasx_prompt_attention_device(FAKE, 512, 128, FAKE, 512, 128, FAKE, 512, 128, 0, 4, 4, 4, 4, 128, FAKE,
+                                               FAKE, 1, 1, s, 0, FAKE, None, None) == -3
+        assert b"scale" in L.ojasx_get_last_error()
