@@ -655,6 +655,7 @@ class PagedCodeKVCache:
 
 # The calls below serve single tokens, where the host's time is the call's: their checks
 # read each property once, and hold devices by index.
+_MOST_INT = 0x7fffffff      # the entry points' counts are C ints: a larger one would lose its high bits
 _INFERENCE_TAGS = {}        # dtype -> (C-ABI tag, torch's forward-mode module)
 
 
@@ -877,6 +878,8 @@ class PagedInt4KVCache:
         what = "PagedInt4KVCache.append"
         tag = self._tag(what, key, value) if query is None else self._tag(what, key, value, query)
         n = key.shape[0] if key.dim() else 0
+        if n > _MOST_INT:
+            raise ValueError(f"{what}: {n} tokens")
         self._check_rows(key, n, self.num_kv_heads, "key")
         self._check_rows(value, n, self.num_kv_heads, "value")
         at, cu = self._packed(n, start, cu_seqlens)
@@ -1016,6 +1019,8 @@ class PackedPromptAttention:
         if B < 1:
             raise ValueError(f"cu_seqlens must hold the B + 1 bounds of B sequences, got "
                              f"{tuple(cu_seqlens.shape)}")
+        if m > _MOST_INT or B > _MOST_INT:
+            raise ValueError(f"{m} keys, {B} sequences")
         cq = ck = _lengths_tensor(cu_seqlens, B + 1, dev, "cu_seqlens")
         if cu_seqlens_kv is not None:
             ck = _lengths_tensor(cu_seqlens_kv, B + 1, dev, "cu_seqlens_kv")

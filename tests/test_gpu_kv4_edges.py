@@ -149,3 +149,17 @@ def test_forward_tangents_are_refused(lc, dev):
             call(k), call(fw.unpack_dual(d).primal)
             with torch.inference_mode():
                 call(k)
+
+
+def test_counts_past_an_int_are_refused(lc, dev):
+    """Rows of stride 0 can be more than 2^32: their count must not lose its high bits on the way."""
+    import torch
+    c = lc.PagedInt4KVCache(1, 64, max_resident_pages=4, rope_theta=None, device=dev)
+    a = lc.PackedPromptAttention(1, 1, 64)
+    row = torch.ones(1, 1, 64, device=dev)
+    many = row.expand(2 ** 32 + 3, 1, 64)
+    cu = i32(dev, [0, 3])
+    for call in (lambda: c.append(many, many, i32(dev, [0]), cu), lambda: a(row, many, many, i32(dev, [0, 1]), cu)):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+    assert not c.k_steps.any()
