@@ -126,15 +126,18 @@ __device__ __forceinline__ float kv4_out(float o, float l, float m) {
     return m == -INFINITY ? 0.f : o / l;         // l = 0: only scores of -inf, no softmax, NaN
 }
 
-// The tiles of all sequences, and those before sequence b.  Whole waves call it.
-__device__ __forceinline__ int kv4_all_tiles(const Kv4View &c, const int *seen, int b, int *before) {
+// The tiles of all sequences, those before sequence b and its own, from one look at
+// each length.  Whole waves call it.
+__device__ __forceinline__ int kv4_all_tiles(const Kv4View &c, const int *seen, int b, int *before, int *own) {
     const int lane = threadIdx.x & 63;
-    int all = 0, bef = 0;
+    int all = 0, bef = 0, mine = 0;
     for (int i = lane; i < c.B; i += 64) {
         const int n = kv4_tiles(c, seen[i]);
         all += n;
         if (i < b) bef += n;
+        if (i == b) mine = n;
     }
+    *own = __builtin_amdgcn_readlane(mine, b & 63);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o), bef += __shfl_xor(bef, o);
     *before = bef;
@@ -256,13 +259,14 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
         b = p.c.B == 1 ? 0 : __builtin_ctzll(__ballot(up > pos));
         first = __builtin_amdgcn_readlane(up - own, b);
     } else {
-        int none;
-        const Runs runs(kv4_all_tiles(p.c, p.seen, 0, &none), p.W);
+        int none, own0;
+        const Runs runs(kv4_all_tiles(p.c, p.seen, 0, &none, &own0), p.W);
         if ((int)blockIdx.x >= runs.W) return;
         pos = runs.start(blockIdx.x);
         end = runs.start(blockIdx.x + 1);
         first = 0;
-        for (int i0 = 0;; i0 += 64) {
+        b = p.c.B;
+        for (int i0 = 0; i0 < p.c.B; i0 += 64) {
             const int i = i0 + lane, own = i < p.c.B ? kv4_tiles(p.c, p.seen[i]) : 0, up = wave_scan(own);
             const unsigned long long over = __ballot(first + up > pos);
             if (over) {
@@ -280,7 +284,7 @@ __global__ __launch_bounds__(kNT) __attribute__((amdgpu_waves_per_eu(D == 256 ? 
     first = __builtin_amdgcn_readfirstlane(first);
     uint32_t magic = 0x64006400u;
     asm volatile("" : "+v"(magic));
-    for (; pos < end; ++b) {
+    for (; pos < end && b < p.c.B; ++b) {      // whatever the lengths are by now
     const Kv4Extent ext = kv4_extent(p.c, uniform_int(p.seen + b));
     const int tiles = ((ext.entries << bps) + 3) >> 2;
     if (tiles == 0) continue;
@@ -587,7 +591,8 @@ __global__ __launch_bounds__(kNT) void kv4_merge_kernel(Kv4DecodeParams p) {
     __shared__ float4 os[SG][DQ];
     const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const int d = tid % DQ, sg = tid / DQ;
-    const int tiles = kv4_tiles(p.c, p.seen[b]);
+    int first, tiles;
+    const Runs runs(kv4_all_tiles(p.c, p.seen, b, &first, &tiles), p.W);
     T *out = static_cast<T *>(p.out) + ((size_t)b * p.Hq + head) * D;
     if (tiles == 0) {
         if (tid < DQ)
@@ -595,8 +600,6 @@ __global__ __launch_bounds__(kNT) void kv4_merge_kernel(Kv4DecodeParams p) {
             for (int e = 0; e < 4; ++e) store_act(out, 4 * d + e, 0.f);
         return;
     }
-    int first;
-    const Runs runs(kv4_all_tiles(p.c, p.seen, b, &first), p.W);
     const int i0 = runs.of(first), used = runs.of(first + tiles - 1) - i0 + 1;
     if (used == 1) return;                               // written whole
     const size_t row0 = (size_t)(i0 + b) * p.Hq + head;
