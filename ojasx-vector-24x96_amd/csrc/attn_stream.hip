@@ -810,12 +810,8 @@ int launch_tiles(const AttnParams &p, int n_work, int B, int RB, hipStream_t st)
                                : reinterpret_cast<const void *>(&attn_tile_kernel<KT, 8>);
     // The limit bounds the dynamic part; the default admits 64 KB in total
     // with the static arrays, so it is raised whenever the v rows are staged.
-    static size_t granted[4] = {};
-    size_t &g = granted[RB == 1 ? 0 : RB == 2 ? 1 : RB == 4 ? 2 : 3];
-    if (lds > g) {
-        OJX_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        g = lds;
-    }
+    static DynLds granted[4];
+    if (lds) OJX_HIP(raise_dyn_lds(fn, lds, &granted[RB == 1 ? 0 : RB == 2 ? 1 : RB == 4 ? 2 : 3]));
     switch (RB) {
         case 1: OJX_LAUNCH((attn_tile_kernel<KT, 1>), grid, dim3(kANT), lds, st, p); break;
         case 2: OJX_LAUNCH((attn_tile_kernel<KT, 2>), grid, dim3(kANT), lds, st, p); break;
@@ -829,7 +825,7 @@ int launch_tiles(const AttnParams &p, int n_work, int B, int RB, hipStream_t st)
 template <int KT, int D>
 int launch_rows_d(const AttnParams &p, double *state, int n_work, dim3 grid, hipStream_t st) {
     constexpr size_t lds = (size_t)2 * kRT * (pad_to(D, 2) + pad_to(D, 16) + 2) * sizeof(double);
-    static size_t granted = 0;
+    static DynLds granted;
     int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&attn_rows_kernel<KT, D>), lds, &granted);
     if (rc) return rc;
     OJX_LAUNCH((attn_rows_kernel<KT, D>), grid, dim3(kRNT), lds, st, p, state, n_work);

@@ -12,6 +12,7 @@
 #include <cstring>
 #include <string>
 
+#include "dyn_lds.h"
 #include "ojasx_lut_c_api.h"
 
 namespace ojx {
@@ -274,12 +275,10 @@ int launch_lut_build(const void *x, const float *cb, int B, int K, int D, int G,
 
 inline size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 
-// Raise a kernel's dynamic-LDS limit when a launch needs more than the 64 KB
-// default (gfx950 has 160 KB per workgroup).  `granted` caches the last value.
-inline int ensure_dyn_lds(const void *fn, size_t bytes, size_t *granted) {
-    if (bytes <= 65536 || bytes <= *granted) return OJASX_OK;
-    OJX_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    *granted = bytes;
+// Raise a kernel's dynamic-LDS limit on the current device when a launch needs more
+// than the 64 KB default (gfx950 has 160 KB per workgroup).
+inline int ensure_dyn_lds(const void *fn, size_t bytes, DynLds *granted) {
+    if (bytes > 65536) OJX_HIP(raise_dyn_lds(fn, bytes, granted));
     return OJASX_OK;
 }
 

@@ -207,13 +207,13 @@ int kv_encode_append(const float *k, const float *v, int num_tokens,
                        (reinterpret_cast<uintptr_t>(k_codebook) & 15) == 0 &&
                        (reinterpret_cast<uintptr_t>(v_codebook) & 15) == 0;
     if (reg16) {
-        static size_t granted = 0;
+        static DynLds granted;
         int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&kv_encode_append_kernel<16>), lds,
                                 &granted);
         if (rc) return rc;
         OJX_LAUNCH(kv_encode_append_kernel<16>, grid, dim3(kNT), lds, st, p);
     } else {
-        static size_t granted = 0;
+        static DynLds granted;
         int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&kv_encode_append_kernel<0>), lds,
                                 &granted);
         if (rc) return rc;

@@ -645,14 +645,10 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(const int *idx, const fl
 
 namespace {
 template <typename F>
-int set_dyn_lds(F *fn, size_t lds, size_t *granted) {
+int set_dyn_lds(F *fn, size_t lds, DynLds *granted) {
     // The attribute bounds the dynamic part; with the 64 KB of static LUT the
     // total passes the 64 KB default for any input.
-    if (lds > *granted) {
-        OJX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(fn),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        *granted = lds;
-    }
+    OJX_HIP(raise_dyn_lds(reinterpret_cast<const void *>(fn), lds, granted));
     return OJASX_OK;
 }
 }  // namespace
@@ -664,7 +660,7 @@ bool bank_fits(int K) {
 int launch_bank(const GroupItem *items_dev, const int2 *work_dev, int n_work, int max_K,
                 hipStream_t st) {
     const size_t lds = round_up((size_t)(max_K / 16), 32) * kXRow * sizeof(float);
-    static size_t granted = 0;
+    static DynLds granted;
     int rc = set_dyn_lds(&lut_bank_kernel, lds, &granted);
     if (rc) return rc;
     OJX_LAUNCH(lut_bank_kernel, dim3(n_work), dim3(kBNT), lds, st, items_dev, work_dev);
@@ -675,12 +671,9 @@ int launch_bank(const GroupItem *items_dev, const int2 *work_dev, int n_work, in
 int launch_moe_plan(const int *idx, const float *w, int P, int E, int nb_gu, int nb_dn,
                     int2 *work_gu, int2 *work_dn, int *n_work, hipStream_t st) {
     const size_t lds = (size_t)(3 * E + P) * sizeof(int);
-    static size_t granted = 0;
-    if (lds > 65536 && lds > granted) {
-        OJX_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(&moe_plan_kernel),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        granted = lds;
-    }
+    static DynLds granted;
+    const int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&moe_plan_kernel), lds, &granted);
+    if (rc) return rc;
     OJX_LAUNCH(moe_plan_kernel, dim3(1), dim3(1024), lds, st, idx, w, P, E, nb_gu, nb_dn, work_gu,
                work_dn, n_work);
     OJX_HIP(hipGetLastError());
@@ -695,15 +688,15 @@ int launch_moe_bank(const MoEBankLaunch &l, hipStream_t st) {
     const int grid = l.work ? 8 * ((l.max_work + 7) / 8) : l.max_work;
     int rc = OJASX_OK;
     if (l.xs == XS_SWIGLU) {
-        static size_t gr = 0;
+        static DynLds gr;
         rc = set_dyn_lds(&moe_bank_kernel<XS_SWIGLU>, lds, &gr);
         if (!rc) OJX_LAUNCH(moe_bank_kernel<XS_SWIGLU>, dim3(grid), dim3(kBNT), lds, st, p);
     } else if (l.xs == XS_BF16) {
-        static size_t gr = 0;
+        static DynLds gr;
         rc = set_dyn_lds(&moe_bank_kernel<XS_BF16>, lds, &gr);
         if (!rc) OJX_LAUNCH(moe_bank_kernel<XS_BF16>, dim3(grid), dim3(kBNT), lds, st, p);
     } else {
-        static size_t gr = 0;
+        static DynLds gr;
         rc = set_dyn_lds(&moe_bank_kernel<XS_F32>, lds, &gr);
         if (!rc) OJX_LAUNCH(moe_bank_kernel<XS_F32>, dim3(grid), dim3(kBNT), lds, st, p);
     }
@@ -740,15 +733,15 @@ int launch_moe_resident(const MoEBankLaunch &l, int groups, int slots, hipStream
     const dim3 grid(groups * cpt), block(teams * kBNT);
     int rc = OJASX_OK;
     if (l.xs == XS_SWIGLU) {
-        static size_t gr = 0;
+        static DynLds gr;
         rc = set_dyn_lds(&moe_resident_kernel<XS_SWIGLU, 1>, lds, &gr);
         if (!rc) OJX_LAUNCH((moe_resident_kernel<XS_SWIGLU, 1>), grid, block, lds, st, p);
     } else if (l.xs == XS_BF16) {
-        static size_t gr = 0;
+        static DynLds gr;
         rc = set_dyn_lds(&moe_resident_kernel<XS_BF16, 2>, lds, &gr);
         if (!rc) OJX_LAUNCH((moe_resident_kernel<XS_BF16, 2>), grid, block, lds, st, p);
     } else {
-        static size_t gr = 0;
+        static DynLds gr;
         rc = set_dyn_lds(&moe_resident_kernel<XS_F32, 2>, lds, &gr);
         if (!rc) OJX_LAUNCH((moe_resident_kernel<XS_F32, 2>), grid, block, lds, st, p);
     }

@@ -461,7 +461,7 @@ int launch_gemm_tile(GemmParams p, hipStream_t st) {
     constexpr size_t sums = (size_t)NWR * 32 * (BT + 4) * sizeof(float);
     const size_t lds = p.gptr ? std::max(stage, sums) : stage;
     static_assert(stage <= 160 * 1024 && sums <= 160 * 1024, "LDS");
-    static size_t granted = 0;
+    static DynLds granted;
     int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&lut_gemm_kernel<T, PROD, WT, WR, NWT, NWR, PXD>), lds, &granted);
     if (rc) return rc;
     p.nr = (p.M + BR - 1) / BR;

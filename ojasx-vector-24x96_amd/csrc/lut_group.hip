@@ -134,7 +134,7 @@ int launch_tall_rms(const GroupItem &it, const float *w, float eps, hipStream_t 
         return OJASX_ERR_INVALID;
     }
     const size_t lds = (size_t)it.S * 256 * sizeof(float);
-    static size_t granted = 0;
+    static DynLds granted;
     int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&lut_tall_rms_kernel),
                             lds + slices::lut_bytes(true), &granted);
     if (rc) return rc;

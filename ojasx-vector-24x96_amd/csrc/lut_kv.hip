@@ -959,7 +959,7 @@ int kv_decode(const float *q, const uint8_t *kc, const float *ks, const uint8_t 
                    Hq, Hkv, hd, D, G, (int)C, 4, n_chunks, sf, nullptr, 0};
         const size_t lds = (size_t)(4 * 128 + 256 * 16 + 32 * kLutP + 32) * 4 + (size_t)kWideNT * 16 +
                            (size_t)kWideNT * 16 + (size_t)16 * 32 * 16 * 4;
-        static size_t gw = 0;
+        static DynLds gw;
         int rc = ensure_dyn_lds(reinterpret_cast<const void *>(&kv_decode_wide_kernel), lds, &gw);
         if (rc) return rc;
         OJX_LAUNCH(kv_decode_wide_kernel, dim3(n_chunks, Hkv, nz), dim3(kWideNT), lds, st, p);
@@ -983,7 +983,7 @@ int kv_decode(const float *q, const uint8_t *kc, const float *ks, const uint8_t 
     KVParams p{q, kc, vc, ks, vs, kcb, vcb, bt, wk.po, wk.pml, out, T, P,
                Hq, Hkv, hd, D, G, kNT, RS, n_chunks, sf, nullptr, 0};
     const size_t lds = ((size_t)RS * hd + 256 * D + (size_t)RS * G * 256) * 4 + (size_t)RS * G * kHP * 4;
-    static size_t g0 = 0;
+    static DynLds g0;
     rc = ensure_dyn_lds(reinterpret_cast<const void *>(&kv_decode_chunk_kernel<0, 0, 8, 1>), lds, &g0);
     if (rc) return rc;
     OJX_LAUNCH((kv_decode_chunk_kernel<0, 0, 8, 1>), dim3(n_chunks, Hkv, nz), dim3(kNT), lds, st, p);

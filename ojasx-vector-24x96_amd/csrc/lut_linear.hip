@@ -608,7 +608,7 @@ namespace {
 template <int BT, typename T>
 int launch_gather(const GatherParams &gp, int M, dim3 grid_y, size_t lds, hipStream_t st) {
     constexpr int R = kRows;
-    static size_t granted = 0;
+    static DynLds granted;
     const void *fn = reinterpret_cast<const void *>(&lut_gather_kernel<R, BT, T>);
     int rc = ensure_dyn_lds(fn, lds, &granted);
     if (rc) return rc;
@@ -628,7 +628,7 @@ struct Fuse {
 
 template <typename T, int BT, int RPL, int PRO, bool RES, bool HO>
 int launch_dec_g(const DecParams &dp, dim3 grid, size_t lds, hipStream_t st) {
-    static size_t granted = 0;
+    static DynLds granted;
     const void *fn = reinterpret_cast<const void *>(&lut_dec_kernel<T, BT, RPL, PRO, RES, HO>);
     int rc = ensure_dyn_lds(fn, lds, &granted);
     if (rc) return rc;

@@ -828,7 +828,7 @@ int moe_forward_dec(MoE *m, const void *x, const int *idx, const float *w, void 
         constexpr int NI = 2;
         p.NW = std::min(m->Sin, 16);
         const size_t lds = (size_t)(kCB * 16 + m->Sin * 256) * sizeof(float);
-        static size_t granted = 0;
+        static DynLds granted;
         const void *fn = reinterpret_cast<const void *>(&moe_up_dec_kernel<T, NI>);
         rc = ensure_dyn_lds(fn, lds, &granted);
         if (rc) return rc;
@@ -842,7 +842,7 @@ int moe_forward_dec(MoE *m, const void *x, const int *idx, const float *w, void 
         const bool r2 = (long)T_ * ((m->H + 31) / 32) >= 192;
         const void *fn = r2 ? reinterpret_cast<const void *>(&moe_down_dec_kernel<T, 2>)
                             : reinterpret_cast<const void *>(&moe_down_dec_kernel<T, 1>);
-        static size_t granted1 = 0, granted2 = 0;
+        static DynLds granted1, granted2;
         rc = ensure_dyn_lds(fn, lds, r2 ? &granted2 : &granted1);
         if (rc) return rc;
         if (r2)
@@ -870,7 +870,7 @@ template <int NS>
 int launch_dn(const MoEGroupParams &p, size_t P, size_t lds, hipStream_t st) {
     const void *fn = reinterpret_cast<const void *>(
         &moe_dn_group_kernel<kDnWaves, kDnRows, kGroupDB, kGroupPF, NS>);
-    static size_t granted = 0;
+    static DynLds granted;
     int rc = ensure_dyn_lds(fn, lds + slices::lut_bytes(kGroupDB), &granted);
     if (rc) return rc;
     const int nb = (p.H + 64 * kDnWaves * kDnRows - 1) / (64 * kDnWaves * kDnRows);
@@ -918,7 +918,7 @@ int moe_forward_group(MoE *m, const void *x, const int *idx, const float *w, voi
         const void *fn = reinterpret_cast<const void *>(
             &moe_gu_group_kernel<T, kGuWaves, kGuIdx, kGroupDB, kGroupPF>);
         const size_t lds = (size_t)m->Sin * 256 * sizeof(float);
-        static size_t granted = 0;
+        static DynLds granted;
         rc = ensure_dyn_lds(fn, lds + slices::lut_bytes(kGroupDB), &granted);
         if (rc) return rc;
         const int nb = (m->I + 64 * kGuWaves * kGuIdx - 1) / (64 * kGuWaves * kGuIdx);

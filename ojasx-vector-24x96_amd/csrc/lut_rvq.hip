@@ -456,7 +456,7 @@ bool valid_bits(int bits) { return bits == 1 || bits == 2 || bits == 4 || bits =
 
 template <typename T, int TT, bool B4>
 int launch_rvq_mm_k(const RvqParams &p, size_t lds, hipStream_t st) {
-    static size_t granted = 0;
+    static DynLds granted;
     const void *fn = reinterpret_cast<const void *>(&lut_rvq_mm_kernel<T, TT, B4>);
     int rc = ensure_dyn_lds(fn, lds, &granted);
     if (rc) return rc;
@@ -494,7 +494,7 @@ int try_rvq_mm(RvqParams &p, bool cb_lds, hipStream_t st) {
 
 template <typename T, int DT, int BT>
 int launch_rvq_bt(RvqParams &p, size_t lds, hipStream_t st) {
-    static size_t granted = 0;
+    static DynLds granted;
     const void *fn = reinterpret_cast<const void *>(&lut_rvq_kernel<T, DT, BT>);
     int rc = ensure_dyn_lds(fn, lds, &granted);
     if (rc) return rc;

@@ -950,7 +950,7 @@ int heads_shift(const PromptParams &p, int wr) {
     return share < most ? share : most;
 }
 // Sets p.hw, the LDS limit of kernel `fn` and the launch's size, or returns an error.
-int prepare(const void *fn, PromptParams &p, int wr, size_t lds, size_t *granted, int *slots, unsigned *groups) {
+int prepare(const void *fn, PromptParams &p, int wr, size_t lds, DynLds *granted, int *slots, unsigned *groups) {
     const int rc = ensure_dyn_lds(fn, lds, granted);
     if (rc) return rc;
     p.hw = heads_shift(p, wr);
@@ -966,7 +966,7 @@ int prepare(const void *fn, PromptParams &p, int wr, size_t lds, size_t *granted
 }
 template <typename E, int DP, int KS>
 int launch16_split(PromptParams p, hipStream_t st) {
-    static size_t granted = 0;
+    static DynLds granted;
     const size_t lds = (size_t)4 * kKeys * 2 * DP + kFlags;
     int slots;
     unsigned groups;
@@ -985,7 +985,7 @@ int launch16(const PromptParams &p, hipStream_t st) {
 }
 template <int DP, int BUFFERS>
 int launch32(PromptParams p, hipStream_t st) {
-    static size_t granted = 0;
+    static DynLds granted;
     const size_t lds = (size_t)BUFFERS * 6 * 32 * 2 * DP + kFlags;
     int slots;
     unsigned groups;
