@@ -163,3 +163,21 @@ def test_counts_past_an_int_are_refused(lc, dev):
         with pytest.raises((ValueError, RuntimeError)):
             call()
     assert not c.k_steps.any()
+
+
+def test_single_tokens_of_a_large_batch(lc, dev):
+    """Append and read of one token a sequence with one wave for a whole token (more than 4096 waves)."""
+    import torch
+    B = 5000
+    c = [lc.PagedInt4KVCache(2, 64, num_sequences=B, max_resident_pages=7, device=dev) for _ in range(2)]
+    k, v, q = (rand(dev, "bfloat16", B, h, 64, seed=s) for s, h in enumerate((2, 2, 6)))
+    starts = [7 * b % 100 for b in range(B)]
+    start = i32(dev, starts)
+    a = c[0].append(k, v, start, query=q)[0]
+    b = c[1].append(k, v, start, i32(dev, range(B + 1)), query=q)[0]
+    assert torch.equal(a, b)
+    _, hk, hv = want_kv(k, v, np.array(starts), 64, 32)
+    for x, y, want in zip(c[0].read(start), c[1].read(start, i32(dev, range(B + 1)), B), (hk, hv)):
+        assert torch.equal(x, y) and np.array_equal(f64(x), want.astype(np.float32).astype(np.float64))
+    qf = kv4.rotate(f64(q), starts, kv4.inv_freq(64, 1e6))
+    assert (np.abs(f64(a) - qf) <= 2 * eps_half("bfloat16") * np.abs(qf)).all()

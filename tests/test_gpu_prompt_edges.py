@@ -235,3 +235,30 @@ def test_single_rows_over_long_keys(lc, dev, dtype, Hq, Hkv, D):
     got[-1, 0] = out[-1, 0]
     q[-1, 0, 0] = 0
     check(got[:-1], q[:-1], k[:-65], v[:-65], cum(nq[:-1]), cum(nk[:-1]), True, D ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_over_the_cache(lc, dev, dtype):
+    """A prompt that arrives in parts: each part's rows over all the sequence's keys so far, read back
+    from the 4-bit cache, through cu_seqlens_kv."""
+    import torch
+    Hq, Hkv, D, group = 4, 2, 128, 32
+    cache = lc.PagedInt4KVCache(Hkv, D, num_sequences=2, max_resident_pages=32, group_size=group, device=dev)
+    a = lc.PackedPromptAttention(Hq, Hkv, D)
+    seen, dt = np.zeros(2, int), getattr(torch, dtype)
+    hist = [[np.zeros((0, Hkv, D))] * 2 for _ in range(2)]
+    for part, lengths in enumerate(([100, 7], [65, 0], [1, 200], [130, 33])):
+        N = sum(lengths)
+        q, k, v = (rand(dev, dtype, N, h, D, seed=10 * part + s) for h, s in ((Hq, 1), (Hkv, 2), (Hkv, 3)))
+        qr, _ = cache.append(k, v, i32(dev, seen), i32(dev, cum(lengths)), query=q)
+        _, hk, hv = want_kv(k, v, positions(seen, lengths), D, group)
+        for b, (lo, hi) in enumerate(zip(cum(lengths), cum(lengths)[1:])):
+            hist[b] = [np.concatenate([hist[b][0], hk[lo:hi]]), np.concatenate([hist[b][1], hv[lo:hi]])]
+            seen[b] += hi - lo
+        ck = cum(seen)
+        rk, rv = cache.read(i32(dev, [0, 0]), i32(dev, ck), ck[-1], dtype=dt)
+        for got, i in ((rk, 0), (rv, 1)):
+            want = torch.from_numpy(np.concatenate([hist[0][i], hist[1][i]]).astype(np.float32)).to(dt)
+            assert torch.equal(got.cpu(), want)
+        out = a(qr, rk, rv, i32(dev, cum(lengths)), i32(dev, ck))
+        check(out, qr, rk, rv, cum(lengths), ck, True, D ** -0.5, dtype)
