@@ -282,6 +282,13 @@ inline int ensure_dyn_lds(const void *fn, size_t bytes, DynLds *granted) {
     return OJASX_OK;
 }
 
+// Rows a kernel reads with 16-byte loads: aligned, token and head strides (elements of es
+// bytes) not negative and multiples of 16 bytes.
+inline bool rows_of_16(const void *p, long token_stride, long head_stride, size_t es) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && token_stride >= 0 && head_stride >= 0 &&
+           token_stride * es % 16 == 0 && head_stride * es % 16 == 0;
+}
+
 // ---- device helpers ------------------------------------------------------
 // Load through a global-address-space pointer.  Pointers read from device
 // memory (not kernel arguments) are otherwise generic, their loads become

@@ -367,11 +367,6 @@ unsigned wave_groups(int n, int parts) { return (unsigned)(((long)n * parts + kN
             OJX_KV4_DISPATCH(KERNEL, __hip_bfloat16, D, GS, __VA_ARGS__);                     \
         else OJX_KV4_DISPATCH(KERNEL, __half, D, GS, __VA_ARGS__);                            \
     } while (0)
-
-bool rows_ok(const void *p, long ts, long hs, size_t es) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ts >= 0 && hs >= 0 &&
-           (ts * es) % 16 == 0 && (hs * es) % 16 == 0;
-}
 }  // namespace
 
 }  // namespace ojx
@@ -400,9 +395,9 @@ OJASX_API int ojasx_kv4_append_device(const OjasxKV4Cache *cache, const void *q,
     if (num_tokens == 0) return OJASX_OK;
     if (!k || !v || !start || (num_q_heads && (!q || !q_out))) return OJASX_ERR_NULL;
     const size_t es = dtype == OJASX_DTYPE_F32 ? 4 : 2;
-    if (!rows_ok(k, k_token_stride, k_head_stride, es) || !rows_ok(v, v_token_stride, v_head_stride, es) ||
-        (num_q_heads && (!rows_ok(q, q_token_stride, q_head_stride, es) || !rows_ok(q_out, 0, 0, es))) ||
-        (k_out && !rows_ok(k_out, 0, 0, es))) {
+    if (!rows_of_16(k, k_token_stride, k_head_stride, es) || !rows_of_16(v, v_token_stride, v_head_stride, es) ||
+        (num_q_heads && (!rows_of_16(q, q_token_stride, q_head_stride, es) || !rows_of_16(q_out, 0, 0, es))) ||
+        (k_out && !rows_of_16(k_out, 0, 0, es))) {
         set_error("4-bit KV append: rows are 16-byte aligned");
         return OJASX_ERR_INVALID;
     }
@@ -440,7 +435,7 @@ OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start
     }
     if (num_tokens == 0) return OJASX_OK;
     if (!start || !k_out || !v_out) return OJASX_ERR_NULL;
-    if (!rows_ok(k_out, 0, 0, 4) || !rows_ok(v_out, 0, 0, 4)) {
+    if (!rows_of_16(k_out, 0, 0, 4) || !rows_of_16(v_out, 0, 0, 4)) {
         set_error("4-bit KV read: outputs are 16-byte aligned");
         return OJASX_ERR_INVALID;
     }

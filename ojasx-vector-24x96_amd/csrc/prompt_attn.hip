@@ -805,7 +805,7 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
             }
             if (BUFFERS == 2) load(tile + 2);
             s0 += s1;
-            if (k0 + KEYS - 1 > lim_lo) {
+            if (k0 + KEYS - 1 > lim_lo) {            // mask_tile, whose array of one costs a spill here
                 int rel = lim - k0 - 4 * h;
                 asm volatile("" : "+v"(rel));
 #pragma unroll
@@ -996,11 +996,6 @@ int launch32(PromptParams p, hipStream_t st) {
     OJX_HIP(hipGetLastError());
     return OJASX_OK;
 }
-
-bool rows16(const void *p, long ts, long hs, size_t es) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ts >= 0 && hs >= 0 && ts * es % 16 == 0 &&
-           hs * es % 16 == 0;
-}
 }  // namespace
 
 }  // namespace ojx
@@ -1039,9 +1034,9 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
     if (num_q_tokens == 0) return OJASX_OK;
     if (!q || !out || !cu_seqlens_q || !cu_seqlens_kv || (num_kv_tokens && (!k || !v))) return OJASX_ERR_NULL;
     const size_t es = dtype == OJASX_DTYPE_F32 ? 4 : 2;
-    if (!rows16(q, q_token_stride, q_head_stride, es) || !rows16(out, 0, 0, es) ||
-        (num_kv_tokens && (!rows16(k, k_token_stride, k_head_stride, es) ||
-                           !rows16(v, v_token_stride, v_head_stride, es)))) {
+    if (!rows_of_16(q, q_token_stride, q_head_stride, es) || !rows_of_16(out, 0, 0, es) ||
+        (num_kv_tokens && (!rows_of_16(k, k_token_stride, k_head_stride, es) ||
+                           !rows_of_16(v, v_token_stride, v_head_stride, es)))) {
         set_error("prompt attention: rows are 16-byte aligned");
         return OJASX_ERR_INVALID;
     }
