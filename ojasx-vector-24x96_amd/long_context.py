@@ -809,10 +809,10 @@ class PagedInt4KVCache:
         self.rotary_dim, self.interleaved = rotary_dim, bool(interleaved)
         self.num_pages = num_sequences * max_resident_pages if num_pages is None else num_pages
         rows = self.num_pages * num_kv_heads * page_size
-        self.k_codes = torch.zeros(rows * head_dim // 2, dtype=torch.uint8, device=dev)
-        self.v_codes = torch.zeros_like(self.k_codes)
-        self.k_steps = torch.zeros(rows * head_dim // group_size * 2, dtype=torch.float16, device=dev)
-        self.v_steps = torch.zeros_like(self.k_steps)
+        self._k_codes = torch.zeros(rows * head_dim // 2, dtype=torch.uint8, device=dev)
+        self._v_codes = torch.zeros_like(self._k_codes)
+        self._k_steps = torch.zeros(rows * head_dim // group_size * 2, dtype=torch.float16, device=dev)
+        self._v_steps = torch.zeros_like(self._k_steps)
         if num_pages is None:
             table = torch.arange(self.num_pages, dtype=torch.int32, device=dev)
         else:
@@ -826,6 +826,12 @@ class PagedInt4KVCache:
                                 num_kv_heads, head_dim, group_size, rotary_dim, int(self.interleaved))
         self._ref = ctypes.addressof(self._c)
         self._workspace_bytes = {}       # (query heads, max_seen) -> bytes
+
+    # The kernels hold these tensors by address: they are filled in, never replaced.
+    k_codes = property(lambda self: self._k_codes, doc="Codes of the keys, as csrc/kv4.h lays them out.")
+    v_codes = property(lambda self: self._v_codes, doc="Codes of the values.")
+    k_steps = property(lambda self: self._k_steps, doc="Steps and smallest values of the keys' groups.")
+    v_steps = property(lambda self: self._v_steps, doc="Steps and smallest values of the values' groups.")
 
     @property
     def block_table(self):

@@ -181,3 +181,14 @@ def test_single_tokens_of_a_large_batch(lc, dev):
         assert torch.equal(x, y) and np.array_equal(f64(x), want.astype(np.float32).astype(np.float64))
     qf = kv4.rotate(f64(q), starts, kv4.inv_freq(64, 1e6))
     assert (np.abs(f64(a) - qf) <= 2 * eps_half("bfloat16") * np.abs(qf)).all()
+
+
+@pytest.mark.parametrize("name", ["k_codes", "v_codes", "k_steps", "v_steps", "block_table"])
+def test_buffers_are_filled_in_not_replaced(lc, dev, name):
+    """The kernels hold the buffers' addresses: a tensor put in a buffer's place would be ignored, and
+    the memory that they go on writing freed."""
+    c = lc.PagedInt4KVCache(1, 64, max_resident_pages=4, device=dev)
+    t = getattr(c, name)
+    with pytest.raises(AttributeError):
+        setattr(c, name, t.clone())
+    assert getattr(c, name) is t
