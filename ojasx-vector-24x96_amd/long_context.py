@@ -789,20 +789,24 @@ class PagedInt4KVCache:
             rotary_dim = head_dim
         if rotary_dim < 0 or rotary_dim > head_dim or rotary_dim % 16:
             raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim, got {rotary_dim}")
+        turns = None
+        if rotary_dim:
+            if inv_freq is None:
+                if not 0.0 < float(rope_theta) < math.inf:
+                    raise ValueError(f"rope_theta must be positive and finite, got {rope_theta}")
+                inv_freq = float(rope_theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+                                                 / rotary_dim)
+            inv_freq = torch.as_tensor(inv_freq).detach().to(device="cpu", dtype=torch.float64)
+            if tuple(inv_freq.shape) != (rotary_dim // 2,) or not torch.isfinite(inv_freq).all():
+                raise ValueError(f"inv_freq must hold {rotary_dim // 2} finite values, got "
+                                 f"{tuple(inv_freq.shape)}")
+            turns = inv_freq / (2.0 * math.pi)
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         dev = self.device
         self._index = dev.index
-        turns = None
-        if rotary_dim:
-            if inv_freq is None:
-                inv_freq = float(rope_theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64)
-                                                 / rotary_dim)
-            inv_freq = torch.as_tensor(inv_freq).to(device="cpu", dtype=torch.float64)
-            if tuple(inv_freq.shape) != (rotary_dim // 2,):
-                raise ValueError(f"inv_freq must hold {rotary_dim // 2} values, got "
-                                 f"{tuple(inv_freq.shape)}")
-            turns = (inv_freq / (2.0 * math.pi)).to(dev)
+        if turns is not None:
+            turns = turns.to(dev)
         self.num_kv_heads, self.head_dim, self.group_size = num_kv_heads, head_dim, group_size
         self.num_sequences, self.page_size = num_sequences, page_size
         self.max_resident_pages, self.sink_pages = max_resident_pages, sink_pages

@@ -192,3 +192,15 @@ def test_scales_that_are_not_finite_are_refused(pkg):
         assert L.ojasx_prompt_attention_device(FAKE, 512, 128, FAKE, 512, 128, FAKE, 512, 128, 0, 4, 4, 4, 4, 128, FAKE,
                                                FAKE, 1, 1, s, 0, FAKE, None, None) == -3
         assert b"scale" in L.ojasx_get_last_error()
+
+
+def test_frequencies_that_are_not_finite_are_refused(pkg):
+    """They would rotate every key into NaN, which the cache then holds."""
+    import torch
+    from importlib import import_module
+    lc = import_module(pkg.__name__ + ".long_context")
+    for kw in (dict(rope_theta=0.0), dict(rope_theta=-1e4), dict(rope_theta=float("nan")), dict(rope_theta=float("inf")),
+               dict(inv_freq=torch.full((64,), float("nan"))), dict(inv_freq=[float("inf")] + [0.0] * 63),
+               dict(inv_freq=torch.ones(63))):
+        with pytest.raises(ValueError):
+            lc.PagedInt4KVCache(2, **kw)
