@@ -363,7 +363,8 @@ OJASX_API int ojasx_kv4_read_device(const OjasxKV4Cache *cache, const int *start
 /* Attention of one query token per sequence over its resident tokens:
  * q, out [num_sequences][num_q_heads][head_dim] in dtype (F32, BF16, F16), head
  * j reading kv head j / (num_q_heads / num_kv_heads); seen: the tokens of each
- * sequence so far (0: a row of zeros).  scale_factor <= 0: 1/sqrt(head_dim);
+ * sequence so far (0: a row of zeros; tokens that all score -inf: NaN).  Scores and
+ * sums are fp32, weights 11 bits for BF16 outputs, 22 else.  scale_factor <= 0: 1/sqrt(head_dim);
  * one that is NaN or not finite times log2(e) is refused.
  * max_seen bounds seen[] (0: the cache's capacity) and with it the size of the
  * launch; larger entries of seen are attended in full all the same.
@@ -384,8 +385,10 @@ OJASX_API int ojasx_kv4_decode_device(const OjasxKV4Cache *cache, const void *q,
  * strides of tokens and heads, rows 16-byte aligned; head_dim a multiple of 8 up
  * to 256; query head h reads kv head h / (num_heads / num_kv_heads).  out
  * [num_q_tokens][num_heads][head_dim] contiguous in dtype; lse [num_q_tokens][num_heads]
- * fp32, the natural log of sum exp(scale * score), or NULL.  Keys that a row does
- * not see reach nothing, whatever they hold.  Rows of no sequence are left as
+ * fp32, the natural log of sum exp(scale * score), or NULL.  A row whose keys all
+ * score -inf is NaN, with lse -inf.  Scores, maxima and sums are fp32; the softmax's
+ * weights are rounded to dtype for the value product.  Keys that a row does not see
+ * reach nothing, whatever they hold.  Rows of no sequence are left as
  * they are, or with zero_rest != 0 written as 0 (lse -inf).  A call that would
  * need 2^24 workgroups (blocks of 32 rows or more by up to four heads) is
  * refused. */

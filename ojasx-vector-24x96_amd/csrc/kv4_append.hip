@@ -15,7 +15,7 @@
 // 128, queries rotated along: bf16 45 to 49 us for 178 MB, 3.8 TB/s, fp32 88 us for
 // 346 MB, 3.9 TB/s (a copy runs at 4.9 here).  One token: 4 us, a launch and three
 // loads that wait for each other.  Reading the 8192 tokens back as bf16: 15 us for
-// 44 MB.
+// 44 MB (a lane loads its values' codes byte by byte).
 #include "kv4.h"
 
 namespace ojx {

@@ -44,11 +44,12 @@
 // sequence that lies in one run is written whole, of the others each run leaves
 // (out, max, sum) in slot run + sequence, and kv4_merge_kernel joins them.
 //
-// Bound by the reading of the pages: 131072 bf16 tokens, 32 / 8 heads of 128, groups
-// of 64, 32 us for 151 MB, 4.6 TB/s (a copy runs at 4.9 here); 64 sequences of 192000
-// tokens in all, groups of 32, 56 us for 246 MB, 4.4 TB/s; with narrow heads by a
-// wave's way through its tiles: 16 sequences of 32000 held fp16 tokens, 16 heads of 64,
-// 15 us for 38 MB.  The merge is a second launch, 4 to 5 us.
+// Bound by the reading of the pages (a copy runs at 4.9 TB/s here): 131072 bf16 tokens,
+// 32 / 8 heads of 128, groups of 64, 39 us for 151 MB, 3.8 TB/s (32 where the last-level
+// cache holds them all); 64 sequences of 192000 tokens in all, groups of 32, 58 us for 247
+// MB, 4.2 TB/s, and 100 us with 64 / 8 heads, which take two passes over the cache; with
+// narrow heads by a wave's way through its tiles: 16 sequences of 32000 held fp16
+// tokens, 16 heads of 64, 15 to 16.5 us for 35 MB.  The merge is a second launch, 4 to 5 us.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

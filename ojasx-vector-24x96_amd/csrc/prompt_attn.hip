@@ -23,11 +23,12 @@
 // Bound by the matrix instructions where rows are long, and by exponentials with
 // narrow heads: a score costs 4 D operations there and one exp2 at a quarter of the
 // vector rate, about as long as its products at D = 64.  Measured, one pass, causal,
-// 32 / 8 heads of 128 but where said: 16384 bf16 tokens of one sequence 2.06 to 2.29
-// ms by the card's clock, 960 to 1070 TFLOP/s (a large bf16 matrix product of the
-// library runs at 1200); 8192 of eight 0.12 ms; 4999 fp16 tokens of five sequences, 16
-// heads of 64, 30 us; 2048 fp32 of two 138 to 147 us; 150 bf16 of three 7.4 us, of
-// which a launch with nothing to do is half.
+// 32 / 8 heads of 128 but where said: 16384 bf16 tokens of one sequence 2.10 to 2.34
+// ms by the card's clock, 940 to 1050 TFLOP/s (a large bf16 matrix product of the
+// library runs at 1200); 8192 of eight 0.11 to 0.12 ms, 0.155 with 16 / 8 heads of 256;
+// 4999 fp16 tokens of five sequences, 16 heads of 64, 30 us; 2048 fp32 of two 130 to 140
+// us, 412 with 16 / 8 heads of 256; 150 bf16 of three 7.6 us, of which a launch with
+// nothing to do is half.
 #include <cmath>
 #include <type_traits>
 

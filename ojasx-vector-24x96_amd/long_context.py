@@ -916,7 +916,8 @@ class PagedInt4KVCache:
         ``append``: (k, v), each [num_tokens, num_kv_heads, head_dim] in
         ``dtype`` (float32 unless given).  ``seen`` (int32 [num_sequences]): the
         tokens of each sequence so far, where that is more than the last one
-        read; a token its sequence has evicted reads as 0."""
+        read; a token its sequence has evicted reads as 0 (as a key it would
+        take weight: leave such rows out of an attention over them)."""
         torch = _torch()
         dtype = torch.float32 if dtype is None else dtype
         tag = _attn_tag(dtype)
@@ -942,8 +943,10 @@ class PagedInt4KVCache:
         float16), over the resident ones of the ``seen[b]`` tokens (int32
         [num_sequences], the current one included) of each sequence; q head j
         reads kv head j // (num_q_heads // num_kv_heads).  ``scale_factor <= 0``
-        means 1/sqrt(head_dim); a sequence without tokens gives 0.  ``out`` may be
-        the query itself.
+        means 1/sqrt(head_dim); a sequence without tokens gives 0, one whose
+        tokens all score -inf NaN.  Scores and sums are float32; for bfloat16
+        outputs a softmax weight is rounded to 11 bits in the product with the
+        values.  ``out`` may be the query itself.
         ``max_seen``, a bound on ``seen`` where the caller knows one, keeps the
         launch of short sequences as small as they are."""
         torch = _torch()
@@ -980,10 +983,12 @@ class PagedInt4KVCache:
 class PackedPromptAttention:
     """Attention of packed prompts: the queries of every sequence over its own
     keys, in one launch.  float32, bfloat16 or float16; head_dim a multiple of
-    8 up to 256; scores times ``scale`` (1/sqrt(head_dim) unless given), sums
-    and softmax in float32.  Where OnlineSoftmaxBlockAttention is exact (fp64)
-    over one sequence's tiles, this is the batch's prefill at the speed of the
-    inputs' own type."""
+    8 up to 256; scores times ``scale`` (1/sqrt(head_dim) unless given).
+    Scores, the softmax's maxima and sums and the outputs' sums are float32;
+    the softmax's weights are rounded to bfloat16 or float16 inputs' type for
+    the product with the values, as the output is once more.  Where
+    OnlineSoftmaxBlockAttention is exact (fp64) over one sequence's tiles, this
+    is the batch's prefill at the speed of the inputs' own type."""
 
     def __init__(self, num_heads: int, num_kv_heads: Optional[int] = None, head_dim: int = 128, *,
                  causal: bool = True, scale: Optional[float] = None) -> None:
@@ -1013,7 +1018,11 @@ class PackedPromptAttention:
         cu_seqlens[b + 1] - 1 (int32 [B + 1] on the device) are sequence b's.
         With ``cu_seqlens_kv`` its keys are those rows instead, and query i of
         Lq sees keys j <= i + Lk - Lq: a prompt's last rows over keys that
-        begin earlier.  A row that sees no key is 0.
+        begin earlier.  A row that sees no key is 0; one whose keys all score
+        -inf is NaN.  What a row does not see reaches it in no way; an infinity
+        or NaN that it sees, or scores past 2^20, cost its call a second pass
+        over the keys (about 2.3 times the time; 5 times where all values are
+        infinite or NaN).
 
         Returns the output [N, num_heads, head_dim] in the query's dtype, or
         (output, lse float32 [N, num_heads]) with ``return_lse``.  Rows of no
