@@ -252,7 +252,7 @@ class OnlineSoftmaxBlockAttention:
         if min(num_heads, head_dim, q_block_size, kv_block_size) <= 0:
             raise ValueError("Attention dimensions and block sizes must be positive")
         self.num_heads = int(num_heads)
-        self.num_kv_heads = int(num_kv_heads or num_heads)
+        self.num_kv_heads = self.num_heads if num_kv_heads is None else int(num_kv_heads)
         if self.num_heads % self.num_kv_heads != 0:
             raise ValueError(f"num_heads ({self.num_heads}) must be divisible by num_kv_heads "
                              f"({self.num_kv_heads})")
@@ -993,7 +993,7 @@ class PackedPromptAttention:
     def __init__(self, num_heads: int, num_kv_heads: Optional[int] = None, head_dim: int = 128, *,
                  causal: bool = True, scale: Optional[float] = None) -> None:
         self.num_heads = int(num_heads)
-        self.num_kv_heads = int(num_kv_heads or num_heads)
+        self.num_kv_heads = self.num_heads if num_kv_heads is None else int(num_kv_heads)
         self.head_dim = int(head_dim)
         if self.num_heads <= 0 or self.num_kv_heads <= 0 or self.num_heads % self.num_kv_heads:
             raise ValueError(f"num_heads ({self.num_heads}) must be divisible by num_kv_heads "

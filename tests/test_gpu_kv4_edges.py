@@ -192,3 +192,28 @@ def test_buffers_are_filled_in_not_replaced(lc, dev, name):
     with pytest.raises(AttributeError):
         setattr(c, name, t.clone())
     assert getattr(c, name) is t
+
+
+def test_two_streams_at_once(lc, dev):
+    """Decodes of one cache and prompts on two streams at the same time, one prompt with a NaN that
+    takes its second pass: each has its own workspace, the results are the calls' own."""
+    import torch
+    c, q, hk, hv = decode_case(lc, dev, 128, 32, "bfloat16", 16, 2, 4, [900, 3, 2000, 77], 128)
+    seen, n = i32(dev, [900, 3, 2000, 77]), 700
+    pq, pk, pv = (rand(dev, "bfloat16", n, h, 128, seed=s) for h, s in ((8, 1), (2, 2), (2, 3)))
+    pn = pv.clone()
+    pn[100, 0, 3] = float("nan")
+    a, cu = lc.PackedPromptAttention(8, 2, 128), i32(dev, [0, 300, n])
+    qs = [q, q * 0.5]
+    want = [(c.decode(x, seen), a(pq, pk, v, cu)) for x, v in zip(qs, (pv, pn))]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((c.decode(qs[i], seen), a(pq, pk, (pv, pn)[i], cu)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for d, p in got[i]:
+            assert torch.equal(d, want[i][0]) and torch.equal(p.nan_to_num(7), want[i][1].nan_to_num(7))

@@ -204,3 +204,12 @@ def test_frequencies_that_are_not_finite_are_refused(pkg):
                dict(inv_freq=torch.ones(63))):
         with pytest.raises(ValueError):
             lc.PagedInt4KVCache(2, **kw)
+
+
+def test_no_kv_heads_are_refused(pkg):
+    """0 kv heads are not the default."""
+    from importlib import import_module
+    lc = import_module(pkg.__name__ + ".long_context")
+    with pytest.raises(ValueError):
+        lc.PackedPromptAttention(4, 0, 64)
+    assert lc.PackedPromptAttention(4, None, 64).num_kv_heads == 4
