@@ -174,7 +174,8 @@ def test_a_nan_does_not_stall_a_batch(lc, dev):
     assert took(v2) < 6 * took(v)
 
 
-@pytest.mark.parametrize("dtype,Hq,Hkv,n", [("bfloat16", 4, 2, 400), ("bfloat16", 32, 32, 900), ("float32", 4, 1, 300)])
+@pytest.mark.parametrize("dtype,Hq,Hkv,n", [("bfloat16", 4, 2, 400), ("bfloat16", 32, 32, 900), ("float32", 4, 1, 300),
+                                            ("bfloat16", 32, 8, 3000), ("float16", 48, 48, 2500)])
 def test_out_is_the_query_with_a_nan(lc, dev, dtype, Hq, Hkv, n):
     """A second pass reads the queries again: rows already written into them take no part."""
     import torch
@@ -262,3 +263,44 @@ def test_prompt_over_the_cache(lc, dev, dtype):
             assert torch.equal(got.cpu(), want)
         out = a(qr, rk, rv, i32(dev, cum(lengths)), i32(dev, ck))
         check(out, qr, rk, rv, cum(lengths), ck, True, D ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype,H,D", [("bfloat16", 80, 64), ("float16", 64, 128), ("bfloat16", 64, 128), ("float16", 32, 256),
+                                       ("float16", 80, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_infinities_in_large_grids(lc, dev, dtype, H, D, causal):
+    """As test_infinities_that_many_rows_see, past the rule that splits a tile's keys over two waves: each
+    wave has rows of its own, and those without a NaN are written before the second pass."""
+    import torch
+    lengths = [450, 70, 333]
+    N, cu = sum(lengths), cum(lengths)
+    assert (N // 128 + 5) * H > (768 if D <= 64 else 512 if D <= 128 else 256)
+    q, k, v = (rand(dev, dtype, N, H, D, seed=s) for s in (1, 2, 3))
+    a = lc.PackedPromptAttention(H, H, D, causal=causal)
+    v2 = v.clone()
+    inf = float("inf")
+    v2[140, 0, 3], v2[200, 0, 4], v2[300, 0, 4], v2[cu[1] + 69, 1, 5], v2[310, H - 1, 6] = inf, -inf, inf, -inf, float("nan")
+    out, lse = a(q, k, v2, i32(dev, cu), return_lse=True)
+    got, l2 = f64(out), f64(lse)
+    for b in range(3):
+        s, n = slice(cu[b], cu[b + 1]), lengths[b]
+        for h in (0, 1, 2, H - 1):
+            x, K, V = f64(q)[s, h], f64(k)[s, h], f64(v2)[s, h]
+            sc = x @ K.T * D ** -0.5
+            if causal:
+                sc = np.where(np.tri(n, dtype=bool), sc, -np.inf)
+            w = np.exp(sc - sc.max(1, keepdims=True))
+            total = w.sum(1, keepdims=True)
+            seen = np.tri(n) if causal else np.ones((n, n))
+            up, down, nan = (seen @ m for m in (V == inf, V == -inf, np.isnan(V)))
+            F = np.where(np.isfinite(V), V, 0)
+            want = (w @ F) / total
+            score = 2 ** -24 * (16 * D ** -0.5 * np.abs(x).max(0) @ np.abs(K).max(0) + 30)
+            tol = (w @ np.abs(F)) / total * (2 * score + eps_half(dtype) + 2 ** -21) + eps_half(dtype) * np.abs(want) + 1e-7
+            ok = np.abs(got[s, h] - want) <= tol
+            g = got[s, h]
+            both = (up > 0) & (down > 0) | (nan > 0)
+            ok = np.where(both, np.isnan(g), np.where(up > 0, g == inf, np.where(down > 0, g == -inf, ok)))
+            assert ok.all(), (b, h, np.argwhere(~ok)[:3])
+            want_l = (sc.max(1, keepdims=True) + np.log(total))[:, 0]
+            assert (np.abs(l2[s, h] - want_l) <= score + 2 ** -21 * (1 + np.abs(want_l))).all()
