@@ -559,22 +559,22 @@ __device__ __forceinline__ int prompt_block_attn(const PromptParams &p, int slot
                 }
             } else {
 #pragma unroll
-            for (int i = 0; i < VB; ++i) read_v(i);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) weight(0, e);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < 2 * NB * NT2; ++i) {
-                const int f = i / NT2, t = i % NT2;
-                if (i + VB < 2 * NB * NT2) read_v(i + VB);
+                for (int i = 0; i < VB; ++i) read_v(i);
                 __builtin_amdgcn_sched_barrier(0);
-                acc[t] = E::mma(v_of(i), pf[f], acc[t]);
-                if (f < 2 * NB - 1)
 #pragma unroll
-                    for (int e = 0; e < PART; ++e) weight(f + 1, t * PART + e);
+                for (int e = 0; e < 8; ++e) weight(0, e);
                 __builtin_amdgcn_sched_barrier(0);
-            }
+#pragma unroll
+                for (int i = 0; i < 2 * NB * NT2; ++i) {
+                    const int f = i / NT2, t = i % NT2;
+                    if (i + VB < 2 * NB * NT2) read_v(i + VB);
+                    __builtin_amdgcn_sched_barrier(0);
+                    acc[t] = E::mma(v_of(i), pf[f], acc[t]);
+                    if (f < 2 * NB - 1)
+#pragma unroll
+                        for (int e = 0; e < PART; ++e) weight(f + 1, t * PART + e);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             l += lt;
         }
@@ -880,20 +880,20 @@ __device__ __forceinline__ int prompt_block_f32(const PromptParams &p, int slots
                     __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
-            read_v(0);
-            __builtin_amdgcn_sched_barrier(0);
-            weights(0, 0, 8);
-            __builtin_amdgcn_sched_barrier(0);
+                read_v(0);
+                __builtin_amdgcn_sched_barrier(0);
+                weights(0, 0, 8);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 2 * NT2; ++i) {
-                if (i + 1 < 2 * NT2) read_v(i + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                bf16x8_t z[3];
-                v_of(i, z);
-                mma6(z, pf[i / NT2], acc[i % NT2], acc[(SETS - 1) * NT2 + i % NT2]);
-                if (i * PART < 8) weights(1, i * PART, i * PART + PART);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                for (int i = 0; i < 2 * NT2; ++i) {
+                    if (i + 1 < 2 * NT2) read_v(i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    bf16x8_t z[3];
+                    v_of(i, z);
+                    mma6(z, pf[i / NT2], acc[i % NT2], acc[(SETS - 1) * NT2 + i % NT2]);
+                    if (i * PART < 8) weights(1, i * PART, i * PART + PART);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             l += lt;
         }
