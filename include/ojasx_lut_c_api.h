@@ -401,6 +401,101 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
                                             float scale, int zero_rest, void *out, float *lse,
                                             void *stream);
 
+/* ---- evicting KV cache (no reference counterpart) ------------------------- */
+/* A cache of num_sequences sequences in the element type dtype (F32, BF16 or
+ * F16) that counts the attention its tokens get and drops those that get
+ * least.  Token slot t of a sequence lies in slot t % page_size of page
+ * block_table[sequence][t / page_size]; an entry outside [0, num_pages) is a page
+ * that is not there: its tokens are not written and not attended.  A page holds
+ * for each kv head page_size rows of keys and values, weights (the softmax
+ * weights that a token got, fp32) and positions; the order is [num_pages]
+ * [num_kv_heads][page_size]([head_dim]).  Pages that decode counts into or that
+ * evict moves belong to one sequence.  How many tokens a sequence holds is the
+ * caller's: int32 arrays on the device, so every call can be captured and
+ * replayed while they change.  head_dim 64, 128 or 256; page_size a power of
+ * two from 16 to 32768; keys and values 16-byte aligned.  The struct is read during
+ * the call. */
+typedef struct OjasxKVECache {
+    void *keys, *values;
+    float *weights;
+    int *positions;
+    const int *block_table;        /* [num_sequences][max_pages] */
+    const double *turns;           /* [rotary_dim / 2]: frequency / (2 pi), turns per position */
+    int num_sequences, max_pages, page_size, num_pages;
+    int num_kv_heads, head_dim, dtype;
+    int rotary_dim;                /* dimensions that rotate: a multiple of 16, 0: none */
+    int interleaved;               /* pairs (2 i, 2 i + 1) instead of (i, i + rotary_dim / 2) */
+} OjasxKVECache;
+/* Rotates queries and keys by their positions and writes keys and values.
+ * Rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32, num_sequences + 1) go to
+ * sequence b's slots start[b], start[b] + 1, ... and stand at positions
+ * position[b], position[b] + 1, ... (NULL: the slots' numbers); cu_seqlens NULL:
+ * one token for each sequence.  weight [num_tokens][num_kv_heads]: the tokens'
+ * weights (NULL: 0).  q, k, v, their strides, q_out and rows of no sequence as in
+ * ojasx_kv4_append_device, in the cache's dtype; a slot outside the sequence's
+ * pages is not written. */
+OJASX_API int ojasx_kve_append_device(const OjasxKVECache *cache, const void *q, long q_token_stride,
+                                      long q_head_stride, int num_q_heads, void *q_out, const void *k,
+                                      long k_token_stride, long k_head_stride, const void *v,
+                                      long v_token_stride, long v_head_stride, const float *weight,
+                                      int num_tokens, const int *start, const int *position,
+                                      const int *cu_seqlens, void *stream);
+/* Attention of one query token per sequence over its first held[b] slots: q, out
+ * [num_sequences][num_q_heads][head_dim] in the cache's dtype, 16-byte aligned,
+ * head j reading kv head j / (num_q_heads / num_kv_heads) (at most 128 query heads
+ * of a kv head); a sequence without tokens gives 0, one whose tokens all score
+ * -inf NaN.  With count != 0 each token's softmax weights, summed over the query
+ * heads of its kv head, are added to its weight.  Scores, sums and weights are
+ * fp32; BF16 and F16 round the softmax's weights for the value product.
+ * scale_factor <= 0: 1/sqrt(head_dim).  max_held bounds held[] (0: the pages'
+ * slots) and with it launch and workspace; of a longer sequence the first
+ * max_held tokens are attended.  workspace: ojasx_kve_decode_workspace(...) bytes
+ * for the same arguments, 16-byte aligned, one for each call that may run at the
+ * same time. */
+OJASX_API long ojasx_kve_decode_workspace(const OjasxKVECache *cache, int num_q_heads, int max_held, int count);
+OJASX_API int ojasx_kve_decode_device(const OjasxKVECache *cache, const void *q, int num_q_heads, const int *held,
+                                      int max_held, float scale_factor, int count, void *out, void *workspace,
+                                      long workspace_bytes, void *stream);
+/* Of each sequence and kv head that holds more than budget tokens, budget stay:
+ * those at positions below sink_tokens, those of the recent_tokens newest positions,
+ * and of the others the ones of largest weight, ties to the lowest slot (NaN
+ * least of all).  A kept token from behind the budget takes the place of a
+ * dropped one before it, the i-th of them the i-th place, with its weight and
+ * position; nothing else is written.  held is read: it is min(held, budget) after
+ * the call.  sink_tokens + recent_tokens <= budget; where more tokens than the
+ * budget stand at such positions, the lowest slots of them stay.  max_held as
+ * above. */
+OJASX_API long ojasx_kve_evict_workspace(const OjasxKVECache *cache, int budget, int max_held);
+OJASX_API int ojasx_kve_evict_device(const OjasxKVECache *cache, const int *held, int budget, int sink_tokens,
+                                     int recent_tokens, int max_held, void *workspace, long workspace_bytes,
+                                     void *stream);
+
+/* ---- sampling (no reference counterpart) ---------------------------------- */
+/* One token of every row of logits [num_rows][vocab] (dtype F32, BF16 or F16,
+ * row_stride elements apart) from the random number uniform[row] in [0, 1).  With
+ * e_i = exp((l_i - max l) / temperature) and the tokens in order of falling logits,
+ * equal ones of rising index: top_k > 0 keeps the first top_k, top_p < 1 of those the
+ * shortest beginning with at least top_p of their sum of e, min_p > 0 of those the ones
+ * with e_i >= min_p; the token is the first kept one, in the vocabulary's order, at
+ * which the running sum of e passes uniform times the kept sum.  temperature 0:
+ * the largest logit, of equal ones the first.  Each setting is one value for all rows,
+ * or an array of a value for each on the device (NULL: the value; values out of range
+ * count as the nearest one in it, a temperature that is negative, NaN or infinite
+ * gives -1).  e is fp64; a token of e below 2^-51 is not drawn.  A row
+ * with a NaN or +inf, or of -inf alone, gives -1.  vocab at most 2^22.  workspace:
+ * ojasx_sample_workspace(...) bytes, 16-byte aligned, one for each call that may
+ * run at the same time. */
+typedef struct OjasxSampling {
+    double temperature, top_p, min_p;
+    const float *temperatures, *top_ps, *min_ps;   /* [num_rows] or NULL */
+    const int *top_ks;                             /* [num_rows] or NULL */
+    int top_k;
+} OjasxSampling;
+OJASX_API long ojasx_sample_workspace(int num_rows, int vocab);
+OJASX_API int ojasx_sample_device(const void *logits, int dtype, int num_rows, int vocab, long row_stride,
+                                  const float *uniform, const OjasxSampling *settings, int *tokens,
+                                  void *workspace, long workspace_bytes, void *stream);
+
 /* ---- MoE (ref.h:125-150) ---------------------------------------------- */
 OJASX_API OjasxMoEHandle ojasx_create_moe(int num_experts, int hidden_dim,
                                           int intermediate_dim, int top_k, int block_dim,

@@ -83,6 +83,14 @@ SIGNATURES = {
     "ojasx_kv4_read_device": (ci, [vp, vp, vp, vp, ci, vp, vp, ci, vp]),
     "ojasx_kv4_decode_workspace": (cl, [vp, ci, ci]),
     "ojasx_kv4_decode_device": (ci, [vp, vp, ci, ci, vp, ci, cf, vp, vp, cl, vp]),
+    "ojasx_kve_append_device": (ci, [vp, vp, cl, cl, ci, vp, vp, cl, cl, vp, cl, cl, vp, ci, vp, vp, vp,
+                                     vp]),
+    "ojasx_kve_decode_workspace": (cl, [vp, ci, ci, ci]),
+    "ojasx_kve_decode_device": (ci, [vp, vp, ci, vp, ci, cf, ci, vp, vp, cl, vp]),
+    "ojasx_kve_evict_workspace": (cl, [vp, ci, ci]),
+    "ojasx_kve_evict_device": (ci, [vp, vp, ci, ci, ci, ci, vp, cl, vp]),
+    "ojasx_sample_workspace": (cl, [ci, ci]),
+    "ojasx_sample_device": (ci, [vp, ci, ci, ci, cl, vp, vp, vp, vp, cl, vp]),
     "ojasx_prompt_attention_device": (ci, [vp, cl, cl, vp, cl, cl, vp, cl, cl, ci, ci, ci, ci, ci, ci,
                                            vp, vp, ci, ci, cf, ci, vp, vp, vp]),
 }
@@ -106,6 +114,21 @@ class KV4Cache(ctypes.Structure):
                 ("num_sequences", ci), ("max_pages", ci), ("sink_pages", ci), ("page_size", ci),
                 ("num_pages", ci), ("num_kv_heads", ci), ("head_dim", ci), ("group_size", ci),
                 ("rotary_dim", ci), ("interleaved", ci)]
+
+
+class KVECache(ctypes.Structure):
+    """OjasxKVECache: the buffers and shape of an evicting paged KV cache."""
+    _fields_ = [("keys", vp), ("values", vp), ("weights", vp), ("positions", vp),
+                ("block_table", vp), ("turns", vp),
+                ("num_sequences", ci), ("max_pages", ci), ("page_size", ci), ("num_pages", ci),
+                ("num_kv_heads", ci), ("head_dim", ci), ("dtype", ci), ("rotary_dim", ci),
+                ("interleaved", ci)]
+
+
+class Sampling(ctypes.Structure):
+    """OjasxSampling: the settings of a draw, each one value or an array of one for each row."""
+    _fields_ = [("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double),
+                ("temperatures", vp), ("top_ps", vp), ("min_ps", vp), ("top_ks", vp), ("top_k", ci)]
 
 
 DTYPE_F32 = 0

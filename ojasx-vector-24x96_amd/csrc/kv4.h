@@ -61,6 +61,49 @@ __device__ __forceinline__ void load8(const __half *p, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
 }
 
+__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
+    *reinterpret_cast<f4_t *>(p) = f4_t{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f4_t *>(p + 4) = f4_t{x[4], x[5], x[6], x[7]};
+}
+__device__ __forceinline__ void store8(__hip_bfloat16 *p, const float (&x)[8]) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    b8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (__bf16)x[i];
+    *reinterpret_cast<b8 *>(p) = a;
+}
+__device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    h8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (_Float16)x[i];
+    *reinterpret_cast<h8 *>(p) = a;
+}
+
+// The angles of position pos, as the factors of a lane's dimensions d0 .. d0 + 7: x_e <-
+// x_e co[e] + (the value it turns with) sn[e].  turns: frequencies / (2 pi) of the `half` =
+// rotary_dim / 2 pairs.  Whole waves call it, each with `half` entries of LDS of its own.
+__device__ __forceinline__ void token_angles(const double *turns, int half, bool interleaved, int pos, int d0,
+                                             double2 *cs, double (&co)[8], double (&sn)[8]) {
+    for (int i = threadIdx.x & 63; i < half; i += 64) {
+        const double f = turns[i], t = (double)pos * f;
+        const double frac = (t - rint(t)) + fma((double)pos, f, -t);
+        double s, c;
+        sincospi(2.0 * frac, &s, &c);
+        cs[i] = make_double2(c, s);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const bool rotates = d0 < 2 * half, low = d0 < half;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int i = interleaved ? (d0 + e) / 2 : low ? d0 + e : d0 - half + e;
+        const double2 a = rotates ? cs[i] : make_double2(1.0, 0.0);
+        co[e] = a.x;
+        sn[e] = (interleaved ? e % 2 == 0 : low) ? -a.y : a.y;
+    }
+}
+
 // Entry of the block table that holds page j of a sequence.
 __device__ __forceinline__ int kv4_entry(const Kv4View &c, int j) {
     return j < c.sink ? j : c.sink + (j - c.sink) % (c.max_pages - c.sink);

@@ -23,8 +23,6 @@ namespace ojx {
 namespace {
 constexpr int kNT = 256;
 
-typedef float v4f __attribute__((ext_vector_type(4)));
-
 struct Kv4AppendParams {
     Kv4View c;
     const void *q, *k, *v;
@@ -33,25 +31,6 @@ struct Kv4AppendParams {
     const int *start, *cu;
     int n, Hq, parts;
 };
-
-__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
-    *reinterpret_cast<v4f *>(p) = v4f{x[0], x[1], x[2], x[3]};
-    *reinterpret_cast<v4f *>(p + 4) = v4f{x[4], x[5], x[6], x[7]};
-}
-__device__ __forceinline__ void store8(__hip_bfloat16 *p, const float (&x)[8]) {
-    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-    b8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (__bf16)x[i];
-    *reinterpret_cast<b8 *>(p) = a;
-}
-__device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
-    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    h8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (_Float16)x[i];
-    *reinterpret_cast<h8 *>(p) = a;
-}
 
 // Minimum, maximum and sum over the LANES (4, 8 or 16) lanes of a group.
 template <int LANES>
@@ -167,23 +146,8 @@ __global__ __launch_bounds__(kNT) void kv4_append_kernel(Kv4AppendParams p) {
     // the token's block of kv head 0; head h's is h pages of blocks further
     const long blk0 = r.b < 0 ? -1 : kv4_block(p.c, r.b, r.pos, r.seen, 0);
     double2 *cs = angles[w];
-    for (int i = lane; i < half; i += 64) {
-        const double f = p.c.turns[i], t = (double)r.pos * f;
-        const double frac = (t - rint(t)) + fma((double)r.pos, f, -t);
-        double sn, co;
-        sincospi(2.0 * frac, &sn, &co);
-        cs[i] = make_double2(co, sn);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
     double co[8], sn[8];                         // x_e <- x_e co + (its other) sn
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int i = p.c.interleaved ? (d0 + e) / 2 : low ? d0 + e : d0 - half + e;
-        const double2 a = turns ? cs[i] : make_double2(1.0, 0.0);
-        co[e] = a.x;
-        sn[e] = (p.c.interleaved ? e % 2 == 0 : low) ? -a.y : a.y;
-    }
+    token_angles(p.c.turns, half, p.c.interleaved, r.pos, d0, cs, co, sn);
     for (int row0 = part * RPW + lane / UPR; row0 - lane / UPR < rows; row0 += kAtOnce * step) {
         float x[kAtOnce][8], y[kAtOnce][8];
         // past the last row: row 0's values, not used

@@ -1,0 +1,653 @@
+// kve_decode.hip -- attention of one query token per sequence over the evicting KV cache
+// (layout: kve.h), with the softmax's weights added to each token's count.
+//
+//   s_t = (q . k_t) scale,   p_t = exp(s_t - max s) / sum,   out = sum_t p_t v_t,
+//   weight_t += the sum of p_t over the query heads of the kv head.
+//
+// Matrix products without a shuffle.  A workgroup takes the query heads of a kv head as the 16
+// columns of v_mfma_f32_16x16x32 (bf16, fp16) or 16x16x4 (fp32): the scores are K Q^T, the
+// output is V^T P^T, and both products give a lane the column (query head) lane % 16, so maxima,
+// sums and rescaling stay in the lane.  The order of the terms within a product is free as long
+// as both operands agree: row i of the score product's half u is token 8 (i / 4) + 4 u + i % 4
+// of a tile of 32, and so a lane of quarter c = lane / 16 ends with the scores of tokens 8 c ..
+// 8 c + 7, exactly the eight weights that the value product wants from it as its operand (fp32:
+// row i is token i, and the four scores of a lane are its operands of four products).  The other
+// operand, V^T, needs eight tokens of one dimension in a lane: a lane loads eight rows of eight
+// dimensions, whole rows by sixteen lanes, and turns the 8 x 8 values in registers with byte
+// permutations.  K, V and P never pass through LDS.
+//
+// Work: the tiles of all sequences are cut into chunks of equal size, as many as the card takes
+// workgroups, whatever the lengths are; a workgroup's four waves take turns at the tiles of
+// its chunk, join in LDS and leave (out, max, sums) to kve_join_kernel, which also turns the
+// scores kept by the first kernel (fp32, a thirtieth of the cache's bytes) into weights, once
+// the sums over whole sequences are known.
+//
+// Scores, maxima, sums and outputs are fp32.  Weights are rounded to bf16 or fp16 for the value
+// product (fp16: times 2^15, so that the smallest keep their share), and the sum that divides
+// the output is that of the rounded ones; the counted weights are divided by the exact sum.
+#include <cfloat>
+#include <cmath>
+
+#include "kve.h"
+
+namespace ojx {
+
+namespace {
+constexpr int kNT = 256;
+constexpr int kNW = kNT / 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMostGroup = 128;          // query heads of a kv head
+constexpr int kChunks = 2048;            // workgroups that a launch is cut into, at least
+constexpr int kLeastTiles = 4;           // tiles of a chunk, one for each wave
+
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef unsigned int u2_t __attribute__((ext_vector_type(2)));
+
+struct KveDecodeParams {
+    KveView c;
+    const void *q;              // [B][Hq][D]
+    void *out;
+    const int *held;
+    float *part_o;              // [item][Rb][D]
+    float *part_ml;             // [item][Rb][4]: max, sum, sum of the rounded weights
+    float *scores;              // [B][Hkv][R][tokens] times log2(e), or null: no weights
+    int Hq, R, HB, Rb;          // query heads, of a kv head, blocks of those, heads of a block
+    int most, stride;           // bound on a sequence's tokens; tokens of a row of scores
+    int chunks;                 // chunks that the launch and the partial results have room for
+    float scale;                // scale factor x log2(e)
+};
+
+// Sum of v over the workgroup, in order of the threads' numbers; sh: kNW + 1 ints.
+__device__ __forceinline__ int block_sum(int v, int *sh) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < kNW; ++i) s += sh[i];
+    return s;
+}
+
+// What workgroup blockIdx.x has: chunk j of k of sequence b, heads block hb of kv head h, and its
+// tokens [t0, t1) of n held ones.  b < 0: nothing.  Chunks are numbered by sequence, then by
+// place; the groups (kv head, heads block) of a chunk are neighbours.
+struct KveItem {
+    int b, h, hb, j, k, n, t0, t1;
+    long first;                 // number of the item of chunk 0 of this group; the next is `groups` on
+};
+template <int TT>
+__device__ __forceinline__ KveItem kve_item(const KveDecodeParams &p, int *sh) {
+    const int groups = p.c.Hkv * p.HB, B = p.c.B, tid = threadIdx.x;
+    const long ci = blockIdx.x / groups;
+    const int grp = blockIdx.x % groups;
+    auto tiles = [&](int b) { return (min(max(p.held[b], 0), p.most) + TT - 1) / TT; };
+    // tiles of a chunk; the sum of tiles stays within an int (the host's check)
+    int mine = 0;
+    for (int b = tid; b < B; b += kNT) mine += tiles(b);
+    const long total = block_sum(mine, sh);
+    const long size = max((long)kLeastTiles, (total * groups + kChunks - 1) / kChunks);
+    long before = 0;
+    KveItem it{-1, 0, 0, 0, 0, 0, 0, 0, 0};
+    for (int b0 = 0; b0 < B; b0 += kNT) {
+        const int b = b0 + tid, nt = b < B ? tiles(b) : 0;
+        const int k = b < B ? max(1, (int)((nt + size - 1) / size)) : 0;     // no tokens: a chunk of none
+        int incl = k;                                                        // scan over the workgroup
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(incl, o);
+            if ((tid & 63) >= o) incl += x;
+        }
+        __syncthreads();
+        if ((tid & 63) == 63) sh[tid >> 6] = incl;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int i = 0; i < kNW; ++i) {
+            if (i < tid >> 6) incl += sh[i];
+            all += sh[i];
+        }
+        const long j = ci - before - (incl - k);
+        if (j >= 0 && j < k) {                    // one thread at most
+            sh[kNW + 0] = b;
+            sh[kNW + 1] = (int)j;
+            sh[kNW + 2] = k;
+        }
+        if (ci >= before && ci < before + all) {  // the same for all threads
+            __syncthreads();
+            it.b = sh[kNW], it.j = sh[kNW + 1], it.k = sh[kNW + 2];
+            break;
+        }
+        before += all;
+    }
+    // lengths that another stream changes meanwhile may ask for more chunks than there is room for
+    it.k = min((long)it.k, p.chunks - (ci - it.j));
+    if (it.b < 0 || it.j >= it.k) {
+        it.b = -1;
+        return it;
+    }
+    it.h = grp / p.HB, it.hb = grp % p.HB;
+    it.first = (long)blockIdx.x - (long)it.j * groups;
+    it.n = min(max(p.held[it.b], 0), p.most);
+    const long nt = (it.n + TT - 1) / TT;
+    it.t0 = (int)(nt * it.j / it.k) * TT;
+    it.t1 = min(it.n, (int)(nt * (it.j + 1) / it.k) * TT);
+    return it;
+}
+constexpr int kItemInts = kNW + 3;
+
+__device__ __forceinline__ float swap32(float v, bool max_) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float x = __uint_as_float(a[0]), y = __uint_as_float(a[1]);
+    return max_ ? fmaxf(x, y) : x + y;
+}
+__device__ __forceinline__ float swap16(float v, bool max_) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float x = __uint_as_float(a[0]), y = __uint_as_float(a[1]);
+    return max_ ? fmaxf(x, y) : x + y;
+}
+// Over the four lanes of one column.
+__device__ __forceinline__ float column_max(float v) { return swap16(swap32(v, true), true); }
+__device__ __forceinline__ float column_sum(float v) { return swap16(swap32(v, false), false); }
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__hip_bfloat16> {
+    typedef b8_t V8;
+    static constexpr float kScale = 1.f;
+    static __device__ __forceinline__ f4_t mma(V8 a, V8 b, f4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ __bf16 from(float f) { return (__bf16)f; }
+};
+template <>
+struct Half<__half> {
+    typedef h8_t V8;
+    static constexpr float kScale = 32768.f;
+    static __device__ __forceinline__ f4_t mma(V8 a, V8 b, f4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ _Float16 from(float f) { return (_Float16)f; }
+};
+
+// One tile of TT tokens of a page (or of two pages) in registers.
+template <typename T, int D>
+struct Tile {                                   // bf16, fp16: 32 tokens
+    static constexpr int TT = 32, E = 8;        // tokens of a tile, and of a lane's scores
+    static constexpr int NK = D / 32, DL = D / 16 < 8 ? D / 16 : 8, NV = D / 16 / DL;
+    typedef typename Half<T>::V8 V8;
+    V8 k[2][NK];
+    unsigned v[E][NV][DL / 2];
+    // a lane's token within the tile whose row of K it loads for half u
+    static __device__ __forceinline__ int key(int i, int u) { return (i >> 2) * 8 + u * 4 + (i & 3); }
+    static __device__ __forceinline__ int key_block(int i) { return i >> 3; }       // of 16 slots
+    static __device__ __forceinline__ int value_block(int c) { return c >> 1; }
+    __device__ __forceinline__ void load_k(const T *rows, int i, int c) {           // row of slot 0 of key_block
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+                k[u][j] = *reinterpret_cast<const V8 *>(rows + (key(i, u) & 15) * D + j * 32 + c * 8);
+    }
+    __device__ __forceinline__ void load_v(const T *rows, int i, int c) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const T *src = rows + ((c & 1) * 8 + e) * D + n * 128 + i * DL;
+                if constexpr (DL == 8) {
+                    const u4_t x = *reinterpret_cast<const u4_t *>(src);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) v[e][n][w] = x[w];
+                } else {
+                    const u2_t x = *reinterpret_cast<const u2_t *>(src);
+                    v[e][n][0] = x[0], v[e][n][1] = x[1];
+                }
+            }
+    }
+    __device__ __forceinline__ void clear_value(int e) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int w = 0; w < DL / 2; ++w) v[e][n][w] = 0;
+    }
+    // scores of the lane's tokens with 16 columns of queries
+    __device__ __forceinline__ void scores(const V8 (&q)[NK], float (&s)[E]) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NK; ++j) a = Half<T>::mma(k[u][j], q[j], a);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[u * 4 + r] = a[r];
+        }
+    }
+    // eight tokens of one dimension: dimension d of the lane's in half n
+    __device__ __forceinline__ V8 column(int n, int d) const {
+        u4_t x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = __builtin_amdgcn_perm(v[2 * i + 1][n][d / 2], v[2 * i][n][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+        return __builtin_bit_cast(V8, x);
+    }
+    // o += V^T P^T; returns the sum of the weights as the product takes them
+    template <int NT>
+    __device__ __forceinline__ void values(const float (&p)[NT][E], f4_t (&o)[NT][D / 16], float (&sum)[NT]) const {
+        V8 w[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                w[t][e] = Half<T>::from(p[t][e] * Half<T>::kScale);
+                sum[t] += (float)w[t][e];
+            }
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int d = 0; d < DL; ++d) {
+                const V8 a = column(n, d);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[t][n * DL + d] = Half<T>::mma(a, w[t], o[t][n * DL + d]);
+            }
+    }
+    static __device__ __forceinline__ void load_q(const T *q, int c, V8 (&f)[NK]) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j) f[j] = *reinterpret_cast<const V8 *>(q + j * 32 + c * 8);
+    }
+    // dimension of row 4 c + r of the value product's block a
+    static __device__ __forceinline__ int dim(int a, int c, int r) { return a / DL * 128 + (c * 4 + r) * DL + a % DL; }
+};
+
+template <int D>
+struct Tile<float, D> {                         // 16 tokens
+    static constexpr int TT = 16, E = 4, NK = D / 16, NV = D / 64;
+    typedef f4_t V8;
+    f4_t k[NK], v[E][NV];
+    static __device__ __forceinline__ int key_block(int) { return 0; }
+    static __device__ __forceinline__ int value_block(int) { return 0; }
+    __device__ __forceinline__ void load_k(const float *rows, int i, int c) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j) k[j] = *reinterpret_cast<const f4_t *>(rows + i * D + j * 16 + c * 4);
+    }
+    __device__ __forceinline__ void load_v(const float *rows, int i, int c) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+                v[e][n] = *reinterpret_cast<const f4_t *>(rows + (c * 4 + e) * D + n * 64 + i * 4);
+    }
+    __device__ __forceinline__ void clear_value(int e) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) v[e][n] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void scores(const V8 (&q)[NK], float (&s)[E]) const {
+        // two sums at once: a product of this shape waits long for the one before
+        f4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int m = 0; m < 4; m += 2) {
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][m], q[j][m], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][m + 1], q[j][m + 1], b, 0, 0, 0);
+            }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = a[r] + b[r];
+    }
+    template <int NT>
+    __device__ __forceinline__ void values(const float (&p)[NT][E], f4_t (&o)[NT][D / 16], float (&sum)[NT]) const {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[t] += p[t][e];
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        o[t][n * 4 + m] =
+                            __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][n][m], p[t][e], o[t][n * 4 + m], 0, 0, 0);
+    }
+    static __device__ __forceinline__ void load_q(const float *q, int c, V8 (&f)[NK]) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j) f[j] = *reinterpret_cast<const f4_t *>(q + j * 16 + c * 4);
+    }
+    static __device__ __forceinline__ int dim(int a, int c, int r) { return a / 4 * 64 + (c * 4 + r) * 4 + a % 4; }
+};
+}  // namespace
+
+// NT: blocks of 16 query heads that share a pass over the chunk.
+template <typename T, int D, int NT>
+__global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
+#pragma clang fp contract(off)                   // s - m with both rounded alike: 0 for the largest score
+    typedef Tile<T, D> Tl;
+    constexpr int TT = Tl::TT, E = Tl::E, NA = D / 16;
+    __shared__ int ish[kItemInts];
+    __shared__ float ml[kNW][NT * 16][3];
+    __shared__ float buf[kNW / 2][NT * NA * 4][64];
+    const KveItem it = kve_item<TT>(p, ish);
+    if (it.b < 0) return;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, i = lane & 15, c = lane >> 4;
+    const int head0 = it.hb * p.Rb, heads = min(p.Rb, p.R - head0);     // of the kv head
+    typename Tl::V8 q[NT][Tl::NK] = {};
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+        if (t * 16 + i < heads)
+            Tl::load_q(static_cast<const T *>(p.q) + ((size_t)it.b * p.Hq + it.h * p.R + head0 + t * 16 + i) * D, c, q[t]);
+    f4_t o[NT][NA];
+    float m[NT], l[NT], lr[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY, l[t] = 0.f, lr[t] = 0.f;
+#pragma unroll
+        for (int a = 0; a < NA; ++a) o[t][a] = f4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    // block table entries of the lane's key and value rows, a tile ahead of their use
+    const int *bt = p.c.bt + (long)it.b * p.c.max_pages;
+    const int pmask = (1 << p.c.pshift) - 1, kb = Tl::key_block(i) * 16, vb = Tl::value_block(c) * 16;
+    auto entry = [&](int t) { return bt[min(t >> p.c.pshift, p.c.max_pages - 1)]; };
+    int t = it.t0 + wv * TT;
+    int kp = 0, vp = 0;
+    if (t < it.t1) kp = entry(t + kb), vp = entry(t + vb);
+    for (; t < it.t1; t += kNW * TT) {
+        const bool kin = kp >= 0 && kp < p.c.num_pages, vin = vp >= 0 && vp < p.c.num_pages;
+        auto row = [&](int page, bool in, int t) {
+            return ((((long)(in ? page : 0) * p.c.Hkv) + it.h) << p.c.pshift) + (t & pmask);
+        };
+        Tl tl;
+        tl.load_k(reinterpret_cast<const T *>(p.c.k) + row(kp, kin, t + kb) * D, i, c);
+        tl.load_v(reinterpret_cast<const T *>(p.c.v) + row(vp, vin, t + vb) * D, i, c);
+        const int left = it.n - t - c * E;        // tokens from the lane's first one on
+        const int next = t + kNW * TT;
+        if (next < it.t1) kp = entry(next + kb), vp = entry(next + vb);
+        const bool whole = __all(vin && left >= E);
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (!vin || e >= left) tl.clear_value(e);
+        }
+        float w[NT][E];
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            float s[E], most = -FLT_MAX;          // not -inf: some token is there, if all score that
+            tl.scores(q[b], s);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[e] *= p.scale;
+            if (p.scores && b * 16 + i < heads) {
+                float *to = p.scores + (((long)it.b * p.c.Hkv + it.h) * p.R + head0 + b * 16 + i) * p.stride + t + c * E;
+#pragma unroll
+                for (int e = 0; e < E; e += 4) *reinterpret_cast<f4_t *>(to + e) = f4_t{s[e], s[e + 1], s[e + 2], s[e + 3]};
+            }
+            if (whole) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) most = fmaxf(most, s[e]);
+            } else {
+                if (!vin || left <= 0) most = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    if (!vin || e >= left) s[e] = -INFINITY;
+                    most = fmaxf(most, s[e]);
+                }
+            }
+            if (__any(most > m[b])) {
+                most = fmaxf(m[b], column_max(most));
+                const float f = most == -INFINITY ? 1.f : exp2f(m[b] - most);
+                m[b] = most;
+                l[b] *= f, lr[b] *= f;
+#pragma unroll
+                for (int a = 0; a < NA; ++a) o[b][a] *= f;
+            }
+            const float base = m[b] == -INFINITY ? 0.f : m[b];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                w[b][e] = __builtin_amdgcn_exp2f(s[e] - base);
+                l[b] += w[b][e];
+            }
+        }
+        tl.template values<NT>(w, o, lr);
+    }
+    // the four waves' (max, sums, out) joined: 2 into 0 and 3 into 1, then 1 into 0
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        l[b] = column_sum(l[b]), lr[b] = column_sum(lr[b]);
+        if (c == 0) ml[wv][b * 16 + i][0] = m[b], ml[wv][b * 16 + i][1] = l[b], ml[wv][b * 16 + i][2] = lr[b];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        float most = ml[0][b * 16 + i][0];
+#pragma unroll
+        for (int x = 1; x < kNW; ++x) most = fmaxf(most, ml[x][b * 16 + i][0]);
+        const float f = m[b] == -INFINITY ? 0.f : exp2f(m[b] - most);
+        l[b] = lr[b] = 0.f;
+#pragma unroll
+        for (int x = 0; x < kNW; ++x) {
+            const float mx = ml[x][b * 16 + i][0], g = mx == -INFINITY ? 0.f : exp2f(mx - most);
+            l[b] += ml[x][b * 16 + i][1] * g;
+            lr[b] += ml[x][b * 16 + i][2] * g;
+        }
+        if (f != 1.f) {                           // a wave without tokens has sums of 0, and no infinity to turn into NaN
+#pragma unroll
+            for (int a = 0; a < NA; ++a) o[b][a] *= f;
+        }
+        m[b] = most;
+    }
+    auto give = [&](float (*to)[64]) {
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[(b * NA + a) * 4 + r][lane] = o[b][a][r];
+    };
+    auto take = [&](float (*of)[64]) {
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[b][a][r] += of[(b * NA + a) * 4 + r][lane];
+    };
+    if (wv >= 2) give(buf[wv - 2]);
+    __syncthreads();
+    if (wv < 2) take(buf[wv]);
+    __syncthreads();
+    if (wv == 1) give(buf[0]);
+    __syncthreads();
+    if (wv) return;
+    take(buf[0]);
+    const long item = blockIdx.x;
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        const int head = b * 16 + i;
+        if (head >= heads) continue;
+        float *to = p.part_o + (item * p.Rb + head) * D;
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) to[Tl::dim(a, c, r)] = o[b][a][r];
+        if (c == 0) *reinterpret_cast<f4_t *>(p.part_ml + (item * p.Rb + head) * 4) = f4_t{m[b], l[b], lr[b], 0.f};
+    }
+}
+
+// The chunks of a sequence joined, and its weights: workgroup = item, as in the first kernel.
+// Its share of the output is every k-th part of the group's, summed over all chunks; its share
+// of the weights the tokens of its own chunk, over all query heads of the kv head (the first
+// heads block's item does it).
+template <typename T, int D, int TT>
+__global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
+    __shared__ int ish[kItemInts];
+    __shared__ float most[kMostGroup], inv[kMostGroup], rounded[kMostGroup];
+    const KveItem it = kve_item<TT>(p, ish);
+    if (it.b < 0) return;
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, groups = p.c.Hkv * p.HB;
+    const bool counts = p.scores && it.hb == 0;
+    // maxima and sums of the heads that this item needs: its own block's, or all of the kv head
+    const int h0 = counts ? 0 : it.hb * p.Rb, h1 = counts ? p.R : min(p.R, h0 + p.Rb);
+    for (int r = h0 + wv; r < h1; r += kNW) {
+        const long first = it.first + r / p.Rb - it.hb;
+        const float *of = p.part_ml + (first * p.Rb + r % p.Rb) * 4;
+        const long step = (long)groups * p.Rb * 4;
+        float m = -INFINITY, l = 0.f, lr = 0.f;
+        for (int j = lane; j < it.k; j += 64) m = fmaxf(m, of[j * step]);
+        m = wave_max_f(m);
+        for (int j = lane; j < it.k; j += 64) {
+            const f4_t x = *reinterpret_cast<const f4_t *>(of + j * step);
+            const float f = x[0] == -INFINITY ? 0.f : exp2f(x[0] - m);
+            l += x[1] * f;
+            lr += x[2] * f;
+        }
+        l = wave_sum_f(l), lr = wave_sum_f(lr);
+        if (lane == 0) most[r] = m, inv[r] = 1.f / l, rounded[r] = lr;
+    }
+    __syncthreads();
+    // outputs: units of four values, each summed by `lanes` lanes
+    const int heads = min(p.Rb, p.R - it.hb * p.Rb), units = heads * (D / 4);
+    int lanes = 1;
+    while (lanes < 64 && lanes < it.k) lanes *= 2;
+    const int u0 = (int)((long)units * it.j / it.k), u1 = (int)((long)units * (it.j + 1) / it.k);
+    const int sub = threadIdx.x % lanes;
+    for (int u = u0; u < u1; u += kNT / lanes) {           // whole waves stay in it: the sum below is theirs
+        const int mine = u + threadIdx.x / lanes, at = min(mine, u1 - 1), head = at / (D / 4), r = it.hb * p.Rb + head;
+        const float m = most[r];
+        f4_t sum = {0.f, 0.f, 0.f, 0.f};
+        for (int j = sub; j < it.k; j += lanes) {
+            const long row = (it.first + (long)j * groups) * p.Rb + head;
+            const float mj = p.part_ml[row * 4];
+            if (mj == -INFINITY) continue;
+            sum += *reinterpret_cast<const f4_t *>(p.part_o + row * D + at % (D / 4) * 4) * exp2f(mj - m);
+        }
+        for (int o = 1; o < lanes; o *= 2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], o);
+        if (sub == 0 && mine < u1) {
+            // no tokens: 0; tokens that all score -inf: 0 / 0
+            T *to = static_cast<T *>(p.out) + ((size_t)it.b * p.Hq + it.h * p.R + r) * D + at % (D / 4) * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_act(to, e, m == -INFINITY ? 0.f : sum[e] / rounded[r]);
+        }
+    }
+    if (!counts) return;
+    const float *s = p.scores + (((long)it.b * p.c.Hkv + it.h) * p.R) * p.stride;
+    for (int t = it.t0 + threadIdx.x; t < it.t1; t += kNT) {
+        const long row = kve_row(p.c, it.b, t);
+        if (row < 0) continue;
+        float sum = 0.f;
+        for (int r = 0; r < p.R; ++r) sum += exp2f(s[(long)r * p.stride + t] - most[r]) * inv[r];
+        p.c.w[row + ((long)it.h << p.c.pshift)] += sum;
+    }
+}
+
+namespace {
+struct KvePlan {
+    int R, NT, HB, Rb, TT, most, stride;
+    long chunks, items, o_bytes, ml_bytes, s_bytes;
+};
+int kve_plan(const OjasxKVECache *c, const KveView &v, int num_q_heads, int max_held, int count, KvePlan *p) {
+    if (num_q_heads <= 0 || num_q_heads % v.Hkv || max_held < 0) {
+        set_error("KV decode: %d query heads for %d kv heads, max_held %d", num_q_heads, v.Hkv, max_held);
+        return OJASX_ERR_INVALID;
+    }
+    p->R = num_q_heads / v.Hkv;
+    if (p->R > kMostGroup) {
+        set_error("KV decode: %d query heads of a kv head (at most %d)", p->R, kMostGroup);
+        return OJASX_ERR_INVALID;
+    }
+    p->TT = v.dtype == OJASX_DTYPE_F32 ? 16 : 32;
+    p->NT = p->R > 16 && !(v.dtype == OJASX_DTYPE_F32 && v.D == 256) ? 2 : 1;   // two would spill there
+    p->HB = (p->R + p->NT * 16 - 1) / (p->NT * 16);
+    p->Rb = (p->R + p->HB - 1) / p->HB;
+    p->most = max_held && max_held < v.cap ? max_held : v.cap;
+    const long groups = (long)v.Hkv * p->HB, tiles = ((long)p->most + p->TT - 1) / p->TT;
+    p->stride = (int)(tiles * p->TT);
+    // the chunks of a kv head: of size tiles * groups / kChunks (all sequences' tiles), one more for each
+    // sequence, and none smaller than kLeastTiles
+    const long a = kChunks / groups + v.B, b = v.B * ((tiles + kLeastTiles - 1) / kLeastTiles);
+    p->chunks = a < b ? a : b;
+    p->items = p->chunks * groups;
+    if (p->items > 0xffffff || tiles * v.B > 0x7fffffffL) {
+        set_error("KV decode: %d sequences of up to %d tokens with %d kv heads are more than a launch takes", v.B,
+                  p->most, v.Hkv);
+        return OJASX_ERR_INVALID;
+    }
+    p->o_bytes = p->items * p->Rb * v.D * 4;
+    p->ml_bytes = p->items * p->Rb * 16;
+    p->s_bytes = count ? (long)v.B * num_q_heads * p->stride * 4 : 0;
+    return OJASX_OK;
+}
+
+template <typename T, int D>
+void decode(const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
+    const dim3 grid((unsigned)pl.items), block(kNT);
+    constexpr int kNT2 = sizeof(T) == 4 && D == 256 ? 1 : 2;
+    if (pl.NT == 1) OJX_LAUNCH((kve_decode_kernel<T, D, 1>), grid, block, 0, st, p);
+    else OJX_LAUNCH((kve_decode_kernel<T, D, kNT2>), grid, block, 0, st, p);
+    OJX_LAUNCH((kve_join_kernel<T, D, Tile<T, D>::TT>), grid, block, 0, st, p);
+}
+template <typename T>
+void decode(int D, const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
+    if (D == 64) decode<T, 64>(pl, st, p);
+    else if (D == 128) decode<T, 128>(pl, st, p);
+    else decode<T, 256>(pl, st, p);
+}
+}  // namespace
+
+}  // namespace ojx
+
+extern "C" {
+
+OJASX_API long ojasx_kve_decode_workspace(const OjasxKVECache *cache, int num_q_heads, int max_held, int count) {
+    using namespace ojx;
+    KveView v{};
+    KvePlan pl{};
+    int rc = kve_view(cache, &v);
+    if (!rc) rc = kve_plan(cache, v, num_q_heads, max_held, count, &pl);
+    return rc ? rc : pl.o_bytes + pl.ml_bytes + pl.s_bytes;
+}
+
+OJASX_API int ojasx_kve_decode_device(const OjasxKVECache *cache, const void *q, int num_q_heads, const int *held,
+                                      int max_held, float scale_factor, int count, void *out, void *workspace,
+                                      long workspace_bytes, void *stream) {
+    using namespace ojx;
+    KveDecodeParams p{};
+    KvePlan pl{};
+    int rc = kve_view(cache, &p.c);
+    if (!rc) rc = kve_plan(cache, p.c, num_q_heads, max_held, count, &pl);
+    if (rc) return rc;
+    if (!q || !held || !out) return OJASX_ERR_NULL;
+    p.scale = (scale_factor > 0.f || scale_factor != scale_factor ? scale_factor : 1.f / sqrtf((float)p.c.D)) * kLog2e;
+    if (!(p.scale > 0.f) || p.scale > FLT_MAX) {
+        set_error("KV decode: scale factor %g times log2(e) is not finite", (double)scale_factor);
+        return OJASX_ERR_INVALID;
+    }
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) {
+        set_error("KV decode: queries and outputs are 16-byte aligned");
+        return OJASX_ERR_INVALID;
+    }
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < pl.o_bytes + pl.ml_bytes + pl.s_bytes) {
+        set_error("KV decode: the workspace has to be 16-byte aligned and of %ld bytes, got %ld",
+                  pl.o_bytes + pl.ml_bytes + pl.s_bytes, workspace_bytes);
+        return OJASX_ERR_INVALID;
+    }
+    char *ws = static_cast<char *>(workspace);
+    p.part_o = reinterpret_cast<float *>(ws);
+    p.part_ml = reinterpret_cast<float *>(ws + pl.o_bytes);
+    p.scores = count ? reinterpret_cast<float *>(ws + pl.o_bytes + pl.ml_bytes) : nullptr;
+    p.q = q, p.out = out, p.held = held;
+    p.Hq = num_q_heads, p.R = pl.R, p.HB = pl.HB, p.Rb = pl.Rb, p.most = pl.most, p.stride = pl.stride,
+    p.chunks = (int)pl.chunks;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (p.c.dtype == OJASX_DTYPE_F32) decode<float>(p.c.D, pl, st, p);
+    else if (p.c.dtype == OJASX_DTYPE_BF16) decode<__hip_bfloat16>(p.c.D, pl, st, p);
+    else decode<__half>(p.c.D, pl, st, p);
+    OJX_HIP(hipGetLastError());
+    return OJASX_OK;
+}
+
+}  // extern "C"

@@ -38,6 +38,85 @@ def _dev_f32(a, device):
     return t.to(device).contiguous()
 
 
+def _setting(value, rows, dtype, index, name):
+    """(value for all rows, address of a value for each row or None) of a sampling setting."""
+    torch = _torch()
+    if not torch.is_tensor(value):
+        return value, None
+    if value.dtype != dtype or tuple(value.shape) != (rows,) or not value.is_contiguous() or \
+            value.get_device() != index:
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor of {rows} entries on "
+                         f"cuda:{index}, got {value.dtype} {tuple(value.shape)} on {value.device}")
+    return 0, value.data_ptr()
+
+
+def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """One token of every row of ``logits`` [rows, vocab] (float32, bfloat16 or
+    float16, any strides; vocab at most 2^22), drawn with the random number
+    ``uniform[row]`` (float32 [rows], in [0, 1)): int32 [rows], in ``out`` where
+    given.
+
+    With e_i = exp((l_i - max l) / temperature) and the tokens in order of
+    falling logits, equal ones of rising index: ``top_k > 0`` keeps the first
+    top_k, ``top_p < 1`` of those the shortest beginning that has at least top_p
+    of their sum of e, ``min_p > 0`` of those the ones with e_i >= min_p.  The
+    token is the first kept one, in the vocabulary's order, at which the running
+    sum of e passes uniform times the kept sum.  ``temperature=0``: the largest
+    logit, of equal ones the first.  Each setting is a number, or a tensor of
+    one for each row (float32, top_k int32) on the logits' device; entries out
+    of range count as the nearest one in it.  A row without a distribution (a
+    NaN or +inf among its logits, -inf alone, or a temperature that is negative,
+    NaN or infinite) gives -1.
+
+    e and sums are fp64, so the token is the definition's own unless uniform lies
+    within about 1e-11 of a border; one whose e is below 2^-51 is not drawn.
+    The result does not depend on the other rows."""
+    torch = _torch()
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    if not logits.is_cuda:
+        raise RuntimeError(f"sample_tokens runs on the GPU only (got a {logits.device} tensor)")
+    tag = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
+           torch.float16: _lib.DTYPE_F16}.get(logits.dtype)
+    if tag is None:
+        raise TypeError(f"unsupported dtype {logits.dtype}: float32, bfloat16 or float16")
+    rows, vocab = logits.shape
+    index = logits.get_device()
+    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (rows,) or not uniform.is_contiguous() or \
+            uniform.get_device() != index:
+        raise ValueError(f"uniform must be a contiguous float32 tensor of {rows} entries on cuda:{index}, got "
+                         f"{uniform.dtype} {tuple(uniform.shape)} on {uniform.device}")
+    s = _lib.Sampling()
+    s.temperature, s.temperatures = _setting(temperature, rows, torch.float32, index, "temperature")
+    s.top_p, s.top_ps = _setting(top_p, rows, torch.float32, index, "top_p")
+    s.min_p, s.min_ps = _setting(min_p, rows, torch.float32, index, "min_p")
+    top_k, s.top_ks = _setting(top_k, rows, torch.int32, index, "top_k")
+    s.top_k = min(max(int(top_k), 0), 0x7fffffff)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    elif out.dtype != torch.int32 or tuple(out.shape) != (rows,) or not out.is_contiguous() or \
+            out.get_device() != index:
+        raise ValueError(f"out must be a contiguous int32 tensor of {rows} entries on cuda:{index}")
+    if vocab > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    need = _lib.lib().ojasx_sample_workspace(min(rows, 0x7fffffff), min(vocab, 0x7fffffff))
+    if need < 0:
+        raise ValueError(_lib.lib().ojasx_get_last_error().decode(errors="replace"))
+    ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    call = lambda: _lib.lib().ojasx_sample_device(  # noqa: E731
+        logits.data_ptr(), tag, rows, vocab, logits.stride(0), uniform.data_ptr(), ctypes.addressof(s),
+        out.data_ptr(), ws.data_ptr(), need, _lib.raw_stream(index))
+    if torch.cuda.current_device() == index:
+        rc = call()
+    else:
+        with torch.cuda.device(index):
+            rc = call()
+    if rc == -3:
+        raise ValueError(_lib.lib().ojasx_get_last_error().decode(errors="replace"))
+    _lib.check(rc, "ojasx_sample_device")
+    return out
+
+
 @dataclass
 class DecoderConfig:
     hidden: int = 2560

@@ -29,7 +29,10 @@ csrc/lut_kv.hip.
   several sequences in 4 bits, with the position rotation applied on the way
   in (csrc/kv4_append.hip, csrc/kv4_decode.hip).  The sequences' lengths are
   the caller's, in device memory, so its calls can be captured.
-* ``PackedPromptAttention`` is the prefill beside it: attention of a batch of
+* ``PagedEvictingKVCache`` holds keys and values of a serving batch in their own
+  type, counts the attention that each token gets and drops those that get
+  least (csrc/kve_append.hip, csrc/kve_decode.hip, csrc/kve_evict.hip).
+* ``PackedPromptAttention`` is the prefill beside them: attention of a batch of
   prompts of different lengths, packed row by row, causal, grouped heads
   (csrc/prompt_attn.hip).
 
@@ -733,6 +736,31 @@ def _launch(index, what, *args):
         _lib.check(rc, what)
 
 
+def _rotation(head_dim, rotary_dim, rope_theta, inv_freq):
+    """(rotary_dim, the frequencies in turns per position or None) of a cache's arguments."""
+    torch = _torch()
+    if inv_freq is None and rope_theta is None:
+        if rotary_dim:
+            raise ValueError("rotary_dim without rope_theta or inv_freq")
+        rotary_dim = 0
+    elif rotary_dim is None:
+        rotary_dim = head_dim
+    if rotary_dim < 0 or rotary_dim > head_dim or rotary_dim % 16:
+        raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim, got {rotary_dim}")
+    if not rotary_dim:
+        return 0, None
+    if inv_freq is None:
+        if not 0.0 < float(rope_theta) < math.inf:
+            raise ValueError(f"rope_theta must be positive and finite, got {rope_theta}")
+        inv_freq = float(rope_theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+                                         / rotary_dim)
+    inv_freq = torch.as_tensor(inv_freq).detach().to(device="cpu", dtype=torch.float64)
+    if tuple(inv_freq.shape) != (rotary_dim // 2,) or not torch.isfinite(inv_freq).all():
+        raise ValueError(f"inv_freq must hold {rotary_dim // 2} finite values, got "
+                         f"{tuple(inv_freq.shape)}")
+    return rotary_dim, inv_freq / (2.0 * math.pi)
+
+
 class PagedInt4KVCache:
     """Paged KV cache of one attention layer for ``num_sequences`` sequences, in
     4 bits, on the GPU.
@@ -781,26 +809,7 @@ class PagedInt4KVCache:
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise RuntimeError("PagedInt4KVCache runs on the GPU only")
-        if inv_freq is None and rope_theta is None:
-            if rotary_dim:
-                raise ValueError("rotary_dim without rope_theta or inv_freq")
-            rotary_dim = 0
-        elif rotary_dim is None:
-            rotary_dim = head_dim
-        if rotary_dim < 0 or rotary_dim > head_dim or rotary_dim % 16:
-            raise ValueError(f"rotary_dim must be a multiple of 16 up to head_dim, got {rotary_dim}")
-        turns = None
-        if rotary_dim:
-            if inv_freq is None:
-                if not 0.0 < float(rope_theta) < math.inf:
-                    raise ValueError(f"rope_theta must be positive and finite, got {rope_theta}")
-                inv_freq = float(rope_theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64)
-                                                 / rotary_dim)
-            inv_freq = torch.as_tensor(inv_freq).detach().to(device="cpu", dtype=torch.float64)
-            if tuple(inv_freq.shape) != (rotary_dim // 2,) or not torch.isfinite(inv_freq).all():
-                raise ValueError(f"inv_freq must hold {rotary_dim // 2} finite values, got "
-                                 f"{tuple(inv_freq.shape)}")
-            turns = inv_freq / (2.0 * math.pi)
+        rotary_dim, turns = _rotation(head_dim, rotary_dim, rope_theta, inv_freq)
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         dev = self.device
@@ -978,6 +987,239 @@ class PagedInt4KVCache:
         _launch(self._index, "ojasx_kv4_decode_device", self._ref, q.data_ptr(), heads, tag, sp, max_seen,
                 scale_factor, out.data_ptr(), ws.data_ptr(), need)
         return out
+
+
+class PagedEvictingKVCache:
+    """Paged KV cache of one attention layer for ``num_sequences`` sequences, on
+    the GPU, that counts the attention its tokens get and can drop those that
+    get least: long generations in bounded memory, with the tokens kept that
+    the model looks at, where the other caches keep the first and newest pages.
+
+    Token slot t of a sequence lies in slot t % page_size (a power of two from
+    16) of page ``block_table[sequence, t // page_size]`` (int32 [num_sequences,
+    max_pages]): by default every sequence has pages of its own.  With
+    ``num_pages`` given, the pool has that many pages and the table starts as
+    -1, no page; the caller fills it in.  ``keys`` and ``values`` [num_pages,
+    num_kv_heads, page_size, head_dim] hold ``dtype`` (float32, bfloat16 or
+    float16), ``weights`` (float32) and ``positions`` (int32) [num_pages,
+    num_kv_heads, page_size] a token's attention so far and where it stands.
+    The caller may fill these tensors in, too.
+
+    Keys, and queries given to ``append``, are rotated by their positions as
+    PagedInt4KVCache does it (rope_theta, inv_freq, rotary_dim, interleaved);
+    ``rope_theta=None`` without ``inv_freq``: no rotation.
+
+    The sequences' lengths are the caller's: int32 tensors on the cache's
+    device, one for all layers, that a captured graph advances itself.  Calls on
+    one cache write its pages: order them on one stream.  Sequences may share
+    pages only where nothing writes them: no append, no eviction, and decode
+    with ``count=False``."""
+
+    def __init__(self, num_kv_heads: int, head_dim: int = 128, *, num_sequences: int = 1,
+                 page_size: int = 16, max_pages: int = 512, rope_theta: Optional[float] = 1e6,
+                 inv_freq=None, rotary_dim: Optional[int] = None, interleaved: bool = False,
+                 num_pages: Optional[int] = None, dtype=None, device="cuda") -> None:
+        torch = _torch()
+        dtype = torch.bfloat16 if dtype is None else dtype
+        tag = _attn_tag(dtype)
+        if tag is None or tag == _lib.DTYPE_F64:
+            raise TypeError(f"unsupported dtype {dtype}: float32, bfloat16 or float16")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+        if not 16 <= page_size <= 32768 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 32768, got {page_size}")
+        if num_kv_heads <= 0 or num_sequences <= 0 or max_pages <= 0 or \
+                (num_pages is not None and num_pages <= 0):
+            raise ValueError("Invalid page configuration for PagedEvictingKVCache")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError("PagedEvictingKVCache runs on the GPU only")
+        rotary_dim, turns = _rotation(head_dim, rotary_dim, rope_theta, inv_freq)
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        dev = self.device
+        self._index = dev.index
+        if turns is not None:
+            turns = turns.to(dev)
+        self.num_kv_heads, self.head_dim, self.dtype = num_kv_heads, head_dim, dtype
+        self.num_sequences, self.page_size, self.max_pages = num_sequences, page_size, max_pages
+        self.rotary_dim, self.interleaved = rotary_dim, bool(interleaved)
+        self.num_pages = num_sequences * max_pages if num_pages is None else num_pages
+        slots = (self.num_pages, num_kv_heads, page_size)
+        self._keys = torch.zeros(*slots, head_dim, dtype=dtype, device=dev)
+        self._values = torch.zeros_like(self._keys)
+        self._weights = torch.zeros(slots, dtype=torch.float32, device=dev)
+        self._positions = torch.zeros(slots, dtype=torch.int32, device=dev)
+        if num_pages is None:
+            table = torch.arange(self.num_pages, dtype=torch.int32, device=dev)
+        else:
+            table = torch.full((num_sequences * max_pages,), -1, dtype=torch.int32, device=dev)
+        self._block_table = table.view(num_sequences, max_pages)
+        self._turns = turns
+        self._c = _lib.KVECache(_vp(self._keys), _vp(self._values), _vp(self._weights),
+                                _vp(self._positions), _vp(table),
+                                _vp(turns) if turns is not None else None, num_sequences, max_pages,
+                                page_size, self.num_pages, num_kv_heads, head_dim, tag, rotary_dim,
+                                int(self.interleaved))
+        self._ref = ctypes.addressof(self._c)
+        self._workspace_bytes = {}       # arguments of a workspace's size -> bytes
+
+    # The kernels hold these tensors by address: they are filled in, never replaced.
+    keys = property(lambda self: self._keys, doc="Keys, rotated.")
+    values = property(lambda self: self._values, doc="Values.")
+    weights = property(lambda self: self._weights, doc="The softmax weights that each token got, summed.")
+    positions = property(lambda self: self._positions, doc="The tokens' positions.")
+    block_table = property(lambda self: self._block_table, doc="The pages of each sequence.")
+
+    @property
+    def capacity(self) -> int:
+        """Tokens of one sequence that its pages hold at most."""
+        return self.max_pages * self.page_size
+
+    @property
+    def storage_bytes(self) -> int:
+        """Bytes of the pool: keys, values, weights, positions and block table."""
+        return sum(t.numel() * t.element_size() for t in
+                   (self._keys, self._values, self._weights, self._positions, self._block_table))
+
+    def _check(self, what, *tensors):
+        """The cache's dtype and device, and no gradient."""
+        tag, index = _inference_tag(what, *tensors)
+        if index != self._index or tag != self._c.dtype:
+            raise ValueError(f"{what}: tensors of {tensors[0].dtype} on {tensors[0].device}, the cache of "
+                             f"{self.dtype} on {self.device}")
+
+    def _check_rows(self, t, n, heads, name):
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != n or shape[2] != self.head_dim or \
+                (heads is not None and shape[1] != heads):
+            raise ValueError(f"{name} must be [{n}, {heads or 'heads'}, {self.head_dim}], got "
+                             f"{tuple(shape)}")
+
+    def _workspace(self, name, *args):
+        """An uninitialised workspace of the size that the entry point ``name`` gives, and its bytes."""
+        key = (name, *args)
+        need = self._workspace_bytes.get(key)
+        if need is None:
+            need = getattr(_lib.lib(), name)(self._ref, *args)
+            if need < 0:
+                _lib.check(need, name)
+            if len(self._workspace_bytes) > 64:
+                self._workspace_bytes.clear()
+            self._workspace_bytes[key] = need
+        return _torch().empty(need, dtype=_torch().uint8, device=self.device), need
+
+    def append(self, key, value, start, cu_seqlens=None, *, position=None, query=None, weight=None):
+        """Rotate ``key`` and write it with ``value`` [N, num_kv_heads, head_dim]
+        (the cache's dtype, any strides): rows cu_seqlens[b] .. cu_seqlens[b +
+        1] - 1 go to sequence b's slots start[b], start[b] + 1, ...; without
+        ``cu_seqlens`` row b is sequence b's one token.  They stand at positions
+        position[b], position[b] + 1, ... (int32 [num_sequences]; ``start``
+        unless given, right as long as nothing has been evicted).  ``start`` and
+        ``position`` are read, not advanced.  ``weight`` (float32 [N,
+        num_kv_heads]) is the attention that the tokens got already, 0 unless
+        given.  Slots past the sequence's pages are not written.
+
+        Returns the query [N, heads, head_dim] rotated by the same positions, in
+        its dtype (zeros in rows that belong to no sequence), or None."""
+        what = "PagedEvictingKVCache.append"
+        if query is None:
+            self._check(what, key, value)
+        else:
+            self._check(what, key, value, query)
+        n, B = key.shape[0] if key.dim() else 0, self.num_sequences
+        if n > _MOST_INT:
+            raise ValueError(f"{what}: {n} tokens")
+        self._check_rows(key, n, self.num_kv_heads, "key")
+        self._check_rows(value, n, self.num_kv_heads, "value")
+        at = _lengths_tensor(start, B, self._index, "start")
+        pa = None if position is None else _lengths_tensor(position, B, self._index, "position")
+        cu = None
+        if cu_seqlens is not None:
+            cu = _lengths_tensor(cu_seqlens, B + 1, self._index, "cu_seqlens")
+        elif n != B:
+            raise ValueError(f"{n} tokens: without cu_seqlens each of the {B} sequences gets one")
+        wa = None
+        if weight is not None:
+            if weight.dtype != _torch().float32 or tuple(weight.shape) != (n, self.num_kv_heads) or \
+                    weight.get_device() != self._index or not weight.is_contiguous():
+                raise ValueError(f"weight must be contiguous float32 [{n}, {self.num_kv_heads}] on "
+                                 f"{self.device}, got {weight.dtype} {tuple(weight.shape)} on {weight.device}")
+            wa = weight.data_ptr()
+        es = 4 if self._c.dtype == _lib.DTYPE_F32 else 2
+        k, ka, kt, kh = _aligned_rows(key, es)
+        v, va, vt, vh = _aligned_rows(value, es)
+        qo = qa = qp = None
+        heads = qt = qh = 0
+        if query is not None:
+            self._check_rows(query, n, None, "query")
+            heads = query.shape[1]
+            q, qa, qt, qh = _aligned_rows(query, es)
+            qo = _new_like(q)
+            qp = qo.data_ptr()
+        _launch(self._index, "ojasx_kve_append_device", self._ref, qa, qt, qh, heads, qp, ka, kt, kh, va, vt,
+                vh, wa, n, at, pa, cu)
+        return qo
+
+    def decode(self, query, held, scale_factor: float = -1.0, *, max_held: int = 0, count: bool = True,
+               out=None):
+        """Attention of one query token per sequence, ``query``
+        [num_sequences, num_q_heads, head_dim] (rotated; the cache's dtype),
+        over the first ``held[b]`` slots (int32 [num_sequences], the current
+        token included) of each sequence; q head j reads kv head j //
+        (num_q_heads // num_kv_heads), at most 128 of them one kv head.
+        ``scale_factor <= 0`` means 1/sqrt(head_dim); a sequence without tokens
+        gives 0, one whose tokens all score -inf NaN.  With ``count`` each
+        token's softmax weights, summed over the query heads of its kv head, are
+        added to its entry of ``weights``.  Scores, sums and counted weights are
+        float32; for bfloat16 and float16 the softmax's weights are rounded to
+        that type for the product with the values.  ``out`` may be the query
+        itself.  ``max_held``, a bound on ``held`` where the caller knows one,
+        keeps launch and workspace as small as the sequences are; of a longer
+        one the first ``max_held`` tokens are attended."""
+        self._check("PagedEvictingKVCache.decode", query)
+        self._check_rows(query, self.num_sequences, None, "query")
+        heads = query.shape[1]
+        if heads == 0 or heads % self.num_kv_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {self.num_kv_heads} kv heads")
+        if not 0 <= max_held <= _MOST_INT:
+            raise ValueError(f"max_held must not be negative, got {max_held}")
+        hp = _lengths_tensor(held, self.num_sequences, self._index, "held")
+        count = 1 if count else 0
+        ws, need = self._workspace("ojasx_kve_decode_workspace", heads, max_held, count)
+        if out is None:
+            out = _new_like(query)
+        elif out.shape != query.shape or out.dtype != query.dtype or out.device != query.device or \
+                not out.is_contiguous() or out.data_ptr() & 15:
+            raise ValueError("out must be contiguous, 16-byte aligned and of the query's shape, dtype and "
+                             "device")
+        q = query if query.is_contiguous() else query.contiguous()
+        if q.data_ptr() & 15:
+            q = q.clone()
+        _launch(self._index, "ojasx_kve_decode_device", self._ref, q.data_ptr(), heads, hp, max_held,
+                scale_factor, count, out.data_ptr(), ws.data_ptr(), need)
+        return out
+
+    def evict(self, held, budget: int, *, sink_tokens: int = 4, recent_tokens: int = 0,
+              max_held: int = 0) -> None:
+        """Of each sequence and kv head that holds more than ``budget`` tokens
+        (``held``, int32 [num_sequences]), keep ``budget``: those at positions
+        below ``sink_tokens``, those of the ``recent_tokens`` newest positions,
+        and of the others the ones of largest weight, ties to the lowest slot
+        (NaN last).  A kept token from behind the budget takes the place of a
+        dropped one before it, the i-th of them the i-th place, with its weight
+        and position; nothing else is written.  The caller then holds
+        min(held, budget) tokens; ``held`` is read, not changed, so that the
+        layers of a model can share it.  ``max_held`` as in ``decode``."""
+        budget, sink_tokens, recent_tokens = int(budget), int(sink_tokens), int(recent_tokens)
+        if min(sink_tokens, recent_tokens, max_held) < 0 or max(budget, max_held) > _MOST_INT or \
+                not 0 < budget >= sink_tokens + recent_tokens:
+            raise ValueError(f"budget {budget} for {sink_tokens} sink and {recent_tokens} recent tokens, "
+                             f"max_held {max_held}")
+        hp = _lengths_tensor(held, self.num_sequences, self._index, "held")
+        ws, need = self._workspace("ojasx_kve_evict_workspace", budget, max_held)
+        _launch(self._index, "ojasx_kve_evict_device", self._ref, hp, budget, sink_tokens, recent_tokens,
+                max_held, ws.data_ptr(), need)
 
 
 class PackedPromptAttention:

@@ -1,0 +1,263 @@
+"""decoder.sample_tokens on the GPU: the token is the fp64 oracle's own (oracle/kve.py), at cuts, ties,
+masks and sizes where it can go wrong."""
+import math
+
+import numpy as np
+import pytest
+
+from oracle import kve
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def sample(pkg):
+    from importlib import import_module
+    return import_module(pkg.__name__ + ".decoder").sample_tokens
+
+
+def logits(rows, vocab, dtype, seed, spread=2.0, peaks=12):
+    import torch
+    r = np.random.default_rng(seed)
+    x = r.normal(size=(rows, vocab)) * spread
+    for b in range(rows):
+        x[b, r.integers(0, vocab, size=peaks)] += 4 + 3 * r.normal(size=peaks)
+    return torch.from_numpy(x.astype(np.float32)).to(getattr(torch, dtype))
+
+
+def check(sample, dev, x, u, T=1.0, k=0, p=1.0, m=0.0):
+    """Settings: numbers, or lists of one for each row."""
+    import torch
+    rows = x.shape[0]
+
+    def given(v, dtype):
+        return torch.tensor(v, dtype=dtype, device=dev) if isinstance(v, list) else v
+
+    got = sample(x.to(dev), torch.tensor(u, dtype=torch.float32, device=dev), temperature=given(T, torch.float32),
+                 top_k=given(k, torch.int32), top_p=given(p, torch.float32), min_p=given(m, torch.float32))
+    assert got.dtype == torch.int32 and tuple(got.shape) == (rows,)
+    f = lambda v: np.asarray(v, np.float32).astype(np.float64) if isinstance(v, list) else np.full(rows, v)  # noqa: E731
+    xs, uf = x.double().cpu().numpy(), np.asarray(u, np.float32).astype(np.float64)
+    want = [kve.draw(xs[b], uf[b], a, int(kk), pp, mm) for b, (a, kk, pp, mm) in
+            enumerate(zip(f(T), k if isinstance(k, list) else [k] * rows, f(p), f(m)))]
+    assert got.tolist() == want
+    return want
+
+
+def grid(n):
+    """n numbers over [0, 1), both ends among them."""
+    return [min(i / (n - 1), 1 - 2.0 ** -24) for i in range(n)]
+
+
+SETTINGS = [dict(), dict(T=0.3), dict(T=1.7), dict(k=1), dict(k=50), dict(k=5000), dict(p=0.9), dict(p=0.5, T=0.7),
+            dict(p=0.999), dict(m=0.05), dict(m=0.5, T=1.3), dict(k=40, p=0.8), dict(k=1000, p=0.95, m=0.01, T=0.8),
+            dict(k=3, m=0.9), dict(T=0.0), dict(T=0.0, k=5, p=0.5), dict(T=0.05, k=50, p=0.9), dict(T=1e-4),
+            dict(T=25.0, p=0.6), dict(T=25.0, k=20000), dict(T=1e6, p=0.3, k=9000), dict(p=0.0), dict(m=1.0),
+            dict(p=1e-9), dict(p=1 - 1e-12), dict(k=2**31 - 1, p=2.0)]
+
+
+@pytest.mark.parametrize("s", SETTINGS, ids=lambda s: "-".join(f"{k}{v}" for k, v in s.items()) or "plain")
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_settings(sample, dev, s, dtype):
+    """A vocabulary of several slices with an odd end; bfloat16 has many equal logits."""
+    check(sample, dev, logits(24, 30011, dtype, seed=1), grid(24), **s)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 9, 255, 1000, 8191, 8192, 8193, 16384, 151936, 262144])
+def test_vocabularies(sample, dev, vocab):
+    x = logits(5, vocab, "float32", seed=vocab)
+    for s in (dict(), dict(k=20, p=0.9), dict(p=0.95, T=1.2), dict(T=0.0), dict(m=0.1)):
+        check(sample, dev, x, grid(5), **s)
+
+
+def test_largest_vocabulary(sample, dev):
+    x = logits(2, 1 << 22, "bfloat16", seed=5)
+    for s in (dict(), dict(p=0.9), dict(k=100000, p=0.99)):
+        check(sample, dev, x, [0.31, 0.83], **s)
+
+
+def test_settings_of_each_row(sample, dev):
+    r = np.random.default_rng(4)
+    rows = 200
+    check(sample, dev, logits(rows, 9001, "bfloat16", seed=6), r.random(rows).tolist(),
+          T=[float(r.choice([0.0, 0.2, 0.7, 1.0, 1.5, 30.0])) for _ in range(rows)],
+          k=[int(r.choice([0, -5, 1, 2, 40, 700, 9000, 9001, 10000])) for _ in range(rows)],
+          p=[float(r.choice([1.0, 0.9, 0.5, 0.05, 0.0, -1.0, 1.5])) for _ in range(rows)],
+          m=[float(r.choice([0.0, 0.02, 0.3, 1.0, 1.5, -0.5])) for _ in range(rows)])
+
+
+def test_equal_logits(sample, dev):
+    """Cuts within equal logits keep the first ones of the vocabulary, over slices too."""
+    import torch
+    V = 20000
+    flat = torch.zeros(16, V)
+    u = grid(16)
+    for s in (dict(), dict(k=1), dict(k=8192), dict(k=8193), dict(k=12345), dict(p=0.25), dict(p=0.5), dict(p=0.75),
+              dict(k=16000, p=0.5), dict(m=1.0), dict(T=0.0), dict(T=3.0, k=100, p=0.5), dict(p=0.99999)):
+        want = check(sample, dev, flat, u, **s)
+        n = s.get("k") or V
+        assert max(want) < (n if "p" not in s else math.ceil(n * s["p"]))
+    two = torch.where(torch.arange(V) % 3 == 0, 0.5, -0.25).repeat(16, 1)
+    for s in (dict(k=100), dict(k=6667), dict(k=6668), dict(k=15000), dict(p=0.3), dict(p=0.8), dict(k=9000, p=0.9)):
+        check(sample, dev, two, u, **s)
+        check(sample, dev, -two * 1e-3 + 1e4, u, **s)
+        check(sample, dev, two.bfloat16(), u, T=0.4, **s)
+
+
+def test_masked_logits(sample, dev):
+    """Logits of -inf are never drawn, the type's lowest value only where nothing else is."""
+    import torch
+    for low in (-math.inf, torch.finfo(torch.float32).min):
+        x = logits(12, 20001, "float32", seed=7)
+        x[:, 3:19000] = low
+        x[1, :] = low
+        x[1, [77, 15000]] = torch.tensor([1.0, 2.0])
+        x[2, :8192] = low                             # whole slices of it
+        x[3, 8192:] = low
+        x[4, :20000] = low
+        for s in (dict(), dict(p=0.9), dict(k=30), dict(k=5000, p=0.99), dict(m=0.1), dict(T=0.0), dict(T=1e-3, p=0.5)):
+            got = check(sample, dev, x, grid(12), **s)
+            assert all(x[b, t] > -1e30 for b, t in enumerate(got))
+    x = torch.full((2, 9000), torch.finfo(torch.float32).min)
+    for s in (dict(), dict(k=100), dict(p=0.5), dict(T=0.0)):
+        check(sample, dev, x, [0.0, 0.9999], **s)
+
+
+def test_rows_without_a_distribution(sample, dev):
+    import torch
+    x = logits(8, 10000, "bfloat16", seed=8)
+    x[0] = -math.inf
+    x[1, 9999] = math.nan
+    x[2, 0] = math.inf
+    x[3, 4000] = -math.nan
+    for s in (dict(), dict(k=20), dict(p=0.9), dict(m=0.2), dict(T=0.0)):
+        got = check(sample, dev, x, grid(8), **s)
+        assert got[:4] == [-1] * 4 and min(got[4:]) >= 0
+    T = [1.0, 1.0, 1.0, 1.0, -1.0, math.nan, math.inf, 1.0]
+    got = sample(x.to(dev), torch.tensor(grid(8), device=dev), temperature=torch.tensor(T, device=dev), top_p=0.9)
+    assert got.tolist()[:7] == [-1] * 7 and got[7] >= 0
+
+
+def test_extreme_values(sample, dev):
+    """Logits at the ends of the type, tiny and huge temperatures, a cut at a value next to 0."""
+    import torch
+    big = torch.finfo(torch.float32).max
+    x = torch.tensor([[big, -big, 0.0, big, 1e-45, -1e-45, -0.0, 0.0, 1e38, -1e38]] * 6)
+    u = grid(6)
+    for s in (dict(), dict(k=2), dict(k=5), dict(p=0.5), dict(m=0.5), dict(T=1e38), dict(T=1e38, k=5), dict(T=1e-38, k=2),
+              dict(T=3e38, p=0.7), dict(T=1e-45), dict(T=1e38, m=0.1), dict(T=1e38, k=7, p=0.9)):
+        check(sample, dev, x, u, **s)
+    near = torch.tensor([[0.0, -0.0, 1e-45, 0.0, -0.0, -1e-45, 2e-45, -1e-3, 1e-3, -0.0]] * 6)
+    for k in range(1, 10):
+        check(sample, dev, near, u, k=k)
+        check(sample, dev, near, u, k=k, p=0.6, T=0.5)
+    check(sample, dev, near, u, m=0.9999)
+    for v in (0.0, 1e4, -1e4, 60000.0):
+        check(sample, dev, torch.full((3, 9000), v, dtype=torch.float16), [0.0, 0.4, 0.99], k=8500, p=0.7)
+
+
+def test_random_numbers_out_of_range(sample, dev):
+    import torch
+    x = torch.full((5, 9000), -math.inf)
+    x[:, 10:8990] = 0.0
+    u = torch.tensor([1.0, 7.0, -1.0, math.nan, math.inf], device=dev)
+    for kw in (dict(), dict(top_k=100), dict(top_p=0.5)):
+        got = sample(x.to(dev), u, **kw).tolist()
+        last = {0: 8989, 100: 109}.get(kw.get("top_k", 0)) if "top_p" not in kw else 4499
+        assert got == [last, last, 10, 10, last], kw
+
+
+def test_many_tokens_of_one_bin(sample, dev):
+    """More candidates of a cut than the list in LDS takes, over a wide range of keys."""
+    r = np.random.default_rng(9)
+    import torch
+    x = torch.from_numpy((r.random((6, 60000)) * 0.1).astype(np.float32))
+    x[3:] -= 0.05                                     # both signs
+    for s in (dict(k=20000), dict(p=0.4), dict(k=50000, p=0.7), dict(m=0.95), dict(k=30000, m=0.93, p=0.99)):
+        check(sample, dev, x, grid(6), **s)
+
+
+def test_strides_and_rows(sample, dev):
+    import torch
+    base = logits(6, 5003, "bfloat16", seed=10).to(dev)
+    u = torch.tensor(grid(6), device=dev)
+    want = sample(base, u, top_p=0.9)
+    wide = torch.empty(6, 9001, dtype=base.dtype, device=dev)
+    wide[:, 7:5010] = base
+    assert torch.equal(sample(wide[:, 7:5010], u, top_p=0.9), want)          # rows 2-byte aligned
+    assert torch.equal(sample(base.t().contiguous().t(), u, top_p=0.9), want)
+    one = base[2:3].expand(6, -1)                     # a row for all
+    assert torch.equal(sample(one, u, top_p=0.9), sample(one.contiguous(), u, top_p=0.9))
+    out = torch.empty(6, dtype=torch.int32, device=dev)
+    assert sample(base, u, top_p=0.9, out=out) is out and torch.equal(out, want)
+    # a row alone is what it is among others
+    for b in range(6):
+        assert sample(base[b:b + 1], u[b:b + 1], top_p=0.9).item() == want[b]
+    assert sample(base[:0], u[:0]).shape == (0,)
+
+
+def test_many_rows(sample, dev):
+    """More rows than a grid's second dimension would take."""
+    import torch
+    x = logits(70000, 40, "float32", seed=11, peaks=2)
+    r = np.random.default_rng(12)
+    u = r.random(70000).astype(np.float32)
+    got = sample(x.to(dev), torch.from_numpy(u).to(dev), top_k=10, top_p=0.9).tolist()
+    xs = x.double().numpy()
+    for b in range(0, 70000, 701):
+        assert got[b] == kve.draw(xs[b], float(u[b]), 1.0, 10, 0.9)
+    assert min(got) >= 0 and max(got) < 40
+
+
+def test_frequencies(sample, dev):
+    """Over an even grid of random numbers every token comes as often as its probability, to one."""
+    import torch
+    p = np.array([0.5, 0.25, 0.125, 0.0625, 0.0625])
+    n = 4096
+    x = torch.from_numpy(np.log(p).astype(np.float32)).repeat(n, 1)
+    u = (torch.arange(n) + 0.5) / n
+    got = np.bincount(sample(x.to(dev), u.to(dev)).cpu().numpy(), minlength=5)
+    assert (np.abs(got - p * n) <= 1).all()
+
+
+def test_captured_and_on_a_stream(sample, dev):
+    import torch
+    x, u = logits(9, 20000, "bfloat16", seed=13).to(dev), torch.rand(9, device=dev)
+    T, out = torch.full((9,), 0.7, device=dev), torch.empty(9, dtype=torch.int32, device=dev)
+    sample(x, u, temperature=T, top_k=50, top_p=0.9, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sample(x, u, temperature=T, top_k=50, top_p=0.9, out=out)
+    for i in range(4):
+        u.copy_(torch.rand(9, device=dev))
+        T.fill_(0.3 + 0.4 * i)
+        x.copy_(logits(9, 20000, "bfloat16", seed=20 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, sample(x, u, temperature=T, top_k=50, top_p=0.9))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a = sample(x, u, temperature=T, top_k=50, top_p=0.9)
+    s.synchronize()
+    assert torch.equal(a, got)
+
+
+def test_refusals(sample, dev):
+    import torch
+    x, u = torch.zeros(2, 50, device=dev), torch.zeros(2, device=dev)
+    for bad in (lambda: sample(x[0], u[:1]), lambda: sample(x, u[:1]), lambda: sample(x, u.double()),
+                lambda: sample(x, u.cpu()), lambda: sample(x[:, :0], u), lambda: sample(x, u, temperature=-1.0),
+                lambda: sample(x, u, temperature=math.nan), lambda: sample(x, u, temperature=math.inf),
+                lambda: sample(x, u, top_p=-0.1), lambda: sample(x, u, top_p=math.nan), lambda: sample(x, u, min_p=1.1),
+                lambda: sample(x, u, min_p=math.nan), lambda: sample(x, u, temperature=u.double()),
+                lambda: sample(x, u, top_k=u), lambda: sample(x, u, top_p=u[:1]), lambda: sample(x, u, out=u),
+                lambda: sample(x, u, out=torch.zeros(2, dtype=torch.int64, device=dev))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (x.double(), x.long()):
+        with pytest.raises(TypeError):
+            sample(bad, u)
+    with pytest.raises(RuntimeError):
+        sample(x.cpu(), u.cpu())
