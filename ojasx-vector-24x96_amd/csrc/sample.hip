@@ -6,13 +6,17 @@
 //   ones, in the vocabulary's order, at which the running sum of e passes u times their sum.
 //
 // All three cuts keep a beginning of one order, so together they are one logit kappa and a count:
-// kept is what lies above kappa, and of the tokens that equal it the first `ties`.  No sort: the
-// first kernel counts, by slices of the vocabulary, tokens and sums of e in 255 bins of the logit
-// (width T / 7, on one grid for all slices, from the slice's largest down to where e is
-// below 2^-51 of it and is not drawn); the second, a workgroup per row, adds the slices' bins,
-// finds the bin that a cut falls into, takes that bin's tokens from the row and selects among
-// them byte by byte of their logits' order; then it finds the slice that the draw falls into from
-// the slices' kept sums, and the token within it.
+// kept is what lies above kappa, and of the tokens that equal it the first `ties`.  No sort, and
+// no token is looked at more than three times:
+//   1. by slices of the vocabulary, counts of tokens and sums of e in 255 bins of the logit (width
+//      T / 7, on one grid for all slices, from the slice's largest down to where e is below 2^-51
+//      of it and is not drawn);
+//   2. by slices again, with the slices' bins added up: the tokens of the bins that the cuts fall
+//      into go to a list of the row;
+//   3. by rows: the cuts themselves, selected among the list's tokens byte by byte of their
+//      logits' order; then the slice that the draw falls into, from the slices' kept sums, and the
+//      token within it.
+// A row without cuts needs of 1. its slices' sums alone, and nothing of 2.
 //
 // A drawn token is a whole number: it has to be the definition's own.  So e is fp64 to about
 // 2^-50, sums are fp64, or in LDS, where they are added in any order, 64-bit integers: a fixed
@@ -31,48 +35,62 @@ constexpr int kNW = kNT / 64;
 constexpr int kPer = 8;                  // tokens of a thread
 constexpr int kSlice = kNT * kPer;
 constexpr int kBins = 256;               // the last: e below kLeast
-constexpr int kCopies = 4;               // of the bins' counters, so that a wave's lanes collide less
+constexpr int kCopies = 16;              // of the bins' counters, so that a wave's lanes collide less
 constexpr double kBinsPerE = 7.0;        // 255 / 7 = 36.4 > 51 ln 2
 constexpr int kFrac = 50;                // bits behind the point of a slice's sums (8192 of them: 2^63)
-constexpr int kList = 8192;              // tokens of a bin that are selected among in LDS
+constexpr int kList = 8192;              // tokens that are selected among in LDS; more: in memory
 constexpr int kMostSlices = 512;
 constexpr double kLeast = 0x1p-51;       // tokens of a smaller e are not drawn
 
 typedef unsigned long long u64;
 
 struct SliceHead {
-    double top;                          // bin of the slice's largest logit
     double total;                        // rows without cuts: the slice's sum of e, relative to its largest
     float most;
     int at;                              // index of the largest logit
+    int top;                             // its bin
     int bad;                             // a NaN or +inf among the logits
+};
+struct SliceBins {                       // up to and with the bin; the last two alike
+    u64 sum[kBins];
+    unsigned count[kBins];               // rows with a top-k cut
+};
+struct RowBins {                         // of the whole row, up to and with the bin
+    double sum[kBins];
+    int count[kBins];
+    int cut[6];                          // CutBins
+    unsigned listed;                     // tokens in the row's list
     int pad;
 };
-struct SliceBins {
-    u64 sum[kBins];
-    unsigned count[kBins];
+struct Work {
+    SliceBins *bins;                     // [row][slice]
+    SliceHead *heads;                    // [row][slice]
+    RowBins *rows;                       // [row]
+    uint2 *list;                         // [row][vocab]: key, index and in the high byte the bin
 };
 
-// 2^x for x <= 0, to about 2^-52: 2^f as its Taylor polynomial of degree 12, |f| <= 1/2 (the next
-// term is below 2^-52), scaled by the exponent; below 2^-1000: that.
-__device__ __forceinline__ double exp2_f64(double x) {
-    x = fmax(x, -1000.0);
-    const double n = rint(x), f = x - n;
-    constexpr double c1 = 0.69314718055994530942, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4,
-                     c5 = c4 * c1 / 5, c6 = c5 * c1 / 6, c7 = c6 * c1 / 7, c8 = c7 * c1 / 8, c9 = c8 * c1 / 9,
-                     c10 = c9 * c1 / 10, c11 = c10 * c1 / 11, c12 = c11 * c1 / 12;
-    double p = fma(c12, f, c11);
-    p = fma(p, f, c10);
-    p = fma(p, f, c9);
-    p = fma(p, f, c8);
-    p = fma(p, f, c7);
-    p = fma(p, f, c6);
-    p = fma(p, f, c5);
-    p = fma(p, f, c4);
-    p = fma(p, f, c3);
-    p = fma(p, f, c2);
-    p = fma(p, f, c1);
-    return ldexp(fma(p, f, 1.0), (int)n);
+// A constant held in scalar registers: one instruction adds its multiple, where the compiler would
+// copy it to two vector registers first.
+__device__ __forceinline__ double held(double c) {
+    asm("" : "+s"(c));
+    return c;
+}
+// 2^(x c), x <= 0, x c > -1020, to about 2^-51.5: 2^f, |f| <= 1/2, by the polynomial of degree 10
+// through its values at the 11 Chebyshev nodes (off by 3e-16), scaled by the exponent.
+__device__ __forceinline__ double exp2_f64(double x, double c) {
+    const double whole = held(0x1.8p52);         // the sum's last bits are x c rounded to whole numbers
+    const double t = fma(x, c, whole), f = fma(x, c, whole - t);
+    double p = fma(held(0x1.e6063f7217bc6p-28), f, held(0x1.b675bca4eeebbp-24));
+    p = fma(p, f, held(0x1.62bfd47773353p-20));
+    p = fma(p, f, held(0x1.ffcb54062e698p-17));
+    p = fma(p, f, held(0x1.430913096fd9fp-13));
+    p = fma(p, f, held(0x1.5d87fe9d7a584p-10));
+    p = fma(p, f, held(0x1.3b2ab6fba1ddap-7));
+    p = fma(p, f, held(0x1.c6b08d703ce49p-5));
+    p = fma(p, f, held(0x1.ebfbdff82c598p-3));
+    p = fma(p, f, held(0x1.62e42fefa3a19p-1));
+    p = fma(p, f, 1.0);                          // 0.7 .. 1.42
+    return __longlong_as_double(__double_as_longlong(p) + (__double_as_longlong(t) << 52));
 }
 // Bits of e in [0, 1] behind the point, rounded: e + 2^(52 - frac) has its last bit there.
 __device__ __forceinline__ u64 fixed(double e, int frac) {
@@ -88,11 +106,22 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Row {
-    double c, bins;                      // log2(e) / T, bins per unit of the logit
+    double c;                            // log2(e) / T
+    double bins;                         // bins per unit of the logit
+    float limit;                         // logits past it are one bin: 2^29 bins from 0
+    double depth;                        // e of a logit further below the largest is that of this distance
     double p, m;
     int k;
     bool greedy, bad, k_cut, p_cut, m_cut;
     __device__ __forceinline__ bool cuts() const { return k_cut || p_cut || m_cut; }
+    // A logit's bin on the grid of all slices: its product rounded to the nearest whole number, so that
+    // larger logits have no smaller one.
+    __device__ __forceinline__ int bin(float x) const {
+        return __double2loint(fma((double)__builtin_amdgcn_fmed3f(x, -limit, limit), bins, 0x1.8p52));
+    }
+    __device__ __forceinline__ double e(float x, float most) const {
+        return exp2_f64(fmax((double)x - (double)most, -depth), c);
+    }
 };
 __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
     Row s;
@@ -102,8 +131,11 @@ __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
     s.m = fmin(a.min_ps ? (double)a.min_ps[r] : a.min_p, 1.0);
     s.bad = !(T >= 0.0) || T > (double)FLT_MAX;
     s.greedy = T == 0.0;
-    s.c = 1.4426950408889634074 / T;
-    s.bins = kBinsPerE / T;
+    const double inv = 1.0 / T;                  // the others are its multiples or T's: a division costs 20 products
+    s.c = 1.4426950408889634074 * inv;
+    s.bins = kBinsPerE * inv;
+    s.limit = (float)fmin(0x1p29 / kBinsPerE * T, (double)FLT_MAX);
+    s.depth = 1000.0 / 1.4426950408889634074 * T;
     s.k_cut = s.k > 0 && s.k < a.vocab;
     s.p_cut = s.p < 1.0;
     s.m_cut = s.m > 0.0;
@@ -114,21 +146,38 @@ __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(__hip_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float as_f32(__half x) { return __half2float(x); }
 
-// Eight logits from i on (i a multiple of 8), -inf past the vocabulary's end.
+// Eight logits from i on, -inf past the vocabulary's end.  Rows begin anywhere: global loads need no
+// alignment, only the compiler has to know.
 template <typename T>
 __device__ __forceinline__ void load_logits(const T *row, int i, int V, float (&x)[kPer]) {
-    if ((reinterpret_cast<uintptr_t>(row) & 15) == 0 && i + kPer <= V) {
-        load8(row + i, x);
+    if (i + kPer <= V) {
+        typedef unsigned int u4_any __attribute__((ext_vector_type(4), aligned(2)));
+        T raw[kPer];
+#pragma unroll
+        for (unsigned j = 0; j < sizeof(T) / 2; ++j)
+            reinterpret_cast<u4_any *>(raw)[j] = reinterpret_cast<const u4_any *>(row + i)[j];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[e] = as_f32(raw[e]);
     } else {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[e] = i + e < V ? as_f32(row[i + e]) : -INFINITY;
     }
 }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    return __hiloint2double(dpp_i<CTRL>(__double2hiint(v)), dpp_i<CTRL>(__double2loint(v)));
+}
+__device__ __forceinline__ double lane_d(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane),
+                            __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v += dpp_d<0xB1>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    v += dpp_d<0x140>(v);
+    return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
 }
 __device__ __forceinline__ double wave_scan_d(double v) {       // with this lane's
 #pragma unroll
@@ -146,22 +195,49 @@ __device__ __forceinline__ int wave_scan_i(int v) {
     }
     return v;
 }
+
+// What the slices' heads say of the row.
+struct RowHead {
+    float most;
+    int at, top, bad;
+};
+__device__ __forceinline__ RowHead row_head(const Row &row, const SliceHead *heads, int S) {
+    RowHead h{-INFINITY, INT_MAX, 0, 0};
+    for (int s = threadIdx.x & 63; s < S; s += 64) {       // by every wave
+        const SliceHead x = heads[s];
+        if (x.most > h.most) h.most = x.most, h.at = x.at;
+        h.bad |= x.bad;
+    }
+    const float most = wave_max_f(h.most);
+    h.at = wave_min_i(h.most == most ? h.at : INT_MAX);
+    h.bad = __any(h.bad);
+    h.most = most;
+    h.top = row.bin(most);
+    return h;
+}
+// Bins that a slice's first one is behind the row's.
+__device__ __forceinline__ int slice_off(const SliceHead &h, int top) {
+    return h.most == -INFINITY ? kBins : min(max(top - h.top, 0), kBins);
+}
 }  // namespace
 
 // Workgroup row * slices + slice.
 template <typename T>
-__global__ __launch_bounds__(kNT) void sample_slice_kernel(SampleParams a, SliceHead *heads, SliceBins *bins) {
+__global__ __launch_bounds__(kNT) void sample_slice_kernel(SampleParams a, Work wk) {
     __shared__ u64 sum[kBins * kCopies];
     __shared__ unsigned count[kBins * kCopies];
     __shared__ float wm[kNW];
     __shared__ int wi[kNW], wbad[kNW];
     __shared__ double wt[kNW];
+    __shared__ u64 wsum[kBins / 64];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
-    const Row row = row_of(a, r);
     float x[kPer];
     const int i0 = s * kSlice + tid * kPer;
     load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0, a.vocab, x);
+    const Row row = row_of(a, r);
+    if (row.cuts())
+        for (int i = tid; i < kBins * kCopies; i += kNT) sum[i] = 0, count[i] = 0;
     float most = -INFINITY;
     int at = INT_MAX;
     bool bad = false;
@@ -174,7 +250,6 @@ __global__ __launch_bounds__(kNT) void sample_slice_kernel(SampleParams a, Slice
     const int wat = wave_min_i(most == wmost ? at : INT_MAX);
     const bool any = __any(bad);
     if (lane == 0) wm[wv] = wmost, wi[wv] = wat, wbad[wv] = any;
-    for (int i = tid; i < kBins * kCopies; i += kNT) sum[i] = 0, count[i] = 0;
     __syncthreads();
     most = wm[0], at = wi[0];
     int bads = wbad[0];
@@ -184,377 +259,433 @@ __global__ __launch_bounds__(kNT) void sample_slice_kernel(SampleParams a, Slice
         most = fmaxf(most, wm[w]);
         bads |= wbad[w];
     }
-    SliceHead *head = heads + blockIdx.x;
-    SliceHead h{0.0, 0.0, most, at, bads || row.bad, 0};
+    SliceHead h{0.0, most, at, 0, bads || row.bad};
+    if (s == 0 && tid == 0) wk.rows[r].listed = 0;
     if (row.greedy || h.bad || most == -INFINITY) {
-        if (tid == 0) *head = h;
-        // a slice of -inf: empty bins, which the second kernel adds
-        if (!row.greedy && !h.bad && row.cuts())
-            for (int i = tid; i < kBins; i += kNT) bins[blockIdx.x].sum[i] = 0, bins[blockIdx.x].count[i] = 0;
+        if (tid == 0) wk.heads[blockIdx.x] = h;
         return;
     }
     if (!row.cuts()) {
         double t = 0.0;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) t += x[e] == -INFINITY ? 0.0 : exp2_f64(((double)x[e] - (double)most) * row.c);
+        for (int e = 0; e < kPer; ++e) t += row.e(x[e], most);      // of -inf 2^-1000: nothing beside the largest's 1
         t = wave_sum_d(t);
         if (lane == 0) wt[wv] = t;
         __syncthreads();
         if (tid == 0) {
             for (int w = 0; w < kNW; ++w) h.total += wt[w];
-            *head = h;
+            wk.heads[blockIdx.x] = h;
         }
         return;
     }
-    h.top = floor((double)most * row.bins);
+    h.top = row.bin(most);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        const double d = h.top - floor((double)x[e] * row.bins);
-        if (d < kBins - 1) {                     // of -inf: no
-            const int b = (int)d * kCopies + (lane & (kCopies - 1));
-            atomicAdd(&sum[b], fixed(exp2_f64(((double)x[e] - (double)most) * row.c), kFrac));
-            atomicAdd(&count[b], 1u);
+        const int d = h.top - row.bin(x[e]);
+        const u64 q = fixed(row.e(x[e], most), kFrac);
+        if (d < kBins - 1 && x[e] > -INFINITY) {
+            const int b = d * kCopies + (lane & (kCopies - 1));
+            atomicAdd(&sum[b], q);
+            if (row.k_cut) atomicAdd(&count[b], 1u);
         }
     }
     __syncthreads();
-    for (int i = tid; i < kBins; i += kNT) {
-        u64 t = 0;
-        unsigned n = 0;
+    u64 t = 0;
+    int n = 0;
+    if (tid < kBins) {
 #pragma unroll
-        for (int c = 0; c < kCopies; ++c) t += sum[i * kCopies + c], n += count[i * kCopies + c];
-        bins[blockIdx.x].sum[i] = t;
-        bins[blockIdx.x].count[i] = n;
+        for (int c = 0; c < kCopies; ++c) {      // each lane begins at a copy of its own: other banks
+            const int i = tid * kCopies + ((c + tid) & (kCopies - 1));
+            t += sum[i], n += (int)count[i];
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u64 y = __shfl_up(t, o);
+            if (lane >= o) t += y;
+        }
+        n = wave_scan_i(n);
+        if (lane == 63) wsum[wv] = t, wi[wv] = n;
     }
-    if (tid == 0) *head = h;
+    __syncthreads();
+    if (tid < kBins) {
+        for (int w = 0; w < wv; ++w) t += wsum[w], n += wi[w];
+        wk.bins[blockIdx.x].sum[tid] = t;
+        wk.bins[blockIdx.x].count[tid] = n;
+    }
+    if (tid == 0) wk.heads[blockIdx.x] = h;
+}
+
+namespace {
+struct CutLds {
+    double scale[kMostSlices];           // e of a slice's largest logit
+    int off[kMostSlices];                // bins that the slice's first one is behind the row's
+    double gsum[4][kBins];
+    int gcount[4][kBins];
+    double wsum[kBins];                  // the row's bins: sums and counts up to and with the bin
+    int wcount[kBins];
+    unsigned key;
+};
+// scale and off of all slices.
+__device__ __forceinline__ void load_slices(CutLds &L, const Row &row, const RowHead &h, const SliceHead *heads, int S) {
+    for (int s = threadIdx.x; s < S; s += kNT) {
+        const SliceHead x = heads[s];
+        L.scale[s] = x.most == -INFINITY ? 0.0 : row.e(x.most, h.most);
+        L.off[s] = slice_off(x, h.top);
+    }
+    __syncthreads();
+}
+// The row's bins: four shares of the slices, then the shares in order.
+__device__ __forceinline__ void add_bins(CutLds &L, const SliceBins *bins, int S, bool counts) {
+    const int tid = threadIdx.x, j = tid & (kBins - 1), g = tid / kBins;
+    double w = 0.0;
+    int n = 0;
+    for (int s0 = g; s0 < S; s0 += 5 * (kNT / kBins)) {    // five slices' loads in flight
+        u64 t[5];
+        int c[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            const int s = min(s0 + i * (kNT / kBins), S - 1), b = max(j - L.off[s], 0);
+            t[i] = bins[s].sum[b];
+            c[i] = counts ? (int)bins[s].count[b] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            const int s = s0 + i * (kNT / kBins);
+            const bool in = s < S && j >= L.off[min(s, S - 1)];
+            w += in ? (double)t[i] * L.scale[min(s, S - 1)] : 0.0;
+            n += in ? c[i] : 0;
+        }
+    }
+    L.gsum[g][j] = w, L.gcount[g][j] = n;
+    __syncthreads();
+    if (tid < kBins) {
+        L.wsum[j] = (((L.gsum[0][j] + L.gsum[1][j]) + L.gsum[2][j]) + L.gsum[3][j]) * 0x1p-50;
+        L.wcount[j] = L.gcount[0][j] + L.gcount[1][j] + L.gcount[2][j] + L.gcount[3][j];
+    }
+    __syncthreads();
+}
+// The first bin with tokens that reaches `need`, or kBins: none does.  Every wave finds it by itself.
+__device__ __forceinline__ int reaches(const CutLds &L, bool by_sum, double need) {
+    const int lane = threadIdx.x & 63;
+    int first = kBins;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+        const int j = lane * 4 + i;
+        const bool some = by_sum ? L.wsum[j] > (j ? L.wsum[j - 1] : 0.0) : L.wcount[j] > (j ? L.wcount[j - 1] : 0);
+        if (some && (by_sum ? L.wsum[j] >= need : (double)L.wcount[j] >= need)) first = j;
+    }
+    return wave_min_i(first);
+}
+// The lowest finite key up to the largest logit's with e >= m, by one wave (e rises with the logit).
+__device__ __forceinline__ unsigned key_of_e(const Row &row, float most) {
+    const int lane = threadIdx.x & 63;
+    unsigned lo = key_of(-FLT_MAX), hi = key_of(most);
+    while (lo < hi) {                            // 64 probes at once, six or seven times
+        const unsigned step = (hi - lo) / 64 + 1, probe = min(lo + lane * step, hi);
+        const u64 yes = __ballot(row.e(of_key(probe), most) >= row.m);
+        const int f = yes ? __ffsll(yes) - 1 : 64;
+        if (f < 64) hi = min(lo + f * step, hi);
+        if (f > 0) lo = min(lo + (f - 1) * step + 1, hi);
+    }
+    return lo;
+}
+// Which bins the cuts fall into: top-k's, those that top-p's may (its sum is known only between two
+// bounds while top-k's cut is not selected), min-p's; kBins: no cut there.
+struct CutBins {
+    int k, p0, p1, m;
+    unsigned m_key;
+    int pad;
+    __device__ __forceinline__ bool has(int b) const {
+        return b < kBins - 1 && (b == k || (b >= p0 && b <= p1) || b == m);
+    }
+};
+__device__ __forceinline__ CutBins cut_bins(CutLds &L, const Row &row, const RowHead &h) {
+    CutBins c{kBins, kBins, kBins - 1, kBins, 0, 0};
+    double low = L.wsum[kBins - 1], high = low;
+    if (row.m_cut) {
+        if (threadIdx.x < 64) {
+            const unsigned key = key_of_e(row, h.most);
+            if (threadIdx.x == 0) L.key = key;
+        }
+        __syncthreads();
+        c.m_key = L.key;
+        c.m = h.top - row.bin(of_key(c.m_key));
+        if (c.m >= kBins - 1) c.m = kBins;
+    }
+    if (row.k_cut && L.wcount[kBins - 1] > row.k) {
+        c.k = reaches(L, false, row.k);
+        low = c.k ? L.wsum[c.k - 1] : 0.0, high = L.wsum[c.k];
+    }
+    if (row.p_cut) {
+        c.p0 = reaches(L, true, row.p * low);
+        c.p1 = min(reaches(L, true, row.p * high), kBins - 1);
+    }
+    return c;
+}
+}  // namespace
+
+// Workgroup row * slices + slice: its tokens of the cuts' bins to the row's list; the first slice's
+// leaves the row's bins too.
+template <typename T>
+__global__ __launch_bounds__(kNT) void sample_list_kernel(SampleParams a, Work wk) {
+    __shared__ CutLds L;
+    __shared__ unsigned found, base;
+    const int tid = threadIdx.x, r = blockIdx.x / a.slices, s = blockIdx.x % a.slices, S = a.slices;
+    const Row row = row_of(a, r);
+    if (!row.cuts() || row.greedy || row.bad) return;
+    const SliceHead *heads = wk.heads + (long)r * S;
+    const RowHead h = row_head(row, heads, S);
+    if (h.bad || h.most == -INFINITY) return;
+    float x[kPer];
+    const int i0 = s * kSlice + tid * kPer;
+    load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0, a.vocab, x);
+    if (tid == 0) found = 0;
+    load_slices(L, row, h, heads, S);
+    add_bins(L, wk.bins + (long)r * S, S, row.k_cut);
+    if (s == 0 && tid < kBins) wk.rows[r].sum[tid] = L.wsum[tid], wk.rows[r].count[tid] = L.wcount[tid];
+    const CutBins cut = cut_bins(L, row, h);
+    if (s == 0 && tid == 0) *reinterpret_cast<CutBins *>(wk.rows[r].cut) = cut;
+    if (L.off[s] >= kBins) return;
+    int bin[kPer];
+    unsigned mine = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        bin[e] = h.top - row.bin(x[e]);
+        mine |= (unsigned)(x[e] > -INFINITY && cut.has(bin[e])) << e;
+    }
+    // places in the list: of the wave's tokens, of the workgroup's, of the row's
+    const int n = __popc(mine), upto = wave_scan_i(n), all = __builtin_amdgcn_readlane(upto, 63);
+    unsigned at = 0;
+    if ((tid & 63) == 0 && all) at = atomicAdd(&found, (unsigned)all);
+    at = __builtin_amdgcn_readfirstlane(at) + (unsigned)(upto - n);
+    __syncthreads();
+    if (found == 0) return;
+    if (tid == 0) base = atomicAdd(&wk.rows[r].listed, found);
+    __syncthreads();
+    uint2 *to = wk.list + (long)r * a.vocab + base + at;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+        if (mine >> e & 1) *to++ = make_uint2(key_of(x[e]), (unsigned)(i0 + e) | (unsigned)bin[e] << 24);
 }
 
 namespace {
 struct RowLds {
-    u64 hsum[kBins];                     // a digit's sums, counts
-    unsigned hcount[kBins];
-    double wsum[kBins];                  // the row's bins: sums and counts up to and with the bin
-    int wcount[kBins];
-    double gsum[4][kBins];
-    int gcount[4][kBins];
-    unsigned lkey[kList];
-    int lidx[kList];
-    double scale[kMostSlices];           // e of a slice's largest logit
+    CutLds c;
+    u64 hsum[2][kBins];                  // a digit's sums, counts: one set in use, the other cleared
+    unsigned hcount[2][kBins];
+    uint2 list[kList];
     double kept[kMostSlices];
-    int off[kMostSlices];                // bins that the slice's first one is behind the row's
     u64 csum[kMostSlices];               // of the cut's bin: sum of e above kappa, tokens at kappa
     int cties[kMostSlices];
-    double dw[kNW];
-    int iw[kNW], jw[kNW];
-    double picked_sum, target, rest;
-    int picked, listed, hit, last, slice;
-    unsigned klo, khi;
+    double dw[kNW], picked_sum, rest;
+    unsigned kmin[2], kmax[2];
+    int iw[kNW], picked, picked_n, picked_c, hit, last, slice, before;
 };
 
-// What the second kernel's parts share.
+// The selection among the row's listed tokens.
 template <typename T>
-struct Draw {
-    const SampleParams &a;
+struct Chosen {
+    // low bits of a key that T's values have alike: of bf16 16, of fp16 13
+    static constexpr int kLow = sizeof(T) == 4 ? 0 : __is_same(T, __half) ? 13 : 16;
     const Row &row;
     RowLds &L;
-    const T *logits;
-    float most;
-    double top;
+    const RowHead &h;
+    const uint2 *list;
+    int n;                               // tokens of the list; in LDS if kList of them are enough
     int frac;                            // bits behind the point of sums over the row
-    unsigned klo, khi;                   // the tokens in view: keys from .. to
-    bool in_lds;                         // and whether they are listed
+    int set;                             // of the digits' sums and counts, the one that is clear
 
-    __device__ __forceinline__ double e_of(float x) const { return exp2_f64(((double)x - (double)most) * row.c); }
-    // Bins of a logit behind the row's first one.
-    __device__ __forceinline__ double bin_of(float x) const { return top - floor((double)x * row.bins); }
-    // The lowest finite key up to the largest logit's with in(its logit), which is false below some
-    // key and true from there on, and for the largest; by one wave.
+    // f(index, key) for the listed tokens of bin b
     template <typename F>
-    __device__ unsigned first_key(F in) const {
-        const int lane = threadIdx.x & 63;
-        unsigned lo = key_of(-FLT_MAX), hi = key_of(most);
-        while (lo < hi) {                        // 64 probes at once, six or seven times
-            const unsigned step = (hi - lo) / 64 + 1, probe = min(lo + lane * step, hi);
-            const u64 yes = __ballot(in(of_key(probe)));
-            const int f = yes ? __ffsll(yes) - 1 : 64;
-            if (f < 64) hi = min(lo + f * step, hi);
-            if (f > 0) lo = min(lo + (f - 1) * step + 1, hi);
-        }
-        return lo;
-    }
-    // f(index, key) for the row's tokens with klo <= key <= khi, from memory
-    template <typename F>
-    __device__ __forceinline__ void scan(F f) const {
-        const float lo = of_key(klo), hi = of_key(khi);
-        for (int i = threadIdx.x * kPer; i < a.vocab; i += kSlice) {
-            float x[kPer];
-            load_logits(logits, i, a.vocab, x);
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-                if (x[e] >= lo && x[e] <= hi && i + e < a.vocab) f(i + e, key_of(x[e]));
+    __device__ __forceinline__ void each(int b, F f) const {
+        for (int i = threadIdx.x; i < n; i += kNT) {
+            const uint2 t = n <= kList ? L.list[i] : list[i];
+            if ((int)(t.y >> 24) == b) f((int)(t.y & 0xffffffu), t.x);
         }
     }
-    template <typename F>
-    __device__ __forceinline__ void each(F f) const {
-        if (in_lds)
-            for (int i = threadIdx.x; i < L.listed; i += kNT) f(L.lidx[i], L.lkey[i]);
-        else
-            scan(f);
-    }
-    // Brings the tokens of bin j into view.
-    __device__ void view_bin(int j) {
+    // Of the tokens of bin b, in falling order: the key at which `need` of them (by_sum: of their sum of
+    // e) are reached, and how many of that key it takes; *sum: their sum of e up to there.  Byte by byte
+    // of the key's distance to the bin's lowest, without the bits that T's values never use.  call: 0, 1.
+    __device__ void select(int call, int b, bool by_sum, double need, unsigned *kappa, int *ties, double *sum) {
+        unsigned kmin = 0xffffffffu, kmax = 0;
+        each(b, [&](int, unsigned k) { kmin = min(kmin, k), kmax = max(kmax, k); });
+        kmin = (unsigned)wave_min_i((int)(kmin ^ 0x80000000u)) ^ 0x80000000u;
+        kmax = ~((unsigned)wave_min_i((int)(~kmax ^ 0x80000000u)) ^ 0x80000000u);
+        if ((threadIdx.x & 63) == 0 && kmin <= kmax) atomicMin(&L.kmin[call], kmin), atomicMax(&L.kmax[call], kmax);
         __syncthreads();
-        if (threadIdx.x < 64) {
-            const unsigned lo = first_key([&](float x) { return bin_of(x) <= j; });
-            if (threadIdx.x == 0) L.klo = lo, L.listed = 0;
-        } else if (threadIdx.x < 128) {
-            const unsigned above = j ? first_key([&](float x) { return bin_of(x) <= j - 1; }) : key_of(most) + 1;
-            if (threadIdx.x == 64) L.khi = above - 1;
-        }
-        __syncthreads();
-        klo = L.klo, khi = L.khi;
-        scan([&](int i, unsigned k) {
-            const int at = atomicAdd(&L.listed, 1);
-            if (at < kList) L.lidx[at] = i, L.lkey[at] = k;
-        });
-        __syncthreads();
-        in_lds = L.listed <= kList;
-    }
-    // Of the tokens in view, in falling order: the key at which `need` of them (by_sum: of their sum
-    // of e) are reached, and how many of that key it takes; *sum: their sum of e up to there.
-    __device__ void select(bool by_sum, double need, unsigned *kappa, int *ties, double *sum) {
+        kmin = L.kmin[call] >> kLow, kmax = L.kmax[call] >> kLow;
         unsigned prefix = 0;
         double sums = 0.0;               // above the prefix
         int counts = 0, last_count = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            const unsigned high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-            if (((klo ^ khi) >> shift) == 0) {   // one digit for all of them
-                prefix = khi & (0xffffffffu << shift);
-                if (shift == 0) last_count = INT_MAX;
-                continue;
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < kBins; i += kNT) L.hsum[i] = 0, L.hcount[i] = 0;
-            __syncthreads();
-            each([&](int, unsigned k) {
-                if ((k & high) != (prefix & high)) return;
-                atomicAdd(&L.hsum[k >> shift & 255], fixed(e_of(of_key(k)), frac));
-                atomicAdd(&L.hcount[k >> shift & 255], 1u);
+        // of one key alone this is one pass, of no token none
+        for (int shift = kmin <= kmax ? (32 - __clz(kmax - kmin | 1u) + 7) / 8 * 8 - 8 : -1; shift >= 0; shift -= 8) {
+            u64 *hsum = L.hsum[set];
+            unsigned *hcount = L.hcount[set];
+            set ^= 1;
+            each(b, [&](int, unsigned k) {
+                const unsigned q = (k >> kLow) - kmin;
+                if ((u64)(q ^ prefix) >> (shift + 8)) return;
+                atomicAdd(&hsum[q >> shift & 255], fixed(row.e(of_key(k), h.most), frac));
+                atomicAdd(&hcount[q >> shift & 255], 1u);
             });
             __syncthreads();
+            if (threadIdx.x >= kNT - kBins) {
+                const int i = threadIdx.x - (kNT - kBins);
+                L.hsum[set][i] = 0, L.hcount[set][i] = 0;
+            }
             if (threadIdx.x < 64) {      // four digits a lane, the largest first
                 const int lane = threadIdx.x;
                 const double unit = ldexp(1.0, -frac);
-                double s = 0.0;
-                int n = 0, last = -1;
+                double ds[4], s = 0.0;
+                int c[4], c4 = 0, last = -1;
+#pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int d = 255 - (lane * 4 + i);
-                    s += (double)L.hsum[d] * unit;
-                    n += L.hcount[d];
-                    if (L.hcount[d]) last = d;
+                    s += ds[i] = (double)hsum[d] * unit;
+                    c4 += c[i] = (int)hcount[d];
+                    if (c[i]) last = d;
                 }
                 double s0 = sums + (wave_scan_d(s) - s);
-                int n0 = counts + (wave_scan_i(n) - n);
+                int n0 = counts + (wave_scan_i(c4) - c4);
                 // the lowest digit that has tokens: where rounding leaves the need unreached
                 const int lowest = wave_min_i(last < 0 ? INT_MAX : last);
-                if (lane == 0) L.picked = -1;
+                if (lane == 0) L.picked = 0;
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
+#pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int d = 255 - (lane * 4 + i), c = L.hcount[d];
-                    const double ds = (double)L.hsum[d] * unit;
-                    const bool there = by_sum ? c && s0 < need && (s0 + ds >= need || d == lowest)
-                                              : (double)n0 < need && (double)(n0 + c) >= need;
-                    const bool first = by_sum && need <= s0 && n0 == counts && c;   // nothing needed: the largest
-                    if (there || first) L.picked = d, L.iw[0] = n0, L.iw[1] = c, L.picked_sum = s0;
-                    s0 += ds, n0 += c;
+                    const int d = 255 - (lane * 4 + i);
+                    const bool there = by_sum ? c[i] && s0 < need && (s0 + ds[i] >= need || d == lowest)
+                                              : (double)n0 < need && (double)(n0 + c[i]) >= need;
+                    const bool first = by_sum && need <= s0 && n0 == counts && c[i];   // nothing needed: the largest
+                    if (there || first) L.picked = d, L.picked_n = n0, L.picked_c = c[i], L.picked_sum = s0;
+                    s0 += ds[i], n0 += c[i];
                 }
             }
             __syncthreads();
-            if (L.picked < 0) break;     // nothing in view
             prefix |= (unsigned)L.picked << shift;
-            sums = L.picked_sum, counts = L.iw[0], last_count = L.iw[1];
+            counts = L.picked_n, last_count = L.picked_c, sums = L.picked_sum;
         }
-        const double e = e_of(of_key(prefix));
-        double n = by_sum ? ceil((need - sums) / e) : need - counts;
-        n = fmin(fmax(n, 1.0), (double)last_count);
+        // the key itself: of all that T's values have with these high bits the one that is there
+        prefix = (prefix + kmin) << kLow;
+        if (kLow && prefix < 0x80000000u) prefix |= (1u << kLow) - 1;      // a negative value's low bits are ones
+        const double e = row.e(of_key(prefix), h.most);
+        double t = by_sum ? ceil((need - sums) / e) : need - counts;
+        t = fmin(fmax(t, 1.0), (double)last_count);
         *kappa = prefix;
-        *ties = (int)n;
-        *sum = sums + n * e;
+        *ties = (int)t;
+        *sum = sums + t * e;
     }
 };
 }  // namespace
 
 // Workgroup = row.
 template <typename T>
-__global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, const SliceHead *heads, const SliceBins *bins) {
+__global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk) {
     __shared__ RowLds L;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, r = blockIdx.x, S = a.slices;
+    const SliceHead *heads = wk.heads + (long)r * S;
+    const SliceBins *bins = wk.bins + (long)r * S;
     const Row row = row_of(a, r);
-    heads += (long)r * S, bins += (long)r * S;
-    float most = -INFINITY;
-    int at = INT_MAX, bad = 0;
-    for (int s = 0; s < S; ++s) {                // the same for every thread
-        const float m = heads[s].most;
-        if (m > most) most = m, at = heads[s].at;
-        bad |= heads[s].bad;
-    }
-    if (bad || row.bad || most == -INFINITY || row.greedy) {
-        if (tid == 0) a.tokens[(long)r * a.token_stride] = bad || row.bad || most == -INFINITY ? -1 : at;
+    const RowHead h = row_head(row, heads, S);
+    if (h.bad || row.bad || h.most == -INFINITY || row.greedy) {
+        if (tid == 0) a.tokens[(long)r * a.token_stride] = h.bad || row.bad || h.most == -INFINITY ? -1 : h.at;
         return;
     }
-    Draw<T> d{a, row, L, static_cast<const T *>(a.logits) + (long)r * a.stride, most, floor((double)most * row.bins),
-              min(kFrac, 62 - (32 - __clz(a.vocab))), 0, 0, false};
-    for (int s = tid; s < S; s += kNT) {
-        const SliceHead h = heads[s];
-        const double f = h.most == -INFINITY ? 0.0 : exp2_f64(((double)h.most - (double)most) * row.c);
-        L.scale[s] = f;
-        L.off[s] = h.most == -INFINITY ? kBins : (int)fmin(d.top - h.top, (double)kBins);
-        L.kept[s] = h.total * f;                 // without cuts
-        L.csum[s] = 0, L.cties[s] = 0;
-    }
-    __syncthreads();
+    for (int s = tid; s < S; s += kNT) L.csum[s] = 0, L.cties[s] = 0;
+    if (tid < 2) L.kmin[tid] = 0xffffffffu, L.kmax[tid] = 0;
+    if (tid < kBins) L.hsum[0][tid] = 0, L.hcount[0][tid] = 0;
+    if (tid == 0) L.hit = INT_MAX, L.last = -1;
     unsigned kappa = 0;
-    int ties = INT_MAX;
+    int ties = INT_MAX, jc = kBins - 1;
+    const int frac = min(kFrac, 62 - (32 - __clz(a.vocab)));
     if (row.cuts()) {
-        {   // the row's bins: four shares of the slices, then the shares in order
-            const int j = tid & (kBins - 1), g = tid / kBins;
-            double w = 0.0;
-            int n = 0;
-            for (int s = g; s < S; s += kNT / kBins) {
-                const int b = j - L.off[s];
-                if (b >= 0 && b < kBins - 1) w += (double)bins[s].sum[b] * L.scale[s], n += bins[s].count[b];
-            }
-            L.gsum[g][j] = w * ldexp(1.0, -kFrac), L.gcount[g][j] = n;
-        }
-        __syncthreads();
-        if (wv == 0) {
-            double w[4], t = 0.0;
-            int n[4], m = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = lane * 4 + i;
-                t += w[i] = ((L.gsum[0][j] + L.gsum[1][j]) + L.gsum[2][j]) + L.gsum[3][j];
-                m += n[i] = L.gcount[0][j] + L.gcount[1][j] + L.gcount[2][j] + L.gcount[3][j];
-            }
-            double t0 = wave_scan_d(t) - t;
-            int m0 = wave_scan_i(m) - m;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t0 += w[i], m0 += n[i], L.wsum[lane * 4 + i] = t0, L.wcount[lane * 4 + i] = m0;
-        }
-        __syncthreads();
-        int viewed = -1;
-        double all = L.wsum[kBins - 1];
-        // the first bin that reaches `need`, or kBins: none does
-        auto bin_of = [&](bool by_sum, double need) {
-            __syncthreads();
-            if (tid == 0) L.picked = kBins;
-            __syncthreads();
-            if (tid < kBins && (by_sum ? L.wsum[tid] >= need : (double)L.wcount[tid] >= need) &&
-                (tid == 0 ? L.wcount[0] > 0 || !by_sum : L.wcount[tid] > L.wcount[tid - 1]))
-                atomicMin(&L.picked, tid);
-            __syncthreads();
-            return L.picked;
-        };
-        if (row.k_cut && L.wcount[kBins - 1] > row.k) {
-            const int j = bin_of(false, row.k);
-            d.view_bin(viewed = j);
+        const RowBins &of = wk.rows[r];
+        Chosen<T> d{row, L, h, wk.list + (long)r * a.vocab, (int)of.listed, frac, 0};
+        const CutBins cut = *reinterpret_cast<const CutBins *>(of.cut);
+        if (tid < kBins) L.c.wsum[tid] = of.sum[tid], L.c.wcount[tid] = of.count[tid];
+        if (d.n <= kList)
+            for (int i = tid; i < d.n; i += kNT) L.list[i] = d.list[i];
+        load_slices(L.c, row, h, heads, S);
+        double all = L.c.wsum[kBins - 1];
+        if (cut.k < kBins) {
+            const int j = cut.k;
             double sum;
-            d.select(false, (double)row.k - (j ? L.wcount[j - 1] : 0), &kappa, &ties, &sum);
-            all = (j ? L.wsum[j - 1] : 0.0) + sum;
+            d.select(0, j, false, (double)row.k - (j ? L.c.wcount[j - 1] : 0), &kappa, &ties, &sum);
+            all = (j ? L.c.wsum[j - 1] : 0.0) + sum;
         }
         if (row.p_cut) {
             const double need = row.p * all;
-            const int j = bin_of(true, need);
-            if (j < kBins) {
-                if (j != viewed) d.view_bin(viewed = j);
+            const int j = min(max(reaches(L.c, true, need), cut.p0), cut.p1);
+            if (j < kBins - 1) {
                 unsigned key;
                 int n;
                 double sum;
-                d.select(true, need - (j ? L.wsum[j - 1] : 0.0), &key, &n, &sum);
+                d.select(1, j, true, need - (j ? L.c.wsum[j - 1] : 0.0), &key, &n, &sum);
                 if (key > kappa) kappa = key, ties = n;
                 else if (key == kappa) ties = min(ties, n);
             }
         }
-        if (row.m_cut) {
-            __syncthreads();
-            if (wv == 0) {
-                const unsigned key = d.first_key([&](float x) { return d.e_of(x) >= row.m; });
-                if (lane == 0) L.klo = key;
-            }
-            __syncthreads();
-            if (L.klo > kappa) kappa = L.klo, ties = INT_MAX;
-        }
+        if (row.m_cut && cut.m_key > kappa) kappa = cut.m_key, ties = INT_MAX;
         // the bin of the cut; a slice keeps its bins before that, and of its tokens in that bin those above kappa
-        int jc = kBins - 1;
-        if (kappa) jc = (int)fmin(fmax(d.bin_of(of_key(kappa)), 0.0), kBins - 1.0);
-        if (jc < kBins - 1 && jc != viewed) d.view_bin(jc);
+        if (kappa) jc = min(max(h.top - row.bin(of_key(kappa)), 0), kBins - 1);
+        d.each(jc, [&](int i, unsigned k) {
+            if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(row.e(of_key(k), h.most), frac));
+            if (k == kappa) atomicAdd(&L.cties[i / kSlice], 1);
+        });
         __syncthreads();
-        if (jc < kBins - 1) {
-            d.each([&](int i, unsigned k) {
-                if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(d.e_of(of_key(k)), d.frac));
-                if (k == kappa) atomicAdd(&L.cties[i / kSlice], 1);
-            });
-            __syncthreads();
-        }
-        const double e = kappa ? d.e_of(of_key(kappa)) : 0.0;
-        for (int s = wv; s < S; s += kNW) {
-            double w = 0.0;
-            for (int b = lane; b < min(jc - L.off[s], kBins - 1); b += 64) w += (double)bins[s].sum[b];
-            w = wave_sum_d(w);
-            int before = 0;
-            for (int q = lane; q < s; q += 64) before += L.cties[q];
-#pragma unroll
-            for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
-            if (lane == 0)
-                L.kept[s] = w * ldexp(1.0, -kFrac) * L.scale[s] + (double)L.csum[s] * ldexp(1.0, -d.frac) +
-                            (double)min(max(ties - before, 0), L.cties[s]) * e;
-        }
-        __syncthreads();
+    } else {
+        load_slices(L.c, row, h, heads, S);
     }
     // the slice that the draw falls into
     if (wv == 0) {
-        double mine = 0.0;
         const int per = (S + 63) / 64, s0 = min(S, lane * per), s1 = min(S, s0 + per);
-        for (int s = s0; s < s1; ++s) mine += L.kept[s];
-        const double incl = wave_scan_d(mine);
-        const double total = __shfl(incl, 63);
+        int before = 0;
+        for (int s = s0; s < s1; ++s) before += L.cties[s];
+        before = wave_scan_i(before) - before;   // ties of the slices before
+        const int ties0 = before;
+        const double e = kappa ? row.e(of_key(kappa), h.most) : 0.0, unit = ldexp(1.0, -frac);
+        double mine = 0.0;
+        for (int s = s0; s < s1; ++s) {
+            const int b = jc - 1 - L.c.off[s];
+            const double w = !row.cuts() ? heads[s].total : b >= 0 ? (double)bins[s].sum[b] * 0x1p-50 : 0.0;
+            L.kept[s] = w * L.c.scale[s] + (double)L.csum[s] * unit + (double)min(max(ties - before, 0), L.cties[s]) * e;
+            before += L.cties[s];
+            mine += L.kept[s];
+        }
+        const double incl = wave_scan_d(mine), total = lane_d(incl, 63);
         double u = (double)a.uniform[a.step ? *a.step : r];
         u = u >= 0.0 ? fmin(u, 1.0) : 0.0;       // NaN: 0
         const double t = u * total;
-        double run = incl - mine;
-        int pick = INT_MAX, last = -1;
-        double rest = 0.0;
+        double run = incl - mine, rest = 0.0;
+        int pick = INT_MAX, last = -1, pick_ties = 0, last_ties = 0;
+        before = ties0;
         for (int s = s0; s < s1; ++s) {
             // a slice that keeps any token keeps its largest
-            const bool some = L.kept[s] > 0.0 && L.scale[s] >= kLeast;
-            if (some) last = s;
-            if (pick == INT_MAX && some && run + L.kept[s] > t) pick = s, rest = t - run;
+            const bool some = L.kept[s] > 0.0 && L.c.scale[s] >= kLeast;
+            if (some) last = s, last_ties = before;
+            if (pick == INT_MAX && some && run + L.kept[s] > t) pick = s, pick_ties = before, rest = t - run;
             run += L.kept[s];
+            before += L.cties[s];
         }
         const int slice = wave_min_i(pick), end = -wave_min_i(-last);
-        if (slice == INT_MAX) {                  // u = 1, or a rounding at the end: the last token
-            if (lane == 0) L.slice = end, L.rest = INFINITY;
-        } else if (pick == slice) {
-            L.slice = slice, L.rest = rest;
-        }
+        if (slice != INT_MAX && pick == slice) L.slice = slice, L.rest = rest, L.before = pick_ties;
+        // u = 1, or a rounding at the end: the last token
+        if (slice == INT_MAX && last == end) L.slice = end, L.rest = INFINITY, L.before = last_ties;
     }
-    if (tid == 0) L.hit = INT_MAX, L.last = -1;
     __syncthreads();
     const int s = L.slice, i0 = s * kSlice + tid * kPer;
     const double rest = L.rest;
     float x[kPer];
-    load_logits(d.logits, i0, a.vocab, x);
-    // ties before the slice, and before the thread's tokens within it
-    int mine = 0, before = 0;
+    load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0, a.vocab, x);
+    // ties before the thread's tokens
+    int mine = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) mine += kappa && i0 + e < a.vocab && key_of(x[e]) == kappa;
-    for (int q = lane; q < s; q += 64) before += L.cties[q];
-#pragma unroll
-    for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o);
     const int incl = wave_scan_i(mine);
     if (lane == 63) L.iw[wv] = incl;
     __syncthreads();
-    before += incl - mine;
+    int before = L.before + incl - mine;
     for (int w = 0; w < wv; ++w) before += L.iw[w];
     double e[kPer], sum = 0.0;
 #pragma unroll
@@ -564,7 +695,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, const S
             const unsigned k = key_of(x[i]);
             keep = k > kappa || (k == kappa && before++ < ties);
         }
-        e[i] = keep ? d.e_of(x[i]) : 0.0;
+        e[i] = keep ? row.e(x[i], h.most) : 0.0;
         sum += e[i];
     }
     const double scan = wave_scan_d(sum);
@@ -596,9 +727,13 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, const S
 
 namespace {
 template <typename T>
-void sample(const SampleParams &a, SliceHead *heads, SliceBins *bins, hipStream_t st) {
-    OJX_LAUNCH((sample_slice_kernel<T>), dim3((unsigned)a.rows * a.slices), dim3(kNT), 0, st, a, heads, bins);
-    OJX_LAUNCH((sample_row_kernel<T>), dim3(a.rows), dim3(kNT), 0, st, a, heads, bins);
+void sample(const SampleParams &a, const Work &wk, hipStream_t st) {
+    const dim3 slices((unsigned)a.rows * a.slices);
+    OJX_LAUNCH((sample_slice_kernel<T>), slices, dim3(kNT), 0, st, a, wk);
+    // no row can have a cut: nothing to list
+    if (a.top_ks || a.top_ps || a.min_ps || (a.top_k > 0 && a.top_k < a.vocab) || a.top_p < 1.0 || a.min_p > 0.0)
+        OJX_LAUNCH((sample_list_kernel<T>), slices, dim3(kNT), 0, st, a, wk);
+    OJX_LAUNCH((sample_row_kernel<T>), dim3(a.rows), dim3(kNT), 0, st, a, wk);
 }
 }  // namespace
 
@@ -612,16 +747,21 @@ long sample_workspace(int rows, int vocab) {
         set_error("sampling: %d rows of %d logits are more than a launch takes", rows, vocab);
         return OJASX_ERR_INVALID;
     }
-    return rows * slices * (long)(sizeof(SliceHead) + sizeof(SliceBins));
+    return rows * (slices * (long)(sizeof(SliceHead) + sizeof(SliceBins)) + (long)sizeof(RowBins) +
+                   (long)round_up((size_t)vocab * sizeof(uint2), 16));
 }
 
 int launch_sample(SampleParams a, int dtype, void *workspace, hipStream_t st) {
     a.slices = (a.vocab + kSlice - 1) / kSlice;
-    SliceBins *bins = static_cast<SliceBins *>(workspace);
-    SliceHead *heads = reinterpret_cast<SliceHead *>(bins + (long)a.rows * a.slices);
-    if (dtype == OJASX_DTYPE_F32) sample<float>(a, heads, bins, st);
-    else if (dtype == OJASX_DTYPE_BF16) sample<__hip_bfloat16>(a, heads, bins, st);
-    else sample<__half>(a, heads, bins, st);
+    Work wk;
+    const long n = (long)a.rows * a.slices;
+    wk.bins = static_cast<SliceBins *>(workspace);
+    wk.heads = reinterpret_cast<SliceHead *>(wk.bins + n);
+    wk.rows = reinterpret_cast<RowBins *>(wk.heads + n);
+    wk.list = reinterpret_cast<uint2 *>(wk.rows + a.rows);
+    if (dtype == OJASX_DTYPE_F32) sample<float>(a, wk, st);
+    else if (dtype == OJASX_DTYPE_BF16) sample<__hip_bfloat16>(a, wk, st);
+    else sample<__half>(a, wk, st);
     OJX_HIP(hipGetLastError());
     return OJASX_OK;
 }
