@@ -13,7 +13,7 @@
 //      of it and is not drawn);
 //   2. by slices again, with the slices' bins added up: the tokens of the bins that the cuts fall
 //      into go to a list of the row;
-//   3. by rows: the cuts themselves, selected among the list's tokens byte by byte of their
+//   3. by rows: the cuts themselves, selected among the list's tokens digit by digit of their
 //      logits' order; then the slice that the draw falls into, from the slices' kept sums, and the
 //      token within it.
 // A row without cuts needs of 1. its slices' sums alone, and nothing of 2.
@@ -30,16 +30,23 @@
 namespace ojx {
 
 namespace {
-constexpr int kNT = 1024;
+constexpr int kNT = 1024;                // threads of a row's workgroup
 constexpr int kNW = kNT / 64;
-constexpr int kPer = 8;                  // tokens of a thread
+constexpr int kPer = 8;                  // tokens that a thread takes at a time
 constexpr int kSlice = kNT * kPer;
+// Threads of a slice's workgroup, each with four times kPer tokens: what a wave does once, its settings,
+// maxima and sums, is as much as the work on 8 tokens a lane (256 rows of 32000: 15.5 us with 1024 threads).
+constexpr int kSliceNT = 256;
+constexpr int kSliceNW = kSliceNT / 64;
+constexpr int kSteps = kSlice / (kSliceNT * kPer);
 constexpr int kBins = 256;               // the last: e below kLeast
-constexpr int kCopies = 16;              // of the bins' counters, so that a wave's lanes collide less
+constexpr int kCopies = 8;               // of the bins' counters, so that a wave's lanes collide less
 constexpr double kBinsPerE = 7.0;        // 255 / 7 = 36.4 > 51 ln 2
 constexpr int kFrac = 50;                // bits behind the point of a slice's sums (8192 of them: 2^63)
 constexpr int kList = 8192;              // tokens that are selected among in LDS; more: in memory
 constexpr int kMostSlices = 512;
+constexpr int kDigitBits = 9;            // of a selection's pass: two passes over an fp32 bin's keys
+constexpr int kDigits = 1 << kDigitBits;
 constexpr double kLeast = 0x1p-51;       // tokens of a smaller e are not drawn
 
 typedef unsigned long long u64;
@@ -51,9 +58,12 @@ struct SliceHead {
     int top;                             // its bin
     int bad;                             // a NaN or +inf among the logits
 };
-struct SliceBins {                       // up to and with the bin; the last two alike
-    u64 sum[kBins];
-    unsigned count[kBins];               // rows with a top-k cut
+struct Bin {
+    u64 sum;
+    unsigned count, pad;                 // of rows with a top-k cut
+};
+struct SliceBins {
+    Bin upto[kBins];                     // sums and counts up to and with the bin; the last two alike
 };
 struct RowBins {                         // of the whole row, up to and with the bin
     double sum[kBins];
@@ -119,6 +129,11 @@ struct Row {
     __device__ __forceinline__ int bin(float x) const {
         return __double2loint(fma((double)__builtin_amdgcn_fmed3f(x, -limit, limit), bins, 0x1.8p52));
     }
+    // Bins behind bin `top`, at most the last.
+    __device__ __forceinline__ int behind(int top, float x) const {
+        const int b = min(top - bin(x), kBins - 1);
+        return x == -INFINITY ? kBins - 1 : b;
+    }
     __device__ __forceinline__ double e(float x, float most) const {
         return exp2_f64(fmax((double)x - (double)most, -depth), c);
     }
@@ -179,31 +194,47 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     v += dpp_d<0x140>(v);
     return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
 }
-__device__ __forceinline__ double wave_scan_d(double v) {       // with this lane's
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(v, o);
-        if ((threadIdx.x & 63) >= o) v += x;
-    }
-    return v;
+// Sums over the lanes up to and with each: within rows of 16 lanes by shifts, then row by row (DPP
+// row_shr and row_bcast; lanes without a source add 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp0_i(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ int wave_scan_i(int v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(v, o);
-        if ((threadIdx.x & 63) >= o) v += x;
-    }
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp0_u(u64 v) {
+    return (u64)(unsigned)dpp0_i<CTRL, ROWS>((int)(v >> 32)) << 32 | (unsigned)dpp0_i<CTRL, ROWS>((int)v);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp0_d(double v) {
+    return __longlong_as_double((long long)dpp0_u<CTRL, ROWS>((u64)__double_as_longlong(v)));
+}
+#define OJX_WAVE_SCAN(NAME, T, DPP)                     \
+    __device__ __forceinline__ T NAME(T v) {            \
+        v += DPP<0x111, 0xF>(v);                        \
+        v += DPP<0x112, 0xF>(v);                        \
+        v += DPP<0x114, 0xF>(v);                        \
+        v += DPP<0x118, 0xF>(v);                        \
+        v += DPP<0x142, 0xA>(v);                        \
+        v += DPP<0x143, 0xC>(v);                        \
+        return v;                                       \
+    }
+OJX_WAVE_SCAN(wave_scan_i, int, dpp0_i)
+OJX_WAVE_SCAN(wave_scan_u, u64, dpp0_u)
+OJX_WAVE_SCAN(wave_scan_d, double, dpp0_d)
+#undef OJX_WAVE_SCAN
 
-// What the slices' heads say of the row.
+// What the slices' heads say of the row; mine: the head of slice number lane.
 struct RowHead {
     float most;
     int at, top, bad;
+    SliceHead mine;
 };
 __device__ __forceinline__ RowHead row_head(const Row &row, const SliceHead *heads, int S) {
-    RowHead h{-INFINITY, INT_MAX, 0, 0};
-    for (int s = threadIdx.x & 63; s < S; s += 64) {       // by every wave
+    const int lane = threadIdx.x & 63;           // by every wave
+    RowHead h;
+    h.mine = heads[min(lane, S - 1)];
+    h.most = h.mine.most, h.at = h.mine.at, h.bad = h.mine.bad;
+    for (int s = 64 + lane; s < S; s += 64) {
         const SliceHead x = heads[s];
         if (x.most > h.most) h.most = x.most, h.at = x.at;
         h.bad |= x.bad;
@@ -223,39 +254,51 @@ __device__ __forceinline__ int slice_off(const SliceHead &h, int top) {
 
 // Workgroup row * slices + slice.
 template <typename T>
-__global__ __launch_bounds__(kNT) void sample_slice_kernel(SampleParams a, Work wk) {
+__global__ __launch_bounds__(kSliceNT) void sample_slice_kernel(SampleParams a, Work wk) {
     __shared__ u64 sum[kBins * kCopies];
     __shared__ unsigned count[kBins * kCopies];
-    __shared__ float wm[kNW];
-    __shared__ int wi[kNW], wbad[kNW];
-    __shared__ double wt[kNW];
-    __shared__ u64 wsum[kBins / 64];
+    __shared__ float wm[kSliceNW];
+    __shared__ int wi[kSliceNW], wbad[kSliceNW];
+    __shared__ double wt[kSliceNW];
+    __shared__ u64 wsum[kSliceNW];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
-    float x[kPer];
+    float x[kSteps][kPer];
     const int i0 = s * kSlice + tid * kPer;
-    load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0, a.vocab, x);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+        load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0 + i * (kSliceNT * kPer), a.vocab, x[i]);
     const Row row = row_of(a, r);
     if (row.cuts())
-        for (int i = tid; i < kBins * kCopies; i += kNT) sum[i] = 0, count[i] = 0;
+        for (int i = tid; i < kBins * kCopies; i += kSliceNT) sum[i] = 0, count[i] = 0;
     float most = -INFINITY;
-    int at = INT_MAX;
     bool bad = false;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        bad |= !(x[e] < INFINITY);
-        if (x[e] > most) most = x[e], at = i0 + e;
-    }
-    const float wmost = wave_max_f(most);
-    const int wat = wave_min_i(most == wmost ? at : INT_MAX);
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            bad |= !(x[i][e] < INFINITY);
+            most = fmaxf(most, x[i][e]);
+        }
+    most = wave_max_f(most);
     const bool any = __any(bad);
-    if (lane == 0) wm[wv] = wmost, wi[wv] = wat, wbad[wv] = any;
+    int at = INT_MAX;
+    if (row.greedy) {
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i)
+#pragma unroll
+            for (int e = kPer - 1; e >= 0; --e)
+                if (x[i][e] == most) at = i0 + i * (kSliceNT * kPer) + e;
+        at = wave_min_i(at);
+    }
+    if (lane == 0) wm[wv] = most, wi[wv] = at, wbad[wv] = any;
     __syncthreads();
     most = wm[0], at = wi[0];
     int bads = wbad[0];
 #pragma unroll
-    for (int w = 1; w < kNW; ++w) {
-        if (wm[w] > most || (wm[w] == most && wi[w] < at)) at = wi[w];
+    for (int w = 1; w < kSliceNW; ++w) {
+        if (wm[w] > most) at = wi[w];
+        else if (wm[w] == most) at = min(at, wi[w]);
         most = fmaxf(most, wm[w]);
         bads |= wbad[w];
     }
@@ -268,50 +311,50 @@ __global__ __launch_bounds__(kNT) void sample_slice_kernel(SampleParams a, Work 
     if (!row.cuts()) {
         double t = 0.0;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) t += row.e(x[e], most);      // of -inf 2^-1000: nothing beside the largest's 1
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) t += row.e(x[i][e], most);   // of -inf 2^-1000: nothing beside the largest's 1
         t = wave_sum_d(t);
         if (lane == 0) wt[wv] = t;
         __syncthreads();
         if (tid == 0) {
-            for (int w = 0; w < kNW; ++w) h.total += wt[w];
+            for (int w = 0; w < kSliceNW; ++w) h.total += wt[w];
             wk.heads[blockIdx.x] = h;
         }
         return;
     }
     h.top = row.bin(most);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const int d = h.top - row.bin(x[e]);
-        const u64 q = fixed(row.e(x[e], most), kFrac);
-        if (d < kBins - 1 && x[e] > -INFINITY) {
-            const int b = d * kCopies + (lane & (kCopies - 1));
-            atomicAdd(&sum[b], q);
-            if (row.k_cut) atomicAdd(&count[b], 1u);
+    for (int i = 0; i < kSteps; ++i) {           // eight chains of products at once; what is not drawn to the last bin
+        int b[kPer];
+        u64 q[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            b[e] = row.behind(h.top, x[i][e]) * kCopies + (lane & (kCopies - 1));
+            q[e] = fixed(row.e(x[i][e], most), kFrac);
         }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) atomicAdd(&sum[b[e]], q[e]);
+        if (row.k_cut)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) atomicAdd(&count[b[e]], 1u);
     }
     __syncthreads();
+    static_assert(kSliceNT == kBins, "a thread for each bin");
     u64 t = 0;
     int n = 0;
-    if (tid < kBins) {
 #pragma unroll
-        for (int c = 0; c < kCopies; ++c) {      // each lane begins at a copy of its own: other banks
-            const int i = tid * kCopies + ((c + tid) & (kCopies - 1));
-            t += sum[i], n += (int)count[i];
-        }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const u64 y = __shfl_up(t, o);
-            if (lane >= o) t += y;
-        }
-        n = wave_scan_i(n);
-        if (lane == 63) wsum[wv] = t, wi[wv] = n;
+    for (int c = 0; c < kCopies; ++c) {          // each lane begins at a copy of its own: other banks
+        const int i = tid * kCopies + ((c + tid) & (kCopies - 1));
+        t += sum[i], n += (int)count[i];
     }
+    if (tid == kBins - 1) t = 0, n = 0;
+    t = wave_scan_u(t);
+    n = wave_scan_i(n);
+    if (lane == 63) wsum[wv] = t, wi[wv] = n;
     __syncthreads();
-    if (tid < kBins) {
-        for (int w = 0; w < wv; ++w) t += wsum[w], n += wi[w];
-        wk.bins[blockIdx.x].sum[tid] = t;
-        wk.bins[blockIdx.x].count[tid] = n;
-    }
+    for (int w = 0; w < wv; ++w) t += wsum[w], n += wi[w];
+    wk.bins[blockIdx.x].upto[tid] = Bin{t, (unsigned)n, 0};
     if (tid == 0) wk.heads[blockIdx.x] = h;
 }
 
@@ -319,62 +362,54 @@ namespace {
 struct CutLds {
     double scale[kMostSlices];           // e of a slice's largest logit
     int off[kMostSlices];                // bins that the slice's first one is behind the row's
-    double gsum[4][kBins];
-    int gcount[4][kBins];
     double wsum[kBins];                  // the row's bins: sums and counts up to and with the bin
     int wcount[kBins];
     unsigned key;
 };
 // scale and off of all slices.
 __device__ __forceinline__ void load_slices(CutLds &L, const Row &row, const RowHead &h, const SliceHead *heads, int S) {
-    for (int s = threadIdx.x; s < S; s += kNT) {
-        const SliceHead x = heads[s];
+    for (int s = threadIdx.x; s < S; s += blockDim.x) {
+        const SliceHead x = s < 64 ? h.mine : heads[s];    // of the first wave
         L.scale[s] = x.most == -INFINITY ? 0.0 : row.e(x.most, h.most);
         L.off[s] = slice_off(x, h.top);
     }
     __syncthreads();
 }
-// The row's bins: four shares of the slices, then the shares in order.
-__device__ __forceinline__ void add_bins(CutLds &L, const SliceBins *bins, int S, bool counts) {
-    const int tid = threadIdx.x, j = tid & (kBins - 1), g = tid / kBins;
+// The row's bins, a thread for each, the slices in order.
+__device__ __forceinline__ void add_bins(CutLds &L, const SliceBins *bins, int S) {
+    constexpr int kAtOnce = 20;                  // slices' loads in flight
+    const int j = threadIdx.x;
     double w = 0.0;
     int n = 0;
-    for (int s0 = g; s0 < S; s0 += 5 * (kNT / kBins)) {    // five slices' loads in flight
-        u64 t[5];
-        int c[5];
+    for (int s0 = 0; s0 < S; s0 += kAtOnce) {
+        u4_t t[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-            const int s = min(s0 + i * (kNT / kBins), S - 1), b = max(j - L.off[s], 0);
-            t[i] = bins[s].sum[b];
-            c[i] = counts ? (int)bins[s].count[b] : 0;
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int s = min(s0 + i, S - 1);
+            t[i] = *reinterpret_cast<const u4_t *>(&bins[s].upto[max(j - L.off[s], 0)]);
         }
 #pragma unroll
-        for (int i = 0; i < 5; ++i) {
-            const int s = s0 + i * (kNT / kBins);
-            const bool in = s < S && j >= L.off[min(s, S - 1)];
-            w += in ? (double)t[i] * L.scale[min(s, S - 1)] : 0.0;
-            n += in ? c[i] : 0;
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int s = min(s0 + i, S - 1);
+            const bool in = (s0 + i < S) & (j >= L.off[s]);
+            const double sum = (double)((u64)t[i][1] << 32 | t[i][0]) * L.scale[s];
+            w += in ? sum : 0.0;
+            n += in ? (int)t[i][2] : 0;
         }
     }
-    L.gsum[g][j] = w, L.gcount[g][j] = n;
-    __syncthreads();
-    if (tid < kBins) {
-        L.wsum[j] = (((L.gsum[0][j] + L.gsum[1][j]) + L.gsum[2][j]) + L.gsum[3][j]) * 0x1p-50;
-        L.wcount[j] = L.gcount[0][j] + L.gcount[1][j] + L.gcount[2][j] + L.gcount[3][j];
-    }
+    L.wsum[j] = w * 0x1p-50, L.wcount[j] = n;
     __syncthreads();
 }
-// The first bin with tokens that reaches `need`, or kBins: none does.  Every wave finds it by itself.
+// The first bin that reaches `need`, or kBins: none does; sums and counts never fall from bin to bin.
+// Every wave finds it by itself.
 __device__ __forceinline__ int reaches(const CutLds &L, bool by_sum, double need) {
-    const int lane = threadIdx.x & 63;
-    int first = kBins;
+    int before = 0;
 #pragma unroll
-    for (int i = 3; i >= 0; --i) {
-        const int j = lane * 4 + i;
-        const bool some = by_sum ? L.wsum[j] > (j ? L.wsum[j - 1] : 0.0) : L.wcount[j] > (j ? L.wcount[j - 1] : 0);
-        if (some && (by_sum ? L.wsum[j] >= need : (double)L.wcount[j] >= need)) first = j;
+    for (int i = 0; i < kBins; i += 64) {
+        const int j = i + (threadIdx.x & 63);
+        before += __popcll(__ballot((by_sum ? L.wsum[j] : (double)L.wcount[j]) < need));
     }
-    return wave_min_i(first);
+    return before;
 }
 // The lowest finite key up to the largest logit's with e >= m, by one wave (e rises with the logit).
 __device__ __forceinline__ unsigned key_of_e(const Row &row, float most) {
@@ -395,8 +430,14 @@ struct CutBins {
     int k, p0, p1, m;
     unsigned m_key;
     int pad;
-    __device__ __forceinline__ bool has(int b) const {
-        return b < kBins - 1 && (b == k || (b >= p0 && b <= p1) || b == m);
+    // Bits 32 w .. 32 w + 31 of the set of them.
+    __device__ __forceinline__ unsigned word(int w) const {
+        unsigned bits = 0;
+        for (int i = 0; i < 32; ++i) {
+            const int b = w * 32 + i;
+            bits |= (unsigned)((b < kBins - 1) & ((b == k) | ((b >= p0) & (b <= p1)) | (b == m))) << i;
+        }
+        return bits;
     }
 };
 __device__ __forceinline__ CutBins cut_bins(CutLds &L, const Row &row, const RowHead &h) {
@@ -427,32 +468,37 @@ __device__ __forceinline__ CutBins cut_bins(CutLds &L, const Row &row, const Row
 // Workgroup row * slices + slice: its tokens of the cuts' bins to the row's list; the first slice's
 // leaves the row's bins too.
 template <typename T>
-__global__ __launch_bounds__(kNT) void sample_list_kernel(SampleParams a, Work wk) {
+__global__ __launch_bounds__(kSliceNT) void sample_list_kernel(SampleParams a, Work wk) {
     __shared__ CutLds L;
-    __shared__ unsigned found, base;
+    __shared__ unsigned found, base, words[kBins / 32];
     const int tid = threadIdx.x, r = blockIdx.x / a.slices, s = blockIdx.x % a.slices, S = a.slices;
+    const SliceHead *heads = wk.heads + (long)r * S;
+    float x[kSteps][kPer];
+    const int i0 = s * kSlice + tid * kPer;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+        load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0 + i * (kSliceNT * kPer), a.vocab, x[i]);
     const Row row = row_of(a, r);
     if (!row.cuts() || row.greedy || row.bad) return;
-    const SliceHead *heads = wk.heads + (long)r * S;
     const RowHead h = row_head(row, heads, S);
     if (h.bad || h.most == -INFINITY) return;
-    float x[kPer];
-    const int i0 = s * kSlice + tid * kPer;
-    load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0, a.vocab, x);
     if (tid == 0) found = 0;
     load_slices(L, row, h, heads, S);
-    add_bins(L, wk.bins + (long)r * S, S, row.k_cut);
-    if (s == 0 && tid < kBins) wk.rows[r].sum[tid] = L.wsum[tid], wk.rows[r].count[tid] = L.wcount[tid];
+    add_bins(L, wk.bins + (long)r * S, S);
+    if (s == 0) wk.rows[r].sum[tid] = L.wsum[tid], wk.rows[r].count[tid] = L.wcount[tid];
     const CutBins cut = cut_bins(L, row, h);
     if (s == 0 && tid == 0) *reinterpret_cast<CutBins *>(wk.rows[r].cut) = cut;
     if (L.off[s] >= kBins) return;
-    int bin[kPer];
+    if (tid < kBins / 32) words[tid] = cut.word(tid);
+    __syncthreads();
     unsigned mine = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        bin[e] = h.top - row.bin(x[e]);
-        mine |= (unsigned)(x[e] > -INFINITY && cut.has(bin[e])) << e;
-    }
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            const int b = row.behind(h.top, x[i][e]);
+            mine |= (words[b >> 5] >> (b & 31) & 1) << (i * kPer + e);
+        }
     // places in the list: of the wave's tokens, of the workgroup's, of the row's
     const int n = __popc(mine), upto = wave_scan_i(n), all = __builtin_amdgcn_readlane(upto, 63);
     unsigned at = 0;
@@ -464,22 +510,32 @@ __global__ __launch_bounds__(kNT) void sample_list_kernel(SampleParams a, Work w
     __syncthreads();
     uint2 *to = wk.list + (long)r * a.vocab + base + at;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e)
-        if (mine >> e & 1) *to++ = make_uint2(key_of(x[e]), (unsigned)(i0 + e) | (unsigned)bin[e] << 24);
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+            if (mine >> (i * kPer + e) & 1)
+                *to++ = make_uint2(key_of(x[i][e]), (unsigned)(i0 + i * (kSliceNT * kPer) + e) |
+                                                        (unsigned)(h.top - row.bin(x[i][e])) << 24);
 }
 
 namespace {
+struct Found {                           // a digit, the sum and count of what lies above it, its own count
+    u64 above;
+    int digit, counts, count, pad;
+};
 struct RowLds {
     CutLds c;
-    u64 hsum[2][kBins];                  // a digit's sums, counts: one set in use, the other cleared
-    unsigned hcount[2][kBins];
+    u64 hsum[2][kDigits];                // a digit's sums, counts: one set in use, the other cleared
+    unsigned hcount[2][kDigits];
     uint2 list[kList];
     double kept[kMostSlices];
     u64 csum[kMostSlices];               // of the cut's bin: sum of e above kappa, tokens at kappa
     int cties[kMostSlices];
-    double dw[kNW], picked_sum, rest;
+    double dw[kNW], rest;
     unsigned kmin[2], kmax[2];
-    int iw[kNW], picked, picked_n, picked_c, hit, last, slice, before;
+    u64 uw[kDigits / 64];
+    Found found[kDigits / 64];
+    int iw[kNW], hit, last, slice, before;
 };
 
 // The selection among the row's listed tokens.
@@ -495,80 +551,102 @@ struct Chosen {
     int frac;                            // bits behind the point of sums over the row
     int set;                             // of the digits' sums and counts, the one that is clear
 
-    // f(index, key) for the listed tokens of bin b
-    template <typename F>
+    // f(index, key, e) for the listed tokens of bin b; with_e: e is formed, for four tokens at once
+    template <bool with_e, typename F>
     __device__ __forceinline__ void each(int b, F f) const {
-        for (int i = threadIdx.x; i < n; i += kNT) {
-            const uint2 t = n <= kList ? L.list[i] : list[i];
-            if ((int)(t.y >> 24) == b) f((int)(t.y & 0xffffffu), t.x);
+        constexpr int kAtOnce = 4;
+        for (int i0 = threadIdx.x; i0 < n; i0 += kAtOnce * kNT) {
+            uint2 t[kAtOnce];
+            double e[kAtOnce];
+            if (n <= kList) {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) t[i] = L.list[min(i0 + i * kNT, n - 1)];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) t[i] = list[min(i0 + i * kNT, n - 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) e[i] = with_e ? row.e(of_key(t[i].x), h.most) : 0.0;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (i0 + i * kNT < n && (int)(t[i].y >> 24) == b) f((int)(t[i].y & 0xffffffu), t[i].x, e[i]);
         }
     }
+    // The key of T's values whose high bits they are.
+    static __device__ __forceinline__ unsigned whole_key(unsigned high) {
+        const unsigned k = high << kLow;
+        return kLow && k < 0x80000000u ? k | ((1u << kLow) - 1) : k;       // a negative value's low bits are ones
+    }
     // Of the tokens of bin b, in falling order: the key at which `need` of them (by_sum: of their sum of
-    // e) are reached, and how many of that key it takes; *sum: their sum of e up to there.  Byte by byte
+    // e) are reached, and how many of that key it takes; *sum: their sum of e up to there.  Digit by digit
     // of the key's distance to the bin's lowest, without the bits that T's values never use.  call: 0, 1.
     __device__ void select(int call, int b, bool by_sum, double need, unsigned *kappa, int *ties, double *sum) {
         unsigned kmin = 0xffffffffu, kmax = 0;
-        each(b, [&](int, unsigned k) { kmin = min(kmin, k), kmax = max(kmax, k); });
+        each<false>(b, [&](int, unsigned k, double) { kmin = min(kmin, k), kmax = max(kmax, k); });
         kmin = (unsigned)wave_min_i((int)(kmin ^ 0x80000000u)) ^ 0x80000000u;
         kmax = ~((unsigned)wave_min_i((int)(~kmax ^ 0x80000000u)) ^ 0x80000000u);
         if ((threadIdx.x & 63) == 0 && kmin <= kmax) atomicMin(&L.kmin[call], kmin), atomicMax(&L.kmax[call], kmax);
         __syncthreads();
         kmin = L.kmin[call] >> kLow, kmax = L.kmax[call] >> kLow;
         unsigned prefix = 0;
-        double sums = 0.0;               // above the prefix
-        int counts = 0, last_count = 0;
+        // all in whole numbers, sums with frac bits behind the point: exactly one digit is the first to reach
+        u64 above = 0;                   // sum of what lies above the prefix
+        int counts = 0, last_count = 0;  // tokens above it, tokens of it
         // of one key alone this is one pass, of no token none
-        for (int shift = kmin <= kmax ? (32 - __clz(kmax - kmin | 1u) + 7) / 8 * 8 - 8 : -1; shift >= 0; shift -= 8) {
+        for (int shift = kmin <= kmax ? (31 - __clz((kmax - kmin) | 1u)) / kDigitBits * kDigitBits : -1; shift >= 0;
+             shift -= kDigitBits) {
             u64 *hsum = L.hsum[set];
             unsigned *hcount = L.hcount[set];
             set ^= 1;
-            each(b, [&](int, unsigned k) {
+            auto add = [&](int, unsigned k, double e) {
                 const unsigned q = (k >> kLow) - kmin;
-                if ((u64)(q ^ prefix) >> (shift + 8)) return;
-                atomicAdd(&hsum[q >> shift & 255], fixed(row.e(of_key(k), h.most), frac));
-                atomicAdd(&hcount[q >> shift & 255], 1u);
-            });
+                if ((u64)(q ^ prefix) >> (shift + kDigitBits)) return;
+                if (shift) atomicAdd(&hsum[q >> shift & (kDigits - 1)], fixed(e, frac));
+                atomicAdd(&hcount[q >> shift & (kDigits - 1)], 1u);
+            };
+            // the last digit's tokens have one key each: their sum is a multiple of its e
+            if (shift) each<true>(b, add);
+            else each<false>(b, add);
             __syncthreads();
-            if (threadIdx.x >= kNT - kBins) {
-                const int i = threadIdx.x - (kNT - kBins);
-                L.hsum[set][i] = 0, L.hcount[set][i] = 0;
-            }
-            if (threadIdx.x < 64) {      // four digits a lane, the largest first
-                const int lane = threadIdx.x;
-                const double unit = ldexp(1.0, -frac);
-                double ds[4], s = 0.0;
-                int c[4], c4 = 0, last = -1;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = 255 - (lane * 4 + i);
-                    s += ds[i] = (double)hsum[d] * unit;
-                    c4 += c[i] = (int)hcount[d];
-                    if (c[i]) last = d;
-                }
-                double s0 = sums + (wave_scan_d(s) - s);
-                int n0 = counts + (wave_scan_i(c4) - c4);
-                // the lowest digit that has tokens: where rounding leaves the need unreached
-                const int lowest = wave_min_i(last < 0 ? INT_MAX : last);
-                if (lane == 0) L.picked = 0;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = 255 - (lane * 4 + i);
-                    const bool there = by_sum ? c[i] && s0 < need && (s0 + ds[i] >= need || d == lowest)
-                                              : (double)n0 < need && (double)(n0 + c[i]) >= need;
-                    const bool first = by_sum && need <= s0 && n0 == counts && c[i];   // nothing needed: the largest
-                    if (there || first) L.picked = d, L.picked_n = n0, L.picked_c = c[i], L.picked_sum = s0;
-                    s0 += ds[i], n0 += c[i];
-                }
+            // a digit for each of the first threads, the largest first
+            const int d = kDigits - 1 - (int)threadIdx.x, w = threadIdx.x / 64;
+            u64 mine = 0, upto = 0;
+            int c = 0, n_upto = 0;
+            if (threadIdx.x < kDigits) {
+                c = (int)hcount[d];
+                const double e = row.e(fminf(of_key(whole_key((prefix | (unsigned)d) + kmin)), h.most), h.most);
+                mine = shift ? hsum[d] : c ? c * fixed(e, frac) : 0;                // no token: e of any key
+                upto = wave_scan_u(mine), n_upto = wave_scan_i(c);
+                if ((threadIdx.x & 63) == 63) L.uw[w] = upto, L.iw[w] = n_upto;
+                L.hsum[set][d] = 0, L.hcount[set][d] = 0;
             }
             __syncthreads();
-            prefix |= (unsigned)L.picked << shift;
-            counts = L.picked_n, last_count = L.picked_c, sums = L.picked_sum;
+            if (threadIdx.x < kDigits) {
+                u64 before = above, all = above;
+                int n_before = counts;
+#pragma unroll
+                for (int i = 0; i < kDigits / 64; ++i) {
+                    if (i < w) before += L.uw[i], n_before += L.iw[i];
+                    all += L.uw[i];
+                }
+                // what rounding leaves unreached is all of it
+                const u64 goal = by_sum ? min((u64)ceil(fmax(ldexp(need, frac), 0.0)), all) : 0;
+                const bool there = c && (by_sum ? before + upto >= goal : n_before + n_upto >= (int)need);
+                const u64 who = __ballot(there);
+                if ((threadIdx.x & 63) == 0) L.found[w].digit = -1;
+                if (there && (threadIdx.x & 63) == __ffsll(who) - 1)
+                    L.found[w] = Found{before + (upto - mine), d, n_before + n_upto - c, c, 0};
+            }
+            __syncthreads();
+            Found f = L.found[0];
+#pragma unroll
+            for (int i = 1; i < kDigits / 64; ++i)
+                if (f.digit < 0) f = L.found[i];
+            prefix |= (unsigned)f.digit << shift;
+            above = f.above, counts = f.counts, last_count = f.count;
         }
-        // the key itself: of all that T's values have with these high bits the one that is there
-        prefix = (prefix + kmin) << kLow;
-        if (kLow && prefix < 0x80000000u) prefix |= (1u << kLow) - 1;      // a negative value's low bits are ones
+        const double sums = (double)above * ldexp(1.0, -frac);
+        prefix = whole_key(prefix + kmin);
         const double e = row.e(of_key(prefix), h.most);
         double t = by_sum ? ceil((need - sums) / e) : need - counts;
         t = fmin(fmax(t, 1.0), (double)last_count);
@@ -594,7 +672,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
     }
     for (int s = tid; s < S; s += kNT) L.csum[s] = 0, L.cties[s] = 0;
     if (tid < 2) L.kmin[tid] = 0xffffffffu, L.kmax[tid] = 0;
-    if (tid < kBins) L.hsum[0][tid] = 0, L.hcount[0][tid] = 0;
+    if (tid < kDigits) L.hsum[0][tid] = 0, L.hcount[0][tid] = 0;
     if (tid == 0) L.hit = INT_MAX, L.last = -1;
     unsigned kappa = 0;
     int ties = INT_MAX, jc = kBins - 1;
@@ -629,8 +707,8 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         if (row.m_cut && cut.m_key > kappa) kappa = cut.m_key, ties = INT_MAX;
         // the bin of the cut; a slice keeps its bins before that, and of its tokens in that bin those above kappa
         if (kappa) jc = min(max(h.top - row.bin(of_key(kappa)), 0), kBins - 1);
-        d.each(jc, [&](int i, unsigned k) {
-            if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(row.e(of_key(k), h.most), frac));
+        d.template each<true>(jc, [&](int i, unsigned k, double e) {
+            if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(e, frac));
             if (k == kappa) atomicAdd(&L.cties[i / kSlice], 1);
         });
         __syncthreads();
@@ -648,7 +726,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         double mine = 0.0;
         for (int s = s0; s < s1; ++s) {
             const int b = jc - 1 - L.c.off[s];
-            const double w = !row.cuts() ? heads[s].total : b >= 0 ? (double)bins[s].sum[b] * 0x1p-50 : 0.0;
+            const double w = !row.cuts() ? heads[s].total : b >= 0 ? (double)bins[s].upto[b].sum * 0x1p-50 : 0.0;
             L.kept[s] = w * L.c.scale[s] + (double)L.csum[s] * unit + (double)min(max(ties - before, 0), L.cties[s]) * e;
             before += L.cties[s];
             mine += L.kept[s];
@@ -690,12 +768,15 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
     double e[kPer], sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        bool keep = x[i] > -INFINITY;            // also false past the end
-        if (kappa && keep) {
-            const unsigned k = key_of(x[i]);
-            keep = k > kappa || (k == kappa && before++ < ties);
+        const unsigned k = key_of(x[i]);         // kappa 0: below every key
+        const bool same = k == kappa, keep = (k > kappa) | (same & (before < ties));
+        before += same;
+        e[i] = 0.0;
+        const bool some = keep & (x[i] > -INFINITY);       // not past the end
+        if (__any(some)) {                       // few of a cut's tokens are kept
+            const double v = row.e(x[i], h.most);
+            e[i] = some ? v : 0.0;
         }
-        e[i] = keep ? row.e(x[i], h.most) : 0.0;
         sum += e[i];
     }
     const double scan = wave_scan_d(sum);
@@ -729,10 +810,10 @@ namespace {
 template <typename T>
 void sample(const SampleParams &a, const Work &wk, hipStream_t st) {
     const dim3 slices((unsigned)a.rows * a.slices);
-    OJX_LAUNCH((sample_slice_kernel<T>), slices, dim3(kNT), 0, st, a, wk);
+    OJX_LAUNCH((sample_slice_kernel<T>), slices, dim3(kSliceNT), 0, st, a, wk);
     // no row can have a cut: nothing to list
     if (a.top_ks || a.top_ps || a.min_ps || (a.top_k > 0 && a.top_k < a.vocab) || a.top_p < 1.0 || a.min_p > 0.0)
-        OJX_LAUNCH((sample_list_kernel<T>), slices, dim3(kNT), 0, st, a, wk);
+        OJX_LAUNCH((sample_list_kernel<T>), slices, dim3(kSliceNT), 0, st, a, wk);
     OJX_LAUNCH((sample_row_kernel<T>), dim3(a.rows), dim3(kNT), 0, st, a, wk);
 }
 }  // namespace
