@@ -473,11 +473,6 @@ __global__ __launch_bounds__(kSliceNT) void sample_list_kernel(SampleParams a, W
     __shared__ unsigned found, base, words[kBins / 32];
     const int tid = threadIdx.x, r = blockIdx.x / a.slices, s = blockIdx.x % a.slices, S = a.slices;
     const SliceHead *heads = wk.heads + (long)r * S;
-    float x[kSteps][kPer];
-    const int i0 = s * kSlice + tid * kPer;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-        load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0 + i * (kSliceNT * kPer), a.vocab, x[i]);
     const Row row = row_of(a, r);
     if (!row.cuts() || row.greedy || row.bad) return;
     const RowHead h = row_head(row, heads, S);
@@ -486,6 +481,12 @@ __global__ __launch_bounds__(kSliceNT) void sample_list_kernel(SampleParams a, W
     load_slices(L, row, h, heads, S);
     add_bins(L, wk.bins + (long)r * S, S);
     if (s == 0) wk.rows[r].sum[tid] = L.wsum[tid], wk.rows[r].count[tid] = L.wcount[tid];
+    // loaded no earlier: the registers that they take leave room for fewer waves beside this one
+    float x[kSteps][kPer];
+    const int i0 = s * kSlice + tid * kPer;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+        load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0 + i * (kSliceNT * kPer), a.vocab, x[i]);
     const CutBins cut = cut_bins(L, row, h);
     if (s == 0 && tid == 0) *reinterpret_cast<CutBins *>(wk.rows[r].cut) = cut;
     if (L.off[s] >= kBins) return;
