@@ -37,12 +37,26 @@ constexpr int kNT = 256;
 constexpr int kNW = kNT / 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMostGroup = 128;          // query heads of a kv head
-constexpr int kChunks = 2048;            // workgroups that a launch is cut into, at least
 constexpr int kLeastTiles = 4;           // tiles of a chunk, one for each wave
+// Chunks that the tiles are cut into: four times what the card takes at once, so that the last ones end
+// together; fewer where a kv head has many query heads, whose maxima and sums every item of the second
+// kernel reads of all chunks.  64 sequences of 192000 bf16 tokens, 32 / 8 heads of 128, us with 512, 768,
+// 1024 and 1536: 202, 192, 193, 186; one of 131072: 129, 132, 129, 133; 256 of 500: 131, 131, 131, 143;
+// four of 20000 with 40 / 1 heads: 56, 66, 85, 97.
+constexpr int kMostChunks = 1024, kFewestChunks = 256, kChunkHeads = 8192;
+constexpr int kScoreFloats = 12288;      // scores of a whole sequence in LDS: two workgroups of a CU have room
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef unsigned int u2_t __attribute__((ext_vector_type(2)));
+
+// What a workgroup has: chunk j of k of sequence b, heads block hb of kv head h, and its tokens [t0, t1)
+// of n held ones.  b < 0: nothing.  Chunks are numbered by sequence, then by place; the groups (kv head,
+// heads block) of a chunk are neighbours.
+struct KveItem {
+    int b, h, hb, j, k, n, t0, t1;
+    long first;                 // number of the item of chunk 0 of this group; the next is `groups` on
+};
 
 struct KveDecodeParams {
     KveView c;
@@ -51,10 +65,12 @@ struct KveDecodeParams {
     const int *held;
     float *part_o;              // [item][Rb][D]
     float *part_ml;             // [item][Rb][4]: max, sum, sum of the rounded weights
-    float *scores;              // [B][Hkv][R][tokens] times log2(e), or null: no weights
+    KveItem *items;      // what the first kernel's workgroups had, for the second's
+    float *scores;              // [B][Hkv][tiles][R][tokens of a tile] times log2(e), or null: no weights
     int Hq, R, HB, Rb;          // query heads, of a kv head, blocks of those, heads of a block
-    int most, stride;           // bound on a sequence's tokens; tokens of a row of scores
-    int chunks;                 // chunks that the launch and the partial results have room for
+    int most, stride;           // bound on a sequence's tokens; the same in whole tiles
+    int chunks, target;         // chunks that launch and partial results have room for; that the tiles are cut into
+    int lds_scores;             // floats of scores in LDS
     float scale;                // scale factor x log2(e)
 };
 
@@ -71,13 +87,7 @@ __device__ __forceinline__ int block_sum(int v, int *sh) {
     return s;
 }
 
-// What workgroup blockIdx.x has: chunk j of k of sequence b, heads block hb of kv head h, and its
-// tokens [t0, t1) of n held ones.  b < 0: nothing.  Chunks are numbered by sequence, then by
-// place; the groups (kv head, heads block) of a chunk are neighbours.
-struct KveItem {
-    int b, h, hb, j, k, n, t0, t1;
-    long first;                 // number of the item of chunk 0 of this group; the next is `groups` on
-};
+// The workgroup's item.  The tiles of all sequences are cut into chunks of one size, whatever the lengths are.
 template <int TT>
 __device__ __forceinline__ KveItem kve_item(const KveDecodeParams &p, int *sh) {
     const int groups = p.c.Hkv * p.HB, B = p.c.B, tid = threadIdx.x;
@@ -88,7 +98,7 @@ __device__ __forceinline__ KveItem kve_item(const KveDecodeParams &p, int *sh) {
     int mine = 0;
     for (int b = tid; b < B; b += kNT) mine += tiles(b);
     const long total = block_sum(mine, sh);
-    const long size = max((long)kLeastTiles, (total * groups + kChunks - 1) / kChunks);
+    const long size = max((long)kLeastTiles, (total * groups + p.target - 1) / p.target);
     long before = 0;
     KveItem it{-1, 0, 0, 0, 0, 0, 0, 0, 0};
     for (int b0 = 0; b0 < B; b0 += kNT) {
@@ -187,9 +197,9 @@ struct Tile {                                   // bf16, fp16: 32 tokens
     static __device__ __forceinline__ int value_block(int c) { return c >> 1; }
     __device__ __forceinline__ void load_k(const T *rows, int i, int c) {           // row of slot 0 of key_block
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int j = 0; j < NK; ++j)              // in the order of the products
 #pragma unroll
-            for (int j = 0; j < NK; ++j)
+            for (int u = 0; u < 2; ++u)
                 k[u][j] = *reinterpret_cast<const V8 *>(rows + (key(i, u) & 15) * D + j * 32 + c * 8);
     }
     __device__ __forceinline__ void load_v(const T *rows, int i, int c) {
@@ -216,14 +226,13 @@ struct Tile {                                   // bf16, fp16: 32 tokens
     }
     // scores of the lane's tokens with 16 columns of queries
     __device__ __forceinline__ void scores(const V8 (&q)[NK], float (&s)[E]) const {
+        f4_t a[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f4_t a = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NK; ++j)
 #pragma unroll
-            for (int j = 0; j < NK; ++j) a = Half<T>::mma(k[u][j], q[j], a);
+            for (int u = 0; u < 2; ++u) a[u] = Half<T>::mma(k[u][j], q[j], a[u]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[u * 4 + r] = a[r];
-        }
+        for (int r = 0; r < 4; ++r) s[r] = a[0][r], s[4 + r] = a[1][r];
     }
     // eight tokens of one dimension: dimension d of the lane's in half n
     __device__ __forceinline__ V8 column(int n, int d) const {
@@ -257,13 +266,13 @@ struct Tile {                                   // bf16, fp16: 32 tokens
 #pragma unroll
         for (int j = 0; j < NK; ++j) f[j] = *reinterpret_cast<const V8 *>(q + j * 32 + c * 8);
     }
-    // dimension of row 4 c + r of the value product's block a
-    static __device__ __forceinline__ int dim(int a, int c, int r) { return a / DL * 128 + (c * 4 + r) * DL + a % DL; }
+    // Row 4 c + r of the value product's block a is dimension dim(a / DL, c, r) + a % DL.
+    static __device__ __forceinline__ int dim(int n, int c, int r) { return n * 128 + (c * 4 + r) * DL; }
 };
 
 template <int D>
 struct Tile<float, D> {                         // 16 tokens
-    static constexpr int TT = 16, E = 4, NK = D / 16, NV = D / 64;
+    static constexpr int TT = 16, E = 4, NK = D / 16, NV = D / 64, DL = 4;
     typedef f4_t V8;
     f4_t k[NK], v[E][NV];
     static __device__ __forceinline__ int key_block(int) { return 0; }
@@ -317,8 +326,46 @@ struct Tile<float, D> {                         // 16 tokens
 #pragma unroll
         for (int j = 0; j < NK; ++j) f[j] = *reinterpret_cast<const f4_t *>(q + j * 16 + c * 4);
     }
-    static __device__ __forceinline__ int dim(int a, int c, int r) { return a / 4 * 64 + (c * 4 + r) * 4 + a % 4; }
+    static __device__ __forceinline__ int dim(int n, int c, int r) { return n * 64 + (c * 4 + r) * 4; }
 };
+
+// Adds to the weights of the item's tokens [t0, t1) of their kv head: the sum over its query heads of 2^(score -
+// most(head)) inv(head).  scores: tiles [R][TT] from token 0 on.  A thread has kTokens tokens under way at a
+// time: each needs its block table entry before its weight.
+template <int TT, typename S, typename M, typename I>
+__device__ __forceinline__ void add_weights(const KveDecodeParams &p, const KveItem &it, int t0, int t1, S scores, M most,
+                                            I inv) {
+    constexpr int kTokens = 4;
+    const long hrow = (long)it.h << p.c.pshift;
+    for (int first = t0 + (int)threadIdx.x; first < t1; first += kTokens * kNT) {
+        long row[kTokens];
+        float weight[kTokens], sum[kTokens];
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) {
+            const int t = first + i * kNT;
+            row[i] = kve_row(p.c, it.b, min(t, t1 - 1));
+            if (t >= t1) row[i] = -1;
+            sum[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i) weight[i] = row[i] < 0 ? 0.f : p.c.w[row[i] + hrow];
+#pragma unroll 2
+        for (int r = 0; r < p.R; ++r) {
+            float s[kTokens];
+#pragma unroll
+            for (int i = 0; i < kTokens; ++i) {
+                const int t = min(first + i * kNT, t1 - 1);
+                s[i] = scores[(long)(t / TT) * (p.R * TT) + r * TT + t % TT];
+            }
+            const float m = most(r), f = inv(r);
+#pragma unroll
+            for (int i = 0; i < kTokens; ++i) sum[i] += exp2f(s[i] - m) * f;
+        }
+#pragma unroll
+        for (int i = 0; i < kTokens; ++i)
+            if (row[i] >= 0) p.c.w[row[i] + hrow] = weight[i] + sum[i];
+    }
+}
 }  // namespace
 
 // NT: blocks of 16 query heads that share a pass over the chunk.
@@ -330,9 +377,17 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
     __shared__ int ish[kItemInts];
     __shared__ float ml[kNW][NT * 16][3];
     __shared__ float buf[kNW / 2][NT * NA * 4][64];
+    extern __shared__ float lds_scores[];
     const KveItem it = kve_item<TT>(p, ish);
+    // a whole sequence is done here, unless its weights take other workgroups' heads too
+    const bool alone = it.k == 1 && (!p.scores || p.HB == 1);
+    if (threadIdx.x == 0) {
+        KveItem left = it;
+        if (alone) left.b = -1;
+        p.items[blockIdx.x] = left;
+    }
     if (it.b < 0) return;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, i = lane & 15, c = lane >> 4;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, c = lane >> 4;
     const int head0 = it.hb * p.Rb, heads = min(p.Rb, p.R - head0);     // of the kv head
     typename Tl::V8 q[NT][Tl::NK] = {};
 #pragma unroll
@@ -347,69 +402,107 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
 #pragma unroll
         for (int a = 0; a < NA; ++a) o[t][a] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
-    // block table entries of the lane's key and value rows, a tile ahead of their use
+    // Keys are loaded a tile ahead, into the registers of those that the scores are done with, values
+    // as soon as their product is.  Loads come back in order, so the block table entries that the next
+    // ones' addresses need are asked for before them, two tiles ahead: behind them, they would be there
+    // only when all that was asked for before is (4.6 TB/s, where the pages can be read at 6).  For the
+    // same reason no load of the loop hangs on a condition, under which the compiler would not know how
+    // many to wait for: past its last tile a wave loads that one again, from the cache.
     const int *bt = p.c.bt + (long)it.b * p.c.max_pages;
     const int pmask = (1 << p.c.pshift) - 1, kb = Tl::key_block(i) * 16, vb = Tl::value_block(c) * 16;
     auto entry = [&](int t) { return bt[min(t >> p.c.pshift, p.c.max_pages - 1)]; };
-    int t = it.t0 + wv * TT;
-    int kp = 0, vp = 0;
-    if (t < it.t1) kp = entry(t + kb), vp = entry(t + vb);
-    for (; t < it.t1; t += kNW * TT) {
-        const bool kin = kp >= 0 && kp < p.c.num_pages, vin = vp >= 0 && vp < p.c.num_pages;
-        auto row = [&](int page, bool in, int t) {
-            return ((((long)(in ? page : 0) * p.c.Hkv) + it.h) << p.c.pshift) + (t & pmask);
-        };
-        Tl tl;
-        tl.load_k(reinterpret_cast<const T *>(p.c.k) + row(kp, kin, t + kb) * D, i, c);
-        tl.load_v(reinterpret_cast<const T *>(p.c.v) + row(vp, vin, t + vb) * D, i, c);
-        const int left = it.n - t - c * E;        // tokens from the lane's first one on
-        const int next = t + kNW * TT;
-        if (next < it.t1) kp = entry(next + kb), vp = entry(next + vb);
-        const bool whole = __all(vin && left >= E);
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (!vin || e >= left) tl.clear_value(e);
-        }
-        float w[NT][E];
+    auto mapped = [&](int page) { return page >= 0 && page < p.c.num_pages; };
+    auto row = [&](int page, int t) {
+        return ((((long)(mapped(page) ? page : 0) * p.c.Hkv) + it.h) << p.c.pshift) + (t & pmask);
+    };
+    Tl tl;
+    auto load_k = [&](int page, int t) {
+        tl.load_k(reinterpret_cast<const T *>(p.c.k) + row(page, t + kb) * D, i, c);
+    };
+    auto load_v = [&](int page, int t) {
+        tl.load_v(reinterpret_cast<const T *>(p.c.v) + row(page, t + vb) * D, i, c);
+    };
+    // A tile's scores, [R][tokens]: of a whole sequence in LDS, as far as they find room.
+    float *scores = p.scores + ((long)it.b * p.c.Hkv + it.h) * p.R * p.stride;
+    auto store = [&](float *tile, const float (&raw)[NT][E]) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-            float s[E], most = -FLT_MAX;          // not -inf: some token is there, if all score that
-            tl.scores(q[b], s);
+            if (b * 16 + i >= heads) continue;
+            float *to = tile + (head0 + b * 16 + i) * TT + c * E;
 #pragma unroll
-            for (int e = 0; e < E; ++e) s[e] *= p.scale;
-            if (p.scores && b * 16 + i < heads) {
-                float *to = p.scores + (((long)it.b * p.c.Hkv + it.h) * p.R + head0 + b * 16 + i) * p.stride + t + c * E;
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<f4_t *>(to + e) = f4_t{raw[b][e], raw[b][e + 1], raw[b][e + 2], raw[b][e + 3]};
+        }
+    };
+    constexpr int kStep = kNW * TT;
+    int t = it.t0 + wv * TT;
+    int vp = 0, kp1 = 0, vp1 = 0;                 // of the tile's values, and of the next one's keys and values
+    if (t < it.t1) {                              // and the loop with it, which no other way leads into
+        const int kp = entry(t + kb);
+        vp = entry(t + vb);
+        const int next = t + kStep < it.t1 ? t + kStep : t;
+        kp1 = entry(next + kb), vp1 = entry(next + vb);
+        load_k(kp, t);
+        __builtin_amdgcn_sched_barrier(0);        // in this order, as in the loop
+        load_v(vp, t);
+        do {
+            const int next = t + kStep < it.t1 ? t + kStep : t, next2 = next + kStep < it.t1 ? next + kStep : next;
+            const int kp2 = entry(next2 + kb), vp2 = entry(next2 + vb);
+            __builtin_amdgcn_sched_barrier(0);        // no later
+            const bool vin = mapped(vp);
+            const int left = it.n - t - c * E;        // tokens from the lane's first one on
+            const bool whole = __all(vin && left >= E);
+            float w[NT][E];
 #pragma unroll
-                for (int e = 0; e < E; e += 4) *reinterpret_cast<f4_t *>(to + e) = f4_t{s[e], s[e + 1], s[e + 2], s[e + 3]};
-            }
-            if (whole) {
+            for (int b = 0; b < NT; ++b) tl.scores(q[b], w[b]);
+            load_k(kp1, next);
+            float raw[NT][E];
 #pragma unroll
-                for (int e = 0; e < E; ++e) most = fmaxf(most, s[e]);
-            } else {
-                if (!vin || left <= 0) most = -INFINITY;
+            for (int b = 0; b < NT; ++b) {
+                float (&s)[E] = w[b], most = -FLT_MAX;   // not -inf: some token is there, if all score that
+#pragma unroll
+                for (int e = 0; e < E; ++e) raw[b][e] = s[e] *= p.scale;
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) most = fmaxf(most, s[e]);
+                } else {
+                    if (!vin || left <= 0) most = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if (!vin || e >= left) s[e] = -INFINITY;
+                        most = fmaxf(most, s[e]);
+                    }
+                }
+                if (__any(most > m[b])) {
+                    most = fmaxf(m[b], column_max(most));
+                    const float f = most == -INFINITY ? 1.f : exp2f(m[b] - most);
+                    m[b] = most;
+                    l[b] *= f, lr[b] *= f;
+#pragma unroll
+                    for (int a = 0; a < NA; ++a) o[b][a] *= f;
+                }
+                const float base = m[b] == -INFINITY ? 0.f : m[b];
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    if (!vin || e >= left) s[e] = -INFINITY;
-                    most = fmaxf(most, s[e]);
+                    s[e] = __builtin_amdgcn_exp2f(s[e] - base);
+                    l[b] += s[e];
                 }
             }
-            if (__any(most > m[b])) {
-                most = fmaxf(m[b], column_max(most));
-                const float f = most == -INFINITY ? 1.f : exp2f(m[b] - most);
-                m[b] = most;
-                l[b] *= f, lr[b] *= f;
+            if (!whole) {
 #pragma unroll
-                for (int a = 0; a < NA; ++a) o[b][a] *= f;
+                for (int e = 0; e < E; ++e)
+                    if (!vin || e >= left) tl.clear_value(e);
             }
-            const float base = m[b] == -INFINITY ? 0.f : m[b];
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                w[b][e] = __builtin_amdgcn_exp2f(s[e] - base);
-                l[b] += w[b][e];
+            tl.template values<NT>(w, o, lr);
+            load_v(vp1, next);
+            if (p.scores) {
+                const long tile = (long)t * p.R;
+                if (alone && tile + p.R * TT <= p.lds_scores) store(lds_scores + tile, raw);
+                else store(scores + tile, raw);
             }
-        }
-        tl.template values<NT>(w, o, lr);
+            vp = vp1, kp1 = kp2, vp1 = vp2;
+            t += kStep;
+        } while (t < it.t1);
     }
     // the four waves' (max, sums, out) joined: 2 into 0 and 3 into 1, then 1 into 0
 #pragma unroll
@@ -459,51 +552,80 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
     __syncthreads();
     if (wv == 1) give(buf[0]);
     __syncthreads();
-    if (wv) return;
-    take(buf[0]);
-    const long item = blockIdx.x;
+    if (wv == 0) {
+        take(buf[0]);
 #pragma unroll
-    for (int b = 0; b < NT; ++b) {
-        const int head = b * 16 + i;
-        if (head >= heads) continue;
-        float *to = p.part_o + (item * p.Rb + head) * D;
+        for (int b = 0; b < NT; ++b) {
+            const int head = b * 16 + i;
+            if (head >= heads) continue;
+            if (alone) {
+                // no tokens: 0; tokens that all score -inf: 0 / 0
+                T *to = static_cast<T *>(p.out) + ((size_t)it.b * p.Hq + it.h * p.R + head0 + head) * D;
 #pragma unroll
-        for (int a = 0; a < NA; ++a)
+                for (int n = 0; n < NA / Tl::DL; ++n)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) to[Tl::dim(a, c, r)] = o[b][a][r];
-        if (c == 0) *reinterpret_cast<f4_t *>(p.part_ml + (item * p.Rb + head) * 4) = f4_t{m[b], l[b], lr[b], 0.f};
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int d = 0; d < Tl::DL; ++d)
+                            store_act(to, Tl::dim(n, c, r) + d, m[b] == -INFINITY ? 0.f : o[b][n * Tl::DL + d][r] / lr[b]);
+                if (c == 0) ml[0][head][0] = m[b], ml[0][head][1] = 1.f / l[b];
+            } else {
+                const long at = (long)blockIdx.x * p.Rb + head;
+                float *to = p.part_o + at * D;
+#pragma unroll
+                for (int n = 0; n < NA / Tl::DL; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int d = 0; d < Tl::DL; ++d) to[Tl::dim(n, c, r) + d] = o[b][n * Tl::DL + d][r];
+                if (c == 0) *reinterpret_cast<f4_t *>(p.part_ml + at * 4) = f4_t{m[b], l[b], lr[b], 0.f};
+            }
+        }
     }
+    if (!alone || !p.scores) return;
+    __syncthreads();
+    const int here = p.lds_scores / (p.R * TT) * TT;       // tokens whose scores are in LDS
+    add_weights<TT>(p, it, 0, min(it.n, here), lds_scores, [&](int r) { return ml[0][r][0]; }, [&](int r) { return ml[0][r][1]; });
+    add_weights<TT>(p, it, here, it.n, scores, [&](int r) { return ml[0][r][0]; }, [&](int r) { return ml[0][r][1]; });
 }
 
-// The chunks of a sequence joined, and its weights: workgroup = item, as in the first kernel.
-// Its share of the output is every k-th part of the group's, summed over all chunks; its share
-// of the weights the tokens of its own chunk, over all query heads of the kv head (the first
-// heads block's item does it).
+// The chunks of a sequence joined, and its weights: workgroup = item of the first kernel.  Its share
+// of the output is every k-th part of the group's, summed over all chunks; its share of the weights
+// the tokens of its own chunk, over all query heads of the kv head (the first heads block's item does
+// it).
 template <typename T, int D, int TT>
 __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
-    __shared__ int ish[kItemInts];
     __shared__ float most[kMostGroup], inv[kMostGroup], rounded[kMostGroup];
-    const KveItem it = kve_item<TT>(p, ish);
+    const KveItem it = p.items[blockIdx.x];
     if (it.b < 0) return;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, groups = p.c.Hkv * p.HB;
+    const int tid = threadIdx.x, groups = p.c.Hkv * p.HB;
     const bool counts = p.scores && it.hb == 0;
-    // maxima and sums of the heads that this item needs: its own block's, or all of the kv head
+    // maxima and sums of the heads that this item needs: its own block's, or all of the kv head; `each`
+    // lanes for a head, as many heads at once as the workgroup has
     const int h0 = counts ? 0 : it.hb * p.Rb, h1 = counts ? p.R : min(p.R, h0 + p.Rb);
-    for (int r = h0 + wv; r < h1; r += kNW) {
-        const long first = it.first + r / p.Rb - it.hb;
-        const float *of = p.part_ml + (first * p.Rb + r % p.Rb) * 4;
+    int each = 64;
+    while (each > 4 && each * (h1 - h0) > kNT) each /= 2;
+    for (int r0 = h0; r0 < h1; r0 += kNT / each) {
+        const int r = min(r0 + tid / each, h1 - 1), sub = tid % each;
+        const float *of = p.part_ml + ((it.first + r / p.Rb - it.hb) * p.Rb + r % p.Rb) * 4;
         const long step = (long)groups * p.Rb * 4;
         float m = -INFINITY, l = 0.f, lr = 0.f;
-        for (int j = lane; j < it.k; j += 64) m = fmaxf(m, of[j * step]);
-        m = wave_max_f(m);
-        for (int j = lane; j < it.k; j += 64) {
+#pragma unroll 4
+        for (int j = sub; j < it.k; j += each) {
             const f4_t x = *reinterpret_cast<const f4_t *>(of + j * step);
-            const float f = x[0] == -INFINITY ? 0.f : exp2f(x[0] - m);
-            l += x[1] * f;
-            lr += x[2] * f;
+            const float to = fmaxf(m, x[0]), f = m == -INFINITY ? 0.f : exp2f(m - to), g = x[0] == -INFINITY ? 0.f : exp2f(x[0] - to);
+            l = l * f + x[1] * g;
+            lr = lr * f + x[2] * g;
+            m = to;
         }
-        l = wave_sum_f(l), lr = wave_sum_f(lr);
-        if (lane == 0) most[r] = m, inv[r] = 1.f / l, rounded[r] = lr;
+        for (int o = 1; o < each; o *= 2) {
+            const float xm = __shfl_xor(m, o), xl = __shfl_xor(l, o), xr = __shfl_xor(lr, o);
+            const float to = fmaxf(m, xm), f = m == -INFINITY ? 0.f : exp2f(m - to), g = xm == -INFINITY ? 0.f : exp2f(xm - to);
+            l = l * f + xl * g;
+            lr = lr * f + xr * g;
+            m = to;
+        }
+        if (sub == 0) most[r] = m, inv[r] = 1.f / l, rounded[r] = lr;
     }
     __syncthreads();
     // outputs: units of four values, each summed by `lanes` lanes
@@ -511,16 +633,20 @@ __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
     int lanes = 1;
     while (lanes < 64 && lanes < it.k) lanes *= 2;
     const int u0 = (int)((long)units * it.j / it.k), u1 = (int)((long)units * (it.j + 1) / it.k);
-    const int sub = threadIdx.x % lanes;
+    const int sub = tid % lanes;
     for (int u = u0; u < u1; u += kNT / lanes) {           // whole waves stay in it: the sum below is theirs
-        const int mine = u + threadIdx.x / lanes, at = min(mine, u1 - 1), head = at / (D / 4), r = it.hb * p.Rb + head;
+        const int mine = u + tid / lanes, at = min(mine, u1 - 1), head = at / (D / 4), r = it.hb * p.Rb + head;
         const float m = most[r];
         f4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int j = sub; j < it.k; j += lanes) {
-            const long row = (it.first + (long)j * groups) * p.Rb + head;
-            const float mj = p.part_ml[row * 4];
-            if (mj == -INFINITY) continue;
-            sum += *reinterpret_cast<const f4_t *>(p.part_o + row * D + at % (D / 4) * 4) * exp2f(mj - m);
+            const long of = (it.first + (long)j * groups) * p.Rb + head;
+            const float mj = p.part_ml[of * 4];
+            const f4_t x = *reinterpret_cast<const f4_t *>(p.part_o + of * D + at % (D / 4) * 4);
+            const float f = exp2f(mj - m);
+            // a chunk without tokens has zeros, which no infinity or NaN may meet
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += mj == -INFINITY ? 0.f : x[e] * f;
         }
         for (int o = 1; o < lanes; o *= 2)
 #pragma unroll
@@ -533,20 +659,15 @@ __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
         }
     }
     if (!counts) return;
-    const float *s = p.scores + (((long)it.b * p.c.Hkv + it.h) * p.R) * p.stride;
-    for (int t = it.t0 + threadIdx.x; t < it.t1; t += kNT) {
-        const long row = kve_row(p.c, it.b, t);
-        if (row < 0) continue;
-        float sum = 0.f;
-        for (int r = 0; r < p.R; ++r) sum += exp2f(s[(long)r * p.stride + t] - most[r]) * inv[r];
-        p.c.w[row + ((long)it.h << p.c.pshift)] += sum;
-    }
+    const float *scores = p.scores + ((long)it.b * p.c.Hkv + it.h) * p.R * p.stride;
+    add_weights<TT>(p, it, it.t0, it.t1, scores, [&](int r) { return most[r]; }, [&](int r) { return inv[r]; });
 }
 
 namespace {
 struct KvePlan {
-    int R, NT, HB, Rb, TT, most, stride;
-    long chunks, items, o_bytes, ml_bytes, s_bytes;
+    int R, NT, HB, Rb, TT, most, stride, target, lds_scores;
+    long chunks, items, o_bytes, ml_bytes, item_bytes, s_bytes;
+    long bytes() const { return o_bytes + ml_bytes + item_bytes + s_bytes; }
 };
 int kve_plan(const OjasxKVECache *c, const KveView &v, int num_q_heads, int max_held, int count, KvePlan *p) {
     if (num_q_heads <= 0 || num_q_heads % v.Hkv || max_held < 0) {
@@ -565,9 +686,11 @@ int kve_plan(const OjasxKVECache *c, const KveView &v, int num_q_heads, int max_
     p->most = max_held && max_held < v.cap ? max_held : v.cap;
     const long groups = (long)v.Hkv * p->HB, tiles = ((long)p->most + p->TT - 1) / p->TT;
     p->stride = (int)(tiles * p->TT);
-    // the chunks of a kv head: of size tiles * groups / kChunks (all sequences' tiles), one more for each
+    // the chunks of a kv head: of size tiles * groups / target (all sequences' tiles), one more for each
     // sequence, and none smaller than kLeastTiles
-    const long a = kChunks / groups + v.B, b = v.B * ((tiles + kLeastTiles - 1) / kLeastTiles);
+    const int target = kChunkHeads / p->R;
+    p->target = target > kMostChunks ? kMostChunks : target < kFewestChunks ? kFewestChunks : target;
+    const long a = p->target / groups + v.B, b = v.B * ((tiles + kLeastTiles - 1) / kLeastTiles);
     p->chunks = a < b ? a : b;
     p->items = p->chunks * groups;
     if (p->items > 0xffffff || tiles * v.B > 0x7fffffffL) {
@@ -577,23 +700,32 @@ int kve_plan(const OjasxKVECache *c, const KveView &v, int num_q_heads, int max_
     }
     p->o_bytes = p->items * p->Rb * v.D * 4;
     p->ml_bytes = p->items * p->Rb * 16;
+    p->item_bytes = p->items * (long)sizeof(KveItem);
     p->s_bytes = count ? (long)v.B * num_q_heads * p->stride * 4 : 0;
+    // scores in LDS, where most sequences are not cut: no more than the longest has
+    const long all = (long)p->R * p->stride;
+    p->lds_scores = count && groups * v.B >= p->target && p->HB == 1 ? (int)(all < kScoreFloats ? all : kScoreFloats) : 0;
     return OJASX_OK;
 }
 
-template <typename T, int D>
-void decode(const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
+template <typename T, int D, int NT>
+int decode(const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
     const dim3 grid((unsigned)pl.items), block(kNT);
-    constexpr int kNT2 = sizeof(T) == 4 && D == 256 ? 1 : 2;
-    if (pl.NT == 1) OJX_LAUNCH((kve_decode_kernel<T, D, 1>), grid, block, 0, st, p);
-    else OJX_LAUNCH((kve_decode_kernel<T, D, kNT2>), grid, block, 0, st, p);
+    const size_t lds = (size_t)pl.lds_scores * 4;
+    static DynLds granted;
+    if (lds) OJX_HIP(raise_dyn_lds(reinterpret_cast<const void *>(&kve_decode_kernel<T, D, NT>), lds, &granted));
+    OJX_LAUNCH((kve_decode_kernel<T, D, NT>), grid, block, lds, st, p);
     OJX_LAUNCH((kve_join_kernel<T, D, Tile<T, D>::TT>), grid, block, 0, st, p);
+    return OJASX_OK;
+}
+template <typename T, int D>
+int decode(const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
+    constexpr int kNT2 = sizeof(T) == 4 && D == 256 ? 1 : 2;
+    return pl.NT == 1 ? decode<T, D, 1>(pl, st, p) : decode<T, D, kNT2>(pl, st, p);
 }
 template <typename T>
-void decode(int D, const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
-    if (D == 64) decode<T, 64>(pl, st, p);
-    else if (D == 128) decode<T, 128>(pl, st, p);
-    else decode<T, 256>(pl, st, p);
+int decode(int D, const KvePlan &pl, hipStream_t st, const KveDecodeParams &p) {
+    return D == 64 ? decode<T, 64>(pl, st, p) : D == 128 ? decode<T, 128>(pl, st, p) : decode<T, 256>(pl, st, p);
 }
 }  // namespace
 
@@ -607,7 +739,7 @@ OJASX_API long ojasx_kve_decode_workspace(const OjasxKVECache *cache, int num_q_
     KvePlan pl{};
     int rc = kve_view(cache, &v);
     if (!rc) rc = kve_plan(cache, v, num_q_heads, max_held, count, &pl);
-    return rc ? rc : pl.o_bytes + pl.ml_bytes + pl.s_bytes;
+    return rc ? rc : pl.bytes();
 }
 
 OJASX_API int ojasx_kve_decode_device(const OjasxKVECache *cache, const void *q, int num_q_heads, const int *held,
@@ -630,22 +762,23 @@ OJASX_API int ojasx_kve_decode_device(const OjasxKVECache *cache, const void *q,
         return OJASX_ERR_INVALID;
     }
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
-        workspace_bytes < pl.o_bytes + pl.ml_bytes + pl.s_bytes) {
+        workspace_bytes < pl.bytes()) {
         set_error("KV decode: the workspace has to be 16-byte aligned and of %ld bytes, got %ld",
-                  pl.o_bytes + pl.ml_bytes + pl.s_bytes, workspace_bytes);
+                  pl.bytes(), workspace_bytes);
         return OJASX_ERR_INVALID;
     }
     char *ws = static_cast<char *>(workspace);
     p.part_o = reinterpret_cast<float *>(ws);
     p.part_ml = reinterpret_cast<float *>(ws + pl.o_bytes);
     p.scores = count ? reinterpret_cast<float *>(ws + pl.o_bytes + pl.ml_bytes) : nullptr;
+    p.items = reinterpret_cast<KveItem *>(ws + pl.o_bytes + pl.ml_bytes + pl.s_bytes);
     p.q = q, p.out = out, p.held = held;
     p.Hq = num_q_heads, p.R = pl.R, p.HB = pl.HB, p.Rb = pl.Rb, p.most = pl.most, p.stride = pl.stride,
-    p.chunks = (int)pl.chunks;
+    p.chunks = (int)pl.chunks, p.target = pl.target, p.lds_scores = pl.lds_scores;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (p.c.dtype == OJASX_DTYPE_F32) decode<float>(p.c.D, pl, st, p);
-    else if (p.c.dtype == OJASX_DTYPE_BF16) decode<__hip_bfloat16>(p.c.D, pl, st, p);
-    else decode<__half>(p.c.D, pl, st, p);
+    rc = p.c.dtype == OJASX_DTYPE_F32 ? decode<float>(p.c.D, pl, st, p)
+         : p.c.dtype == OJASX_DTYPE_BF16 ? decode<__hip_bfloat16>(p.c.D, pl, st, p) : decode<__half>(p.c.D, pl, st, p);
+    if (rc) return rc;
     OJX_HIP(hipGetLastError());
     return OJASX_OK;
 }
