@@ -10,6 +10,19 @@
 // A token's rank is 32 bits that order like its weight: all ones where it is protected, 1 for a
 // NaN, 0 where no page is mapped.  A workgroup finds the rank of the last kept token byte by byte
 // from counts in LDS, then numbers the places and the tokens for them with wave ballots.
+//
+// One workgroup for a (sequence, head), since every pass of the selection needs all of its ranks and
+// those of 32768 tokens fit LDS.  What is read is small (8 bytes a token and head; of a moved token
+// its rows besides), so the time is that of a chain of steps that wait for each other: block table,
+// positions and weights, four counts, three walks over the ballots.  11-bit digits, in three passes,
+// took as long as four of 8 bits.  Up to kMoveInPlace moves the workgroup does itself, four units of
+// a thread in flight; more are a second launch over the whole card, one unit of a thread in flight
+// (16.8 us against 23.0 for four, for 8 sequences of 8192 that leave 2048).
+//
+// Measured, bf16, 8 heads of 128, the launches without the append: 64 sequences of 2064 tokens that
+// leave 2048: 24 us (1 sequence, 4 heads of fp32: 13 us); 8 sequences of 8192 that leave 2048: 22 us
+// and 17 us for the 131 MB or so of its moves; a sequence of 65536, whose ranks are formed anew in
+// each pass: 307 us.
 #include <climits>
 
 #include "kve.h"
@@ -17,13 +30,18 @@
 namespace ojx {
 
 namespace {
-constexpr int kNT = 1024;
-constexpr int kNW = kNT / 64;
-constexpr int kCopies = 16;              // counters of a digit, so that equal digits of a wave's lanes collide less
+constexpr int kWideNT = 1024, kSlimNT = 256;   // threads of a selecting workgroup
+constexpr int kDigitBits = 8;            // of a rank's 32: four passes
+constexpr int kDigits = 1 << kDigitBits;
+constexpr int kCopies = 8;               // counters of a digit, so that equal digits of a wave's lanes collide less
 constexpr int kRanksInLds = 32768;       // tokens whose ranks are kept (128 KB); of more they are formed again
 constexpr int kMoveInPlace = 256;        // moves that the selecting workgroup does itself
+// Up to this many tokens a workgroup of 256 threads is faster (64 sequences of 416 tokens, 8 heads: 14.3
+// against 17.9 us), from about 2000 on one of 1024 (4 sequences of 4096: 15.2 against 29.8 us).
+constexpr int kSlimTokens = 1024;
+constexpr int kBatch = 4;                // tokens of a thread whose loads are in flight together
 constexpr int kMoveNT = 256;
-constexpr size_t kSelectLds = 256 * kCopies * 4 + 2048;   // static LDS of the selecting kernel, rounded up
+constexpr size_t kSelectLds = kDigits * kCopies * 4 + 4096;   // static LDS of the selecting kernel, rounded up
 
 struct KveEvictParams {
     KveView c;
@@ -33,17 +51,7 @@ struct KveEvictParams {
     int budget, sink, recent, most, most_moves, in_lds;
 };
 
-__device__ __forceinline__ int block_sum(int v, int *sh) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    int s = 0;
-#pragma unroll
-    for (int i = 0; i < kNW; ++i) s += sh[i];
-    return s;
-}
+template <int NT>
 __device__ __forceinline__ int block_max(int v, int *sh) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
@@ -52,118 +60,153 @@ __device__ __forceinline__ int block_max(int v, int *sh) {
     __syncthreads();
     int s = sh[0];
 #pragma unroll
-    for (int i = 1; i < kNW; ++i) s = max(s, sh[i]);
+    for (int i = 1; i < NT / 64; ++i) s = max(s, sh[i]);
     return s;
 }
 
-// Rows `of` of a kv head to rows `to`: 16-byte unit u of the keys' and the values' row together.
-template <int UNITS>
-__device__ __forceinline__ void move_unit(const KveView &c, long to, long of, int u) {
-    char *base = u < UNITS ? c.k : c.v;
-    const int at = (u & (UNITS - 1)) * 16;
-    *reinterpret_cast<u4_t *>(base + to * (UNITS * 16) + at) = *reinterpret_cast<const u4_t *>(base + of * (UNITS * 16) + at);
-}
-// Moves first, first + step, ... of the n of a (sequence, kv head), by the calling threads.
-template <int UNITS>
-__device__ __forceinline__ void move_rows(const KveEvictParams &p, int b, int h, const int *to, const int *of, int n, int thread,
-                                          int threads) {
-    const long hrow = (long)h << p.c.pshift;
-    for (long i = thread; i < (long)n * (2 * UNITS); i += threads) {
-        const int m = (int)(i / (2 * UNITS)), u = (int)(i % (2 * UNITS));
-        const long d = kve_row(p.c, b, to[m]), s = kve_row(p.c, b, of[m]);
-        if (d < 0 || s < 0) continue;
-        move_unit<UNITS>(p.c, d + hrow, s + hrow, u);
-        if (u == 0) p.c.w[d + hrow] = p.c.w[s + hrow];
-        if (u == 1) p.c.pos[d + hrow] = p.c.pos[s + hrow];
+// The moves first, first + threads, ... of the n of a (sequence, kv head): keys, values, weights and
+// positions of the slots of[m] to the slots to[m].  A thread has kUnits 16-byte units under way at a time.
+template <int UNITS, int kUnits, typename L>
+__device__ __forceinline__ void move_rows(const KveEvictParams &p, int b, int h, L to, L of, int n, int thread, int threads) {
+    const long hrow = (long)h << p.c.pshift, all = (long)n * (2 * UNITS);
+    for (long i0 = thread; i0 < all; i0 += (long)kUnits * threads) {
+        long d[kUnits], s[kUnits];
+        u4_t x[kUnits];
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+            const long i = i0 + (long)j * threads;
+            const int m = (int)((i < all ? i : i0) / (2 * UNITS));
+            d[j] = kve_row(p.c, b, to[m]), s[j] = kve_row(p.c, b, of[m]);
+            if (i >= all || d[j] < 0) s[j] = -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+            const int u = (int)((i0 + (long)j * threads) % (2 * UNITS));
+            if (s[j] < 0) continue;
+            x[j] = *reinterpret_cast<const u4_t *>((u < UNITS ? p.c.k : p.c.v) + (s[j] + hrow) * (UNITS * 16) + (u % UNITS) * 16);
+        }
+#pragma unroll
+        for (int j = 0; j < kUnits; ++j) {
+            const int u = (int)((i0 + (long)j * threads) % (2 * UNITS));
+            if (s[j] < 0) continue;
+            *reinterpret_cast<u4_t *>((u < UNITS ? p.c.k : p.c.v) + (d[j] + hrow) * (UNITS * 16) + (u % UNITS) * 16) = x[j];
+            if (u == 0) p.c.w[d[j] + hrow] = p.c.w[s[j] + hrow];
+            if (u == 1) p.c.pos[d[j] + hrow] = p.c.pos[s[j] + hrow];
+        }
     }
 }
 }  // namespace
 
 // Workgroup (kv head, sequence).  UNITS: 16-byte units of a row; MOVES: it moves the rows too.
-template <int UNITS, bool MOVES>
-__global__ __launch_bounds__(kNT) void kve_select_kernel(KveEvictParams p) {
+template <int UNITS, bool MOVES, int NT>
+__global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
+    constexpr int kNT = NT, kNW = NT / 64;
     extern __shared__ uint32_t ranks[];
-    __shared__ int counts[256 * kCopies], total[256], sh[kNW], picked[2];
+    __shared__ int counts[kDigits * kCopies], sh[kNW], sh2[kNW], picked[2], picked_places[kNW], places_of[MOVES ? 2 * kMoveInPlace : 1];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = min(max(p.held[b], 0), p.most);
     int *number = p.counts + (long)b * p.c.Hkv + h;
     if (n <= p.budget) {
-        if (tid == 0) *number = 0;
+        if (!MOVES && tid == 0) *number = 0;
         return;
     }
     const long hrow = (long)h << p.c.pshift;
-    int newest = INT_MIN;
-    for (int t = tid; t < n; t += kNT) {
-        const long row = kve_row(p.c, b, t);
-        if (row >= 0) newest = max(newest, p.c.pos[row + hrow]);
-    }
-    newest = block_max(newest, sh);
-    auto form = [&](int t) -> uint32_t {
-        const long row = kve_row(p.c, b, t);
+    auto rank_of = [&](long row, int pos, float w, int newest) -> uint32_t {
         if (row < 0) return 0;
-        const int pos = p.c.pos[row + hrow];
-        const float w = p.c.w[row + hrow] + 0.f;           // -0: 0
         if (pos < p.sink || (long)pos > (long)newest - p.recent) return 0xffffffffu;
+        w += 0.f;                                // -0: 0
         if (w != w) return 1;
         const uint32_t u = __float_as_uint(w);
         return u & 0x80000000u ? ~u : u | 0x80000000u;
     };
+    // kBatch tokens from t0 on, kNT apart
+    long row[kBatch];
+    int pos[kBatch];
+    float w[kBatch];
+    auto load = [&](int t0, bool weights) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) row[i] = t0 + i * kNT < n ? kve_row(p.c, b, t0 + i * kNT) : -1;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            pos[i] = row[i] < 0 ? INT_MIN : p.c.pos[row[i] + hrow];
+            if (weights) w[i] = row[i] < 0 ? 0.f : p.c.w[row[i] + hrow];
+        }
+    };
+    int newest = INT_MIN;
+    const bool once = n <= kNT * kBatch;         // all tokens at once: they stay in registers
+    for (int t0 = tid; t0 - tid < n; t0 += kNT * kBatch) {
+        load(t0, once);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) newest = max(newest, pos[i]);
+    }
+    for (int i = tid; i < kDigits * kCopies; i += kNT) counts[i] = 0;
+    newest = block_max<NT>(newest, sh);
+    auto form = [&](int t) {
+        const long at = kve_row(p.c, b, t);
+        return at < 0 ? 0u : rank_of(at, p.c.pos[at + hrow], p.c.w[at + hrow], newest);
+    };
     if (p.in_lds)
-        for (int t = tid; t < n; t += kNT) ranks[t] = form(t);
+        for (int t0 = tid; t0 - tid < n; t0 += kNT * kBatch) {
+            if (!once) load(t0, true);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (t0 + i * kNT < n) ranks[t0 + i * kNT] = rank_of(row[i], pos[i], w[i], newest);
+        }
     auto rank = [&](int t) { return p.in_lds ? ranks[t] : form(t); };
     // the rank of the budget-th largest: `above` are larger
     uint32_t last = 0;
     int above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256 * kCopies; i += kNT) counts[i] = 0;
-        __syncthreads();
+    uint32_t high = 0;                           // the bits of `last` that are known
+    for (int shift = 32 - kDigitBits;; shift -= kDigitBits) {
         for (int t = tid; t < n; t += kNT) {
             const uint32_t r = rank(t);
-            if (shift == 24 || (r ^ last) >> (shift + 8) == 0) atomicAdd(&counts[(r >> shift & 255) * kCopies + lane % kCopies], 1);
+            if (((r ^ last) & high) == 0) atomicAdd(&counts[((r & ~high) >> shift) * kCopies + lane % kCopies], 1);
         }
         __syncthreads();
-        if (tid < 256) {
-            int s = 0;
-            for (int i = 0; i < kCopies; ++i) s += counts[tid * kCopies + i];
-            total[tid] = s;
-        }
-        __syncthreads();
-        if (wv == 0) {                           // four digits a lane, the largest first
-            int mine[4], s = 0;
+        // a digit for each of the first threads, the largest first
+        const int d = kDigits - 1 - tid;
+        int c = 0, upto = 0;
+        if (tid < kDigits) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s += mine[i] = total[255 - (lane * 4 + i)];
-            int before = s;
+            for (int i = 0; i < kCopies; ++i) c += counts[d * kCopies + i], counts[d * kCopies + i] = 0;
+            upto = c;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(before, o);
-                if (lane >= o) before += x;
+                const int x = __shfl_up(upto, o);
+                if (lane >= o) upto += x;
             }
-            before += above - s;
+            if (lane == 63) sh2[wv] = upto;
+        }
+        __syncthreads();
+        if (tid < kDigits) {
+            int before = above + upto - c;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (before < p.budget && before + mine[i] >= p.budget) picked[0] = 255 - (lane * 4 + i), picked[1] = before;
-                before += mine[i];
-            }
+            for (int i = 0; i < kDigits / 64; ++i) before += i < wv ? sh2[i] : 0;
+            if (before < p.budget && before + c >= p.budget) picked[0] = d, picked[1] = before;
         }
         __syncthreads();
         last |= (uint32_t)picked[0] << shift;
         above = picked[1];
+        high = 0xffffffffu << shift;
+        if (shift == 0) break;
     }
     const int ties = p.budget - above;           // tokens of rank `last` that stay, the lowest slots
     // wave w has slots [w * span, (w + 1) * span)
     const int span = ((n + kNW - 1) / kNW + 63) & ~63, s0 = min(n, wv * span), s1 = min(n, s0 + span);
-    auto before_waves = [&](int v) {             // sum of v (one value a wave) over the waves before
+    auto before_waves = [&](int v, int *at, int *all) {    // sum of v (one value a wave) over the waves before
+        if (lane == 0) at[wv] = v;
         __syncthreads();
-        if (lane == 0) sh[wv] = v;
-        __syncthreads();
-        int s = 0;
-        for (int i = 0; i < wv; ++i) s += sh[i];
+        int s = 0, t = 0;
+#pragma unroll
+        for (int i = 0; i < kNW; ++i) t += at[i], s += i < wv ? at[i] : 0;
+        *all = t;
         return s;
     };
+    int any;
     int mine = 0;
     for (int t = s0 + lane; t - lane < s1; t += 64) mine += __popcll(__ballot(t < s1 && rank(min(t, n - 1)) == last));
-    const int tie0 = before_waves(mine);
+    const int tie0 = before_waves(mine, sh, &any);
     const unsigned long below = (1ul << lane) - 1;
     auto kept = [&](int t, int &tie) {           // of the wave's 64 slots from t - lane on; tie: ties before them
         const uint32_t r = rank(min(t, n - 1));
@@ -178,9 +221,11 @@ __global__ __launch_bounds__(kNT) void kve_select_kernel(KveEvictParams p) {
         places += __popcll(__ballot(t < s1 && t < p.budget && !keep));
         tokens += __popcll(__ballot(t < s1 && t >= p.budget && keep));
     }
-    int place = before_waves(places), token = before_waves(tokens);
-    const int n_moves = block_sum(lane == 0 ? tokens : 0, sh);
-    int *to = p.moves + ((long)b * p.c.Hkv + h) * 2 * p.most_moves, *of = to + p.most_moves;
+    if (lane == 0) picked_places[wv] = places;
+    int n_moves, place = 0;
+    int token = before_waves(tokens, sh2, &n_moves);
+    for (int i = 0; i < wv; ++i) place += picked_places[i];
+    int *to = MOVES ? places_of : p.moves + ((long)b * p.c.Hkv + h) * 2 * p.most_moves, *of = to + p.most_moves;
     tie = tie0;
     for (int t = s0 + lane; t - lane < s1; t += 64) {
         const bool keep = kept(t, tie);
@@ -190,11 +235,13 @@ __global__ __launch_bounds__(kNT) void kve_select_kernel(KveEvictParams p) {
         place += __popcll(a);
         token += __popcll(c);
     }
-    if (tid == 0) *number = n_moves;
-    if (MOVES) {
-        __syncthreads();
-        move_rows<UNITS>(p, b, h, to, of, min(n_moves, p.most_moves), tid, kNT);
+    if (!MOVES) {
+        if (tid == 0) *number = n_moves;
+        return;
     }
+    __syncthreads();
+    const int *from = places_of;
+    move_rows<UNITS, 4>(p, b, h, from, from + p.most_moves, min(n_moves, p.most_moves), tid, kNT);
 }
 
 // The moves of the selecting launch: workgroup (part, kv head, sequence).
@@ -203,7 +250,7 @@ __global__ __launch_bounds__(kMoveNT) void kve_move_kernel(KveEvictParams p) {
     const int h = blockIdx.y, b = blockIdx.z;
     const long at = (long)b * p.c.Hkv + h;
     const int *to = p.moves + at * 2 * p.most_moves;
-    move_rows<UNITS>(p, b, h, to, to + p.most_moves, min(p.counts[at], p.most_moves), blockIdx.x * kMoveNT + threadIdx.x,
+    move_rows<UNITS, 1>(p, b, h, to, to + p.most_moves, min(p.counts[at], p.most_moves), blockIdx.x * kMoveNT + threadIdx.x,
                      gridDim.x * kMoveNT);
 }
 
@@ -228,20 +275,22 @@ int evict_plan(const KveView &v, int budget, int sink, int recent, int max_held,
     return OJASX_OK;
 }
 
+template <int UNITS, bool MOVES, int NT>
+int select(const KveEvictParams &p, dim3 grid, size_t lds, hipStream_t st) {
+    static DynLds granted;
+    if (lds + kSelectLds > 65536)
+        OJX_HIP(raise_dyn_lds(reinterpret_cast<const void *>(&kve_select_kernel<UNITS, MOVES, NT>), lds, &granted));
+    OJX_LAUNCH((kve_select_kernel<UNITS, MOVES, NT>), grid, dim3(NT), lds, st, p);
+    return OJASX_OK;
+}
 template <int UNITS>
 int evict(const KveEvictParams &p, hipStream_t st) {
     const dim3 grid(p.c.Hkv, p.c.B);
     const size_t lds = p.in_lds ? round_up((size_t)p.most * 4, 16) : 0;
-    const bool wide = lds + kSelectLds > 65536;
-    if (p.most_moves <= kMoveInPlace) {
-        static DynLds granted;
-        if (wide) OJX_HIP(raise_dyn_lds(reinterpret_cast<const void *>(&kve_select_kernel<UNITS, true>), lds, &granted));
-        OJX_LAUNCH((kve_select_kernel<UNITS, true>), grid, dim3(kNT), lds, st, p);
-        return OJASX_OK;
-    }
-    static DynLds granted;
-    if (wide) OJX_HIP(raise_dyn_lds(reinterpret_cast<const void *>(&kve_select_kernel<UNITS, false>), lds, &granted));
-    OJX_LAUNCH((kve_select_kernel<UNITS, false>), grid, dim3(kNT), lds, st, p);
+    const bool slim = p.most <= kSlimTokens;
+    if (p.most_moves <= kMoveInPlace) return slim ? select<UNITS, true, kSlimNT>(p, grid, lds, st) : select<UNITS, true, kWideNT>(p, grid, lds, st);
+    const int rc = slim ? select<UNITS, false, kSlimNT>(p, grid, lds, st) : select<UNITS, false, kWideNT>(p, grid, lds, st);
+    if (rc) return rc;
     // parts of a (sequence, kv head): 8 moves or more each, no more than four times what fills the card
     const long pairs = (long)p.c.B * p.c.Hkv, wanted = (p.most_moves + 7) / 8, fill = (4096 + pairs - 1) / pairs;
     OJX_LAUNCH((kve_move_kernel<UNITS>), dim3((unsigned)(wanted < fill ? wanted : fill), p.c.Hkv, p.c.B), dim3(kMoveNT), 0, st, p);
