@@ -595,6 +595,15 @@ OJASX_API int ojasx_decoder_reset(OjasxDecoderHandle handle, int position);
  * graph per token (captured on the first such call).  Synchronous. */
 OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token, int num_tokens,
                                      int use_graph, int *tokens_out, float *last_logits);
+/* The same with every token drawn from its logits, as ojasx_sample_device does:
+ * token i with uniform[i] (host, num_tokens numbers in [0, 1)).  tokens_out
+ * has -1 where the logits are no distribution; the step after such a one starts
+ * from token 0.  Settings and numbers may differ from call to call with one
+ * captured graph.  vocab at most 2^22. */
+OJASX_API int ojasx_decoder_generate_sampled(OjasxDecoderHandle handle, int first_token, int num_tokens,
+                                             int use_graph, const float *uniform, float temperature,
+                                             int top_k, float top_p, float min_p, int *tokens_out,
+                                             float *last_logits);
 /* Host copy of one layer's KV cache rows for tokens [first_token,
  * first_token + num_tokens), first_token a multiple of page_size: codes
  * [pages][kv_heads][page_size][8], scales [pages][kv_heads][page_size]. */

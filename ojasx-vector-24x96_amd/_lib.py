@@ -71,6 +71,7 @@ SIGNATURES = {
     "ojasx_decoder_set_context": (ci, [vp, ci, vp, vp, vp, vp, ci]),
     "ojasx_decoder_reset": (ci, [vp, ci]),
     "ojasx_decoder_generate": (ci, [vp, ci, ci, ci, vp, vp]),
+    "ojasx_decoder_generate_sampled": (ci, [vp, ci, ci, ci, vp, cf, ci, cf, cf, vp, vp]),
     "ojasx_decoder_read_kv": (ci, [vp, ci, ci, ci, vp, vp, vp, vp]),
     "ojasx_linear_forward_fused_device": (ci, [vp, vp, vp, ci, vp, cf, vp, vp]),
     "ojasx_attention_stream_init_device": (ci, [vp, vp, ci, ci, ci, vp]),

@@ -1,6 +1,6 @@
 // decoder.hip -- a Qwen3-4B-shaped decoder whose every linear layer is a
 // split-manifold LUT linear (d = 16, 256 centroids, CSR outliers) and whose
-// KV cache is the paged code-domain cache, greedy batch-1 decode on gfx950.
+// KV cache is the paged code-domain cache, batch-1 decode, greedy or sampled, on gfx950.
 //
 // One token step, all state on the device (position, step, token), so the
 // step is a fixed launch sequence that a HIP graph replays:
@@ -17,7 +17,8 @@
 //     5. x   += LUT(Wdown, h)                          residual epilogue
 //   head: logits = LUT(Wlm, RMSNorm(x, w_final)); argmax_embed_kernel picks the
 //   token (ties to the lower id), stores it, loads its embedding row into x
-//   and advances the position.
+//   and advances the position.  Sampled generation draws it with the kernels of
+//   sample.hip instead, and drawn_embed_kernel does the rest.
 // RMSNorm is x * (1 / sqrt(mean(x^2) + eps)) * w; RoPE rotates dimension i
 // with i + hd/2 by the angle fp32(pos) * inv_freq[i], inv_freq[i] =
 // fp32(1 / theta^(2i / hd)), through cos / sin tables computed on the host.
@@ -27,6 +28,7 @@
 #include <vector>
 
 #include "common.h"
+#include "sample.h"
 
 namespace ojx {
 
@@ -466,6 +468,29 @@ __global__ __launch_bounds__(kArgNT) void embed_kernel(const float *emb, int hid
     for (int d = threadIdx.x; d < hidden; d += kArgNT) x[d] = emb[(size_t)tok * hidden + d];
 }
 
+// The drawn token's embedding row into x and its record, as argmax_embed_kernel's: -1 (the
+// logits are no distribution) is recorded, and the step after it starts from token 0.
+__global__ __launch_bounds__(kArgNT) void drawn_embed_kernel(const int *drawn, const float *emb, int hidden,
+                                                            float *x, int *state, int *tokens, int max_steps) {
+    const int tok = max(*drawn, 0), step = state[1];
+    for (int d = threadIdx.x; d < hidden; d += kArgNT) x[d] = emb[(size_t)tok * hidden + d];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if (step >= 0 && step < max_steps) tokens[step] = *drawn;
+        state[0] += 1;
+        state[1] = step + 1;
+        state[2] = tok;
+    }
+}
+
+// What a sampled step reads besides the decoder's state: one row's settings, in device memory so
+// that a captured step follows them, the token drawn last, and after it the steps' random numbers.
+struct DrawInput {
+    float temperature, top_p, min_p;
+    int top_k;
+    int drawn, pad[3];
+};
+
 struct DecoderLayer {
     void *qkv = nullptr, *o = nullptr, *gu = nullptr, *down = nullptr;   // Linear handles (not owned)
     DevBuf in_norm, post_norm, q_norm, k_norm, kcb, vcb, kc, ks, vc, vs;
@@ -478,20 +503,23 @@ struct Decoder {
     std::vector<DecoderLayer> L;
     void *lm = nullptr;
     DevBuf final_norm, emb, cos_t, sin_t, bt, x, qkv, attn, gu, logits, arg_part, part_o, part_ml,
-        state, tokens;
+        state, tokens, draw, draw_ws;       // draw: DrawInput, max_steps random numbers
     hipStream_t stream = nullptr;
-    hipGraph_t graph = nullptr;
-    hipGraphExec_t exec = nullptr;
+    // a greedy step, a sampled one
+    hipGraph_t graph[2] = {nullptr, nullptr};
+    hipGraphExec_t exec[2] = {nullptr, nullptr};
     bool ready_layers = false, ready_head = false;
 
     // The captured step holds the device pointers of every linear handle and
     // buffer it launched on; replacing a handle makes it stale, so the next
     // generate with use_graph captures again.
     void drop_graph() {
-        if (exec) (void)hipGraphExecDestroy(exec);
-        if (graph) (void)hipGraphDestroy(graph);
-        exec = nullptr;
-        graph = nullptr;
+        for (int i = 0; i < 2; ++i) {
+            if (exec[i]) (void)hipGraphExecDestroy(exec[i]);
+            if (graph[i]) (void)hipGraphDestroy(graph[i]);
+            exec[i] = nullptr;
+            graph[i] = nullptr;
+        }
     }
 
     ~Decoder() {
@@ -502,14 +530,31 @@ struct Decoder {
                               &l.ks, &l.vc, &l.vs})
                 b->release();
         for (DevBuf *b : {&final_norm, &emb, &cos_t, &sin_t, &bt, &x, &qkv, &attn, &gu, &logits,
-                          &arg_part, &part_o, &part_ml, &state, &tokens})
+                          &arg_part, &part_o, &part_ml, &state, &tokens, &draw, &draw_ws})
             b->release();
     }
 
     int n_chunks() const { return (max_ctx + kAttnC - 1) / kAttnC; }
 
+    // The token after the logits, drawn, on `st`.
+    int draw_token(hipStream_t st) {
+        DrawInput *in = draw.as<DrawInput>();
+        SampleParams a{};
+        a.logits = logits.ptr, a.stride = vocab, a.rows = 1, a.vocab = vocab;
+        a.uniform = reinterpret_cast<float *>(in + 1), a.step = state.as<int>() + 1;
+        a.tokens = &in->drawn;
+        a.temperatures = &in->temperature, a.top_ps = &in->top_p, a.min_ps = &in->min_p;
+        a.top_ks = &in->top_k;
+        const int rc = launch_sample(a, OJASX_DTYPE_F32, draw_ws.ptr, st);
+        if (rc) return rc;
+        OJX_LAUNCH(drawn_embed_kernel, dim3(1), dim3(kArgNT), 0, st, &in->drawn, emb.as<float>(), hidden,
+                   x.as<float>(), state.as<int>(), tokens.as<int>(), max_steps);
+        OJX_HIP(hipGetLastError());
+        return OJASX_OK;
+    }
+
     // One token step on `st` (device-resident position and token).
-    int step(hipStream_t st) {
+    int step(hipStream_t st, bool sampled) {
         int rc;
         const int *pos = state.as<int>();
         const float sf = 1.0f / sqrtf((float)kHd);
@@ -544,6 +589,7 @@ struct Decoder {
         rc = linear_forward_lm_head(lm, x.as<float>(), logits.as<float>(), final_norm.as<float>(),
                                     eps, arg_part.as<float2>(), &n_part, st);
         if (rc) return rc;
+        if (sampled) return draw_token(st);
         OJX_LAUNCH(argmax_embed_kernel, dim3(1), dim3(kArgNT), 0, st, logits.as<float>(), vocab,
                    arg_part.as<float2>(), n_part, emb.as<float>(), hidden, x.as<float>(),
                    state.as<int>(), tokens.as<int>(), max_steps);
@@ -755,8 +801,13 @@ OJASX_API int ojasx_decoder_reset(OjasxDecoderHandle handle, int position) {
     return OJASX_OK;
 }
 
-OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token, int num_tokens,
-                                     int use_graph, int *tokens_out, float *last_logits) {
+// num_tokens steps from first_token; sampled: with the settings and numbers given, else greedily.
+struct DrawSettings {
+    ojx::DrawInput in;
+    const float *uniform;
+};
+static int generate(OjasxDecoderHandle handle, int first_token, int num_tokens, int use_graph,
+                    const DrawSettings *draw, int *tokens_out, float *last_logits) {
     using namespace ojx;
     if (!handle || !tokens_out) return OJASX_ERR_NULL;
     Decoder *d = static_cast<Decoder *>(handle);
@@ -770,6 +821,19 @@ OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token,
                   first_token);
         return OJASX_ERR_INVALID;
     }
+    const bool sampled = draw != nullptr;
+    long ws = 0;
+    if (sampled) {
+        int rc = check_sampling(draw->in.temperature, draw->in.top_p, draw->in.min_p);
+        if (rc) return rc;
+        for (int i = 0; i < num_tokens; ++i)
+            if (!(draw->uniform[i] >= 0.f && draw->uniform[i] < 1.f)) {
+                set_error("decoder: uniform[%d] is %g, outside [0, 1)", i, draw->uniform[i]);
+                return OJASX_ERR_INVALID;
+            }
+        ws = sample_workspace(1, d->vocab);
+        if (ws < 0) return (int)ws;
+    }
     hipStream_t st = d->stream;
     int state[3];
     OJX_HIP(hipStreamSynchronize(st));
@@ -779,6 +843,15 @@ OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token,
                   d->max_ctx);
         return OJASX_ERR_INVALID;
     }
+    if (sampled) {
+        // of one size for the decoder's life: a captured step holds the addresses
+        int rc = d->draw.ensure(sizeof(DrawInput) + (size_t)d->max_steps * 4);
+        if (!rc) rc = d->draw_ws.ensure((size_t)ws);
+        if (rc) return rc;
+        OJX_HIP(hipMemcpy(d->draw.ptr, &draw->in, sizeof(DrawInput), hipMemcpyHostToDevice));
+        OJX_HIP(hipMemcpy(d->draw.as<DrawInput>() + 1, draw->uniform, (size_t)num_tokens * 4,
+                          hipMemcpyHostToDevice));
+    }
     state[1] = 0;
     state[2] = first_token;
     OJX_HIP(hipMemcpy(d->state.ptr, state, sizeof(state), hipMemcpyHostToDevice));
@@ -786,10 +859,10 @@ OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token,
                d->state.as<int>(), d->x.as<float>());
     int rc = OJASX_OK;
     int done = 0;
-    if (use_graph && !d->exec) {
+    if (use_graph && !d->exec[sampled]) {
         // One eager step first: it sets every kernel attribute, so capture
         // records launches only.
-        rc = d->step(st);
+        rc = d->step(st, sampled);
         if (rc) return rc;
         done = 1;
         if (timing_on()) {
@@ -797,7 +870,7 @@ OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token,
             return OJASX_ERR_INVALID;
         }
         OJX_HIP(hipStreamBeginCapture(st, hipStreamCaptureModeThreadLocal));
-        rc = d->step(st);
+        rc = d->step(st, sampled);
         hipGraph_t g = nullptr;
         const hipError_t e = hipStreamEndCapture(st, &g);
         if (rc) {
@@ -805,14 +878,14 @@ OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token,
             return rc;
         }
         OJX_HIP(e);
-        d->graph = g;
-        OJX_HIP(hipGraphInstantiate(&d->exec, g, nullptr, nullptr, 0));
+        d->graph[sampled] = g;
+        OJX_HIP(hipGraphInstantiate(&d->exec[sampled], g, nullptr, nullptr, 0));
     }
     for (int i = done; i < num_tokens; ++i) {
         if (use_graph) {
-            OJX_HIP(hipGraphLaunch(d->exec, st));
+            OJX_HIP(hipGraphLaunch(d->exec[sampled], st));
         } else {
-            rc = d->step(st);
+            rc = d->step(st, sampled);
             if (rc) return rc;
         }
     }
@@ -823,6 +896,20 @@ OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token,
                                hipMemcpyDeviceToHost, st));
     OJX_HIP(hipStreamSynchronize(st));
     return OJASX_OK;
+}
+
+OJASX_API int ojasx_decoder_generate(OjasxDecoderHandle handle, int first_token, int num_tokens,
+                                     int use_graph, int *tokens_out, float *last_logits) {
+    return generate(handle, first_token, num_tokens, use_graph, nullptr, tokens_out, last_logits);
+}
+
+OJASX_API int ojasx_decoder_generate_sampled(OjasxDecoderHandle handle, int first_token, int num_tokens,
+                                             int use_graph, const float *uniform, float temperature,
+                                             int top_k, float top_p, float min_p, int *tokens_out,
+                                             float *last_logits) {
+    if (!uniform) return OJASX_ERR_NULL;
+    const DrawSettings draw{{temperature, top_p, min_p, top_k, 0, {}}, uniform};
+    return generate(handle, first_token, num_tokens, use_graph, &draw, tokens_out, last_logits);
 }
 
 OJASX_API int ojasx_decoder_read_kv(OjasxDecoderHandle handle, int layer, int first_token,

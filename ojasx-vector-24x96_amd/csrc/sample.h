@@ -10,8 +10,7 @@ struct SampleParams {
     long stride;
     const float *uniform;                // [rows], or with step: of one row, entry *step
     const int *step;
-    int *tokens;                         // row r's at tokens + r * token_stride
-    int token_stride;
+    int *tokens;                         // [rows]
     int rows, vocab, slices;
     // one value for all rows, or an array of a value for each
     double temperature, top_p, min_p;

@@ -668,7 +668,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
     const Row row = row_of(a, r);
     const RowHead h = row_head(row, heads, S);
     if (h.bad || row.bad || h.most == -INFINITY || row.greedy) {
-        if (tid == 0) a.tokens[(long)r * a.token_stride] = h.bad || row.bad || h.most == -INFINITY ? -1 : h.at;
+        if (tid == 0) a.tokens[r] = h.bad || row.bad || h.most == -INFINITY ? -1 : h.at;
         return;
     }
     for (int s = tid; s < S; s += kNT) L.csum[s] = 0, L.cties[s] = 0;
@@ -804,7 +804,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         atomicMax(&L.last, wlast);
     }
     __syncthreads();
-    if (tid == 0) a.tokens[(long)r * a.token_stride] = L.hit == INT_MAX ? L.last : L.hit;
+    if (tid == 0) a.tokens[r] = L.hit == INT_MAX ? L.last : L.hit;
 }
 
 namespace {
@@ -889,7 +889,7 @@ OJASX_API int ojasx_sample_device(const void *logits, int dtype, int num_rows, i
     }
     SampleParams a{};
     a.logits = logits, a.stride = row_stride, a.rows = num_rows, a.vocab = vocab;
-    a.uniform = uniform, a.tokens = tokens, a.token_stride = 1;
+    a.uniform = uniform, a.tokens = tokens;
     a.temperature = s.temperature, a.temperatures = s.temperatures;
     a.top_k = s.top_k, a.top_ks = s.top_ks;
     a.top_p = s.top_p, a.top_ps = s.top_ps;

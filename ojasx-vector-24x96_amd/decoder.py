@@ -190,15 +190,37 @@ class LUTDecoder:
         _lib.check(_lib.lib().ojasx_decoder_reset(self._h, position), "ojasx_decoder_reset")
 
     def generate(self, first_token: int, num_tokens: int, use_graph: bool = True,
-                 return_logits: bool = False):
-        """Greedy tokens after ``first_token`` (and the last step's logits)."""
+                 return_logits: bool = False, *, uniform=None, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0):
+        """Greedy tokens after ``first_token`` (and the last step's logits).
+
+        With ``uniform``, num_tokens numbers in [0, 1), token i is drawn with
+        uniform[i] as :func:`sample_tokens` does, the settings rounded to
+        float32; -1 where the logits are no distribution, and the step after it
+        starts from token 0."""
         toks = np.zeros(num_tokens, np.int32)
         logits = np.zeros(self.cfg.vocab, np.float32) if return_logits else None
-        rc = _lib.lib().ojasx_decoder_generate(
-            self._h, int(first_token), int(num_tokens), 1 if use_graph else 0,
-            toks.ctypes.data_as(ctypes.c_void_p),
-            logits.ctypes.data_as(ctypes.c_void_p) if logits is not None else None)
-        _lib.check(rc, "ojasx_decoder_generate")
+        outs = (toks.ctypes.data_as(ctypes.c_void_p),
+                logits.ctypes.data_as(ctypes.c_void_p) if logits is not None else None)
+        args = (self._h, int(first_token), int(num_tokens), 1 if use_graph else 0)
+        if uniform is None:
+            if (temperature, top_k, top_p, min_p) != (1.0, 0, 1.0, 0.0):
+                raise ValueError("temperature, top_k, top_p and min_p are for drawn tokens: give uniform")
+            rc = _lib.lib().ojasx_decoder_generate(*args, *outs)
+            _lib.check(rc, "ojasx_decoder_generate")
+        else:
+            if hasattr(uniform, "cpu"):
+                uniform = uniform.cpu()
+            wide = np.asarray(uniform)
+            u = np.ascontiguousarray(wide, np.float32)
+            # a number below 1 that float32 rounds to 1: the largest below it
+            u = np.where((wide < 1) & (u == 1), np.nextafter(np.float32(1), np.float32(0)), u)
+            if u.shape != (num_tokens,):
+                raise ValueError(f"uniform must have {num_tokens} entries, got {u.shape}")
+            rc = _lib.lib().ojasx_decoder_generate_sampled(
+                *args, u.ctypes.data_as(ctypes.c_void_p), float(temperature),
+                min(max(int(top_k), 0), 0x7fffffff), float(top_p), float(min_p), *outs)
+            _lib.check(rc, "ojasx_decoder_generate_sampled")
         return (toks, logits) if return_logits else toks
 
     def read_kv(self, layer: int, first_token: int, num_tokens: int):

@@ -168,3 +168,19 @@ def test_oracle_draws():
     assert [kve.draw(x, u, m=0.3) for u in (0.0, 0.99)] == [1, 2]
     assert kve.draw(x, 0.99, T=0) == 1 and kve.draw([1.0, np.nan], 0.5) == -1 and kve.draw([-np.inf] * 3, 0.5) == -1
     assert kve.draw([0.0, np.inf], 0.5) == -1 and kve.draw([0.0, -np.inf], 0.999) == 0
+
+
+def test_bad_sampled_generation_is_refused(pkg):
+    import torch
+    dec = pkg.decoder
+    call = pkg._lib.lib().ojasx_decoder_generate_sampled
+    u, toks = (ctypes.c_float * 2)(0.1, 0.2), (ctypes.c_int * 2)()
+    assert call(None, 0, 2, 0, u, 1.0, 0, 1.0, 0.0, toks, None) == -1
+    assert call(FAKE, 0, 2, 0, None, 1.0, 0, 1.0, 0.0, toks, None) == -1
+    assert call(FAKE, 0, 2, 0, u, 1.0, 0, 1.0, 0.0, None, None) == -1
+    d = object.__new__(dec.LUTDecoder)
+    d.cfg, d._h = dec.DecoderConfig(), None
+    with pytest.raises(ValueError, match="uniform"):
+        d.generate(0, 2, temperature=0.5)
+    with pytest.raises(ValueError, match="uniform"):
+        d.generate(0, 2, uniform=torch.zeros(3))
