@@ -257,6 +257,26 @@ def test_decode(lc, dev, D, dtype, page, Hkv, Hq, lengths):
     assert c.decode(x, held, 0.3, count=False, out=x) is x and torch.equal(x, other)
 
 
+def cycled(lengths, n):
+    return (lengths * n)[:n]
+
+
+@pytest.mark.parametrize("dtype,Hq,lengths", [
+    # 32 query heads a kv head: scores of 384 tokens lie in LDS, chunks have 512
+    ("bfloat16", 64, cycled([590, 600, 540, 600, 500, 0, 600, 385, 384, 600], 130)),
+    # 16: scores of 768 tokens, chunks of 800
+    ("float32", 32, cycled([900, 900, 790, 769, 830, 900, 768, 900, 900, 1], 260)),
+    # a kv head for each query head: all of the longest
+    ("float16", 2, cycled([70, 31, 0, 128, 129, 1], 513)),
+])
+def test_decode_of_whole_sequences(lc, dev, dtype, Hq, lengths):
+    """A batch whose sequences are a workgroup's each, with their scores in LDS and past it, some cut in two."""
+    c = filled(lc, dev, 64, dtype, 16, 2, lengths, seed=31)
+    q = rand(dev, dtype, len(lengths), Hq, 64, seed=32)
+    before = f64(c.weights)
+    check_decode(c, q, lengths, c.decode(q, i32(dev, lengths)), before, dtype)
+
+
 def test_decode_one_long_sequence(lc, dev):
     """More tiles than a launch has chunks for at their least size, with a strided query."""
     import torch
@@ -437,6 +457,14 @@ def test_evict(lc, dev, D, dtype, page, Hkv, held, budget, sink, recent):
     check_evict(c, left, max(1, budget // 2), sink // 2, recent // 2)
     # with a bound below the lengths
     check_evict(c, left, max(1, budget // 4), 0, 0, max_held=max(2, budget // 3))
+
+
+@pytest.mark.parametrize("held,budget", [([1024, 1000, 7], 400), ([1025, 1000, 512], 400), ([1024, 1023], 1020),
+                                         ([1025, 1024], 1020), ([4096, 4097], 4000), ([4097], 1000)])
+def test_evict_at_the_sizes_that_change_the_launch(lc, dev, held, budget):
+    c = filled(lc, dev, 128, "bfloat16", 16, 2, held, seed=41, poison=False)
+    check_evict(c, held, budget, 4, 64, max_held=max(held))
+    check_evict(c, [min(n, budget) for n in held], budget - 3, 4, 64)
 
 
 def test_evict_ties_and_odd_weights(lc, dev):
