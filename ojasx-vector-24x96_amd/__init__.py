@@ -15,10 +15,12 @@ Faces, each mirroring a reference interface:
 * ``long_context``: ``PagedCompressedKVCache`` (reference int8 paged KV cache)
   and ``PagedCodeKVCache`` (paged codebook-code KV cache with device append
   and decode); for a serving batch ``PagedInt4KVCache`` (4-bit paged cache:
-  append with rotation, decode attention) and ``PackedPromptAttention``
-  (causal attention of packed prompts)
-* ``decoder``: ``LUTDecoder`` / ``synthetic_decoder``, the 4B-shaped greedy
-  decoder over LUT linears and the code KV cache (HIP graph per token)
+  append with rotation, decode attention), ``PagedEvictingKVCache`` (16- or
+  32-bit paged cache that counts the attention its tokens get and evicts those
+  of least) and ``PackedPromptAttention`` (causal attention of packed prompts)
+* ``decoder``: ``LUTDecoder`` / ``synthetic_decoder``, the 4B-shaped decoder
+  over LUT linears and the code KV cache (HIP graph per token, greedy or
+  sampled), and ``sample_tokens`` (temperature, top-k, top-p, min-p)
 * ``oqpack``: the reference's oqpack.v1 container (verify, mmap, write) and
   the loader of its residual-VQ linears as GPU LUT layers
 * ``synthetic``: seeded synthetic inputs of the benchmark configurations

@@ -19,8 +19,15 @@
 // Work: the tiles of all sequences are cut into chunks of equal size, as many as the card takes
 // workgroups, whatever the lengths are; a workgroup's four waves take turns at the tiles of
 // its chunk, join in LDS and leave (out, max, sums) to kve_join_kernel, which also turns the
-// scores kept by the first kernel (fp32, a thirtieth of the cache's bytes) into weights, once
-// the sums over whole sequences are known.
+// scores kept by the first kernel (fp32) into weights, once the sums over whole sequences are
+// known.  Writes among the reads cost far more than their bytes: the scores, 3 % of what the
+// kernel reads with four query heads of a kv head, took 27 us of 175 when each tile's were written
+// at once, and 20 now that a chunk's are kept in LDS and written when it is done.  A workgroup with
+// a whole sequence finishes output and weights itself.
+//
+// Bound by reading the pages.  Measured, bf16, 32 / 8 heads of 128: 64 sequences of 192000 tokens in
+// all, 167 us (4.8 TB/s; without counting 146, 5.4) and join 18; one of 131072, 103 to 114 and 13; fp32, one of
+// 2048: 10 and 6.5, both a launch and the chain of its loads.
 //
 // Scores, maxima, sums and outputs are fp32.  Weights are rounded to bf16 or fp16 for the value
 // product (fp16: times 2^15, so that the smallest keep their share), and the sum that divides
@@ -41,10 +48,13 @@ constexpr int kLeastTiles = 4;           // tiles of a chunk, one for each wave
 // Chunks that the tiles are cut into: four times what the card takes at once, so that the last ones end
 // together; fewer where a kv head has many query heads, whose maxima and sums every item of the second
 // kernel reads of all chunks.  64 sequences of 192000 bf16 tokens, 32 / 8 heads of 128, us with 512, 768,
-// 1024 and 1536: 202, 192, 193, 186; one of 131072: 129, 132, 129, 133; 256 of 500: 131, 131, 131, 143;
-// four of 20000 with 40 / 1 heads: 56, 66, 85, 97.
+// 1024 and 1536: 195, 186, 187, 181; one of 131072: 125, 129, 127, 131; 256 of 500: 130, 130, 130, 142;
+// eight of 6000 with 32 / 8 heads of 256: 114, 119, 112, 130.  Four of 20000 with 40 / 1 heads, without the
+// second rule: 56, 66, 85, 97.
 constexpr int kMostChunks = 1024, kFewestChunks = 256, kChunkHeads = 8192;
-constexpr int kScoreFloats = 12288;      // scores of a whole sequence in LDS: two workgroups of a CU have room
+// Scores of a chunk in LDS, so that as many workgroups of a CU find room as its registers take: two, and four
+// of D = 64.
+constexpr int kScoreFloats = 12288, kScoreFloats64 = 7168;
 
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
@@ -422,7 +432,7 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
     auto load_v = [&](int page, int t) {
         tl.load_v(reinterpret_cast<const T *>(p.c.v) + row(page, t + vb) * D, i, c);
     };
-    // A tile's scores, [R][tokens]: of a whole sequence in LDS, as far as they find room.
+    // A tile's scores, [R][tokens]: in LDS, as far as they find room, until the chunk is done.
     float *scores = p.scores + ((long)it.b * p.c.Hkv + it.h) * p.R * p.stride;
     auto store = [&](float *tile, const float (&raw)[NT][E]) {
 #pragma unroll
@@ -496,9 +506,9 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
             tl.template values<NT>(w, o, lr);
             load_v(vp1, next);
             if (p.scores) {
-                const long tile = (long)t * p.R;
-                if (alone && tile + p.R * TT <= p.lds_scores) store(lds_scores + tile, raw);
-                else store(scores + tile, raw);
+                const long tile = (long)(t - it.t0) * p.R;
+                if (tile + p.R * TT <= p.lds_scores) store(lds_scores + tile, raw);
+                else store(scores + (long)t * p.R, raw);
             }
             vp = vp1, kp1 = kp2, vp1 = vp2;
             t += kStep;
@@ -511,6 +521,13 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
         if (c == 0) ml[wv][b * 16 + i][0] = m[b], ml[wv][b * 16 + i][1] = l[b], ml[wv][b * 16 + i][2] = lr[b];
     }
     __syncthreads();
+    const int here = p.lds_scores / (p.R * TT) * TT;       // tokens whose scores are in LDS
+    if (!alone) {
+        const int n = min((it.t1 - it.t0 + TT - 1) / TT * TT, here) * p.R;
+        float *to = scores + (long)it.t0 * p.R;
+        for (int x = threadIdx.x * 4; x < n; x += kNT * 4)
+            *reinterpret_cast<f4_t *>(to + x) = *reinterpret_cast<const f4_t *>(lds_scores + x);
+    }
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
         float most = ml[0][b * 16 + i][0];
@@ -584,7 +601,6 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
     }
     if (!alone || !p.scores) return;
     __syncthreads();
-    const int here = p.lds_scores / (p.R * TT) * TT;       // tokens whose scores are in LDS
     add_weights<TT>(p, it, 0, min(it.n, here), lds_scores, [&](int r) { return ml[0][r][0]; }, [&](int r) { return ml[0][r][1]; });
     add_weights<TT>(p, it, here, it.n, scores, [&](int r) { return ml[0][r][0]; }, [&](int r) { return ml[0][r][1]; });
 }
@@ -702,9 +718,8 @@ int kve_plan(const OjasxKVECache *c, const KveView &v, int num_q_heads, int max_
     p->ml_bytes = p->items * p->Rb * 16;
     p->item_bytes = p->items * (long)sizeof(KveItem);
     p->s_bytes = count ? (long)v.B * num_q_heads * p->stride * 4 : 0;
-    // scores in LDS, where most sequences are not cut: no more than the longest has
-    const long all = (long)p->R * p->stride;
-    p->lds_scores = count && groups * v.B >= p->target && p->HB == 1 ? (int)(all < kScoreFloats ? all : kScoreFloats) : 0;
+    const long all = (long)p->R * p->stride, room = v.D == 64 && p->NT == 1 ? kScoreFloats64 : kScoreFloats;
+    p->lds_scores = count && p->HB == 1 ? (int)(all < room ? all : room) : 0;
     return OJASX_OK;
 }
 

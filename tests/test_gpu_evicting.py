@@ -264,8 +264,10 @@ def cycled(lengths, n):
 @pytest.mark.parametrize("dtype,Hq,lengths", [
     # 32 query heads a kv head: scores of 384 tokens lie in LDS, chunks have 512
     ("bfloat16", 64, cycled([590, 600, 540, 600, 500, 0, 600, 385, 384, 600], 130)),
-    # 16: scores of 768 tokens, chunks of 800
+    # 16: scores of 448 tokens, chunks of 800
     ("float32", 32, cycled([900, 900, 790, 769, 830, 900, 768, 900, 900, 1], 260)),
+    # sequences cut into chunks of 512, more than LDS has room for
+    ("float16", 64, cycled([590, 1000, 540, 600, 500, 0, 600, 385, 384, 600], 130)),
     # a kv head for each query head: all of the longest
     ("float16", 2, cycled([70, 31, 0, 128, 129, 1], 513)),
 ])
