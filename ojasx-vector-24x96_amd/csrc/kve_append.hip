@@ -4,6 +4,11 @@
 // The rotation is that of the 4-bit cache (kv4_append.hip): angles in fp64 turns, products in
 // fp64, one rounding to fp32 and one to the element type.  What does not rotate is copied bit
 // for bit.
+//
+// Bound by the copy of the rows: 8192 bf16 tokens with 32 / 8 heads of 128 take 42 us, 4.8 TB/s of
+// rows in and out; a token each of 64 sequences takes 4.8 us, a launch and the chain of table entry,
+// angles and rows.  Loading a token's first rows before its place and angles are known leaves room
+// for fewer waves (53 us).
 #include "kve.h"
 
 namespace ojx {

@@ -21,6 +21,13 @@
 // A drawn token is a whole number: it has to be the definition's own.  So e is fp64 to about
 // 2^-50, sums are fp64, or in LDS, where they are added in any order, 64-bit integers: a fixed
 // number of bits behind the point, the same result in every order.
+//
+// What is read is small (2 or 4 bytes a logit); bound by the fp64 products of the exponentials and,
+// with cuts, two additions in LDS for each token in 1., and for few rows by the chains of three
+// launches.  Measured: 256 rows of 32000 fp16 logits without cuts 11 + 9 us (1. and 3.), 64 rows of
+// 151936 bf16 ones with settings of their own 20 + 17 + 20 us, one row of 151936 fp32 ones with top-k
+// 50 and top-p 0.9 7 + 9 + 15.5 us.  Keeping a row's workgroups on one die's L2 took 3 % off rows that
+// all have cuts and cost as much where only some have.
 #include <cfloat>
 #include <climits>
 #include <cmath>
