@@ -147,12 +147,13 @@ struct Row {
 };
 __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
     Row s;
-    const double T = a.temperatures ? (double)a.temperatures[r] : a.temperature;
+    const double given = a.temperatures ? (double)a.temperatures[r] : a.temperature;
+    const double T = fmax(given, 0x1p-300);      // as any below: of two fp32 logits the smaller's e is 0, and 1 / T is finite
     s.k = a.top_ks ? a.top_ks[r] : a.top_k;
     s.p = a.top_ps ? (double)a.top_ps[r] : a.top_p;
     s.m = fmin(a.min_ps ? (double)a.min_ps[r] : a.min_p, 1.0);
-    s.bad = !(T >= 0.0) || T > (double)FLT_MAX;
-    s.greedy = T == 0.0;
+    s.bad = !(given >= 0.0) || given > (double)FLT_MAX;
+    s.greedy = given == 0.0;
     const double inv = 1.0 / T;                  // the others are its multiples or T's: a division costs 20 products
     s.c = 1.4426950408889634074 * inv;
     s.bins = kBinsPerE * inv;

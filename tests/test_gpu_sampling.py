@@ -261,3 +261,13 @@ def test_refusals(sample, dev):
             sample(bad, u)
     with pytest.raises(RuntimeError):
         sample(x.cpu(), u.cpu())
+
+
+@pytest.mark.parametrize("T", [5e-324, 1e-310, 1e-300, 1e-90, 1e-60])
+def test_temperatures_below_any_fp32(sample, dev, T):
+    """Only tokens that equal the largest logit are drawn, however near the others are."""
+    import torch
+    big = torch.finfo(torch.float32).max
+    x = torch.tensor([[0.0, 3.0, -1.0, 3.0, big, big], [1e-45, 0.0, -0.0, 1e-45, -1e-45, 1e-45], [-big, big, 1.0, big, -1.0, 5.0]] * 2)
+    for s in (dict(), dict(k=1), dict(k=2), dict(k=4, p=0.9), dict(p=0.3), dict(m=0.5), dict(m=1.0, p=0.6)):
+        check(sample, dev, x, grid(6), T=T, **s)
