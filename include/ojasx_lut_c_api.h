@@ -409,8 +409,9 @@ OJASX_API int ojasx_prompt_attention_device(const void *q, long q_token_stride, 
  * that is not there: its tokens are not written and not attended.  A page holds
  * for each kv head page_size rows of keys and values, weights (the softmax
  * weights that a token got, fp32) and positions; the order is [num_pages]
- * [num_kv_heads][page_size]([head_dim]).  Pages that decode counts into or that
- * evict moves belong to one sequence.  How many tokens a sequence holds is the
+ * [num_kv_heads][page_size]([head_dim]).  Pages that append writes, that decode counts
+ * into or that evict moves belong to one sequence and stand in its row once.  A
+ * sequence has at most 2^31 - 2^20 slots.  How many tokens a sequence holds is the
  * caller's: int32 arrays on the device, so every call can be captured and
  * replayed while they change.  head_dim 64, 128 or 256; page_size a power of
  * two from 16 to 32768; keys and values 16-byte aligned.  The struct is read during

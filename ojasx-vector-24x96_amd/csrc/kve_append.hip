@@ -141,8 +141,9 @@ int kve_view(const OjasxKVECache *c, KveView *v) {
                   c->num_kv_heads, c->num_pages, c->max_pages);
         return OJASX_ERR_INVALID;
     }
-    if ((long)c->max_pages * P > 0x7fffff00L) {
-        set_error("evicting KV cache: %d pages of %d slots of a sequence are more than 2^31 slots", c->max_pages, P);
+    // room for the steps of a loop past a sequence's end
+    if ((long)c->max_pages * P > 0x7ff00000L) {
+        set_error("evicting KV cache: %d pages of %d slots of a sequence are more than 2^31 - 2^20 slots", c->max_pages, P);
         return OJASX_ERR_INVALID;
     }
     if (c->rotary_dim < 0 || c->rotary_dim > D || c->rotary_dim % 16 || (c->rotary_dim && !c->turns)) {

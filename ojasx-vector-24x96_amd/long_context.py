@@ -1011,9 +1011,9 @@ class PagedEvictingKVCache:
 
     The sequences' lengths are the caller's: int32 tensors on the cache's
     device, one for all layers, that a captured graph advances itself.  Calls on
-    one cache write its pages: order them on one stream.  Sequences may share
-    pages only where nothing writes them: no append, no eviction, and decode
-    with ``count=False``."""
+    one cache write its pages: order them on one stream.  A page may stand in
+    the table more than once only where nothing writes it: no append, no
+    eviction, and decode with ``count=False``."""
 
     def __init__(self, num_kv_heads: int, head_dim: int = 128, *, num_sequences: int = 1,
                  page_size: int = 16, max_pages: int = 512, rope_theta: Optional[float] = 1e6,

@@ -21,7 +21,8 @@ def cache(pkg, **over):
 BAD = [dict(head_dim=96), dict(head_dim=0), dict(page_size=24), dict(page_size=8), dict(page_size=65536),
        dict(num_sequences=0), dict(max_pages=0), dict(num_kv_heads=0), dict(num_kv_heads=65536), dict(num_pages=0),
        dict(rotary_dim=24), dict(rotary_dim=144), dict(rotary_dim=-16), dict(turns=None), dict(keys=FAKE + 4),
-       dict(values=FAKE + 8), dict(dtype=3), dict(dtype=4), dict(dtype=-1), dict(max_pages=1 << 27)]
+       dict(values=FAKE + 8), dict(dtype=3), dict(dtype=4), dict(dtype=-1), dict(max_pages=1 << 27),
+       dict(max_pages=(0x7ff00000 >> 4) + 1)]
 
 
 @pytest.mark.parametrize("over", BAD, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
@@ -35,6 +36,13 @@ def test_bad_cache_is_refused(pkg, over):
     assert L.ojasx_kve_evict_workspace(ref, 8, 0) == -3
     assert L.ojasx_kve_evict_device(ref, FAKE, 8, 0, 0, 0, FAKE, 1 << 40, None) == -3
     assert L.ojasx_get_last_error()
+
+
+def test_the_most_slots_are_taken(pkg):
+    """Kernels step past a sequence's end by some thousands of slots, in 32 bits."""
+    L, c = pkg.lib(), cache(pkg, max_pages=0x7ff00000 >> 4, num_sequences=1)
+    assert L.ojasx_kve_decode_workspace(ctypes.addressof(c), 4, 0, 0) > 0
+    assert L.ojasx_kve_evict_workspace(ctypes.addressof(c), 8, 0) > 0
 
 
 def test_null_buffers_are_refused(pkg):
