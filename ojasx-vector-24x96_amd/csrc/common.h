@@ -394,6 +394,22 @@ __device__ __forceinline__ int wave_min_i(int v) {
     const int c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
     return min(min(a, b), min(c, d));
 }
+
+// Sum over the lanes up to and with each: within rows of 16 lanes by shifts, then row by row (DPP
+// row_shr and row_bcast; lanes without a source add 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp0_i(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan_i(int v) {
+    v += dpp0_i<0x111, 0xF>(v);
+    v += dpp0_i<0x112, 0xF>(v);
+    v += dpp0_i<0x114, 0xF>(v);
+    v += dpp0_i<0x118, 0xF>(v);
+    v += dpp0_i<0x142, 0xA>(v);
+    v += dpp0_i<0x143, 0xC>(v);
+    return v;
+}
 // Minima over the wave of N values per lane, the N reductions interleaved
 // (independent DPP chains in one straight-line block); every lane gets them.
 template <int N>

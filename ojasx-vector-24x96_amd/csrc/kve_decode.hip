@@ -86,10 +86,9 @@ struct KveDecodeParams {
 
 // Sum of v over the workgroup, in order of the threads' numbers; sh: kNW + 1 ints.
 __device__ __forceinline__ int block_sum(int v, int *sh) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    v = wave_scan_i(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
     __syncthreads();
     int s = 0;
 #pragma unroll
@@ -114,12 +113,7 @@ __device__ __forceinline__ KveItem kve_item(const KveDecodeParams &p, int *sh) {
     for (int b0 = 0; b0 < B; b0 += kNT) {
         const int b = b0 + tid, nt = b < B ? tiles(b) : 0;
         const int k = b < B ? max(1, (int)((nt + size - 1) / size)) : 0;     // no tokens: a chunk of none
-        int incl = k;                                                        // scan over the workgroup
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(incl, o);
-            if ((tid & 63) >= o) incl += x;
-        }
+        int incl = wave_scan_i(k);                                           // over the workgroup
         __syncthreads();
         if ((tid & 63) == 63) sh[tid >> 6] = incl;
         __syncthreads();

@@ -53,8 +53,7 @@ struct KveEvictParams {
 
 template <int NT>
 __device__ __forceinline__ int block_max(int v, int *sh) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
+    v = ~wave_min_i(~v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -170,12 +169,7 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
         if (tid < kDigits) {
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) c += counts[d * kCopies + i], counts[d * kCopies + i] = 0;
-            upto = c;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(upto, o);
-                if (lane >= o) upto += x;
-            }
+            upto = wave_scan_i(c);
             if (lane == 63) sh2[wv] = upto;
         }
         __syncthreads();

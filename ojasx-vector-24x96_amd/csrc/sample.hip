@@ -202,12 +202,6 @@ __device__ __forceinline__ double wave_sum_d(double v) {
     v += dpp_d<0x140>(v);
     return (lane_d(v, 0) + lane_d(v, 16)) + (lane_d(v, 32) + lane_d(v, 48));
 }
-// Sums over the lanes up to and with each: within rows of 16 lanes by shifts, then row by row (DPP
-// row_shr and row_bcast; lanes without a source add 0).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp0_i(int v) {
-    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
-}
 template <int CTRL, int ROWS>
 __device__ __forceinline__ u64 dpp0_u(u64 v) {
     return (u64)(unsigned)dpp0_i<CTRL, ROWS>((int)(v >> 32)) << 32 | (unsigned)dpp0_i<CTRL, ROWS>((int)v);
@@ -216,6 +210,7 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp0_d(double v) {
     return __longlong_as_double((long long)dpp0_u<CTRL, ROWS>((u64)__double_as_longlong(v)));
 }
+// As wave_scan_i.
 #define OJX_WAVE_SCAN(NAME, T, DPP)                     \
     __device__ __forceinline__ T NAME(T v) {            \
         v += DPP<0x111, 0xF>(v);                        \
@@ -226,7 +221,6 @@ __device__ __forceinline__ double dpp0_d(double v) {
         v += DPP<0x143, 0xC>(v);                        \
         return v;                                       \
     }
-OJX_WAVE_SCAN(wave_scan_i, int, dpp0_i)
 OJX_WAVE_SCAN(wave_scan_u, u64, dpp0_u)
 OJX_WAVE_SCAN(wave_scan_d, double, dpp0_d)
 #undef OJX_WAVE_SCAN
