@@ -17,11 +17,11 @@
 // positions and weights, four counts, three walks over the ballots.  11-bit digits, in three passes,
 // took as long as four of 8 bits.  Up to kMoveInPlace moves the workgroup does itself, four units of
 // a thread in flight; more are a second launch over the whole card, one unit of a thread in flight
-// (16.8 us against 23.0 for four, for 8 sequences of 8192 that leave 2048).
+// (16.8 us against 23.0 for four, for 8 sequences of 4096 that leave 1024).
 //
 // Measured, bf16, 8 heads of 128, the launches without the append: 64 sequences of 2064 tokens that
-// leave 2048: 24 us (1 sequence, 4 heads of fp32: 13 us); 8 sequences of 8192 that leave 2048: 22 us
-// and 17 us for the 131 MB or so of its moves; a sequence of 65536, whose ranks are formed anew in
+// leave 2048: 19.5 us (1 sequence of 1008 fp32 tokens: 11 us); 8 sequences of 4096 that leave 1024: 21 us
+// and 17 us for their moves; a sequence of 65536, whose ranks are formed anew in
 // each pass: 307 us.
 #include <climits>
 
@@ -30,16 +30,16 @@
 namespace ojx {
 
 namespace {
-constexpr int kWideNT = 1024, kSlimNT = 256;   // threads of a selecting workgroup
 constexpr int kDigitBits = 8;            // of a rank's 32: four passes
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kCopies = 8;               // counters of a digit, so that equal digits of a wave's lanes collide less
 constexpr int kRanksInLds = 32768;       // tokens whose ranks are kept (128 KB); of more they are formed again
 constexpr int kMoveInPlace = 256;        // moves that the selecting workgroup does itself
-// Up to this many tokens a workgroup of 256 threads is faster (64 sequences of 416 tokens, 8 heads: 14.3
-// against 17.9 us), from about 2000 on one of 1024 (4 sequences of 4096: 15.2 against 29.8 us).
-constexpr int kSlimTokens = 1024;
-constexpr int kBatch = 4;                // tokens of a thread whose loads are in flight together
+// Threads of a selecting workgroup.  One that has a CU of its own takes kWideNT (8 sequences of 4096 tokens, 8
+// heads: 21 us against 29 with 512); where a CU takes several, each is faster with fewer, which leave fewer
+// idle in its scans (64 sequences of 2064: 19.5 us against 24; 256 of 1016: 26 with 256 threads, 32 with 512).
+constexpr int kWideNT = 1024, kManyNT = 512, kShortNT = 256;
+constexpr int kWidePairs = 256, kShortTokens = 1024;
 constexpr int kMoveNT = 256;
 constexpr size_t kSelectLds = kDigits * kCopies * 4 + 4096;   // static LDS of the selecting kernel, rounded up
 
@@ -100,6 +100,7 @@ __device__ __forceinline__ void move_rows(const KveEvictParams &p, int b, int h,
 template <int UNITS, bool MOVES, int NT>
 __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     constexpr int kNT = NT, kNW = NT / 64;
+    constexpr int kBatch = NT == kManyNT ? 8 : 4;          // tokens of a thread whose loads are in flight together
     extern __shared__ uint32_t ranks[];
     __shared__ int counts[kDigits * kCopies], sh[kNW], sh2[kNW], picked[2], picked_places[kNW], places_of[MOVES ? 2 * kMoveInPlace : 1];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
@@ -281,9 +282,14 @@ template <int UNITS>
 int evict(const KveEvictParams &p, hipStream_t st) {
     const dim3 grid(p.c.Hkv, p.c.B);
     const size_t lds = p.in_lds ? round_up((size_t)p.most * 4, 16) : 0;
-    const bool slim = p.most <= kSlimTokens;
-    if (p.most_moves <= kMoveInPlace) return slim ? select<UNITS, true, kSlimNT>(p, grid, lds, st) : select<UNITS, true, kWideNT>(p, grid, lds, st);
-    const int rc = slim ? select<UNITS, false, kSlimNT>(p, grid, lds, st) : select<UNITS, false, kWideNT>(p, grid, lds, st);
+    const bool wide = (long)p.c.B * p.c.Hkv <= kWidePairs, brief = p.most <= kShortTokens;
+    if (p.most_moves <= kMoveInPlace)
+        return wide    ? select<UNITS, true, kWideNT>(p, grid, lds, st)
+               : brief ? select<UNITS, true, kShortNT>(p, grid, lds, st)
+                       : select<UNITS, true, kManyNT>(p, grid, lds, st);
+    const int rc = wide    ? select<UNITS, false, kWideNT>(p, grid, lds, st)
+                   : brief ? select<UNITS, false, kShortNT>(p, grid, lds, st)
+                           : select<UNITS, false, kManyNT>(p, grid, lds, st);
     if (rc) return rc;
     // parts of a (sequence, kv head): 8 moves or more each, no more than four times what fills the card
     const long pairs = (long)p.c.B * p.c.Hkv, wanted = (p.most_moves + 7) / 8, fill = (4096 + pairs - 1) / pairs;

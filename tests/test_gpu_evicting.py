@@ -469,6 +469,15 @@ def test_evict_at_the_sizes_that_change_the_launch(lc, dev, held, budget):
     check_evict(c, [min(n, budget) for n in held], budget - 3, 4, 64)
 
 
+@pytest.mark.parametrize("B,held,budget", [(86, [1024, 1000, 7], 400), (86, [1025, 1000, 512], 400), (86, [1024, 1023], 1020),
+                                           (86, [1025, 1024], 1020), (85, [1500, 1490], 1480), (86, [4100, 20, 4096], 4000)])
+def test_evict_of_many_sequences(lc, dev, B, held, budget):
+    """More (sequence, kv head) pairs than the card has CUs, and 255 of them."""
+    held = cycled(held, B)
+    c = filled(lc, dev, 64, "float16", 32, 3, held, seed=42, poison=False)
+    check_evict(c, held, budget, 4, 64, max_held=max(held))
+
+
 def test_evict_ties_and_odd_weights(lc, dev):
     """Equal weights (the lowest slots stay), zeros of both signs, negative ones, infinities and NaN."""
     import torch
