@@ -14,15 +14,15 @@
 // One workgroup for a (sequence, head), since every pass of the selection needs all of its ranks and
 // those of 32768 tokens fit LDS.  What is read is small (8 bytes a token and head; of a moved token
 // its rows besides), so the time is that of a chain of steps that wait for each other: block table,
-// positions and weights, four counts, three walks over the ballots.  11-bit digits, in three passes,
+// positions and weights, four counts, two walks over the ballots.  11-bit digits, in three passes,
 // took as long as four of 8 bits.  Up to kMoveInPlace moves the workgroup does itself, four units of
 // a thread in flight; more are a second launch over the whole card, one unit of a thread in flight
 // (16.8 us against 23.0 for four, for 8 sequences of 4096 that leave 1024).
 //
 // Measured, bf16, 8 heads of 128, the launches without the append: 64 sequences of 2064 tokens that
-// leave 2048: 19.5 us (1 sequence of 1008 fp32 tokens: 11 us); 8 sequences of 4096 that leave 1024: 21 us
+// leave 2048: 17.5 us (1 sequence of 1008 fp32 tokens: 9.6 us); 8 sequences of 4096 that leave 1024: 19 us
 // and 17 us for their moves; a sequence of 65536, whose ranks are formed anew in
-// each pass: 307 us.
+// each pass: 272 us.
 #include <climits>
 
 #include "kve.h"
@@ -102,7 +102,8 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     constexpr int kNT = NT, kNW = NT / 64;
     constexpr int kBatch = NT == kManyNT ? 8 : 4;          // tokens of a thread whose loads are in flight together
     extern __shared__ uint32_t ranks[];
-    __shared__ int counts[kDigits * kCopies], sh[kNW], sh2[kNW], picked[2], picked_places[kNW], places_of[MOVES ? 2 * kMoveInPlace : 1];
+    __shared__ int counts[kDigits * kCopies], sh[kNW], sh2[kNW], picked[2], places_of[MOVES ? 2 * kMoveInPlace : 1];
+    __shared__ int4 parts[kNW];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = min(max(p.held[b], 0), p.most);
@@ -189,41 +190,34 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     const int ties = p.budget - above;           // tokens of rank `last` that stay, the lowest slots
     // wave w has slots [w * span, (w + 1) * span)
     const int span = ((n + kNW - 1) / kNW + 63) & ~63, s0 = min(n, wv * span), s1 = min(n, s0 + span);
-    auto before_waves = [&](int v, int *at, int *all) {    // sum of v (one value a wave) over the waves before
-        if (lane == 0) at[wv] = v;
-        __syncthreads();
-        int s = 0, t = 0;
-#pragma unroll
-        for (int i = 0; i < kNW; ++i) t += at[i], s += i < wv ? at[i] : 0;
-        *all = t;
-        return s;
-    };
-    int any;
-    int mine = 0;
-    for (int t = s0 + lane; t - lane < s1; t += 64) mine += __popcll(__ballot(t < s1 && rank(min(t, n - 1)) == last));
-    const int tie0 = before_waves(mine, sh, &any);
+    // tokens of rank `last` and of larger ones, among the wave's slots below the budget and the others
+    int4 mine = {0, 0, 0, 0};
+    for (int t = s0 + lane; t - lane < s1; t += 64) {
+        const uint32_t r = rank(min(t, n - 1));
+        const unsigned long same = __ballot(t < s1 && r == last), more = __ballot(t < s1 && r > last), low = __ballot(t < p.budget);
+        mine.x += __popcll(same & low), mine.y += __popcll(same & ~low);
+        mine.z += __popcll(more & low), mine.w += __popcll(more & ~low);
+    }
+    if (lane == 0) parts[wv] = mine;
+    __syncthreads();
+    // of wave `lane`: ties before its slots, then the places and tokens for them that it has
+    const int4 of_wave = lane < kNW ? parts[lane] : int4{0, 0, 0, 0};
+    const int w0 = min(n, lane * span), w1 = lane < kNW ? min(n, w0 + span) : w0;
+    const int tie_sum = wave_scan_i(of_wave.x + of_wave.y), tie_before = tie_sum - of_wave.x - of_wave.y;
+    const int stay = ties - tie_before;          // of them that stay from the wave's first on
+    const int places = min(w1, p.budget) - min(w0, p.budget) - of_wave.z - min(max(stay, 0), of_wave.x);
+    const int tokens = of_wave.w + min(max(stay - of_wave.x, 0), of_wave.y);
+    const int place_sum = wave_scan_i(places), token_sum = wave_scan_i(tokens);
+    const int n_moves = __builtin_amdgcn_readlane(token_sum, 63);
+    int tie = __builtin_amdgcn_readlane(tie_before, wv);
+    int place = __builtin_amdgcn_readlane(place_sum - places, wv), token = __builtin_amdgcn_readlane(token_sum - tokens, wv);
     const unsigned long below = (1ul << lane) - 1;
-    auto kept = [&](int t, int &tie) {           // of the wave's 64 slots from t - lane on; tie: ties before them
+    int *to = MOVES ? places_of : p.moves + ((long)b * p.c.Hkv + h) * 2 * p.most_moves, *of = to + p.most_moves;
+    for (int t = s0 + lane; t - lane < s1; t += 64) {
         const uint32_t r = rank(min(t, n - 1));
         const unsigned long same = __ballot(t < s1 && r == last);
         const bool keep = r > last || (r == last && tie + __popcll(same & below) < ties);
         tie += __popcll(same);
-        return keep;
-    };
-    int tie = tie0, places = 0, tokens = 0;
-    for (int t = s0 + lane; t - lane < s1; t += 64) {
-        const bool keep = kept(t, tie);
-        places += __popcll(__ballot(t < s1 && t < p.budget && !keep));
-        tokens += __popcll(__ballot(t < s1 && t >= p.budget && keep));
-    }
-    if (lane == 0) picked_places[wv] = places;
-    int n_moves, place = 0;
-    int token = before_waves(tokens, sh2, &n_moves);
-    for (int i = 0; i < wv; ++i) place += picked_places[i];
-    int *to = MOVES ? places_of : p.moves + ((long)b * p.c.Hkv + h) * 2 * p.most_moves, *of = to + p.most_moves;
-    tie = tie0;
-    for (int t = s0 + lane; t - lane < s1; t += 64) {
-        const bool keep = kept(t, tie);
         const unsigned long a = __ballot(t < s1 && t < p.budget && !keep), c = __ballot(t < s1 && t >= p.budget && keep);
         if (a >> lane & 1) to[min(place + (int)__popcll(a & below), p.most_moves - 1)] = t;
         if (c >> lane & 1) of[min(token + (int)__popcll(c & below), p.most_moves - 1)] = t;
