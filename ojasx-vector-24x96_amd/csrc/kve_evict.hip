@@ -12,17 +12,17 @@
 // from counts in LDS, then numbers the places and the tokens for them with wave ballots.
 //
 // One workgroup for a (sequence, head), since every pass of the selection needs all of its ranks and
-// those of 32768 tokens fit LDS.  What is read is small (8 bytes a token and head; of a moved token
-// its rows besides), so the time is that of a chain of steps that wait for each other: block table,
-// positions and weights, four counts, two walks over the ballots.  11-bit digits, in three passes,
-// took as long as four of 8 bits.  Up to kMoveInPlace moves the workgroup does itself, four units of
+// those of 32768 tokens fit LDS (of more they lie in the workspace).  What is read is small (8 bytes
+// a token and head; of a moved token its rows besides), so the time is that of a chain of steps that
+// wait for each other: block table, positions and weights, four counts, two walks with ballots.
+// 11-bit digits, in three passes, took as long as four of 8 bits.  Up to kMoveInPlace moves the workgroup does itself, four units of
 // a thread in flight; more are a second launch over the whole card, one unit of a thread in flight
 // (16.8 us against 23.0 for four, for 8 sequences of 4096 that leave 1024).
 //
 // Measured, bf16, 8 heads of 128, the launches without the append: 64 sequences of 2064 tokens that
-// leave 2048: 17.5 us (1 sequence of 1008 fp32 tokens: 9.6 us); 8 sequences of 4096 that leave 1024: 19 us
-// and 17 us for their moves; a sequence of 65536, whose ranks are formed anew in
-// each pass: 272 us.
+// leave 2048: 18 us (1 sequence of 1008 fp32 tokens: 10 us); 8 sequences of 4096 that leave 1024: 18 us and
+// 17 us for their moves; a sequence of 65536, whose ranks lie in the workspace: 138 us (formed anew
+// in each pass: 272).
 #include <climits>
 
 #include "kve.h"
@@ -33,7 +33,7 @@ namespace {
 constexpr int kDigitBits = 8;            // of a rank's 32: four passes
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kCopies = 8;               // counters of a digit, so that equal digits of a wave's lanes collide less
-constexpr int kRanksInLds = 32768;       // tokens whose ranks are kept (128 KB); of more they are formed again
+constexpr int kRanksInLds = 32768;       // tokens whose ranks lie in LDS (128 KB); those of more in the workspace
 constexpr int kMoveInPlace = 256;        // moves that the selecting workgroup does itself
 // Threads of a selecting workgroup.  One that has a CU of its own takes kWideNT (8 sequences of 4096 tokens, 8
 // heads: 21 us against 29 with 512); where a CU takes several, each is faster with fewer, which leave fewer
@@ -48,6 +48,7 @@ struct KveEvictParams {
     const int *held;
     int *moves;                 // [B][Hkv][2][most_moves]: places, tokens for them
     int *counts;                // [B][Hkv]
+    uint32_t *ranks;            // [B][Hkv][most], where they are too many for LDS
     int budget, sink, recent, most, most_moves, in_lds;
 };
 
@@ -143,27 +144,48 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     }
     for (int i = tid; i < kDigits * kCopies; i += kNT) counts[i] = 0;
     newest = block_max<NT>(newest, sh);
-    auto form = [&](int t) {
-        const long at = kve_row(p.c, b, t);
-        return at < 0 ? 0u : rank_of(at, p.c.pos[at + hrow], p.c.w[at + hrow], newest);
-    };
-    if (p.in_lds)
-        for (int t0 = tid; t0 - tid < n; t0 += kNT * kBatch) {
-            if (!once) load(t0, true);
+    uint32_t *far = p.ranks + ((long)b * p.c.Hkv + h) * p.most;
+    for (int t0 = tid; t0 - tid < n; t0 += kNT * kBatch) {
+        if (!once) load(t0, true);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (t0 + i * kNT < n) ranks[t0 + i * kNT] = rank_of(row[i], pos[i], w[i], newest);
+        for (int i = 0; i < kBatch; ++i) {
+            const int t = t0 + i * kNT;
+            if (t >= n) continue;
+            const uint32_t r = rank_of(row[i], pos[i], w[i], newest);
+            if (p.in_lds) ranks[t] = r;
+            else far[t] = r;
         }
-    auto rank = [&](int t) { return p.in_lds ? ranks[t] : form(t); };
+    }
+    // The counts below read the ranks of the thread's own tokens; others' are read behind their barriers.
+    // f(t, rank of t) for t = first, first + apart, ... by whole waves while any lane's is before `end`; four
+    // ranks under way at a time, where a thread has that many.  At or past the end f gets some rank.
+    auto walk = [&](int first, int end, int apart, auto f) {
+        constexpr int kAtOnce = 4;
+        if (once) {
+            for (int t = first; t - lane < end; t += apart) f(t, ranks[min(t, n - 1)]);
+            return;
+        }
+        for (int t0 = first; t0 - lane < end; t0 += kAtOnce * apart) {
+            uint32_t r[kAtOnce];
+            if (p.in_lds) {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) r[i] = ranks[min(t0 + i * apart, n - 1)];
+            } else {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) r[i] = far[min(t0 + i * apart, n - 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) f(t0 + i * apart, r[i]);
+        }
+    };
     // the rank of the budget-th largest: `above` are larger
     uint32_t last = 0;
     int above = 0;
     uint32_t high = 0;                           // the bits of `last` that are known
     for (int shift = 32 - kDigitBits;; shift -= kDigitBits) {
-        for (int t = tid; t < n; t += kNT) {
-            const uint32_t r = rank(t);
-            if (((r ^ last) & high) == 0) atomicAdd(&counts[((r & ~high) >> shift) * kCopies + lane % kCopies], 1);
-        }
+        walk(tid, n, kNT, [&](int t, uint32_t r) {
+            if (t < n && ((r ^ last) & high) == 0) atomicAdd(&counts[((r & ~high) >> shift) * kCopies + lane % kCopies], 1);
+        });
         __syncthreads();
         // a digit for each of the first threads, the largest first
         const int d = kDigits - 1 - tid;
@@ -192,12 +214,11 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     const int span = ((n + kNW - 1) / kNW + 63) & ~63, s0 = min(n, wv * span), s1 = min(n, s0 + span);
     // tokens of rank `last` and of larger ones, among the wave's slots below the budget and the others
     int4 mine = {0, 0, 0, 0};
-    for (int t = s0 + lane; t - lane < s1; t += 64) {
-        const uint32_t r = rank(min(t, n - 1));
+    walk(s0 + lane, s1, 64, [&](int t, uint32_t r) {
         const unsigned long same = __ballot(t < s1 && r == last), more = __ballot(t < s1 && r > last), low = __ballot(t < p.budget);
         mine.x += __popcll(same & low), mine.y += __popcll(same & ~low);
         mine.z += __popcll(more & low), mine.w += __popcll(more & ~low);
-    }
+    });
     if (lane == 0) parts[wv] = mine;
     __syncthreads();
     // of wave `lane`: ties before its slots, then the places and tokens for them that it has
@@ -213,8 +234,7 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     int place = __builtin_amdgcn_readlane(place_sum - places, wv), token = __builtin_amdgcn_readlane(token_sum - tokens, wv);
     const unsigned long below = (1ul << lane) - 1;
     int *to = MOVES ? places_of : p.moves + ((long)b * p.c.Hkv + h) * 2 * p.most_moves, *of = to + p.most_moves;
-    for (int t = s0 + lane; t - lane < s1; t += 64) {
-        const uint32_t r = rank(min(t, n - 1));
+    walk(s0 + lane, s1, 64, [&](int t, uint32_t r) {
         const unsigned long same = __ballot(t < s1 && r == last);
         const bool keep = r > last || (r == last && tie + __popcll(same & below) < ties);
         tie += __popcll(same);
@@ -223,7 +243,7 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
         if (c >> lane & 1) of[min(token + (int)__popcll(c & below), p.most_moves - 1)] = t;
         place += __popcll(a);
         token += __popcll(c);
-    }
+    });
     if (!MOVES) {
         if (tid == 0) *number = n_moves;
         return;
@@ -260,7 +280,9 @@ int evict_plan(const KveView &v, int budget, int sink, int recent, int max_held,
     p->most = max_held && max_held < v.cap ? max_held : v.cap;
     const int over = p->most - budget;
     p->most_moves = over <= 0 ? 0 : over < budget ? over : budget;
-    p->bytes = p->most_moves ? ((long)v.B * v.Hkv * (2L * p->most_moves + 1) * 4 + 15) / 16 * 16 : 0;
+    // moves and their numbers; ranks
+    const long words = 2L * p->most_moves + 1 + (p->most > kRanksInLds ? p->most : 0);
+    p->bytes = p->most_moves ? ((long)v.B * v.Hkv * words * 4 + 15) / 16 * 16 : 0;
     return OJASX_OK;
 }
 
@@ -324,6 +346,7 @@ OJASX_API int ojasx_kve_evict_device(const OjasxKVECache *cache, const int *held
     p.held = held;
     p.counts = static_cast<int *>(workspace);
     p.moves = p.counts + (long)p.c.B * p.c.Hkv;
+    p.ranks = reinterpret_cast<uint32_t *>(p.moves + (long)p.c.B * p.c.Hkv * 2 * pl.most_moves);
     p.budget = budget, p.sink = sink_tokens, p.recent = recent_tokens;
     p.most = pl.most, p.most_moves = pl.most_moves, p.in_lds = pl.most <= kRanksInLds;
     hipStream_t st = static_cast<hipStream_t>(stream);
