@@ -26,7 +26,7 @@
 // a whole sequence finishes output and weights itself.
 //
 // Bound by reading the pages.  Measured, bf16, 32 / 8 heads of 128: 64 sequences of 192000 tokens in
-// all, 167 us (4.8 TB/s; without counting 146, 5.4) and join 18; one of 131072, 103 to 114 and 13; fp32, one of
+// all, 167 us (4.8 TB/s; without counting 146, 5.4) and join 17; one of 131072, 103 to 114 and 13; fp32, one of
 // 2048: 10 and 6.5, both a launch and the chain of its loads.
 //
 // Scores, maxima, sums and outputs are fp32.  Weights are rounded to bf16 or fp16 for the value
@@ -353,7 +353,7 @@ __device__ __forceinline__ void add_weights(const KveDecodeParams &p, const KveI
         }
 #pragma unroll
         for (int i = 0; i < kTokens; ++i) weight[i] = row[i] < 0 ? 0.f : p.c.w[row[i] + hrow];
-#pragma unroll 2
+#pragma unroll 4
         for (int r = 0; r < p.R; ++r) {
             float s[kTokens];
 #pragma unroll
