@@ -233,6 +233,14 @@ DECODES = [  # D, dtype, page, kv heads, query heads, lengths
     (128, "bfloat16", 16, 1, 128, [75, 130]),                 # the most query heads of a kv head
     (64, "float32", 16, 1, 128, [35]),
     (128, "float16", 16, 2, 46, [99, 32]),
+    # every build's most shared memory: scores of more tokens than it holds
+    (256, "bfloat16", 16, 1, 32, [600, 33]),
+    (256, "float32", 16, 2, 32, [900, 770, 12]),
+    (256, "float16", 16, 2, 8, [3500]),
+    (128, "float32", 16, 1, 32, [500, 390]),
+    (128, "bfloat16", 16, 2, 64, [388, 800]),
+    (64, "float32", 16, 2, 64, [388, 400]),
+    (64, "float16", 16, 2, 32, [449, 900, 448]),
 ]
 
 
