@@ -25,8 +25,8 @@
 // What is read is small (2 or 4 bytes a logit); bound by the fp64 products of the exponentials and,
 // with cuts, two additions in LDS for each token in 1., and for few rows by the chains of three
 // launches.  Measured: 256 rows of 32000 fp16 logits without cuts 11 + 9 us (1. and 3.), 64 rows of
-// 151936 bf16 ones with settings of their own 20 + 17 + 20 us, one row of 151936 fp32 ones with top-k
-// 50 and top-p 0.9 7 + 9 + 15.5 us.  Keeping a row's workgroups on one die's L2 took 3 % off rows that
+// 151936 bf16 ones with settings of their own 19 + 18 + 20 us, 256 such rows with top-k 50 and top-p 0.9
+// 53 + 41 + 14, one row of 151936 fp32 ones with the same 7 + 9 + 15.5 us.  Keeping a row's workgroups on one die's L2 took 3 % off rows that
 // all have cuts and cost as much where only some have.
 #include <cfloat>
 #include <climits>
@@ -187,6 +187,32 @@ __device__ __forceinline__ void load_logits(const T *row, int i, int V, float (&
     }
 }
 
+// A thread's tokens of a slice that begins at s0, all loads of a slice within the vocabulary under way together.
+template <typename T>
+__device__ __forceinline__ void load_slice(const T *row, int s0, int V, float (&x)[kSteps][kPer]) {
+    typedef unsigned int u4_any __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr int kVecs = sizeof(T) / 2;
+    const int i0 = s0 + (int)threadIdx.x * kPer;
+    if (s0 + kSlice <= V) {
+        u4_any raw[kSteps][kVecs];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j)
+                raw[i][j] = reinterpret_cast<const u4_any *>(row + i0 + i * (kSliceNT * kPer))[j];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            T part[kPer];
+            __builtin_memcpy(part, raw[i], sizeof(part));
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) x[i][e] = as_f32(part[e]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) load_logits(row, i0 + i * (kSliceNT * kPer), V, x[i]);
+    }
+}
+
 template <int CTRL>
 __device__ __forceinline__ double dpp_d(double v) {
     return __hiloint2double(dpp_i<CTRL>(__double2hiint(v)), dpp_i<CTRL>(__double2loint(v)));
@@ -267,9 +293,7 @@ __global__ __launch_bounds__(kSliceNT) void sample_slice_kernel(SampleParams a, 
     const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
     float x[kSteps][kPer];
     const int i0 = s * kSlice + tid * kPer;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-        load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0 + i * (kSliceNT * kPer), a.vocab, x[i]);
+    load_slice(static_cast<const T *>(a.logits) + (long)r * a.stride, s * kSlice, a.vocab, x);
     const Row row = row_of(a, r);
     if (row.cuts())
         for (int i = tid; i < kBins * kCopies; i += kSliceNT) sum[i] = 0, count[i] = 0;
@@ -486,22 +510,34 @@ __global__ __launch_bounds__(kSliceNT) void sample_list_kernel(SampleParams a, W
     // loaded no earlier: the registers that they take leave room for fewer waves beside this one
     float x[kSteps][kPer];
     const int i0 = s * kSlice + tid * kPer;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-        load_logits(static_cast<const T *>(a.logits) + (long)r * a.stride, i0 + i * (kSliceNT * kPer), a.vocab, x[i]);
+    load_slice(static_cast<const T *>(a.logits) + (long)r * a.stride, s * kSlice, a.vocab, x);
     const CutBins cut = cut_bins(L, row, h);
     if (s == 0 && tid == 0) *reinterpret_cast<CutBins *>(wk.rows[r].cut) = cut;
     if (L.off[s] >= kBins) return;
     if (tid < kBins / 32) words[tid] = cut.word(tid);
     __syncthreads();
+    // No logit below it is in the cuts' bins, so that few need the product that finds a logit's bin (256 rows of
+    // 151936 with top-k 50 and top-p 0.9: 55 to 45 us; a cut that keeps most tokens takes 0.3 us more).
+    const int lowest = max(max(cut.k < kBins - 1 ? cut.k : 0, cut.m < kBins - 1 ? cut.m : 0), cut.p0 <= cut.p1 ? cut.p1 : 0);
+    const double under = ((double)(h.top - lowest) - 1.0) / row.bins;
+    const float least = under > -(double)row.limit ? (float)(under - fabs(under) * 0x1p-20) : -INFINITY;
+    float most[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        most[i] = x[i][0];
+#pragma unroll
+        for (int e = 1; e < kPer; ++e) most[i] = fmaxf(most[i], x[i][e]);
+    }
     unsigned mine = 0;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
+    for (int i = 0; i < kSteps; ++i) {
+        if (!__any(most[i] >= least)) continue;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
             const int b = row.behind(h.top, x[i][e]);
             mine |= (words[b >> 5] >> (b & 31) & 1) << (i * kPer + e);
         }
+    }
     // places in the list: of the wave's tokens, of the workgroup's, of the row's
     const int n = __popc(mine), upto = wave_scan_i(n), all = __builtin_amdgcn_readlane(upto, 63);
     unsigned at = 0;
