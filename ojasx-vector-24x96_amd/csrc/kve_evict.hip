@@ -161,7 +161,7 @@ __global__ __launch_bounds__(NT) void kve_select_kernel(KveEvictParams p) {
     // ranks under way at a time, where a thread has that many.  At or past the end f gets some rank.
     auto walk = [&](int first, int end, int apart, auto f) {
         constexpr int kAtOnce = 4;
-        if (once) {
+        if (once && p.in_lds) {                  // a few tokens under a bound past LDS have their ranks in the workspace
             for (int t = first; t - lane < end; t += apart) f(t, ranks[min(t, n - 1)]);
             return;
         }

@@ -520,6 +520,38 @@ def test_evict_long(lc, dev, n, budget):
     check_evict(c, [n, n // 2], budget, 4, 1000)
 
 
+def roomy(lc, dev, dtype, Hkv, held, capacity, seed):
+    """Sequences with pages for what they hold alone, in a table of `capacity` slots each; positions from a
+    place of each sequence's own on, in order."""
+    import torch
+    page, B = 64, len(held)
+    pages = [-(-n // page) for n in held]
+    c = lc.PagedEvictingKVCache(Hkv, 64, num_sequences=B, page_size=page, max_pages=capacity // page, num_pages=sum(pages),
+                                dtype=getattr(torch, dtype), device=dev)
+    order, first = np.random.default_rng(seed).permutation(sum(pages)).astype(np.int32), cum(pages)
+    for b in range(B):
+        c.block_table[b, :pages[b]] = torch.from_numpy(order[first[b]:first[b + 1]]).to(dev)
+    for t, s in ((c.keys, 1), (c.values, 2)):
+        t.copy_(rand(dev, dtype, t.shape[0], Hkv, page, 64, seed=seed + s))
+    c.weights.copy_(torch.rand(c.weights.shape, generator=torch.Generator().manual_seed(seed)))
+    for b, n in enumerate(held):
+        p, s = place(c, b, np.arange(n))
+        c.positions[torch.from_numpy(p).long().to(dev), :, torch.from_numpy(s).long().to(dev)] = \
+            (torch.arange(n, device=dev) + 5 * b).to(torch.int32)[:, None]
+    return c
+
+
+@pytest.mark.parametrize("held,Hkv", [([40001, 3000, 4096, 4097, 900, 0], 2), ([2064, 33, 1], 1),
+                                      (cycled([900, 4096, 201, 4097, 20, 1025, 1024], 86), 3)])
+@pytest.mark.parametrize("budget,recent", [(200, 64), (800, 128), (2900, 0)])     # moves in place, by a launch of their own
+@pytest.mark.parametrize("max_held", [0, 40001])
+def test_evict_short_sequences_of_a_large_pool(lc, dev, held, Hkv, budget, recent, max_held):
+    """A bound past the ranks' place in LDS, sequences that hold few tokens: the newest and the first stay,
+    of the others those of largest weight."""
+    c = roomy(lc, dev, "bfloat16", Hkv, held, 40960, seed=51)
+    check_evict(c, held, budget, 4, recent, **(dict(max_held=max_held) if max_held else {}))
+
+
 def test_evict_lengths_out_of_range(lc, dev):
     c = filled(lc, dev, 64, "bfloat16", 16, 2, [96, 96, 96], seed=14, poison=False)
     check_evict(c, [2**31 - 1, -4, 97], 40, 4, 4)
