@@ -73,7 +73,7 @@ struct SliceBins {
     Bin upto[kBins];                     // sums and counts up to and with the bin; the last two alike
 };
 struct RowBins {                         // of the whole row, up to and with the bin
-    double sum[kBins];
+    double sum[kBins];                   // the last two alike
     int count[kBins];
     int cut[6];                          // CutBins
     unsigned listed;                     // tokens in the row's list
@@ -401,10 +401,11 @@ __device__ __forceinline__ void load_slices(CutLds &L, const Row &row, const Row
     }
     __syncthreads();
 }
-// The row's bins, a thread for each, the slices in order.
+// The row's bins, a thread for each, the slices in order; the last as the one before it, as a slice's are: a
+// slice whose first bin is behind the row's has tokens there, and they are not drawn.
 __device__ __forceinline__ void add_bins(CutLds &L, const SliceBins *bins, int S) {
     constexpr int kAtOnce = 20;                  // slices' loads in flight
-    const int j = threadIdx.x;
+    const int j = min((int)threadIdx.x, kBins - 2);
     double w = 0.0;
     int n = 0;
     for (int s0 = 0; s0 < S; s0 += kAtOnce) {
@@ -423,7 +424,7 @@ __device__ __forceinline__ void add_bins(CutLds &L, const SliceBins *bins, int S
             n += in ? (int)t[i][2] : 0;
         }
     }
-    L.wsum[j] = w * 0x1p-50, L.wcount[j] = n;
+    L.wsum[threadIdx.x] = w * 0x1p-50, L.wcount[threadIdx.x] = n;
     __syncthreads();
 }
 // The first bin that reaches `need`, or kBins: none does; sums and counts never fall from bin to bin.

@@ -104,6 +104,26 @@ def test_equal_logits(sample, dev):
         check(sample, dev, two.bfloat16(), u, T=0.4, **s)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_tokens_next_to_those_not_drawn(sample, dev, dtype):
+    """Tokens 36.4 temperatures below the largest, e about 2^-52.5, in a slice whose own largest is below the
+    row's: none is drawn, and a top-k cut among them keeps all that can be."""
+    import torch
+    x = torch.full((12, 24576), -60000.0)
+    x[:, 0] = 0.0
+    for b, top in enumerate((-1.0, -0.125, -3.0, -20.0) * 3):
+        x[b, 8192 + b] = top
+        x[b, 8300:8310] = -25.5
+        x[b, 16384 + b:16390] = -25.5                 # a slice of nothing else
+    x = x.to(getattr(torch, dtype))
+    for k in (1, 2, 3, 5, 11, 12, 13, 18, 30):
+        for s in (dict(), dict(p=0.5), dict(p=0.999999), dict(m=1e-12), dict(p=0.9, m=0.01)):
+            got = check(sample, dev, x, grid(12), T=0.7, k=k, **s)
+            assert all(t in (0, 8192 + b) for b, t in enumerate(got))
+    for s in (dict(), dict(p=0.5), dict(p=1 - 1e-7)):
+        check(sample, dev, x, grid(12), T=0.7, **s)
+
+
 def test_masked_logits(sample, dev):
     """Logits of -inf are never drawn, the type's lowest value only where nothing else is."""
     import torch
