@@ -20,7 +20,10 @@
 //
 // A drawn token is a whole number: it has to be the definition's own.  So e is fp64 to about
 // 2^-50, sums are fp64, or in LDS, where they are added in any order, 64-bit integers: a fixed
-// number of bits behind the point, the same result in every order.
+// number of bits behind the point, the same result in every order.  A slice's sums have 50 bits, relative
+// to its largest e: 8192 equal logits that round alike are off by 2^-38 of it, 3.6e-12.  A bin's sums are
+// relative to the bin's largest.  What is not drawn and lies in a bin that is counted shifts a border by
+// 2^-51 for each such token.
 //
 // What is read is small (2 or 4 bytes a logit); bound by the fp64 products of the exponentials and,
 // with cuts, two additions in LDS for each token in 1., and for few rows by the chains of three
@@ -141,9 +144,7 @@ struct Row {
         const int b = min(top - bin(x), kBins - 1);
         return x == -INFINITY ? kBins - 1 : b;
     }
-    __device__ __forceinline__ double e(float x, float most) const {
-        return exp2_f64(fmax((double)x - (double)most, -depth), c);
-    }
+    __device__ __forceinline__ double e(double x, double most) const { return exp2_f64(fmax(x - most, -depth), c); }
 };
 __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
     Row s;
@@ -571,7 +572,7 @@ struct RowLds {
     double kept[kMostSlices];
     u64 csum[kMostSlices];               // of the cut's bin: sum of e above kappa, tokens at kappa
     int cties[kMostSlices];
-    double dw[kNW], rest;
+    double dw[kNW], rest, unit;           // unit: of csum
     unsigned kmin[2], kmax[2];
     u64 uw[kDigits / 64];
     Found found[kDigits / 64];
@@ -588,12 +589,13 @@ struct Chosen {
     const RowHead &h;
     const uint2 *list;
     int n;                               // tokens of the list; in LDS if kList of them are enough
-    int frac;                            // bits behind the point of sums over the row
+    int frac;                            // bits behind the point of a bin's sums
     int set;                             // of the digits' sums and counts, the one that is clear
 
-    // f(index, key, e) for the listed tokens of bin b; with_e: e is formed, for four tokens at once
+    // f(index, key, e relative to the logit `top`) for the listed tokens of bin b; with_e: e is formed, for four
+    // tokens at once
     template <bool with_e, typename F>
-    __device__ __forceinline__ void each(int b, F f) const {
+    __device__ __forceinline__ void each(int b, double top, F f) const {
         constexpr int kAtOnce = 4;
         for (int i0 = threadIdx.x; i0 < n; i0 += kAtOnce * kNT) {
             uint2 t[kAtOnce];
@@ -606,11 +608,17 @@ struct Chosen {
                 for (int i = 0; i < kAtOnce; ++i) t[i] = list[min(i0 + i * kNT, n - 1)];
             }
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) e[i] = with_e ? row.e(of_key(t[i].x), h.most) : 0.0;
+            for (int i = 0; i < kAtOnce; ++i) e[i] = with_e ? row.e(of_key(t[i].x), top) : 0.0;
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i)
                 if (i0 + i * kNT < n && (int)(t[i].y >> 24) == b) f((int)(t[i].y & 0xffffffu), t[i].x, e[i]);
         }
+    }
+    // A logit that none of bin b is above, nor further below than the bin's width unless the bin is one of all
+    // beyond row.limit.  Sums of the bin are of e relative to it: relative to the row's largest, the step of a
+    // fixed point is as much as the e of a far bin's tokens, and equal logits all round the same way.
+    __device__ __forceinline__ double bin_top(int b) const {
+        return b ? ((double)(h.top - b) + 0.5) / row.bins : (double)h.most;
     }
     // The key of T's values whose high bits they are.
     static __device__ __forceinline__ unsigned whole_key(unsigned high) {
@@ -622,11 +630,13 @@ struct Chosen {
     // of the key's distance to the bin's lowest, without the bits that T's values never use.  call: 0, 1.
     __device__ void select(int call, int b, bool by_sum, double need, unsigned *kappa, int *ties, double *sum) {
         unsigned kmin = 0xffffffffu, kmax = 0;
-        each<false>(b, [&](int, unsigned k, double) { kmin = min(kmin, k), kmax = max(kmax, k); });
+        each<false>(b, 0.0, [&](int, unsigned k, double) { kmin = min(kmin, k), kmax = max(kmax, k); });
         kmin = (unsigned)wave_min_i((int)(kmin ^ 0x80000000u)) ^ 0x80000000u;
         kmax = ~((unsigned)wave_min_i((int)(~kmax ^ 0x80000000u)) ^ 0x80000000u);
         if ((threadIdx.x & 63) == 0 && kmin <= kmax) atomicMin(&L.kmin[call], kmin), atomicMax(&L.kmax[call], kmax);
         __syncthreads();
+        const double top = bin_top(b), unit = row.e(top, h.most);
+        if (by_sum) need /= unit;
         kmin = L.kmin[call] >> kLow, kmax = L.kmax[call] >> kLow;
         unsigned prefix = 0;
         // all in whole numbers, sums with frac bits behind the point: exactly one digit is the first to reach
@@ -645,8 +655,8 @@ struct Chosen {
                 atomicAdd(&hcount[q >> shift & (kDigits - 1)], 1u);
             };
             // the last digit's tokens have one key each: their sum is a multiple of its e
-            if (shift) each<true>(b, add);
-            else each<false>(b, add);
+            if (shift) each<true>(b, top, add);
+            else each<false>(b, top, add);
             __syncthreads();
             // a digit for each of the first threads, the largest first
             const int d = kDigits - 1 - (int)threadIdx.x, w = threadIdx.x / 64;
@@ -654,7 +664,7 @@ struct Chosen {
             int c = 0, n_upto = 0;
             if (threadIdx.x < kDigits) {
                 c = (int)hcount[d];
-                const double e = row.e(fminf(of_key(whole_key((prefix | (unsigned)d) + kmin)), h.most), h.most);
+                const double e = row.e(fmin((double)of_key(whole_key((prefix | (unsigned)d) + kmin)), top), top);
                 mine = shift ? hsum[d] : c ? c * fixed(e, frac) : 0;                // no token: e of any key
                 upto = wave_scan_u(mine), n_upto = wave_scan_i(c);
                 if ((threadIdx.x & 63) == 63) L.uw[w] = upto, L.iw[w] = n_upto;
@@ -687,12 +697,12 @@ struct Chosen {
         }
         const double sums = (double)above * ldexp(1.0, -frac);
         prefix = whole_key(prefix + kmin);
-        const double e = row.e(of_key(prefix), h.most);
+        const double e = row.e(of_key(prefix), top);
         double t = by_sum ? ceil((need - sums) / e) : need - counts;
         t = fmin(fmax(t, 1.0), (double)last_count);
         *kappa = prefix;
         *ties = (int)t;
-        *sum = sums + t * e;
+        *sum = (sums + t * e) * unit;
     }
 };
 }  // namespace
@@ -713,10 +723,10 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
     for (int s = tid; s < S; s += kNT) L.csum[s] = 0, L.cties[s] = 0;
     if (tid < 2) L.kmin[tid] = 0xffffffffu, L.kmax[tid] = 0;
     if (tid < kDigits) L.hsum[0][tid] = 0, L.hcount[0][tid] = 0;
-    if (tid == 0) L.hit = INT_MAX, L.last = -1;
+    if (tid == 0) L.hit = INT_MAX, L.last = -1, L.unit = 0.0;
     unsigned kappa = 0;
     int ties = INT_MAX, jc = kBins - 1;
-    const int frac = min(kFrac, 62 - (32 - __clz(a.vocab)));
+    const int frac = min(kFrac, 62 - (32 - __clz(a.vocab)));   // a sum of e of all tokens fits
     if (row.cuts()) {
         const RowBins &of = wk.rows[r];
         Chosen<T> d{row, L, h, wk.list + (long)r * a.vocab, (int)of.listed, frac, 0};
@@ -747,8 +757,9 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         if (row.m_cut && cut.m_key > kappa) kappa = cut.m_key, ties = INT_MAX;
         // the bin of the cut; a slice keeps its bins before that, and of its tokens in that bin those above kappa
         if (kappa) jc = min(max(h.top - row.bin(of_key(kappa)), 0), kBins - 1);
-        d.template each<true>(jc, [&](int i, unsigned k, double e) {
-            if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(e, frac));
+        if (tid == 0) L.unit = ldexp(row.e(d.bin_top(jc), h.most), -kFrac);
+        d.template each<true>(jc, d.bin_top(jc), [&](int i, unsigned k, double e) {
+            if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(e, kFrac));      // a slice's, as its bins'
             if (k == kappa) atomicAdd(&L.cties[i / kSlice], 1);
         });
         __syncthreads();
@@ -762,7 +773,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         for (int s = s0; s < s1; ++s) before += L.cties[s];
         before = wave_scan_i(before) - before;   // ties of the slices before
         const int ties0 = before;
-        const double e = kappa ? row.e(of_key(kappa), h.most) : 0.0, unit = ldexp(1.0, -frac);
+        const double e = kappa ? row.e(of_key(kappa), h.most) : 0.0, unit = L.unit;
         double mine = 0.0;
         for (int s = s0; s < s1; ++s) {
             const int b = jc - 1 - L.c.off[s];

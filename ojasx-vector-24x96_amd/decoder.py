@@ -68,8 +68,9 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     NaN or +inf among its logits, -inf alone, or a temperature that is negative,
     NaN or infinite) gives -1.
 
-    e and sums are fp64, so the token is the definition's own unless uniform lies
-    within about 1e-11 of a border; one whose e is below 2^-51 is not drawn.
+    e and sums are fp64 or of 50 bits, so the token is the definition's own unless
+    uniform, top_p or min_p lies within about 1e-11 + vocab 2^-51 of a border
+    (8e-11 for 151936 logits); one whose e is below 2^-51 is not drawn.
     The result does not depend on the other rows."""
     torch = _torch()
     if logits.dim() != 2:

@@ -197,6 +197,45 @@ def test_many_tokens_of_one_bin(sample, dev):
         check(sample, dev, x, grid(6), **s)
 
 
+@pytest.mark.parametrize("dtype,V,g", [("bfloat16", 151936, -20.75), ("float16", 151936, -20.75), ("float32", 151936, -20.7),
+                                       ("float32", 151936, -19.9), ("bfloat16", 1 << 22, -18.0), ("float32", 1 << 22, -17.3)])
+def test_top_p_among_many_small_equal_logits(sample, dev, dtype, V, g):
+    """One peak and small e = exp(g) everywhere else: top-p between the sums after the j-th of them and the
+    next one keeps j + 1.  Half an e from either border: 4.8e-10 of all or more, 7.1e-9 with 2^22 logits, where
+    sums may be off by 8e-11 and 1.9e-9."""
+    import torch
+    x = torch.full((6, V), g).to(getattr(torch, dtype))
+    x[:, 0] = 0.0
+    e = math.exp(float(x[0, 1]))
+    u = torch.ones(1, device=dev)                     # counts as the last number: the last kept token
+    for j in (0, 9, 1000, V // 3, V // 2 + 1, V - 3):
+        p = (1 + (j + 0.5) * e) / (1 + (V - 1) * e)
+        assert sample(x[:1].to(dev), u, top_p=p).tolist() == [j + 1], j
+        # top-k takes from the same tokens: their sum is the whole of top-p
+        k = V - V // 10
+        if j < k - 2:
+            p = (1 + (j + 0.5) * e) / (1 + (k - 1) * e)
+            assert sample(x[:1].to(dev), u, top_k=k, top_p=p).tolist() == [j + 1], j
+
+
+@pytest.mark.parametrize("dtype,V,T,a,b", [("bfloat16", 151936, 7.89, -164.0, -165.0), ("float16", 151936, 7.89, -164.0, -165.0),
+                                           ("float32", 151936, 7.84, -164.1, -164.7), ("float32", 151936, 0.858, -18.1, -18.15),
+                                           ("bfloat16", 1 << 22, 7.75, -139.0, -140.0)])
+def test_draws_among_many_small_equal_logits(sample, dev, dtype, V, T, a, b):
+    """Two values of one bin, the cut within the smaller: numbers in the middle of a token's share draw that
+    token, in early and late slices.  Half a share is 3.2e-10 of all or more (2^22 logits: 7e-9)."""
+    import torch
+    n, m, k = V * 2 // 3, V // 4, V * 2 // 3 + V // 8
+    x = torch.full((8, V), -60000.0)
+    x[:, :n], x[:, n:n + m], x[:, n + m] = a, b, 0.0
+    x = x.to(getattr(torch, dtype))
+    ea, eb = (math.exp(float(x[0, i]) / T) for i in (0, n))
+    at = [0, 1, 8191, 8192, n // 2, n - 1, n, n + V // 8 - 2]          # the peak is one of the k
+    total = 1 + n * ea + (k - 1 - n) * eb
+    u = [(min(i, n) * ea + max(i - n, 0) * eb + 0.5 * (ea if i < n else eb)) / total for i in at]
+    assert check(sample, dev, x, u, T=T, k=k) == at
+
+
 def test_strides_and_rows(sample, dev):
     import torch
     base = logits(6, 5003, "bfloat16", seed=10).to(dev)
