@@ -218,9 +218,31 @@ def test_top_p_among_many_small_equal_logits(sample, dev, dtype, V, g):
             assert sample(x[:1].to(dev), u, top_k=k, top_p=p).tolist() == [j + 1], j
 
 
-@pytest.mark.parametrize("dtype,V,T,a,b", [("bfloat16", 151936, 7.89, -164.0, -165.0), ("float16", 151936, 7.89, -164.0, -165.0),
-                                           ("float32", 151936, 7.84, -164.1, -164.7), ("float32", 151936, 0.858, -18.1, -18.15),
-                                           ("bfloat16", 1 << 22, 7.75, -139.0, -140.0)])
+ONE_BIN = [  # dtype, vocabulary, temperature, two logits of one bin
+    ("bfloat16", 151936, 7.89, -164.0, -165.0),
+    ("float16", 151936, 7.89, -164.0, -165.0),
+    ("float32", 151936, 7.84, -164.1, -164.7),
+    ("float32", 151936, 0.858, -18.1, -18.15),
+    ("bfloat16", 1 << 22, 7.75, -139.0, -140.0),
+]
+
+
+@pytest.mark.parametrize("dtype,V,T,a,b", ONE_BIN)
+def test_top_p_behind_many_small_equal_logits(sample, dev, dtype, V, T, a, b):
+    """The cut lies among the smaller of two values of one bin, behind the sum of all of the larger: half a share
+    from either border, as above."""
+    import torch
+    n, m = V * 2 // 3, V // 4
+    x = torch.full((1, V), -60000.0)
+    x[:, 0], x[:, 1:1 + n], x[:, 1 + n:1 + n + m] = 0.0, a, b
+    x = x.to(getattr(torch, dtype))
+    ea, eb = (math.exp(float(x[0, i]) / T) for i in (1, 1 + n))
+    for j in (0, 5, m // 2, m - 2):
+        p = (1 + n * ea + (j + 0.5) * eb) / (1 + n * ea + m * eb)
+        assert sample(x.to(dev), torch.ones(1, device=dev), temperature=T, top_p=p).tolist() == [1 + n + j], j
+
+
+@pytest.mark.parametrize("dtype,V,T,a,b", ONE_BIN)
 def test_draws_among_many_small_equal_logits(sample, dev, dtype, V, T, a, b):
     """Two values of one bin, the cut within the smaller: numbers in the middle of a token's share draw that
     token, in early and late slices.  Half a share is 3.2e-10 of all or more (2^22 logits: 7e-9)."""
