@@ -447,7 +447,8 @@ OJASX_API int ojasx_kve_append_device(const OjasxKVECache *cache, const void *q,
  * of a kv head); a sequence without tokens gives 0, one whose tokens all score
  * -inf NaN.  With count != 0 each token's softmax weights, summed over the query
  * heads of its kv head, are added to its weight.  Scores, sums and weights are
- * fp32; BF16 and F16 round the softmax's weights for the value product.
+ * fp32; for the product with BF16 and F16 values a softmax weight is the sum of two
+ * numbers of the type: to 2^-14 of it, F16 to 2^-20 of it or 2^-40 of the largest.
  * scale_factor <= 0: 1/sqrt(head_dim).  max_held bounds held[] (0: the pages'
  * slots) and with it launch and workspace; of a longer sequence the first
  * max_held tokens are attended.  workspace: ojasx_kve_decode_workspace(...) bytes

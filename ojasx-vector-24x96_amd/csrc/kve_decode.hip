@@ -29,9 +29,12 @@
 // all, 167 us (4.8 TB/s; without counting 146, 5.4) and join 17; one of 131072, 103 to 114 and 13; fp32, one of
 // 2048: 10 and 6.5, both a launch and the chain of its loads.
 //
-// Scores, maxima, sums and outputs are fp32.  Weights are rounded to bf16 or fp16 for the value
-// product (fp16: times 2^15, so that the smallest keep their share), and the sum that divides
-// the output is that of the rounded ones; the counted weights are divided by the exact sum.
+// Scores, maxima, sums, counted weights and outputs are fp32.  For the value product of bf16 and fp16 a
+// weight is the sum of two numbers of the type, and each tile's values are multiplied by both: to 2^-14 of
+// it in bf16, 2^-20 in fp16 (there times 2^15, so that the smallest keep their share, those below 2^-20 to
+// 2^-40 of the largest).  Both are above 0 where the weight is (fp16: from 2^-38 on): a value of infinity
+// meets no 0 that the split has made.  One number each would be off by 2^-8 and 2^-11, as much as the
+// output's own rounding; the matrix units are idle otherwise.
 #include <cfloat>
 #include <cmath>
 
@@ -74,7 +77,7 @@ struct KveDecodeParams {
     void *out;
     const int *held;
     float *part_o;              // [item][Rb][D]
-    float *part_ml;             // [item][Rb][4]: max, sum, sum of the rounded weights
+    float *part_ml;             // [item][Rb][2]: max, sum
     KveItem *items;      // what the first kernel's workgroups had, for the second's
     float *scores;              // [B][Hkv][tiles][R][tokens of a tile] times log2(e), or null: no weights
     int Hq, R, HB, Rb;          // query heads, of a kv head, blocks of those, heads of a block
@@ -166,25 +169,52 @@ __device__ __forceinline__ float swap16(float v, bool max_) {
 __device__ __forceinline__ float column_max(float v) { return swap16(swap32(v, true), true); }
 __device__ __forceinline__ float column_sum(float v) { return swap16(swap32(v, false), false); }
 
+// What the value product's weights are multiplied by.
+template <typename T>
+__device__ __forceinline__ constexpr float weight_scale() {
+    return __is_same(T, __half) ? 32768.f : 1.f;
+}
+
 template <typename T>
 struct Half;
 template <>
 struct Half<__hip_bfloat16> {
     typedef b8_t V8;
-    static constexpr float kScale = 1.f;
     static __device__ __forceinline__ f4_t mma(V8 a, V8 b, f4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
-    static __device__ __forceinline__ __bf16 from(float f) { return (__bf16)f; }
+    // hi: 2^-8 below the weight and cut off, so that lo is at least 2^-8 of it
+    static __device__ __forceinline__ void split(const float (&p)[8], V8 &hi, V8 &lo) {
+        u4_t h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned a = __float_as_uint(p[2 * i] * (1.f - 0x1p-8f)), b = __float_as_uint(p[2 * i + 1] * (1.f - 0x1p-8f));
+            h[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            lo[2 * i] = (__bf16)(p[2 * i] - __uint_as_float(a & 0xffff0000u));
+            lo[2 * i + 1] = (__bf16)(p[2 * i + 1] - __uint_as_float(b & 0xffff0000u));
+        }
+        hi = __builtin_bit_cast(V8, h);
+    }
 };
 template <>
 struct Half<__half> {
     typedef h8_t V8;
-    static constexpr float kScale = 32768.f;
     static __device__ __forceinline__ f4_t mma(V8 a, V8 b, f4_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
-    static __device__ __forceinline__ _Float16 from(float f) { return (_Float16)f; }
+    // hi: 2^-10 below the weight and cut off, so that lo is at least 2^-10 of it; half of one whose 2^-10 is
+    // next to the smallest number
+    static __device__ __forceinline__ void split(const float (&p)[8], V8 &hi, V8 &lo) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = p[2 * i] * weight_scale<__half>(), b = p[2 * i + 1] * weight_scale<__half>();
+            const auto h = __builtin_amdgcn_cvt_pkrtz(a * (a < 0x1p-13f ? 0.5f : 1.f - 0x1p-10f),
+                                                      b * (b < 0x1p-13f ? 0.5f : 1.f - 0x1p-10f));
+            hi[2 * i] = (_Float16)h[0], hi[2 * i + 1] = (_Float16)h[1];
+            lo[2 * i] = (_Float16)(a - (float)hi[2 * i]);
+            lo[2 * i + 1] = (_Float16)(b - (float)hi[2 * i + 1]);
+        }
+    }
 };
 
 // One tile of TT tokens of a page (or of two pages) in registers.
@@ -246,24 +276,25 @@ struct Tile {                                   // bf16, fp16: 32 tokens
             x[i] = __builtin_amdgcn_perm(v[2 * i + 1][n][d / 2], v[2 * i][n][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
         return __builtin_bit_cast(V8, x);
     }
-    // o += V^T P^T; returns the sum of the weights as the product takes them
+    // o += V^T P^T, two columns at a time, so that no product waits for the one before
     template <int NT>
-    __device__ __forceinline__ void values(const float (&p)[NT][E], f4_t (&o)[NT][D / 16], float (&sum)[NT]) const {
-        V8 w[NT];
+    __device__ __forceinline__ void values(const float (&p)[NT][E], f4_t (&o)[NT][D / 16]) const {
+        V8 hi[NT], lo[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                w[t][e] = Half<T>::from(p[t][e] * Half<T>::kScale);
-                sum[t] += (float)w[t][e];
-            }
+        for (int t = 0; t < NT; ++t) Half<T>::split(p[t], hi[t], lo[t]);
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
-            for (int d = 0; d < DL; ++d) {
-                const V8 a = column(n, d);
+            for (int d = 0; d < DL; d += 2) {
+                const V8 a = column(n, d), b = column(n, d + 1);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) o[t][n * DL + d] = Half<T>::mma(a, w[t], o[t][n * DL + d]);
+                for (int t = 0; t < NT; ++t) {
+                    f4_t &x = o[t][n * DL + d], &y = o[t][n * DL + d + 1];
+                    x = Half<T>::mma(a, hi[t], x);
+                    y = Half<T>::mma(b, hi[t], y);
+                    x = Half<T>::mma(a, lo[t], x);
+                    y = Half<T>::mma(b, lo[t], y);
+                }
             }
     }
     static __device__ __forceinline__ void load_q(const T *q, int c, V8 (&f)[NK]) {
@@ -310,11 +341,7 @@ struct Tile<float, D> {                         // 16 tokens
         for (int r = 0; r < 4; ++r) s[r] = a[r] + b[r];
     }
     template <int NT>
-    __device__ __forceinline__ void values(const float (&p)[NT][E], f4_t (&o)[NT][D / 16], float (&sum)[NT]) const {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < E; ++e) sum[t] += p[t][e];
+    __device__ __forceinline__ void values(const float (&p)[NT][E], f4_t (&o)[NT][D / 16]) const {
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
@@ -379,7 +406,7 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
     typedef Tile<T, D> Tl;
     constexpr int TT = Tl::TT, E = Tl::E, NA = D / 16;
     __shared__ int ish[kItemInts];
-    __shared__ float ml[kNW][NT * 16][3];
+    __shared__ float ml[kNW][NT * 16][2];
     __shared__ float buf[kNW / 2][NT * NA * 4][64];
     extern __shared__ float lds_scores[];
     const KveItem it = kve_item<TT>(p, ish);
@@ -399,10 +426,10 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
         if (t * 16 + i < heads)
             Tl::load_q(static_cast<const T *>(p.q) + ((size_t)it.b * p.Hq + it.h * p.R + head0 + t * 16 + i) * D, c, q[t]);
     f4_t o[NT][NA];
-    float m[NT], l[NT], lr[NT];
+    float m[NT], l[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY, l[t] = 0.f, lr[t] = 0.f;
+        m[t] = -INFINITY, l[t] = 0.f;
 #pragma unroll
         for (int a = 0; a < NA; ++a) o[t][a] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -481,7 +508,7 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
                     most = fmaxf(m[b], column_max(most));
                     const float f = most == -INFINITY ? 1.f : exp2f(m[b] - most);
                     m[b] = most;
-                    l[b] *= f, lr[b] *= f;
+                    l[b] *= f;
 #pragma unroll
                     for (int a = 0; a < NA; ++a) o[b][a] *= f;
                 }
@@ -497,7 +524,7 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
                 for (int e = 0; e < E; ++e)
                     if (!vin || e >= left) tl.clear_value(e);
             }
-            tl.template values<NT>(w, o, lr);
+            tl.template values<NT>(w, o);
             load_v(vp1, next);
             if (p.scores) {
                 const long tile = (long)(t - it.t0) * p.R;
@@ -511,8 +538,8 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
     // the four waves' (max, sums, out) joined: 2 into 0 and 3 into 1, then 1 into 0
 #pragma unroll
     for (int b = 0; b < NT; ++b) {
-        l[b] = column_sum(l[b]), lr[b] = column_sum(lr[b]);
-        if (c == 0) ml[wv][b * 16 + i][0] = m[b], ml[wv][b * 16 + i][1] = l[b], ml[wv][b * 16 + i][2] = lr[b];
+        l[b] = column_sum(l[b]);
+        if (c == 0) ml[wv][b * 16 + i][0] = m[b], ml[wv][b * 16 + i][1] = l[b];
     }
     __syncthreads();
     const int here = p.lds_scores / (p.R * TT) * TT;       // tokens whose scores are in LDS
@@ -528,12 +555,11 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
 #pragma unroll
         for (int x = 1; x < kNW; ++x) most = fmaxf(most, ml[x][b * 16 + i][0]);
         const float f = m[b] == -INFINITY ? 0.f : exp2f(m[b] - most);
-        l[b] = lr[b] = 0.f;
+        l[b] = 0.f;
 #pragma unroll
         for (int x = 0; x < kNW; ++x) {
             const float mx = ml[x][b * 16 + i][0], g = mx == -INFINITY ? 0.f : exp2f(mx - most);
             l[b] += ml[x][b * 16 + i][1] * g;
-            lr[b] += ml[x][b * 16 + i][2] * g;
         }
         if (f != 1.f) {                           // a wave without tokens has sums of 0, and no infinity to turn into NaN
 #pragma unroll
@@ -572,13 +598,14 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
             if (alone) {
                 // no tokens: 0; tokens that all score -inf: 0 / 0
                 T *to = static_cast<T *>(p.out) + ((size_t)it.b * p.Hq + it.h * p.R + head0 + head) * D;
+                const float sum = l[b] * weight_scale<T>();
 #pragma unroll
                 for (int n = 0; n < NA / Tl::DL; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int d = 0; d < Tl::DL; ++d)
-                            store_act(to, Tl::dim(n, c, r) + d, m[b] == -INFINITY ? 0.f : o[b][n * Tl::DL + d][r] / lr[b]);
+                            store_act(to, Tl::dim(n, c, r) + d, m[b] == -INFINITY ? 0.f : o[b][n * Tl::DL + d][r] / sum);
                 if (c == 0) ml[0][head][0] = m[b], ml[0][head][1] = 1.f / l[b];
             } else {
                 const long at = (long)blockIdx.x * p.Rb + head;
@@ -589,7 +616,7 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int d = 0; d < Tl::DL; ++d) to[Tl::dim(n, c, r) + d] = o[b][n * Tl::DL + d][r];
-                if (c == 0) *reinterpret_cast<f4_t *>(p.part_ml + at * 4) = f4_t{m[b], l[b], lr[b], 0.f};
+                if (c == 0) *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(m[b], l[b]);
             }
         }
     }
@@ -605,7 +632,7 @@ __global__ __launch_bounds__(kNT) void kve_decode_kernel(KveDecodeParams p) {
 // it).
 template <typename T, int D, int TT>
 __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
-    __shared__ float most[kMostGroup], inv[kMostGroup], rounded[kMostGroup];
+    __shared__ float most[kMostGroup], inv[kMostGroup], total[kMostGroup];
     const KveItem it = p.items[blockIdx.x];
     if (it.b < 0) return;
     const int tid = threadIdx.x, groups = p.c.Hkv * p.HB;
@@ -617,25 +644,23 @@ __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
     while (each > 4 && each * (h1 - h0) > kNT) each /= 2;
     for (int r0 = h0; r0 < h1; r0 += kNT / each) {
         const int r = min(r0 + tid / each, h1 - 1), sub = tid % each;
-        const float *of = p.part_ml + ((it.first + r / p.Rb - it.hb) * p.Rb + r % p.Rb) * 4;
-        const long step = (long)groups * p.Rb * 4;
-        float m = -INFINITY, l = 0.f, lr = 0.f;
+        const float *of = p.part_ml + ((it.first + r / p.Rb - it.hb) * p.Rb + r % p.Rb) * 2;
+        const long step = (long)groups * p.Rb * 2;
+        float m = -INFINITY, l = 0.f;
 #pragma unroll 4
         for (int j = sub; j < it.k; j += each) {
-            const f4_t x = *reinterpret_cast<const f4_t *>(of + j * step);
-            const float to = fmaxf(m, x[0]), f = m == -INFINITY ? 0.f : exp2f(m - to), g = x[0] == -INFINITY ? 0.f : exp2f(x[0] - to);
-            l = l * f + x[1] * g;
-            lr = lr * f + x[2] * g;
+            const float2 x = *reinterpret_cast<const float2 *>(of + j * step);
+            const float to = fmaxf(m, x.x), f = m == -INFINITY ? 0.f : exp2f(m - to), g = x.x == -INFINITY ? 0.f : exp2f(x.x - to);
+            l = l * f + x.y * g;
             m = to;
         }
         for (int o = 1; o < each; o *= 2) {
-            const float xm = __shfl_xor(m, o), xl = __shfl_xor(l, o), xr = __shfl_xor(lr, o);
+            const float xm = __shfl_xor(m, o), xl = __shfl_xor(l, o);
             const float to = fmaxf(m, xm), f = m == -INFINITY ? 0.f : exp2f(m - to), g = xm == -INFINITY ? 0.f : exp2f(xm - to);
             l = l * f + xl * g;
-            lr = lr * f + xr * g;
             m = to;
         }
-        if (sub == 0) most[r] = m, inv[r] = 1.f / l, rounded[r] = lr;
+        if (sub == 0) most[r] = m, inv[r] = 1.f / l, total[r] = l * weight_scale<T>();
     }
     __syncthreads();
     // outputs: units of four values, each summed by `lanes` lanes
@@ -651,7 +676,7 @@ __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
 #pragma unroll 4
         for (int j = sub; j < it.k; j += lanes) {
             const long of = (it.first + (long)j * groups) * p.Rb + head;
-            const float mj = p.part_ml[of * 4];
+            const float mj = p.part_ml[of * 2];
             const f4_t x = *reinterpret_cast<const f4_t *>(p.part_o + of * D + at % (D / 4) * 4);
             const float f = exp2f(mj - m);
             // a chunk without tokens has zeros, which no infinity or NaN may meet
@@ -665,7 +690,7 @@ __global__ __launch_bounds__(kNT) void kve_join_kernel(KveDecodeParams p) {
             // no tokens: 0; tokens that all score -inf: 0 / 0
             T *to = static_cast<T *>(p.out) + ((size_t)it.b * p.Hq + it.h * p.R + r) * D + at % (D / 4) * 4;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) store_act(to, e, m == -INFINITY ? 0.f : sum[e] / rounded[r]);
+            for (int e = 0; e < 4; ++e) store_act(to, e, m == -INFINITY ? 0.f : sum[e] / total[r]);
         }
     }
     if (!counts) return;
@@ -709,7 +734,7 @@ int kve_plan(const OjasxKVECache *c, const KveView &v, int num_q_heads, int max_
         return OJASX_ERR_INVALID;
     }
     p->o_bytes = p->items * p->Rb * v.D * 4;
-    p->ml_bytes = p->items * p->Rb * 16;
+    p->ml_bytes = (p->items * p->Rb * 8 + 15) / 16 * 16;     // what follows is 16-byte aligned
     p->item_bytes = p->items * (long)sizeof(KveItem);
     p->s_bytes = count ? (long)v.B * num_q_heads * p->stride * 4 : 0;
     const long all = (long)p->R * p->stride, room = v.D == 64 && p->NT == 1 ? kScoreFloats64 : kScoreFloats;

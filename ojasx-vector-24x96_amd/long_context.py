@@ -1172,8 +1172,9 @@ class PagedEvictingKVCache:
         gives 0, one whose tokens all score -inf NaN.  With ``count`` each
         token's softmax weights, summed over the query heads of its kv head, are
         added to its entry of ``weights``.  Scores, sums and counted weights are
-        float32; for bfloat16 and float16 the softmax's weights are rounded to
-        that type for the product with the values.  ``out`` may be the query
+        float32; for the product with bfloat16 and float16 values a softmax
+        weight is the sum of two numbers of that type (to 2^-14 of it;
+        float16: 2^-20 of it or 2^-40 of the largest).  ``out`` may be the query
         itself.  ``max_held``, a bound on ``held`` where the caller knows one,
         keeps launch and workspace as small as the sequences are; of a longer
         one the first ``max_held`` tokens are attended."""

@@ -390,6 +390,62 @@ def test_decode_extreme_scores(lc, dev, dtype):
     assert torch.isnan(out[0, 2:]).all() and not torch.isnan(out[0, :2]).any()
 
 
+@pytest.mark.parametrize("D,Hq", [(64, 1), (64, 20), (128, 4), (256, 1), (256, 17)])
+@pytest.mark.parametrize("dtype,p", [("bfloat16", 0.5 + 0.99 * 2.0 ** -9), ("float16", 0.5 + 0.99 * 2.0 ** -12),
+                                     ("bfloat16", 0.3 + 2.0 ** -12), ("float16", 0.7), ("float32", 0.7)])
+@pytest.mark.parametrize("n", [40, 300])
+def test_decode_weights_that_the_type_cannot_hold(lc, dev, D, Hq, dtype, p, n):
+    """Half the tokens of weight 1 and half of p, a number in the middle between two of the type, with values
+    that cancel: what remains shows how weights are rounded.
+
+    Of the scores one product is exact and its scaling off by 2^-23 of |ln p| < 2; exp2 and the maximum's factor
+    2^-22; sums of n terms, two products each, 2 n 2^-24 and 8 2^-24 for joins and the division; the weights'
+    two numbers 2^-14 (bfloat16) or 2^-20."""
+    import torch
+    page = 32
+    c = lc.PagedEvictingKVCache(1, D, num_sequences=1, page_size=page, max_pages=-(-n // page), rope_theta=None,
+                                dtype=getattr(torch, dtype), device=dev)
+    scale = float(np.float32(-math.log(p)))
+    r = rand(dev, dtype, D, seed=61)
+    c.keys[:, 0, 1::2, 0] = -1.0
+    c.values[:, 0, ::2] = r
+    c.values[:, 0, 1::2] = (-r.double() / p).to(c.dtype)
+    q = torch.zeros(1, Hq, D, dtype=c.dtype, device=dev)
+    q[..., 0] = 1.0
+    out = f64(c.decode(q, i32(dev, [n]), scale))
+    k, v = (f64(t).transpose(0, 2, 1, 3).reshape(-1, D)[:n] for t in (c.keys, c.values))
+    want, _, size, _ = kve.attend(f64(q)[0, 0], k, v, scale)
+    own = {"bfloat16": 2.0 ** -14, "float16": 2.0 ** -20, "float32": 0.0}[dtype]
+    tol = half_step(dtype) * np.abs(want) + (2.0 ** -22 + 2.0 ** -22 + (2 * n + 8) * 2.0 ** -24 + own) * size
+    tol += 2.0 ** -25 * (dtype == "float16")
+    assert (np.abs(out[0] - want) <= tol).all(), np.abs((out[0] - want) / size).max()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_decode_infinite_values_of_small_weights(lc, dev, dtype):
+    """An infinite value shows as such, however small its weight is beside the largest one, and a token whose
+    weight is 1 alone is its value bit for bit."""
+    import torch
+    D = 64
+    c = lc.PagedEvictingKVCache(1, D, num_sequences=1, page_size=16, max_pages=4, rope_theta=None,
+                                dtype=getattr(torch, dtype), device=dev)
+    v = rand(dev, dtype, 4, 1, 16, D, seed=62)
+    q = torch.zeros(1, 3, D, dtype=c.dtype, device=dev)
+    q[..., 0] = 1.0
+    for at, bits in ((3, 0.0), (17, 1.0), (40, 11.5), (9, 15.0), (50, 20.25), (33, 28.0), (2, 36.5), (1, 37.9)):
+        for sign in (1, -1):
+            c.values.copy_(v)
+            c.keys.zero_()
+            c.keys[at // 16, 0, at % 16, 0] = -bits
+            c.values[at // 16, 0, at % 16, 5] = sign * math.inf
+            out = c.decode(q, i32(dev, [50 + 14 * (at >= 50)]), math.log(2.0), count=False)
+            assert (out[..., 5] == sign * math.inf).all() and torch.isfinite(out).sum() == 3 * (D - 1), bits
+    c.values.copy_(v), c.keys.zero_()
+    assert torch.equal(c.decode(q, i32(dev, [1])), v[0, 0, :1].expand(3, D)[None])
+    c.keys[1, 0, 4, 0] = 1.0                          # the others' weights are 0 in fp32
+    assert torch.equal(c.decode(q, i32(dev, [60]), 1000.0), v[1, 0, 4:5].expand(3, D)[None])
+
+
 def test_decode_small_weights_keep_their_share(lc, dev):
     """One token of weight 1 and 100000 of 2^-24 each: together they are as much as 0.6 % of it, in fp16
     as well, whose smallest number is 2^-24."""
