@@ -465,8 +465,10 @@ OJASX_API int ojasx_kve_decode_device(const OjasxKVECache *cache, const void *q,
  * dropped one before it, the i-th of them the i-th place, with its weight and
  * position; nothing else is written.  held is read: it is min(held, budget) after
  * the call.  sink_tokens + recent_tokens <= budget; where more tokens than the
- * budget stand at such positions, the lowest slots of them stay.  max_held as
- * above. */
+ * budget stand at such positions, the lowest slots of them stay.  Slots of a page
+ * that is not there go first, but are places all the same: a token whose place lies in
+ * such a page is lost, so the pages of the first budget slots should be there.  max_held
+ * as above. */
 OJASX_API long ojasx_kve_evict_workspace(const OjasxKVECache *cache, int budget, int max_held);
 OJASX_API int ojasx_kve_evict_device(const OjasxKVECache *cache, const int *held, int budget, int sink_tokens,
                                      int recent_tokens, int max_held, void *workspace, long workspace_bytes,

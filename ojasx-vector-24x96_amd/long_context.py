@@ -1209,9 +1209,12 @@ class PagedEvictingKVCache:
         and of the others the ones of largest weight, ties to the lowest slot
         (NaN last).  A kept token from behind the budget takes the place of a
         dropped one before it, the i-th of them the i-th place, with its weight
-        and position; nothing else is written.  The caller then holds
-        min(held, budget) tokens; ``held`` is read, not changed, so that the
-        layers of a model can share it.  ``max_held`` as in ``decode``."""
+        and position; nothing else is written.  Slots of a page that is not there
+        go first, but are places all the same: a token whose place lies in such
+        a page is lost, so the pages of the first ``budget`` slots should be
+        there.  The caller then holds min(held, budget) tokens; ``held`` is read,
+        not changed, so that the layers of a model can share it.  ``max_held`` as
+        in ``decode``."""
         budget, sink_tokens, recent_tokens = int(budget), int(sink_tokens), int(recent_tokens)
         if min(sink_tokens, recent_tokens, max_held) < 0 or max(budget, max_held) > _MOST_INT or \
                 not 0 < budget >= sink_tokens + recent_tokens:

@@ -569,6 +569,23 @@ def test_evict_pages_that_are_not_there(lc, dev):
         check_evict(c, [96, 96], budget, 0, 3)
 
 
+def test_evict_loses_what_goes_to_a_page_that_is_not_there(lc, dev):
+    """As documented: of the tokens behind the budget those whose place is such a page's are gone, the others
+    move."""
+    import torch
+    c = filled(lc, dev, 64, "float32", 16, 1, [64], seed=15, poison=False)
+    c.block_table[0, 1] = -1
+    c.weights.fill_(1.0)
+    p, s = (torch.from_numpy(x).long() for x in place(c, 0, np.arange(64)))
+    c.weights[p[40:], 0, s[40:]] = 2.0                # 24 behind the budget: 8 and then 16 of slots 8 to 31
+    c.weights[p[:8], 0, s[:8]] = 3.0
+    was = c.values[p[40:], 0, s[40:]].clone(), c.values.clone()
+    check_evict(c, [64], 32, 0, 0)
+    assert torch.equal(c.values[p[8:16], 0, s[8:16]], was[0][:8])
+    was[1][p[8:16], 0, s[8:16]] = was[0][:8]
+    assert torch.equal(c.values, was[1])
+
+
 @pytest.mark.parametrize("n,budget", [(33000, 32900), (40001, 8192)])
 def test_evict_long(lc, dev, n, budget):
     """More tokens than the ranks' place in LDS."""
@@ -600,7 +617,7 @@ def roomy(lc, dev, dtype, Hkv, held, capacity, seed):
 @pytest.mark.parametrize("held,Hkv", [([40001, 3000, 4096, 4097, 900, 0], 2), ([2064, 33, 1], 1),
                                       (cycled([900, 4096, 201, 4097, 20, 1025, 1024], 86), 3)])
 @pytest.mark.parametrize("budget,recent", [(200, 64), (800, 128), (2900, 0)])     # moves in place, by a launch of their own
-@pytest.mark.parametrize("max_held", [0, 40001])
+@pytest.mark.parametrize("max_held", [0, 40001, 32768])     # the last: all ranks in LDS, as many as there can be
 def test_evict_short_sequences_of_a_large_pool(lc, dev, held, Hkv, budget, recent, max_held):
     """A bound past the ranks' place in LDS, sequences that hold few tokens: the newest and the first stay,
     of the others those of largest weight."""
