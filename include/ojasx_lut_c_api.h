@@ -484,7 +484,7 @@ OJASX_API int ojasx_kve_evict_device(const OjasxKVECache *cache, const int *held
  * which the running sum of e passes uniform times the kept sum.  temperature 0:
  * the largest logit, of equal ones the first.  Each setting is one value for all rows,
  * or an array of a value for each on the device (NULL: the value; values out of range
- * count as the nearest one in it, a temperature that is negative, NaN or infinite
+ * count as the nearest one in it, a NaN or a temperature that is negative or infinite
  * gives -1).  e is fp64; a token of e below 2^-51 is not drawn.  A row
  * with a NaN or +inf, or of -inf alone, gives -1.  vocab at most 2^22.  workspace:
  * ojasx_sample_workspace(...) bytes, 16-byte aligned, one for each call that may

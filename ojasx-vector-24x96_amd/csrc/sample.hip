@@ -153,7 +153,7 @@ __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
     s.k = a.top_ks ? a.top_ks[r] : a.top_k;
     s.p = a.top_ps ? (double)a.top_ps[r] : a.top_p;
     s.m = fmin(a.min_ps ? (double)a.min_ps[r] : a.min_p, 1.0);
-    s.bad = !(given >= 0.0) || given > (double)FLT_MAX;
+    s.bad = !(given >= 0.0) || given > (double)FLT_MAX || s.p != s.p || (a.min_ps && a.min_ps[r] != a.min_ps[r]);
     s.greedy = given == 0.0;
     const double inv = 1.0 / T;                  // the others are its multiples or T's: a division costs 20 products
     s.c = 1.4426950408889634074 * inv;

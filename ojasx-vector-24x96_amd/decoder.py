@@ -65,8 +65,8 @@ def sample_tokens(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     logit, of equal ones the first.  Each setting is a number, or a tensor of
     one for each row (float32, top_k int32) on the logits' device; entries out
     of range count as the nearest one in it.  A row without a distribution (a
-    NaN or +inf among its logits, -inf alone, or a temperature that is negative,
-    NaN or infinite) gives -1.
+    NaN or +inf among its logits, -inf alone, a NaN among its settings, or a
+    temperature that is negative or infinite) gives -1.
 
     e and sums are fp64 or of 50 bits, so the token is the definition's own unless
     uniform, top_p or min_p lies within about 1e-11 + vocab 2^-51 of a border

@@ -158,6 +158,22 @@ def test_rows_without_a_distribution(sample, dev):
     assert got.tolist()[:7] == [-1] * 7 and got[7] >= 0
 
 
+def test_settings_that_are_nan(sample, dev):
+    """A NaN among a row's settings gives -1, not the row without that cut or with its largest token alone;
+    infinities count as the nearest setting in range."""
+    import torch
+    x, u = logits(8, 10000, "bfloat16", seed=14).to(dev), torch.tensor(grid(8), device=dev)
+    nan, inf = math.nan, math.inf
+    p, m = [nan, 0.9, 0.9, inf, -inf, 0.9, nan, 0.9], [0.0, nan, 0.0, 0.0, 0.0, inf, nan, -inf]
+    for T in (1.0, 0.0):
+        for k in (0, 30):
+            got = sample(x, u, temperature=T, top_k=k, top_p=torch.tensor(p, device=dev),
+                         min_p=torch.tensor(m, device=dev)).tolist()
+            want = [kve.draw(x[b].double().cpu().numpy(), float(u[b]), T, k, min(max(p[b], 0.0), 1.0), min(max(m[b], 0.0), 1.0))
+                    for b in range(8)]
+            assert got == [-1, -1, want[2], want[3], want[4], want[5], -1, want[7]]
+
+
 def test_extreme_values(sample, dev):
     """Logits at the ends of the type, tiny and huge temperatures, a cut at a value next to 0."""
     import torch
