@@ -1145,6 +1145,7 @@ class PagedEvictingKVCache:
                     weight.get_device() != self._index or not weight.is_contiguous():
                 raise ValueError(f"weight must be contiguous float32 [{n}, {self.num_kv_heads}] on "
                                  f"{self.device}, got {weight.dtype} {tuple(weight.shape)} on {weight.device}")
+            _inference_tag(what, weight)
             wa = weight.data_ptr()
         es = 4 if self._c.dtype == _lib.DTYPE_F32 else 2
         k, ka, kt, kh = _aligned_rows(key, es)

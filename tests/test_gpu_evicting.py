@@ -716,6 +716,23 @@ def test_on_other_streams(lc, dev):
         assert np.allclose(grown.sum(0), 5 * 4, rtol=1e-3)      # five steps, four query heads a kv head
 
 
+def test_weights_with_a_gradient_are_refused(lc, dev):
+    """As keys, values and queries with one are: what the cache holds has none."""
+    import torch
+    from torch.autograd import forward_ad
+    c = lc.PagedEvictingKVCache(2, 64, num_sequences=2, max_pages=4, dtype=torch.bfloat16, device=dev)
+    k, one = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=dev), i32(dev, [1, 1])
+    w = torch.ones(2, 2, device=dev)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        c.append(k, k, one, weight=w.clone().requires_grad_())
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        c.append(k, k, one, weight=forward_ad.make_dual(w, w))
+    assert not c.weights.any()
+    with torch.no_grad():
+        c.append(k, k, one, weight=w.clone().requires_grad_())
+    assert c.weights.sum() == 4
+
+
 def test_refusals(lc, dev):
     import torch
     c = lc.PagedEvictingKVCache(2, 64, num_sequences=2, max_pages=4, dtype=torch.float32, device=dev)
