@@ -614,6 +614,16 @@ def roomy(lc, dev, dtype, Hkv, held, capacity, seed):
     return c
 
 
+@pytest.mark.parametrize("dtype,Hkv,Hq", [("bfloat16", 2, 8), ("float32", 1, 3), ("float16", 3, 102)])
+def test_decode_short_sequences_of_a_large_pool(lc, dev, dtype, Hkv, Hq):
+    """Without a bound, sequences of some tokens in a table of 40960 slots each."""
+    held = [700, 0, 1, 64, 65, 129, 2500]
+    c = roomy(lc, dev, dtype, Hkv, held, 40960, seed=52)
+    q = rand(dev, dtype, len(held), Hq, 64, seed=53)
+    before = f64(c.weights)
+    check_decode(c, q, held, c.decode(q, i32(dev, held)), before, dtype)
+
+
 @pytest.mark.parametrize("held,Hkv", [([40001, 3000, 4096, 4097, 900, 0], 2), ([2064, 33, 1], 1),
                                       (cycled([900, 4096, 201, 4097, 20, 1025, 1024], 86), 3)])
 @pytest.mark.parametrize("budget,recent", [(200, 64), (800, 128), (2900, 0)])     # moves in place, by a launch of their own
