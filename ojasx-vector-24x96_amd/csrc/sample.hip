@@ -95,7 +95,7 @@ __device__ __forceinline__ double held(double c) {
     asm("" : "+s"(c));
     return c;
 }
-// 2^(x c), x <= 0, x c > -1020, to about 2^-51.5: 2^f, |f| <= 1/2, by the polynomial of degree 10
+// 2^(x c), -1020 < x c <= 60, to about 2^-51.5: 2^f, |f| <= 1/2, by the polynomial of degree 10
 // through its values at the 11 Chebyshev nodes (off by 3e-16), scaled by the exponent.
 __device__ __forceinline__ double exp2_f64(double x, double c) {
     const double whole = held(0x1.8p52);         // the sum's last bits are x c rounded to whole numbers
@@ -128,6 +128,7 @@ __device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k &
 struct Row {
     double c;                            // log2(e) / T
     double bins;                         // bins per unit of the logit
+    double width;                        // a bin's
     float limit;                         // logits past it are one bin: 2^29 bins from 0
     double depth;                        // e of a logit further below the largest is that of this distance
     double p, m;
@@ -144,6 +145,13 @@ struct Row {
         const int b = min(top - bin(x), kBins - 1);
         return x == -INFINITY ? kBins - 1 : b;
     }
+    // A logit that none of bin b is above, nor further below than the bin's width unless the bin is one of all
+    // beyond the limit; top, most: the row's first bin and largest logit.  Sums of the bin are of e relative to
+    // it: relative to the row's largest, the step of a fixed point is as much as the e of a far bin's tokens, and
+    // equal logits all round the same way.
+    __device__ __forceinline__ double bin_top(int b, int top, float most) const {
+        return b ? ((double)(top - b) + 0.5) * width : (double)most;
+    }
     __device__ __forceinline__ double e(double x, double most) const { return exp2_f64(fmax(x - most, -depth), c); }
 };
 __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
@@ -158,6 +166,7 @@ __device__ __forceinline__ Row row_of(const SampleParams &a, int r) {
     const double inv = 1.0 / T;                  // the others are its multiples or T's: a division costs 20 products
     s.c = 1.4426950408889634074 * inv;
     s.bins = kBinsPerE * inv;
+    s.width = 1.0 / kBinsPerE * T;
     s.limit = (float)fmin(0x1p29 / kBinsPerE * T, (double)FLT_MAX);
     s.depth = 1000.0 / 1.4426950408889634074 * T;
     s.k_cut = s.k > 0 && s.k < a.vocab;
@@ -572,7 +581,7 @@ struct RowLds {
     double kept[kMostSlices];
     u64 csum[kMostSlices];               // of the cut's bin: sum of e above kappa, tokens at kappa
     int cties[kMostSlices];
-    double dw[kNW], rest, unit;           // unit: of csum
+    double dw[kNW], rest;
     unsigned kmin[2], kmax[2];
     u64 uw[kDigits / 64];
     Found found[kDigits / 64];
@@ -614,12 +623,6 @@ struct Chosen {
                 if (i0 + i * kNT < n && (int)(t[i].y >> 24) == b) f((int)(t[i].y & 0xffffffu), t[i].x, e[i]);
         }
     }
-    // A logit that none of bin b is above, nor further below than the bin's width unless the bin is one of all
-    // beyond row.limit.  Sums of the bin are of e relative to it: relative to the row's largest, the step of a
-    // fixed point is as much as the e of a far bin's tokens, and equal logits all round the same way.
-    __device__ __forceinline__ double bin_top(int b) const {
-        return b ? ((double)(h.top - b) + 0.5) / row.bins : (double)h.most;
-    }
     // The key of T's values whose high bits they are.
     static __device__ __forceinline__ unsigned whole_key(unsigned high) {
         const unsigned k = high << kLow;
@@ -635,8 +638,8 @@ struct Chosen {
         kmax = ~((unsigned)wave_min_i((int)(~kmax ^ 0x80000000u)) ^ 0x80000000u);
         if ((threadIdx.x & 63) == 0 && kmin <= kmax) atomicMin(&L.kmin[call], kmin), atomicMax(&L.kmax[call], kmax);
         __syncthreads();
-        const double top = bin_top(b), unit = row.e(top, h.most);
-        if (by_sum) need /= unit;
+        const double top = row.bin_top(b, h.top, h.most);
+        if (by_sum) need *= row.e(h.most, top);
         kmin = L.kmin[call] >> kLow, kmax = L.kmax[call] >> kLow;
         unsigned prefix = 0;
         // all in whole numbers, sums with frac bits behind the point: exactly one digit is the first to reach
@@ -702,7 +705,7 @@ struct Chosen {
         t = fmin(fmax(t, 1.0), (double)last_count);
         *kappa = prefix;
         *ties = (int)t;
-        *sum = (sums + t * e) * unit;
+        *sum = (sums + t * e) * row.e(top, h.most);
     }
 };
 }  // namespace
@@ -723,7 +726,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
     for (int s = tid; s < S; s += kNT) L.csum[s] = 0, L.cties[s] = 0;
     if (tid < 2) L.kmin[tid] = 0xffffffffu, L.kmax[tid] = 0;
     if (tid < kDigits) L.hsum[0][tid] = 0, L.hcount[0][tid] = 0;
-    if (tid == 0) L.hit = INT_MAX, L.last = -1, L.unit = 0.0;
+    if (tid == 0) L.hit = INT_MAX, L.last = -1;
     unsigned kappa = 0;
     int ties = INT_MAX, jc = kBins - 1;
     const int frac = min(kFrac, 62 - (32 - __clz(a.vocab)));   // a sum of e of all tokens fits
@@ -757,8 +760,7 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         if (row.m_cut && cut.m_key > kappa) kappa = cut.m_key, ties = INT_MAX;
         // the bin of the cut; a slice keeps its bins before that, and of its tokens in that bin those above kappa
         if (kappa) jc = min(max(h.top - row.bin(of_key(kappa)), 0), kBins - 1);
-        if (tid == 0) L.unit = ldexp(row.e(d.bin_top(jc), h.most), -kFrac);
-        d.template each<true>(jc, d.bin_top(jc), [&](int i, unsigned k, double e) {
+        d.template each<true>(jc, row.bin_top(jc, h.top, h.most), [&](int i, unsigned k, double e) {
             if (k > kappa) atomicAdd(&L.csum[i / kSlice], fixed(e, kFrac));      // a slice's, as its bins'
             if (k == kappa) atomicAdd(&L.cties[i / kSlice], 1);
         });
@@ -773,7 +775,8 @@ __global__ __launch_bounds__(kNT) void sample_row_kernel(SampleParams a, Work wk
         for (int s = s0; s < s1; ++s) before += L.cties[s];
         before = wave_scan_i(before) - before;   // ties of the slices before
         const int ties0 = before;
-        const double e = kappa ? row.e(of_key(kappa), h.most) : 0.0, unit = L.unit;
+        const double e = kappa ? row.e(of_key(kappa), h.most) : 0.0;
+        const double unit = row.e(row.bin_top(jc, h.top, h.most), h.most) * 0x1p-50;     // of csum
         double mine = 0.0;
         for (int s = s0; s < s1; ++s) {
             const int b = jc - 1 - L.c.off[s];
