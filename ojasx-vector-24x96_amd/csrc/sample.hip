@@ -25,12 +25,13 @@
 // relative to the bin's largest.  What is not drawn and lies in a bin that is counted shifts a border by
 // 2^-51 for each such token.
 //
-// What is read is small (2 or 4 bytes a logit); bound by the fp64 products of the exponentials and,
-// with cuts, two additions in LDS for each token in 1., and for few rows by the chains of three
-// launches.  Measured: 256 rows of 32000 fp16 logits without cuts 11 + 9 us (1. and 3.), 64 rows of
-// 151936 bf16 ones with settings of their own 19 + 18 + 20 us, 256 such rows with top-k 50 and top-p 0.9
-// 53 + 41 + 14, one row of 151936 fp32 ones with the same 7 + 9 + 15.5 us.  Keeping a row's workgroups on one die's L2 took 3 % off rows that
-// all have cuts and cost as much where only some have.
+// What is read is small (2 or 4 bytes a logit), and the fp64 products of the exponentials issue in no more
+// than a third of the cycles.  With cuts 1. is bound by its one or two additions in LDS for each token (half of
+// the LDS cycles are conflicts), 2. by adding the row's bins in every workgroup; the rest, and few rows, by the
+// latency of the launches' chains.  Measured: 256 rows of 32000 fp16 logits without cuts 11 + 10 us (1. and
+// 3.), 64 rows of 151936 bf16 ones with settings of their own 19 + 18 + 20 us, 256 such rows with top-k 50 and
+// top-p 0.9 54 + 42 + 15, one row of 151936 fp32 ones with the same 7 + 9 + 16.5 us.  Keeping a row's
+// workgroups on one die's L2 took 3 % off rows that all have cuts and cost as much where only some have.
 #include <cfloat>
 #include <climits>
 #include <cmath>
